@@ -84,6 +84,14 @@ _SIGS = {
     "aoship_model_reset_cache": (C.c_int, [_P]),
     "aoship_model_cache_len": (C.c_int, [_P]),
     "aoship_model_forward": (C.c_int, [_P, _P, C.c_int, C.c_int, _P, _P]),
+    "aoship_kv_cache_new": (_P, [_P]),
+    "aoship_kv_cache_free": (None, [_P]),
+    "aoship_kv_cache_set_rope": (C.c_int, [_P, _P, _P, C.c_int]),
+    "aoship_kv_cache_set_stream": (C.c_int, [_P, _P]),
+    "aoship_kv_cache_faults": (C.c_int, [_P]),
+    "aoship_kv_append": (C.c_int, [_P, C.c_int, _P, _P]),
+    "aoship_kv_read": (C.c_int, [_P, C.c_int, _P, _P, C.c_int64, _P, C.c_int64]),
+    "aoship_kv_attention": (C.c_int, [_P, C.c_int, _P, _P, C.c_int64, C.c_int, C.c_float, C.c_int, _P, C.c_int64]),
 }
 
 
@@ -707,4 +715,148 @@ class Model:
             for layer in getattr(self, "layers", []):
                 layer.h = None
             _lib.aoship_model_free(self.h)
+            self.h = None
+
+
+KV_FORMATS = {"bf16": 0, "mxfp8": 1, "mxfp4": 2}
+KV_FAULT_BATCH, KV_FAULT_PAGE = 1, 2
+
+
+class _KVConfig(C.Structure):
+    _fields_ = [("num_layers", C.c_int), ("num_kv_heads", C.c_int), ("head_dim", C.c_int), ("page_size", C.c_int),
+                ("num_pages", C.c_int), ("format", C.c_int)]
+
+
+class _KVBatch(C.Structure):
+    _fields_ = [("n_seqs", C.c_int), ("n_tokens", C.c_int), ("max_new", C.c_int), ("max_len", C.c_int),
+                ("starts", _P), ("lens", _P), ("pages", _P), ("page_stride", C.c_int)]
+
+
+class _KVRows(C.Structure):
+    _fields_ = [("q", _P), ("k", _P), ("v", _P), ("q_stride", C.c_int64), ("k_stride", C.c_int64),
+                ("v_stride", C.c_int64), ("q_bias", _P), ("k_bias", _P), ("v_bias", _P), ("q_out", _P),
+                ("q_out_stride", C.c_int64), ("num_heads", C.c_int)]
+
+
+class KVBatch:
+    """The sequences of a KVCache call (aoship_kv_batch_t): device int32 tensors starts [n + 1] (sequence s's new
+    tokens are rows starts[s] .. starts[s + 1] - 1 of the call), lens [n] (positions it holds, the new ones last) and
+    pages [n, stride]; max_new and max_len bound the sequences' new rows and positions. Keeps the tensors alive."""
+
+    def __init__(self, starts, lens, pages, max_new: int, max_len: int):
+        import torch
+
+        for t, dims in ((starts, 1), (lens, 1), (pages, 2)):
+            if t.dtype != torch.int32 or t.dim() != dims or not t.is_cuda or (t.numel() and t.stride(-1) != 1):
+                raise AosError("KVBatch: starts, lens [n] and pages [n, stride] must be device int32 tensors")
+        n = lens.numel()
+        if starts.numel() != n + 1 or pages.shape[0] != n:
+            raise AosError("KVBatch: starts must have one entry more than lens, pages a row for each")
+        self.starts, self.lens, self.pages = starts, lens, pages
+        # (rows may be set apart further than they are wide: the table's own width bounds max_len)
+        self.width = pages.shape[1]
+        self.c = _KVBatch(n, 0, max_new, max_len, starts.data_ptr(), lens.data_ptr(), pages.data_ptr(),
+                          pages.stride(0) if n > 1 else pages.shape[1])
+
+
+class KVCache:
+    """aoship_kv_cache_t: a paged key/value cache of many sequences in bfloat16 ("bf16"), 8 ("mxfp8") or 4 bits
+    ("mxfp4"). Row tensors are bfloat16 (or int16 bits) [tokens, heads, head_dim]; rows may be set apart (slices of a
+    joint projection), heads may not."""
+
+    def __init__(self, num_layers: int, num_kv_heads: int, head_dim: int, page_size: int, num_pages: int,
+                 format: str = "bf16"):
+        if format not in KV_FORMATS:
+            raise AosError(f"KVCache: unknown format {format!r}: {', '.join(KV_FORMATS)}")
+        cfg = _KVConfig(num_layers, num_kv_heads, head_dim, page_size, num_pages, KV_FORMATS[format])
+        self.h = lib().aoship_kv_cache_new(C.byref(cfg))
+        if not self.h:
+            raise AosError(f"aoship_kv_cache_new: {last_error()}")
+        self.num_kv_heads, self.head_dim, self.page_size = num_kv_heads, head_dim, page_size
+        self._rows = _KVRows()
+
+    def set_rope(self, cosines=None, sines=None) -> None:
+        """Host float32 [positions, head_dim / 2]; None for both turns the rotation off."""
+        if cosines is None and sines is None:
+            _check(lib().aoship_kv_cache_set_rope(self.h, None, None, 0), "aoship_kv_cache_set_rope")
+            return
+        c, s = (np.ascontiguousarray(a, dtype=np.float32) for a in (cosines, sines))
+        if c.shape != s.shape or c.ndim != 2 or c.shape[1] != self.head_dim // 2:
+            raise AosError("KVCache.set_rope: tables must be [positions, head_dim / 2]")
+        _check(lib().aoship_kv_cache_set_rope(self.h, c.ctypes.data, s.ctypes.data, c.shape[0]),
+               "aoship_kv_cache_set_rope")
+
+    def set_stream(self, stream_ptr) -> None:
+        _check(lib().aoship_kv_cache_set_stream(self.h, stream_ptr), "aoship_kv_cache_set_stream")
+
+    def faults(self) -> int:
+        """KV_FAULT_* bits of what the launches since the last call found wrong in their batches."""
+        f = lib().aoship_kv_cache_faults(self.h)
+        if f < 0:
+            raise AosError(f"aoship_kv_cache_faults: {last_error()}")
+        return f
+
+    def _batch(self, batch: KVBatch, *rows):
+        """The batch for calls over these row tensors, which have the same number of rows."""
+        n = rows[0].shape[0]
+        for t in rows:
+            if t.dim() != 3 or t.shape[0] != n or t.shape[2] != self.head_dim or t.element_size() != 2 \
+                    or t.is_floating_point() and str(t.dtype) != "torch.bfloat16" or not t.is_cuda \
+                    or t.numel() and (t.stride(2) != 1 or t.shape[1] > 1 and t.stride(1) != self.head_dim):
+                raise AosError("KVCache: rows must be device bfloat16 tensors [tokens, heads, head_dim] of one length")
+        if batch.width * self.page_size < batch.c.max_len:
+            raise AosError("KVCache: the page table is too narrow for max_len")
+        batch.c.n_tokens = n
+        return C.byref(batch.c)
+
+    @staticmethod
+    def _stride(t) -> int:
+        return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
+
+    def _kv_heads(self, *rows) -> None:
+        if any(t.shape[1] != self.num_kv_heads for t in rows):
+            raise AosError(f"KVCache: k and v rows must have {self.num_kv_heads} heads")
+
+    def append(self, layer: int, batch: KVBatch, k, v, q=None, q_out=None, q_bias=None, k_bias=None,
+               v_bias=None) -> None:
+        """Biases (device float32 [heads, head_dim]) and rotary embedding of the new rows; k and v go into the pages,
+        q to q_out."""
+        if (q is None) != (q_out is None) or q is not None and q.shape != q_out.shape:
+            raise AosError("KVCache.append: q and q_out come together, with the same shape")
+        b = self._batch(batch, k, v) if q is None else self._batch(batch, k, v, q, q_out)
+        self._kv_heads(k, v)
+        for t, heads in ((q_bias, 0 if q is None else q.shape[1]), (k_bias, k.shape[1]), (v_bias, v.shape[1])):
+            if t is not None and (str(t.dtype) != "torch.float32" or t.numel() != heads * self.head_dim
+                                  or not t.is_contiguous() or not t.is_cuda):
+                raise AosError("KVCache.append: biases must be device float32 [heads, head_dim]")
+        r = self._rows
+        r.k, r.v, r.k_stride, r.v_stride = k.data_ptr(), v.data_ptr(), self._stride(k), self._stride(v)
+        r.q = r.q_out = None
+        r.num_heads = 0
+        if q is not None:
+            r.q, r.q_stride, r.num_heads = q.data_ptr(), self._stride(q), q.shape[1]
+            r.q_out, r.q_out_stride = q_out.data_ptr(), self._stride(q_out)
+        r.q_bias, r.k_bias, r.v_bias = _ptr(q_bias), _ptr(k_bias), _ptr(v_bias)
+        _check(lib().aoship_kv_append(self.h, layer, b, C.byref(r)), "aoship_kv_append")
+
+    def read(self, layer: int, batch: KVBatch, k, v) -> None:
+        """The values that the cache holds of the batch's new rows, into k and v."""
+        b = self._batch(batch, k, v)
+        self._kv_heads(k, v)
+        _check(lib().aoship_kv_read(self.h, layer, b, k.data_ptr(), self._stride(k), v.data_ptr(), self._stride(v)),
+               "aoship_kv_read")
+
+    def attention(self, layer: int, batch: KVBatch, q, out, scale: float | None = None, window: int = 0) -> None:
+        """Causal attention of the batch's new rows (appended before) over their sequences; scale defaults to
+        head_dim ** -0.5, window 0 is none."""
+        b = self._batch(batch, q, out)
+        if q.shape != out.shape:
+            raise AosError("KVCache.attention: q and out must have the same shape")
+        _check(lib().aoship_kv_attention(self.h, layer, b, q.data_ptr(), self._stride(q), q.shape[1],
+                                         self.head_dim ** -0.5 if scale is None else scale, window, out.data_ptr(),
+                                         self._stride(out)), "aoship_kv_attention")
+
+    def __del__(self):
+        if getattr(self, "h", None) and _lib is not None:
+            _lib.aoship_kv_cache_free(self.h)
             self.h = None

@@ -51,6 +51,8 @@ SOURCES = [
     "aoship_model.hip",
     "aoship_liquid.hip",
     "aoship_mlp1.hip",
+    "aoship_kv.hip",
+    "aoship_kv_attn.hip",
     "aoship_api.cpp",
 ]
 

@@ -15,6 +15,7 @@
 #include <cstdio>
 #include <cstring>
 #include <mutex>
+#include <new>
 #include <string>
 #include <vector>
 
@@ -3439,6 +3440,277 @@ extern "C" int aoship_model_forward(aoship_model_t *m, const int32_t *ids, int T
   if (launch_err(aos_launch_gemv(&g, 0, &ctx), "lm head")) return -1;
   m->cache_len += T;
   return 0;
+}
+
+/* ------------------------------------------------------------------------------------------ */
+/* paged key/value cache                                                                       */
+/* ------------------------------------------------------------------------------------------ */
+
+static_assert(AOSHIP_KV_BF16 == AOS_KV_BF16 && AOSHIP_KV_MXFP8 == AOS_KV_MXFP8 && AOSHIP_KV_MXFP4 == AOS_KV_MXFP4,
+              "formats");
+static_assert(AOSHIP_KV_FAULT_BATCH == AOS_KV_FAULT_BATCH && AOSHIP_KV_FAULT_PAGE == AOS_KV_FAULT_PAGE, "faults");
+
+struct aoship_kv_cache {
+  aoship_kv_config_t cfg;
+  int device = 0, hdp = 0, page_shift = 0;
+  size_t layer_bytes = 0;
+  DevBuf pool, part, counters, faults, rope;
+  int rope_positions = 0;
+  hipStream_t stream = nullptr;
+};
+
+extern "C" aoship_kv_cache_t *aoship_kv_cache_new(const aoship_kv_config_t *c) {
+  if (!c) {
+    set_err("aoship_kv_cache_new: null config");
+    return nullptr;
+  }
+  if (c->num_layers < 1 || c->num_kv_heads < 1 || c->num_kv_heads > 4096 || c->head_dim < 8 || c->head_dim % 8 ||
+      c->head_dim > AOS_KV_MAX_HD || (c->page_size != 64 && c->page_size != 128 && c->page_size != 256) ||
+      c->num_pages < 1 || c->format < AOSHIP_KV_BF16 || c->format > AOSHIP_KV_MXFP4) {
+    set_err("aoship_kv_cache_new: unsupported shape (layers, pages and up to 4096 key/value heads at least 1, head_dim "
+            "a multiple of 8 up to 256, page_size 64, 128 or 256, format AOSHIP_KV_*)");
+    return nullptr;
+  }
+  const int hdp = c->head_dim <= 64 ? 64 : c->head_dim <= 128 ? 128 : 256;
+  const size_t tiles = (size_t)c->num_kv_heads * (size_t)(c->page_size / 64);
+  const size_t tile = aos_kv_tile_bytes(c->format, hdp);
+  if ((double)tiles * (double)tile * c->num_pages * c->num_layers > 1e13) {
+    set_err("aoship_kv_cache_new: the pages would take more than 10 TB");
+    return nullptr;
+  }
+  if (ensure_device()) return nullptr;
+  auto *m = new (std::nothrow) aoship_kv_cache();
+  if (!m) {
+    set_err("aoship_kv_cache_new: out of host memory");
+    return nullptr;
+  }
+  m->cfg = *c;
+  m->device = g_device;
+  m->hdp = hdp;
+  m->page_shift = c->page_size == 64 ? 6 : c->page_size == 128 ? 7 : 8;
+  m->layer_bytes = tiles * tile * (size_t)c->num_pages;
+  if (m->pool.alloc(m->layer_bytes * (size_t)c->num_layers, true) ||
+      m->part.alloc(aos_kv_part_floats(hdp) * sizeof(float), false) ||
+      m->counters.alloc(AOS_KV_MAX_WGS * sizeof(uint32_t), true) || m->faults.alloc(sizeof(uint32_t), true)) {
+    delete m;
+    return nullptr;
+  }
+  return m;
+}
+
+extern "C" void aoship_kv_cache_free(aoship_kv_cache_t *m) {
+  if (!m) return;
+  (void)hipDeviceSynchronize();
+  delete m;
+}
+
+/* The handle's own device is the one that aoship_init() chose last. */
+static int kv_check(const aoship_kv_cache *m, const char *what) {
+  if (!m) return set_err(std::string(what) + ": null cache");
+  if (m->device != g_device) return set_err(std::string(what) + ": the cache is on another device than aoship_init's");
+  return ensure_device();
+}
+
+extern "C" int aoship_kv_cache_set_rope(aoship_kv_cache_t *m, const float *cosines, const float *sines, int positions) {
+  if (!m || (!cosines != !sines) || (cosines && positions < 1))
+    return set_err("aoship_kv_cache_set_rope: null cache, one table without the other, or no positions");
+  if (kv_check(m, "aoship_kv_cache_set_rope")) return -1;
+  HIP_OR_FAIL(hipDeviceSynchronize(), "hipDeviceSynchronize"); /* (a launch may still read the old tables) */
+  m->rope_positions = 0;
+  m->rope.release();
+  if (!cosines) return 0;
+  const size_t table = (size_t)positions * (size_t)(m->cfg.head_dim / 2) * sizeof(float);
+  if (m->rope.alloc(2 * table, false)) return -1;
+  HIP_OR_FAIL(hipMemcpy(m->rope.p, cosines, table, hipMemcpyHostToDevice), "hipMemcpy H2D");
+  HIP_OR_FAIL(hipMemcpy(m->rope.as<unsigned char>() + table, sines, table, hipMemcpyHostToDevice), "hipMemcpy H2D");
+  m->rope_positions = positions;
+  return 0;
+}
+
+extern "C" int aoship_kv_cache_set_stream(aoship_kv_cache_t *m, void *stream) {
+  if (!m) return set_err("aoship_kv_cache_set_stream: null cache");
+  m->stream = (hipStream_t)stream;
+  return 0;
+}
+
+extern "C" int aoship_kv_cache_faults(aoship_kv_cache_t *m) {
+  if (kv_check(m, "aoship_kv_cache_faults")) return -1;
+  HIP_OR_FAIL(hipDeviceSynchronize(), "hipDeviceSynchronize");
+  uint32_t f = 0;
+  HIP_OR_FAIL(hipMemcpy(&f, m->faults.p, sizeof(f), hipMemcpyDeviceToHost), "hipMemcpy D2H");
+  if (f) HIP_OR_FAIL(hipMemset(m->faults.p, 0, sizeof(f)), "hipMemset");
+  return (int)f;
+}
+
+/* The checks that every call makes of its batch. n_seqs, n_tokens or max_new 0 is a call with nothing to do (1). */
+static int kv_batch_check(const char *what, const aoship_kv_config_t &c, int layer, const aoship_kv_batch_t *b) {
+  auto bad = [&](const char *why) { return set_err(std::string(what) + ": " + why); };
+  if (!b) return bad("null batch");
+  if (layer < 0 || layer >= c.num_layers) return bad("layer out of range");
+  if (b->n_seqs < 0 || b->n_tokens < 0 || b->max_new < 0 || b->max_len < 0) return bad("negative size in the batch");
+  if (b->max_len > (1 << 30) || b->n_seqs > (1 << 24) || b->n_tokens > (1 << 28))
+    return bad("batch too large (2^30 positions, 2^24 sequences, 2^28 rows)");
+  if (b->n_seqs == 0 || b->n_tokens == 0 || b->max_new == 0) return 1;
+  if (!b->starts || !b->lens || (!b->pages && b->max_len > 0)) return bad("null array in the batch");
+  if ((uintptr_t)b->starts % 4 || (uintptr_t)b->lens % 4 || (uintptr_t)b->pages % 4)
+    return bad("arrays of the batch must be 4-byte aligned");
+  if (b->page_stride < 0 || (long long)b->page_stride * c.page_size < b->max_len)
+    return bad("page_stride is less than max_len needs");
+  return 0;
+}
+
+/* a checked batch in the launches' form */
+static void kv_batch(const aoship_kv_cache *m, int layer, const aoship_kv_batch_t *b, aos_kv_batch *o) {
+  memset(o, 0, sizeof(*o));
+  o->pool = m->pool.as<unsigned char>() + m->layer_bytes * (size_t)layer;
+  o->format = m->cfg.format;
+  o->hd = m->cfg.head_dim;
+  o->hdp = m->hdp;
+  o->nkv = m->cfg.num_kv_heads;
+  o->page_shift = m->page_shift;
+  o->num_pages = m->cfg.num_pages;
+  o->starts = b->starts;
+  o->lens = b->lens;
+  o->pages = b->pages;
+  o->n_seqs = b->n_seqs;
+  o->n_tokens = b->n_tokens;
+  o->max_new = b->max_new < b->n_tokens ? b->max_new : b->n_tokens;
+  o->max_len = b->max_len;
+  o->stride = b->page_stride;
+  o->faults = m->faults.as<uint32_t>();
+}
+
+/* rows of `width` elements, 16 bytes at a time */
+static bool kv_rows_ok(const void *p, int64_t stride, long long width) {
+  return p && aligned16(p) && stride % 8 == 0 && stride >= width && stride < (1ll << 40);
+}
+
+static int kv_append_check(const aoship_kv_config_t &c, int rope_positions, int layer, const aoship_kv_batch_t *batch,
+                           const aoship_kv_rows_t *r) {
+  const std::string what = "aoship_kv_append";
+  const int empty = kv_batch_check(what.c_str(), c, layer, batch);
+  if (empty < 0) return -1;
+  if (!r) return set_err(what + ": null rows");
+  if (r->num_heads < 0 || r->num_heads % c.num_kv_heads || r->num_heads > 65536 ||
+      (r->num_heads > 0) != (r->q != nullptr) || (r->num_heads > 0) != (r->q_out != nullptr))
+    return set_err(what + ": queries need q, q_out and num_heads, a multiple of num_kv_heads");
+  if (empty) return 1;
+  const long long kw = (long long)c.head_dim * c.num_kv_heads, qw = (long long)c.head_dim * r->num_heads;
+  if (!kv_rows_ok(r->k, r->k_stride, kw) || !kv_rows_ok(r->v, r->v_stride, kw) ||
+      (r->q && (!kv_rows_ok(r->q, r->q_stride, qw) || !kv_rows_ok(r->q_out, r->q_out_stride, qw))))
+    return set_err(what + ": rows must be non-NULL, 16-byte aligned, with strides of at least a row and multiples of 8");
+  if (!aligned16(r->q_bias) || !aligned16(r->k_bias) || !aligned16(r->v_bias))
+    return set_err(what + ": biases must be 16-byte aligned");
+  if (r->q && r->q_out == r->q && r->q_out_stride != r->q_stride)
+    return set_err(what + ": q_out in the place of q needs its stride");
+  if (rope_positions && batch->max_len > rope_positions)
+    return set_err(what + ": max_len passes the rotary tables (" + std::to_string(rope_positions) + " positions)");
+  return 0;
+}
+
+static int kv_read_check(const aoship_kv_config_t &c, int layer, const aoship_kv_batch_t *batch, const void *k,
+                         int64_t k_stride, const void *v, int64_t v_stride) {
+  const std::string what = "aoship_kv_read";
+  const int empty = kv_batch_check(what.c_str(), c, layer, batch);
+  if (empty) return empty;
+  const long long kw = (long long)c.head_dim * c.num_kv_heads;
+  if (!kv_rows_ok(k, k_stride, kw) || !kv_rows_ok(v, v_stride, kw))
+    return set_err(what + ": rows must be non-NULL, 16-byte aligned, with strides of at least a row and multiples of 8");
+  return 0;
+}
+
+static int kv_attention_check(const aoship_kv_config_t &c, int layer, const aoship_kv_batch_t *batch, const void *q,
+                              int64_t q_stride, int num_heads, float scale, int window, const void *out,
+                              int64_t out_stride) {
+  const std::string what = "aoship_kv_attention";
+  const int empty = kv_batch_check(what.c_str(), c, layer, batch);
+  if (empty < 0) return -1;
+  if (num_heads < 1 || num_heads % c.num_kv_heads || num_heads > 65536)
+    return set_err(what + ": num_heads must be a multiple of num_kv_heads");
+  if (window < 0) return set_err(what + ": negative window");
+  if (!std::isfinite(scale)) return set_err(what + ": scale must be finite");
+  if (empty) return 1;
+  const long long qw = (long long)num_heads * c.head_dim;
+  if (!kv_rows_ok(q, q_stride, qw) || !kv_rows_ok(out, out_stride, qw))
+    return set_err(what + ": rows must be non-NULL, 16-byte aligned, with strides of at least a row and multiples of 8");
+  if (q == out) return set_err(what + ": out must not be q");
+  return 0;
+}
+
+/* Diagnostics (no counterpart in the reference), for tests without a device: the checks of the three calls on a
+ * cache of this shape; 0 goes ahead, 1 has nothing to do, -1 is refused. */
+extern "C" int aoship_internal_kv_append_check(const aoship_kv_config_t *c, int rope_positions, int layer,
+                                               const aoship_kv_batch_t *batch, const aoship_kv_rows_t *r) {
+  return kv_append_check(*c, rope_positions, layer, batch, r);
+}
+extern "C" int aoship_internal_kv_read_check(const aoship_kv_config_t *c, int layer, const aoship_kv_batch_t *batch,
+                                             const void *k, int64_t k_stride, const void *v, int64_t v_stride) {
+  return kv_read_check(*c, layer, batch, k, k_stride, v, v_stride);
+}
+extern "C" int aoship_internal_kv_attention_check(const aoship_kv_config_t *c, int layer, const aoship_kv_batch_t *batch,
+                                                  const void *q, int64_t q_stride, int num_heads, float scale, int window,
+                                                  const void *out, int64_t out_stride) {
+  return kv_attention_check(*c, layer, batch, q, q_stride, num_heads, scale, window, out, out_stride);
+}
+
+extern "C" int aoship_kv_append(aoship_kv_cache_t *m, int layer, const aoship_kv_batch_t *batch, const aoship_kv_rows_t *r) {
+  if (kv_check(m, "aoship_kv_append")) return -1;
+  const int rc = kv_append_check(m->cfg, m->rope_positions, layer, batch, r);
+  if (rc) return rc < 0 ? -1 : 0;
+  aos_kv_append_params p;
+  kv_batch(m, layer, batch, &p.b);
+  p.q = r->q;
+  p.k = r->k;
+  p.v = r->v;
+  p.q_ld = r->q_stride;
+  p.k_ld = r->k_stride;
+  p.v_ld = r->v_stride;
+  p.out_ld = r->q_out_stride;
+  p.qb = r->q_bias;
+  p.kb = r->k_bias;
+  p.vb = r->v_bias;
+  p.cosines = m->rope_positions ? m->rope.as<float>() : nullptr;
+  p.sines = m->rope_positions ? p.cosines + (size_t)m->rope_positions * (size_t)(m->cfg.head_dim / 2) : nullptr;
+  p.q_out = r->q_out;
+  p.nh = r->num_heads;
+  const aos_launch_ctx ctx = {m->stream, nullptr, nullptr};
+  return launch_err(aos_launch_kv_append(&p, &ctx), "kv append");
+}
+
+extern "C" int aoship_kv_read(aoship_kv_cache_t *m, int layer, const aoship_kv_batch_t *batch, aoship_bf16_t *k,
+                              int64_t k_stride, aoship_bf16_t *v, int64_t v_stride) {
+  if (kv_check(m, "aoship_kv_read")) return -1;
+  const int rc = kv_read_check(m->cfg, layer, batch, k, k_stride, v, v_stride);
+  if (rc) return rc < 0 ? -1 : 0;
+  aos_kv_read_params p;
+  kv_batch(m, layer, batch, &p.b);
+  p.k = k;
+  p.v = v;
+  p.k_ld = k_stride;
+  p.v_ld = v_stride;
+  const aos_launch_ctx ctx = {m->stream, nullptr, nullptr};
+  return launch_err(aos_launch_kv_read(&p, &ctx), "kv read");
+}
+
+extern "C" int aoship_kv_attention(aoship_kv_cache_t *m, int layer, const aoship_kv_batch_t *batch, const aoship_bf16_t *q,
+                                   int64_t q_stride, int num_heads, float scale, int window, aoship_bf16_t *out,
+                                   int64_t out_stride) {
+  if (kv_check(m, "aoship_kv_attention")) return -1;
+  const int rc = kv_attention_check(m->cfg, layer, batch, q, q_stride, num_heads, scale, window, out, out_stride);
+  if (rc) return rc < 0 ? -1 : 0;
+  aos_kv_attn_params p;
+  kv_batch(m, layer, batch, &p.b);
+  p.q = q;
+  p.out = out;
+  p.q_ld = q_stride;
+  p.out_ld = out_stride;
+  p.nh = num_heads;
+  p.window = window;
+  p.scale = scale;
+  p.part = m->part.as<float>();
+  p.counters = m->counters.as<uint32_t>();
+  const aos_launch_ctx ctx = {m->stream, nullptr, nullptr};
+  return launch_err(aos_launch_kv_attention(&p, &ctx), "kv attention");
 }
 
 /* ---- Liquid blend ---- */

@@ -662,10 +662,62 @@ typedef struct {
   float *y;       /* [out_len] */
 } aos_liquid_params;
 
+/* ---- paged key/value cache ----
+ * A layer's pool is [page][kv head][tile of 64 positions]; a tile holds its keys, then its values, then (quantised
+ * formats) their scale bytes, laid out for the matrix cores (aoship_kv.h). head_dim is stored padded to hdp. */
+#define AOS_KV_BF16 0
+#define AOS_KV_MXFP8 1
+#define AOS_KV_MXFP4 2
+#define AOS_KV_MAX_HD 256
+#define AOS_KV_FAULT_BATCH 1u /* inconsistent rows or lengths of a sequence */
+#define AOS_KV_FAULT_PAGE 2u  /* a page outside the cache */
+typedef struct {
+  unsigned char *pool; /* this layer's pages */
+  int format, hd, hdp, nkv, page_shift /* log2 of a page's positions */, num_pages;
+  const int32_t *starts, *lens, *pages; /* [n_seqs + 1], [n_seqs], [n_seqs][stride] */
+  int n_seqs, n_tokens, max_new, max_len, stride;
+  uint32_t *faults; /* AOS_KV_FAULT_* bits, or-ed in */
+} aos_kv_batch;
+
+typedef struct {
+  aos_kv_batch b;
+  const uint16_t *q, *k, *v; /* rows q_ld / k_ld / v_ld elements apart; q may be NULL */
+  long long q_ld, k_ld, v_ld, out_ld;
+  const float *qb, *kb, *vb; /* biases [heads][hd], NULL = none */
+  const float *cosines, *sines; /* [position][hd / 2], NULL = no rotation */
+  uint16_t *q_out;
+  int nh;
+} aos_kv_append_params;
+
+typedef struct {
+  aos_kv_batch b;
+  uint16_t *k, *v; /* rows k_ld / v_ld elements apart */
+  long long k_ld, v_ld;
+} aos_kv_read_params;
+
+/* Attention splits its work evenly over its workgroups, whatever sequence a share falls in; a row tile cut between
+ * workgroups has its pieces in the slots of those workgroups (two each) and is joined by the last of them. */
+#define AOS_KV_MAX_WGS 1024
+typedef struct {
+  aos_kv_batch b;
+  const uint16_t *q;
+  uint16_t *out;
+  long long q_ld, out_ld;
+  int nh, window; /* window 0: none */
+  float scale;
+  float *part;        /* pieces of cut row tiles (aos_kv_part_floats) */
+  uint32_t *counters; /* [AOS_KV_MAX_WGS], zero between launches */
+} aos_kv_attn_params;
+
 #ifdef __cplusplus
 extern "C" {
 #endif
 /* Host-side launchers (return hipError_t as int). */
+int aos_launch_kv_append(const aos_kv_append_params *p, const aos_launch_ctx *ctx);
+int aos_launch_kv_read(const aos_kv_read_params *p, const aos_launch_ctx *ctx);
+int aos_launch_kv_attention(const aos_kv_attn_params *p, const aos_launch_ctx *ctx);
+size_t aos_kv_part_floats(int hdp); /* workspace of an attention launch over a cache of this padded head_dim */
+size_t aos_kv_tile_bytes(int format, int hdp);
 int aos_launch_route(const aos_route_params *p, const aos_launch_ctx *ctx);
 int aos_launch_embed(const aos_embed_params *p, const aos_launch_ctx *ctx);
 int aos_launch_norm(const aos_norm_params *p, const aos_launch_ctx *ctx);

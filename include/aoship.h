@@ -363,6 +363,97 @@ int aoship_model_cache_len(const aoship_model_t *model);
 int aoship_model_forward(aoship_model_t *model, const int32_t *ids, int T, int position_offset,
                          const aoship_ring_t *rings, float *logits);
 
+/* ---- paged key/value cache: many sequences, 16, 8 or 4 bits ---------------------------------- */
+
+/* The cache of aoship_model_t holds one sequence; a program that serves many keeps their keys and values in a
+ * paged one and runs, per layer, aoship_qkv_forward, aoship_kv_append, aoship_kv_attention and
+ * aoship_proj_forward("o_proj") over the rows of all sequences at once (the reference has one
+ * cache per sequence, mlx_kv_cache_t, wrapper.h:324, and attends over it, mlx_cpp_wrapper_real.cpp:3282-3327).
+ *
+ * A cache is num_pages pages of page_size positions (64, 128 or 256) per layer; which pages are whose is the
+ * caller's, in a page table. head_dim: a multiple of 8 up to 256 (kept padded to 64, 128 or 256). Formats:
+ *   AOSHIP_KV_BF16   bfloat16
+ *   AOSHIP_KV_MXFP8  e4m3 codes  } per row and 32 dimensions a scale 2^e, the smallest that keeps the block's largest
+ *   AOSHIP_KV_MXFP4  e2m1 codes  } magnitude within the codes' range (448, 6), e >= -117 (-125); codes round to
+ *                                  nearest even; a block that holds an infinity or a NaN reads back as NaN (and
+ *                                  a magnitude whose code rounds up to 2^128, as infinity). */
+#define AOSHIP_KV_BF16 0
+#define AOSHIP_KV_MXFP8 1
+#define AOSHIP_KV_MXFP4 2
+
+typedef struct aoship_kv_cache aoship_kv_cache_t;
+typedef struct {
+  int num_layers, num_kv_heads, head_dim, page_size, num_pages, format;
+} aoship_kv_config_t;
+
+/* The pages (zeros at first) and the attention's workspace, allocated here: no call below allocates, and all of
+ * them can be captured into a graph. NULL on error. */
+aoship_kv_cache_t *aoship_kv_cache_new(const aoship_kv_config_t *config);
+void aoship_kv_cache_free(aoship_kv_cache_t *cache);
+
+/* Rotary embedding of aoship_kv_append: cosines and sines [positions][head_dim / 2] (host, copied); NULL for both:
+ * none, as at first. Synchronises the device. Returns 0 / -1. */
+int aoship_kv_cache_set_rope(aoship_kv_cache_t *cache, const float *cosines, const float *sines, int positions);
+
+/* Stream (hipStream_t) for this cache's launches; NULL = null stream. Returns 0 / -1. */
+int aoship_kv_cache_set_stream(aoship_kv_cache_t *cache, void *stream);
+
+/* What the launches found wrong in the device arrays of their batches since the last call (and clears it):
+ * a combination of the bits below, 0 for nothing, -1 on error. Synchronises the device. Such a sequence is left
+ * out whole (BATCH: starts that fall or pass n_tokens, more new rows than max_new, a length outside 0..max_len), or
+ * the positions of such a page are (PAGE): not written, read as zeros, not attended to. */
+#define AOSHIP_KV_FAULT_BATCH 1
+#define AOSHIP_KV_FAULT_PAGE 2
+int aoship_kv_cache_faults(aoship_kv_cache_t *cache);
+
+/* The sequences of a call. Sequence s has the rows starts[s] .. starts[s + 1] - 1 of the call's row arrays as its new
+ * tokens (none is fine) and holds lens[s] positions, the new ones the last of them; position i is in page
+ * pages[s * page_stride + i / page_size]. Rows past starts[n_seqs] are left as they are. With fewer positions than
+ * rows (a sequence padded in front), the first rows have no position: append and read skip them (their outputs are
+ * left as they are) and attention gives zeros. Pages may be shared by sequences that only read them; a page that
+ * two sequences of one append write holds the rows of either. starts, lens and pages are device arrays, read by the
+ * launch; n_tokens, max_new and max_len are bounds that it is made for (so that a captured launch can be replayed
+ * with other contents within them): rows of the arrays, most new rows and most positions of a sequence. */
+typedef struct {
+  int n_seqs, n_tokens, max_new, max_len;
+  const int32_t *starts; /* [n_seqs + 1] */
+  const int32_t *lens;   /* [n_seqs] */
+  const int32_t *pages;  /* [n_seqs][page_stride] */
+  int page_stride;       /* at least max_len / page_size, rounded up */
+} aoship_kv_batch_t;
+
+/* Rows of a call (device): row t at q + t * q_stride (elements, multiples of 8; pointers 16-byte aligned), its heads
+ * head_dim apart, so that the projections' outputs and slices of a joint one both serve. Biases are device float32
+ * [heads * head_dim] or NULL. q, q_out and num_heads (a multiple of num_kv_heads) are 0 where there are no queries;
+ * q_out may be q. */
+typedef struct {
+  const aoship_bf16_t *q, *k, *v;
+  int64_t q_stride, k_stride, v_stride;
+  const float *q_bias, *k_bias, *v_bias;
+  aoship_bf16_t *q_out;
+  int64_t q_out_stride;
+  int num_heads;
+} aoship_kv_rows_t;
+
+/* Biases and rotary embedding of the new rows (float32; (a, b) -> (a c - b s, a s + b c) over the halves of a query
+ * or key row, as the fused forward's, mlx_cpp_wrapper_real.cpp:3249-3279), rounded to bfloat16; queries go to q_out,
+ * keys and values in the cache's format to the pages of `layer`. Asynchronous. Returns 0 / -1. */
+int aoship_kv_append(aoship_kv_cache_t *cache, int layer, const aoship_kv_batch_t *batch, const aoship_kv_rows_t *rows);
+
+/* The rows that an append of the same batch wrote, as the bfloat16 values that the cache holds for them (a batch
+ * whose sequences' rows are all their positions reads them whole): k, v: device rows like those of append.
+ * Asynchronous. Returns 0 / -1. */
+int aoship_kv_read(aoship_kv_cache_t *cache, int layer, const aoship_kv_batch_t *batch, aoship_bf16_t *k,
+                   int64_t k_stride, aoship_bf16_t *v, int64_t v_stride);
+
+/* Attention of the new rows (already appended) over their sequences: o = sum_j softmax_j(scale q . k_j) v_j over the
+ * positions j up to the row's own p, and past p - window (0: all); query heads share key/value heads in
+ * consecutive groups. A row that sees nothing gives zeros. q, out: device rows of num_heads * head_dim (out must
+ * not overlap q). Asynchronous. Returns 0 / -1. */
+int aoship_kv_attention(aoship_kv_cache_t *cache, int layer, const aoship_kv_batch_t *batch, const aoship_bf16_t *q,
+                        int64_t q_stride, int num_heads, float scale, int window, aoship_bf16_t *out,
+                        int64_t out_stride);
+
 /* ---- Liquid blend (crates/adapteros-lora-kernel-api/src/liquid.rs) ------------------------ */
 
 #define AOSHIP_LIQUID_MAX_ADAPTERS 3 /* liquid.rs:12 (LIQUID_MAX_ADAPTERS) */

@@ -1,0 +1,287 @@
+"""Attention over the paged cache against float64 (tests/kv_plain.py: attention and the bound attention_bound derives
+for a result: the roundings of the output and of the probabilities to bfloat16, float32 scores and sums)."""
+import numpy as np
+import pytest
+
+import kv_plain as P
+
+pytestmark = pytest.mark.gpu
+
+
+def _setup(hip, fmt, nh, nkv, hd, page, new, lens, seed=0, sharp=1.0, poison=None):
+    """A cache of sequences whose rows are random, and queries for their last `new` positions."""
+    rng = np.random.default_rng(seed)
+    held = [max(0, n) for n in lens]
+    pool = P.Pool(hip, held, nkv, hd, page, fmt, seed=seed)
+    k, v = (P.bf16(rng.standard_normal((sum(held), nkv, hd))) for _ in range(2))
+    if poison:
+        poison(k, v)
+    if sum(held):
+        pool.cache.append(0, pool.batch(held, held), P.to_gpu(k), P.to_gpu(v))
+    q = P.bf16(sharp * rng.standard_normal((sum(new), nh, hd)))
+    cut = np.cumsum(held)[:-1]
+    seqs = list(zip(np.split(q, np.cumsum(new)[:-1]), np.split(P.quantised(k, fmt), cut), np.split(P.quantised(v, fmt), cut)))
+    return pool, q, seqs
+
+
+def _run(pool, q, new, lens, window=0, scale=None, **kw):
+    import torch
+
+    out = torch.full(q.shape, 7.0, dtype=torch.bfloat16, device="cuda")
+    pool.cache.attention(0, pool.batch(new, lens, **kw), P.to_gpu(q), out, scale=scale, window=window)
+    return P.to_cpu(out)
+
+
+def _check(got, seqs, new, scale, window=0):
+    at = 0
+    for (q, k, v), n in zip(seqs, new):
+        o, a = P.attention(q, k, v, scale, window)
+        g = got[at:at + n]
+        at += n
+        if not n:
+            continue
+        assert np.array_equal(np.isnan(g), np.isnan(o)), "NaN"
+        tol = P.attention_bound(q, k, a, o, scale)
+        fin = np.isfinite(o)
+        assert np.array_equal(g[~fin & ~np.isnan(o)], o[~fin & ~np.isnan(o)])
+        off = np.abs(g - o)[fin] / tol[fin]
+        assert off.size == 0 or off.max() <= 1.0, (float(off.max()), n, k.shape)
+
+
+ONES = [1, 2, 63, 64, 65, 128, 200, 1000]
+
+
+@pytest.mark.parametrize("fmt", P.FORMATS)
+@pytest.mark.parametrize("nh,nkv,hd,page", [(14, 2, 64, 64), (28, 4, 128, 128), (3, 3, 128, 64), (40, 1, 80, 64),
+                                            (4, 2, 256, 256), (6, 2, 8, 64), (5, 1, 136, 64)])
+def test_one_token_each(hip, fmt, nh, nkv, hd, page):
+    """Lengths about the tiles' borders, more query heads than a matrix instruction has columns, none."""
+    new = [1] * len(ONES) + [0]
+    lens = ONES + [77]
+    pool, q, seqs = _setup(hip, fmt, nh, nkv, hd, page, new, lens, seed=hd)
+    _check(_run(pool, q, new, lens), seqs, new, hd ** -0.5)
+    assert pool.cache.faults() == 0
+
+
+@pytest.mark.parametrize("fmt", P.FORMATS)
+@pytest.mark.parametrize("nh,nkv,hd,page", [(14, 2, 64, 64), (7, 1, 128, 64), (2, 2, 128, 128), (3, 1, 80, 64), (8, 2, 256, 64)])
+@pytest.mark.parametrize("window", [0, 1, 70])
+def test_chunks(hip, fmt, nh, nkv, hd, page, window):
+    """Drafted tokens, chunks over what is held, whole prompts and single tokens in one call."""
+    new = [3, 65, 1, 130, 16, 0, 40]
+    past = [100, 0, 300, 64, 0, 5, 171]
+    lens = [a + b for a, b in zip(new, past)]
+    pool, q, seqs = _setup(hip, fmt, nh, nkv, hd, page, new, lens, seed=hd + window)
+    _check(_run(pool, q, new, lens, window), seqs, new, hd ** -0.5, window)
+
+
+@pytest.mark.parametrize("fmt", P.FORMATS)
+@pytest.mark.parametrize("new,lens", [([1], [9001]), ([5], [20011]), ([300], [3001]), ([700], [700]), ([1, 1], [64, 40000])])
+def test_long(hip, fmt, new, lens):
+    """Row tiles that many workgroups share, and uneven lengths."""
+    pool, q, seqs = _setup(hip, fmt, 7, 1, 128, 256, new, lens, seed=lens[-1], sharp=3.0)
+    got = _run(pool, q, new, lens)
+    _check(got, seqs, new, 128 ** -0.5)
+    for _ in range(3):
+        assert np.array_equal(got, _run(pool, q, new, lens))  # (no order depends on timing)
+
+
+@pytest.mark.parametrize("n,new", [(150, 1), (70, 2), (130, 20)])
+def test_many_sequences(hip, n, new):
+    """More sequences than lanes, some without rows or positions."""
+    rng = np.random.default_rng(n)
+    news = [int(x) for x in rng.integers(0, new + 1, n)]
+    lens = [a + int(b) for a, b in zip(news, rng.integers(0, 200, n))]
+    pool, q, seqs = _setup(hip, "mxfp8", 4, 2, 64, 64, news, lens)
+    _check(_run(pool, q, news, lens, max_new=new), seqs, news, 64 ** -0.5)
+
+
+@pytest.mark.parametrize("fmt", P.FORMATS)
+@pytest.mark.parametrize("new,lens", [([6, 4, 1], [2, 0, 0]), ([40, 90, 3], [10, 70, 0])])
+def test_rows_that_see_nothing(hip, fmt, new, lens):
+    """Sequences padded in front, and rows of a sequence without positions: zeros."""
+    pool, q, seqs = _setup(hip, fmt, 4, 2, 128, 64, new, lens)
+    got = _run(pool, q, new, lens)
+    _check(got, seqs, new, 128 ** -0.5)
+    assert (got[:new[0] - lens[0]] == 0).all() and (got[-new[2]:] == 0).all()
+
+
+@pytest.mark.parametrize("fmt", P.FORMATS)
+@pytest.mark.parametrize("new", [1, 4, 90])
+def test_infinities_and_nans(hip, fmt, new):
+    """Visible ones reach the rows that see them, by the formula; those of later positions, of positions left of the
+    window and of stale rows in a page reach nobody."""
+    nh, nkv, hd, L = 4, 2, 64, 230
+    first = L - new
+
+    def poison(k, v):
+        v[first + new // 2, 0, 5] = np.inf       # seen by the second half of the new rows
+        v[first + new // 2, 0, 6] = -np.inf
+        v[L - 1, 1, 40] = np.nan                 # seen by the last row only
+        k[L - 1, 1, 33] = np.nan if new > 1 else 0.0
+        v[2, :, :] = np.nan                      # left of every window
+        k[3, :, :] = np.inf
+        v[L:] = np.nan                           # (stale rows: written by an earlier, longer sequence)
+        k[L:] = np.nan
+
+    pool, q, seqs = _setup(hip, fmt, nh, nkv, hd, 64, [new], [L + 20], poison=poison)
+    q, (_, k, v) = q, seqs[0]
+    got = _run(pool, q, [new], [L], window=100, max_len=256)
+    want = [(q, k[:L], v[:L])]
+    if fmt == "bf16":
+        _check(got, want, [new], hd ** -0.5, 100)
+    else:  # a block of 32 dimensions is NaN whole: compare where the float64 form is finite, and its NaNs
+        o, a = P.attention(q, k[:L], v[:L], hd ** -0.5, 100)
+        assert np.array_equal(np.isnan(got), ~np.isfinite(o))
+        fin = np.isfinite(o)
+        assert (np.abs(got - o)[fin] <= P.attention_bound(q, k[:L], a, o, hd ** -0.5)[fin]).all()
+
+
+@pytest.mark.parametrize("sharp,scale", [(60.0, None), (1.0, 0.0), (2.0, -0.3)])
+def test_scores_of_any_size(hip, sharp, scale):
+    """Scores of hundreds (the running maximum moves far), a scale of zero, a negative one."""
+    new, lens = [1, 30], [500, 400]
+    pool, q, seqs = _setup(hip, "bf16", 4, 2, 64, 64, new, lens, sharp=sharp)
+    _check(_run(pool, q, new, lens, scale=scale), seqs, new, 64 ** -0.5 if scale is None else scale)
+
+
+def test_strides_and_rows_left_alone(hip):
+    """Queries as a slice of a joint projection, outputs into a wider tensor, rows behind the last sequence."""
+    import torch
+
+    new, lens, nh, hd = [1, 70, 2], [80, 90, 300], 4, 128
+    pool, q, seqs = _setup(hip, "mxfp8", nh, 2, hd, 64, new, lens)
+    T = sum(new)
+    joint = torch.zeros((T + 5, nh + 3, hd), dtype=torch.bfloat16, device="cuda")
+    joint[:T, 1:1 + nh] = P.to_gpu(q)
+    wide = torch.full((T + 5, nh + 2, hd), 7.0, dtype=torch.bfloat16, device="cuda")
+    pool.cache.attention(0, pool.batch(new, lens), joint[:, 1:1 + nh], wide[:, 2:])
+    _check(P.to_cpu(wide[:T, 2:]), seqs, new, hd ** -0.5)
+    assert (wide[:T, :2] == 7).all() and (wide[T:] == 7).all()
+
+
+def test_bad_pages_and_rows(hip):
+    """Positions of a page outside the cache are not attended to; a sequence that does not fit is left alone; both are
+    reported and neighbours are served."""
+    import torch
+
+    for new in ([1, 1, 1], [1, 100, 40]):
+        lens, nh, hd = [70, 200, 90], 4, 64
+        pool, q, seqs = _setup(hip, "bf16", nh, 2, hd, 64, new, lens)
+        pool.pages[1, 1] = 10 ** 7
+        got = _run(pool, q, new, lens)
+        assert pool.cache.faults() == hip.KV_FAULT_PAGE
+        _check(got[:1], seqs[:1], new[:1], hd ** -0.5)
+        _check(got[-new[2]:], seqs[2:], new[2:], hd ** -0.5)
+        qq, k, v = seqs[1]
+        for t in (0, new[1] - 1):
+            end = lens[1] - new[1] + t + 1
+            keep = [i for i in range(end) if not 64 <= i < 128]
+            o, a = P.attention(qq[t:t + 1], k[keep], v[keep], hd ** -0.5)
+            assert (np.abs(got[new[0] + t] - o[0]) <= P.attention_bound(qq, k, a, o, hd ** -0.5)[0]).all()
+        pool.pages.copy_(torch.from_numpy(pool.table))
+        for bad in ([70, 201, 90], [70, -3, 90]):
+            got = _run(pool, q, new, bad, max_len=200)
+            assert pool.cache.faults() == hip.KV_FAULT_BATCH
+            assert (got[new[0]:new[0] + new[1]] == 7).all()
+            _check(got[:1], seqs[:1], new[:1], hd ** -0.5)
+        pool.pages[0, 0] = -1  # nothing left to see
+        got = _run(pool, q, new, [64, 200, 90])
+        assert (got[0] == 0).all() and pool.cache.faults() == hip.KV_FAULT_PAGE
+
+
+@pytest.mark.parametrize("new", [1, 40])
+def test_graph_replays(hip, new):
+    """append and attention captured on another stream, replayed while the sequences grow, between eager work."""
+    import torch
+
+    rng = np.random.default_rng(new)
+    n, nh, nkv, hd, cap = 4, 8, 2, 128, 900
+    pool = P.Pool(hip, [cap] * n, nkv, hd, 64, "bf16")
+    start = [3, 500, 64, 250]
+    past = [P.bf16(rng.standard_normal((sum(start), nkv, hd))) for _ in range(2)]
+    pool.cache.append(0, pool.batch(start, start), *map(P.to_gpu, past))
+    held = [list(np.split(x, np.cumsum(start)[:-1])) for x in past]
+    q, k, v = (torch.zeros((n * new, h, hd), dtype=torch.bfloat16, device="cuda") for h in (nh, nkv, nkv))
+    out = torch.empty_like(q)
+    batch = pool.batch([new] * n, [s + new for s in start], max_len=cap)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    pool.cache.set_stream(side.cuda_stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        pool.cache.append(0, batch, k, v)
+        pool.cache.attention(0, batch, q, out)
+    for step in range(4):
+        x = [P.bf16(rng.standard_normal(t.shape)) for t in (q, k, v)]
+        for t, y in zip((q, k, v), x):
+            t.copy_(P.to_gpu(y))
+        if step:
+            batch.lens += new
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        for i in range(2):
+            for s in range(n):
+                held[i][s] = np.concatenate([held[i][s], x[1 + i][s * new:(s + 1) * new]])
+        seqs = [(x[0][s * new:(s + 1) * new], held[0][s], held[1][s]) for s in range(n)]
+        _check(P.to_cpu(out), seqs, [new] * n, hd ** -0.5)
+    pool.cache.set_stream(None)
+
+
+@pytest.mark.parametrize("fmt", P.FORMATS)
+def test_a_layer_as_it_is_served(hip, fmt):
+    """q/k/v projections with adapters, biases, rotary embedding and cache, attention, o projection: a prompt of each
+    of three streams, then tokens one by one, against the same steps in float64 from the projections' outputs."""
+    import torch
+
+    rng = np.random.default_rng(9)
+    hidden, nh, nkv, hd = 512, 8, 2, 64
+    layer = hip.Layer(0)
+    for m, o, i in (("q_proj", nh * hd, hidden), ("k_proj", nkv * hd, hidden), ("v_proj", nkv * hd, hidden),
+                    ("o_proj", hidden, nh * hd)):
+        layer.set_base(m, rng.integers(0, 2 ** 32, (o, i // 8), dtype=np.uint32),
+                       (rng.random((o, i // 64)) * 0.01).astype(np.float16), np.full((o, i // 64), -0.04, np.float16))
+    ad = hip.LoraAdapter(0, 1, 1.0)
+    for m, o, i in (("q_proj", nh * hd, hidden), ("o_proj", hidden, nh * hd)):
+        ad.set_module(0, m, (rng.standard_normal((16, i)) / i ** 0.5).astype(np.float32),
+                      (0.01 * rng.standard_normal((o, 16))).astype(np.float32))
+    layer.set_adapters([ad])
+    ring = np.zeros(1, hip.RING_DTYPE)
+    ring["top_k"], ring["gates_q15"][0, 0] = 1, 32767
+    pool = P.Pool(hip, [150] * 3, nkv, hd, 64, fmt)
+    cos, sin = (f(np.arange(150)[:, None] * 10.0 ** (-np.arange(hd // 2) / 8)).astype(np.float32) for f in (np.cos, np.sin))
+    pool.cache.set_rope(cos, sin)
+    bias = [rng.standard_normal((h, hd)).astype(np.float32) for h in (nh, nkv, nkv)]
+    gb = [torch.from_numpy(b).cuda() for b in bias]
+    kept = [[np.zeros((0, nkv, hd))] * 3 for _ in range(2)]
+    lens = [0, 0, 0]
+    for new in ([100, 37, 5], [1, 1, 1], [1, 1, 0], [1, 2, 9]):
+        T = sum(new)
+        x = P.to_gpu(rng.standard_normal((T, hidden)))
+        rings = torch.from_numpy(np.repeat(ring, T).view(np.uint8)).cuda()
+        q, k, v = (torch.empty((T, h, hd), dtype=torch.bfloat16, device="cuda") for h in (nh, nkv, nkv))
+        layer.qkv_forward(x, rings, q, k, v)
+        raw = [P.to_cpu(t) for t in (q, k, v)]
+        at = list(lens)
+        lens = [a + b for a, b in zip(lens, new)]
+        batch = pool.batch(new, lens)
+        pool.cache.append(0, batch, k, v, q=q, q_out=q, q_bias=gb[0], k_bias=gb[1], v_bias=gb[2])
+        out = torch.empty_like(q)
+        pool.cache.attention(0, batch, q, out)
+        y = torch.empty((T, hidden), dtype=torch.bfloat16, device="cuda")
+        layer.proj_forward("o_proj", out.view(T, nh * hd), rings, y)
+        pos = np.concatenate([np.arange(a, a + n) for a, n in zip(at, new)])
+        full = [r.astype(np.float32) + b for r, b in zip(raw, bias)]
+        rows = [P.bf16(P.rotated(full[0], cos[pos], sin[pos])), P.bf16(P.rotated(full[1], cos[pos], sin[pos])), P.bf16(full[2])]
+        seqs = []
+        for s in range(3):
+            part = slice(sum(new[:s]), sum(new[:s + 1]))
+            for i in range(2):
+                kept[i][s] = np.concatenate([kept[i][s], P.quantised(rows[1 + i][part], fmt)])
+            seqs.append((rows[0][part], kept[0][s], kept[1][s]))
+        _check(P.to_cpu(out), seqs, new, hd ** -0.5)
+        again = torch.empty_like(y)
+        layer.proj_forward("o_proj", out.view(T, nh * hd), rings, again)
+        assert torch.isfinite(y).all() and torch.equal(y, again)
+    assert pool.cache.faults() == 0

@@ -1,0 +1,185 @@
+"""CPU checks of the paged key/value cache: what its calls refuse, with every bound on both sides, how a batch's rows
+are dealt to blocks of 16 positions, and the tests' own plain forms."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+import aoship
+import kv_plain as P
+
+I, V = C.c_int, C.c_void_p
+ALIGNED = 1 << 12  # any aligned address: nothing is read
+
+
+def _fn(name, args):
+    f = getattr(aoship.lib(), name)
+    f.restype, f.argtypes = I, args
+    return f
+
+
+CFG = aoship._KVConfig(2, 4, 128, 64, 100, 0)
+
+
+def _batch(**kw):
+    d = dict(n_seqs=3, n_tokens=40, max_new=20, max_len=640, starts=ALIGNED, lens=ALIGNED, pages=ALIGNED, page_stride=10)
+    d.update(kw)
+    return aoship._KVBatch(**d)
+
+
+def _rows(**kw):
+    d = dict(q=ALIGNED, k=ALIGNED, v=ALIGNED, q_stride=1024, k_stride=512, v_stride=512, q_out=2 * ALIGNED,
+             q_out_stride=1024, num_heads=8)
+    d.update(kw)
+    return aoship._KVRows(**d)
+
+
+def _append(cfg=CFG, layer=0, batch=None, rows=None, rope=0):
+    f = _fn("aoship_internal_kv_append_check", [V, I, I, V, V])
+    b, r = batch or _batch(), rows or _rows()
+    return f(C.byref(cfg), rope, layer, C.byref(b), C.byref(r))
+
+
+def _read(batch=None, k=ALIGNED, ks=512, v=ALIGNED, vs=512, layer=0):
+    f = _fn("aoship_internal_kv_read_check", [V, I, V, V, C.c_int64, V, C.c_int64])
+    return f(C.byref(CFG), layer, C.byref(batch or _batch()), k, ks, v, vs)
+
+
+def _attention(batch=None, q=ALIGNED, qs=1024, nh=8, scale=0.1, window=0, out=2 * ALIGNED, os=1024, layer=1):
+    f = _fn("aoship_internal_kv_attention_check", [V, I, V, V, C.c_int64, I, C.c_float, I, V, C.c_int64])
+    return f(C.byref(CFG), layer, C.byref(batch or _batch()), q, qs, nh, scale, window, out, os)
+
+
+def test_good_calls_pass():
+    assert _append() == 0 and _read() == 0 and _attention() == 0
+    assert _append(rows=_rows(q=None, q_out=None, num_heads=0)) == 0
+    assert _append(rows=_rows(q_out=ALIGNED)) == 0  # queries rotated in place
+    assert _append(rope=640) == 0
+
+
+BAD_BATCHES = [dict(n_seqs=-1), dict(n_tokens=-1), dict(max_new=-1), dict(max_len=-1), dict(max_len=641),
+               dict(starts=None), dict(lens=None), dict(pages=None), dict(starts=ALIGNED + 2), dict(pages=ALIGNED + 1),
+               dict(page_stride=9), dict(page_stride=-1), dict(max_len=(1 << 30) + 1, page_stride=1 << 25),
+               dict(n_seqs=(1 << 24) + 1), dict(n_tokens=(1 << 28) + 1)]
+
+
+@pytest.mark.parametrize("kw", BAD_BATCHES, ids=lambda k: "-".join(k))
+def test_bad_batches_are_refused(kw):
+    for call in (_append, _read, _attention):
+        assert call(batch=_batch(**kw)) == -1
+        assert aoship.last_error().startswith("aoship_kv_")
+
+
+@pytest.mark.parametrize("kw", [dict(n_seqs=0), dict(n_tokens=0), dict(max_new=0)], ids=lambda k: "-".join(k))
+def test_empty_batches_have_nothing_to_do(kw):
+    for call in (_append, _read, _attention):
+        assert call(batch=_batch(**kw)) == 1
+    assert _attention(batch=_batch(**kw), window=-1) == -1  # (bad arguments are refused all the same)
+
+
+def test_a_batch_without_positions_needs_no_pages():
+    assert _attention(batch=_batch(max_len=0, pages=None, page_stride=0)) == 0
+
+
+@pytest.mark.parametrize("kw", [dict(k=None), dict(v=None), dict(k=ALIGNED + 8), dict(k_stride=504), dict(v_stride=516),
+                                dict(q_stride=1016), dict(q_out=None), dict(q=None), dict(num_heads=6),
+                                dict(num_heads=-4), dict(num_heads=65540), dict(q_out=ALIGNED, q_out_stride=1032),
+                                dict(q_out=ALIGNED + 2), dict(q_bias=ALIGNED + 4), dict(k_stride=1 << 40),
+                                dict(v_bias=ALIGNED + 8)], ids=lambda k: "-".join(k))
+def test_bad_rows_are_refused(kw):
+    assert _append(rows=_rows(**kw)) == -1
+    assert aoship.last_error().startswith("aoship_kv_append")
+
+
+def test_other_refusals():
+    assert _append(layer=2) == -1 and _append(layer=-1) == -1 and _read(layer=2) == -1 and _attention(layer=2) == -1
+    assert _append(rope=639) == -1 and "rotary" in aoship.last_error()
+    assert _read(k=None) == -1 and _read(vs=500) == -1 and _read(v=ALIGNED + 4) == -1
+    assert _attention(nh=6) == -1 and _attention(nh=0) == -1 and _attention(window=-1) == -1
+    assert _attention(scale=float("nan")) == -1 and _attention(scale=float("inf")) == -1
+    assert _attention(out=ALIGNED) == -1 and _attention(out=None) == -1 and _attention(os=1020) == -1
+
+
+def test_shapes_that_a_cache_refuses():
+    for bad in (dict(num_layers=0), dict(num_kv_heads=0), dict(num_kv_heads=4097), dict(head_dim=0), dict(head_dim=12),
+                dict(head_dim=264), dict(page_size=32), dict(page_size=96), dict(page_size=512), dict(num_pages=0),
+                dict(format=3), dict(format=-1), dict(num_pages=2 ** 31 - 1, num_layers=1000)):
+        c = aoship._KVConfig(2, 4, 128, 64, 100, 0)
+        for n, v in bad.items():
+            setattr(c, n, v)
+        assert not aoship.lib().aoship_kv_cache_new(C.byref(c)), bad
+        assert aoship.last_error().startswith("aoship_kv_cache_new"), bad
+    assert not aoship.lib().aoship_kv_cache_new(None)
+    L = aoship.lib()
+    for call in (lambda: L.aoship_kv_append(None, 0, None, None), lambda: L.aoship_kv_read(None, 0, None, None, 0, None, 0),
+                 lambda: L.aoship_kv_attention(None, 0, None, None, 0, 1, 1.0, 0, None, 0),
+                 lambda: L.aoship_kv_cache_set_rope(None, None, None, 0), lambda: L.aoship_kv_cache_set_stream(None, None),
+                 lambda: L.aoship_kv_cache_faults(None)):
+        assert call() == -1 and "null cache" in aoship.last_error()
+    L.aoship_kv_cache_free(None)
+    with pytest.raises(aoship.AosError):
+        aoship.KVCache(1, 1, 64, 64, 1, "int8")
+
+
+@pytest.mark.parametrize("seed", range(40))
+def test_blocks_cover_every_row_once(seed):
+    """Random batches (single rows, empty sequences, padding in front, rows past the last sequence): the blocks of the
+    grid, found as the launch finds them, hold every row that has a position exactly once, aligned and in their page."""
+    rng = np.random.default_rng(seed)
+    n = int(rng.integers(1, 150))
+    top = int(rng.choice([1, 2, 17, 70]))
+    new = rng.integers(0, top + 1, n)
+    past = rng.integers(0, 300, n) * rng.integers(0, 2, n)
+    lens = np.maximum(0, past + new - (rng.random(n) < 0.1) * rng.integers(0, 40, n))
+    starts = np.concatenate([[0], np.cumsum(new)])
+    T, most = int(starts[-1] + rng.integers(0, 30)), max(1, int(new.max()))
+    blocks = _fn("aoship_internal_kv_blocks", [I, I, I])(most, n, T)
+    f = _fn("aoship_internal_kv_block", [I, I, I, I, I, I, V, V])
+    base, out = C.c_int(), (C.c_int * 4)()
+    found = np.zeros(T, int)
+    bases = []
+    for s in range(n):
+        f(most, s, int(starts[s]), int(new[s]), int(lens[s]), 0, C.byref(base), out)
+        bases.append(base.value)
+    for x in range(blocks):
+        s = int(np.searchsorted(bases, x, side="right")) - 1
+        if s < 0 or not f(most, s, int(starts[s]), int(new[s]), int(lens[s]), x, C.byref(base), out):
+            continue
+        pos, lo, hi, row = out
+        first = int(lens[s] - new[s])
+        assert pos % 16 == 0 and 0 <= lo < hi <= 16 and pos + hi <= lens[s]
+        assert row - starts[s] == pos + lo - first and 0 <= row - starts[s] and row + hi - lo <= starts[s + 1]
+        found[row:row + hi - lo] += 1
+    want = np.zeros(T, int)
+    for s in range(n):
+        skip = max(0, int(new[s] - lens[s]))
+        want[starts[s] + min(skip, new[s]):starts[s + 1]] = 1
+    assert (found == want).all()
+
+
+def test_plain_quantiser():
+    """The plain form against a search over every code and scale."""
+    rng = np.random.default_rng(3)
+    for fmt, top, codes in (("mxfp4", 6.0, [0, .5, 1, 1.5, 2, 3, 4, 6]),
+                            ("mxfp8", 448.0, [m / 8 * 2.0 ** -6 for m in range(8)] +
+                             [(1 + m / 8) * 2.0 ** e for e in range(-6, 9) for m in range(8)][:-1])):
+        codes = np.array(codes)
+        x = P.bf16(rng.standard_normal((50, 40)) * 2.0 ** rng.integers(-20, 20, (50, 1)))
+        x[0] = 0
+        x[1, 3], x[2, 35] = np.inf, np.nan
+        x[3, :3] = P.bf16(np.array([top, top / 2, 2 * top]))
+        got = P.quantised(x, fmt)
+        for r in range(50):
+            for b in (0, 32):
+                blk = x[r, b:b + 32]
+                if not np.isfinite(blk).all():
+                    assert np.isnan(got[r, b:b + 32]).all()
+                    continue
+                e = next(e for e in range(-126, 130) if np.abs(blk).max() <= top * 2.0 ** e)
+                e = max(e, -117 if fmt == "mxfp8" else -125)
+                for i, v in enumerate(blk):
+                    d = np.abs(codes * 2.0 ** e - abs(v))
+                    near = np.flatnonzero(d == d.min())
+                    best = near[0] if len(near) == 1 else near[near % 2 == 0][0]  # ties to the even code
+                    assert abs(got[r, b + i]) == codes[best] * 2.0 ** e
+                    assert got[r, b + i] == 0 or np.sign(got[r, b + i]) == np.sign(v)
