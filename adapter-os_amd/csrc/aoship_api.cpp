@@ -3454,7 +3454,8 @@ struct aoship_kv_cache {
   aoship_kv_config_t cfg;
   int device = 0, hdp = 0, page_shift = 0;
   size_t layer_bytes = 0;
-  DevBuf pool, part, counters, faults, rope;
+  DevBuf pool, part, counters, rope;
+  DevBuf faults; /* two words: faults, and whether an infinity or a NaN has entered the values */
   int rope_positions = 0;
   hipStream_t stream = nullptr;
 };
@@ -3491,7 +3492,7 @@ extern "C" aoship_kv_cache_t *aoship_kv_cache_new(const aoship_kv_config_t *c) {
   m->layer_bytes = tiles * tile * (size_t)c->num_pages;
   if (m->pool.alloc(m->layer_bytes * (size_t)c->num_layers, true) ||
       m->part.alloc(aos_kv_part_floats(hdp) * sizeof(float), false) ||
-      m->counters.alloc(AOS_KV_MAX_WGS * sizeof(uint32_t), true) || m->faults.alloc(sizeof(uint32_t), true)) {
+      m->counters.alloc(AOS_KV_MAX_WGS * sizeof(uint32_t), true) || m->faults.alloc(2 * sizeof(uint32_t), true)) {
     delete m;
     return nullptr;
   }
@@ -3578,6 +3579,7 @@ static void kv_batch(const aoship_kv_cache *m, int layer, const aoship_kv_batch_
   o->max_len = b->max_len;
   o->stride = b->page_stride;
   o->faults = m->faults.as<uint32_t>();
+  o->nonfinite = o->faults + 1;
 }
 
 /* rows of `width` elements, 16 bytes at a time */

@@ -676,7 +676,8 @@ typedef struct {
   int format, hd, hdp, nkv, page_shift /* log2 of a page's positions */, num_pages;
   const int32_t *starts, *lens, *pages; /* [n_seqs + 1], [n_seqs], [n_seqs][stride] */
   int n_seqs, n_tokens, max_new, max_len, stride;
-  uint32_t *faults; /* AOS_KV_FAULT_* bits, or-ed in */
+  uint32_t *faults;    /* AOS_KV_FAULT_* bits, or-ed in */
+  uint32_t *nonfinite; /* set once an infinity or a NaN has entered the cache's values */
 } aos_kv_batch;
 
 typedef struct {

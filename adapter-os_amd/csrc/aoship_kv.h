@@ -55,6 +55,11 @@ constexpr int vs_off() {
   return ks_off<FMT, HDP>() + scale_bytes<FMT, HDP>();
 }
 
+/* whether a word of two bfloat16 holds an infinity or a NaN */
+__device__ __forceinline__ bool odd2(uint32_t w) {
+  return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
+}
+
 /* byte of a position's key scale within its block's 64 */
 __device__ __forceinline__ int ks_index(int pos) { return (pos & 48) | ((pos & 3) << 2) | ((pos >> 2) & 3); }
 

@@ -159,6 +159,7 @@ __global__ void __launch_bounds__(256) aos_kv_append_kernel(aos_kv_append_params
                  ((uint32_t)aos_f32_to_bf16(aos_bf16_to_f32((uint16_t)(x[i] >> 16)) + bias[2 * i + 1]) << 16);
       }
     }
+    if (FMT == AOS_KV_BF16 && (odd2(x[0]) || odd2(x[1]) || odd2(x[2]) || odd2(x[3]))) *p.b.nonfinite = 1u;
     *(u32x4 *)(vs + t * LD + d) = x;
     if (d >= hd || t < o.lo || t >= o.hi) *(u32x4 *)(ks + t * LD + d) = u32x4{};
   }
@@ -195,6 +196,7 @@ __global__ void __launch_bounds__(256) aos_kv_append_kernel(aos_kv_append_params
       const uint32_t byte = scale_byte<FMT>(block_top(x));
       if (is_v) {
         vsc[blk][t] = byte;
+        if (byte == 255u) *p.b.nonfinite = 1u;
         if (fresh) tile[vs_off<FMT, HDP>() + blk * TILE + tp + t] = (unsigned char)byte;
         continue;
       }

@@ -18,6 +18,7 @@ using namespace kv;
 namespace {
 
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int SC1 = 16; /* buffer cache policy: device-coherent (sc1) */
 constexpr float LOG2E = 1.44269504f;
@@ -76,10 +77,12 @@ __device__ __forceinline__ float byte_scale(uint32_t w, int j) {
   return __builtin_bit_cast(float, (j == 3 ? w >> 1 : j == 2 ? w << 7 : j == 1 ? w << 15 : w << 23) & 0x7f800000u);
 }
 
-/* whether a word of two bfloat16 holds an infinity or a NaN */
-__device__ __forceinline__ bool odd2(uint32_t w) {
-  return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
-}
+/* Infinities and NaNs among the values. In a tile that a row sees only in part, the product of such a value with a
+ * probability of zero would reach rows that do not see it. Once one has entered the cache (a word that append sets), the
+ * kernels look for them in such tiles: the matrix product gets zeros in their place, another one counts for each row and
+ * dimension those that the row sees, by class, and the output takes them at the end (OddMarks). Quantised values need
+ * this only where they pass through LDS as bfloat16: else a block's not-a-number scale is met by a probability that is
+ * set to zero after scaling. */
 /* The word with infinities and NaNs as zeros (cls < 0), or 1.0 where it holds +infinity (cls 0), -infinity (1) or a
  * NaN (2) and zeros elsewhere. */
 __device__ __forceinline__ uint32_t odd_part(uint32_t w, int cls) {
@@ -94,24 +97,45 @@ __device__ __forceinline__ uint32_t odd_part(uint32_t w, int cls) {
   }
   return r;
 }
-__device__ __forceinline__ float odd_value(int cls) {
-  return cls == 0 ? __builtin_inff() : cls == 1 ? -__builtin_inff() : __builtin_nanf("");
+__device__ __forceinline__ u32x4 odd_part(u32x4 w, int cls) {
+  return u32x4{odd_part(w[0], cls), odd_part(w[1], cls), odd_part(w[2], cls), odd_part(w[3], cls)};
 }
+/* N accumulator elements' marks, a bit each for +infinity, -infinity and NaN seen */
+template <int N>
+struct OddMarks {
+  uint32_t bit[3][(N + 31) / 32];
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int c = 0; c < 3; ++c)
+#pragma unroll
+      for (int i = 0; i < (N + 31) / 32; ++i) bit[c][i] = 0u;
+  }
+  __device__ __forceinline__ float apply(int i, float x) const {
+    if (bit[0][i / 32] >> (i % 32) & 1) x = x + __builtin_inff();
+    if (bit[1][i / 32] >> (i % 32) & 1) x = x - __builtin_inff();
+    if (bit[2][i / 32] >> (i % 32) & 1) x = x + __builtin_nanf("");
+    return x;
+  }
+};
+/* weight of a piece whose maximum is m in a sum whose maximum is ms: kept off zero, which an infinity would turn into
+ * a NaN */
+__device__ __forceinline__ float piece_weight(float m, float ms) { return fmaxf(ex2(m - ms), 1.17549435e-38f); }
 
 /* ---- sharing the work ------------------------------------------------------------------------ */
 
 /* What of a sequence the attention walks: rows (token, head) in row tiles of R, each over nt tiles from tile t0 on.
- * A sequence with rows but no positions has one tile, in which nothing is visible. */
+ * A sequence with rows but no positions has one tile, in which nothing is visible; one of more than `few` rows is the
+ * other kernel's. */
 struct Work {
   Seq q;
   int rows, rts, t0, nt;
 };
 template <int R>
-__device__ __forceinline__ Work work_of(const aos_kv_attn_params &p, const Seq &q) {
+__device__ __forceinline__ Work work_of(const aos_kv_attn_params &p, int few, const Seq &q) {
   Work w;
   w.q = q;
   w.rows = q.count * (p.nh / p.b.nkv);
-  w.rts = (w.rows + R - 1) / R;
+  w.rts = w.rows > few ? 0 : (w.rows + R - 1) / R;
   const int first = q.len - q.count - p.window + 1; /* first position that the first row sees */
   w.t0 = p.window > 0 && first > 0 ? first / TILE : 0;
   w.nt = (q.len + TILE - 1) / TILE - w.t0;
@@ -213,7 +237,7 @@ constexpr int part_floats() { /* of a piece: maxima and sums [NB][2][16], then t
 constexpr int rows_waves(int fmt, int hdp) { return hdp == 256 || (fmt == AOS_KV_BF16 && hdp == 128) ? 1 : 2; }
 
 template <int FMT, int HDP, int NB>
-__global__ void __launch_bounds__(256, rows_waves(FMT, HDP)) aos_kv_rows_kernel(aos_kv_attn_params p, int min_share) {
+__global__ void __launch_bounds__(256, rows_waves(FMT, HDP)) aos_kv_rows_kernel(aos_kv_attn_params p, int few, int min_share) {
   constexpr int R = 16 * NB, DB = HDP / 16, KS = HDP / 32, W8 = bits<FMT>() / 4; /* W8: words of 8 codes */
   __shared__ float red[2][NB * DB * 4][64];
   __shared__ float mls[4][2][NB][64];
@@ -226,7 +250,7 @@ __global__ void __launch_bounds__(256, rows_waves(FMT, HDP)) aos_kv_rows_kernel(
   /* all units, this workgroup's share [u0, u1) of them, and the sequence that u0 falls in */
   auto units = [&](int s) {
     if (s >= p.b.n_seqs) return 0;
-    const Work x = work_of<R>(p, seq_at(p.b, s));
+    const Work x = work_of<R>(p, few, seq_at(p.b, s));
     return p.b.nkv * x.rts * x.nt;
   };
   int total = 0;
@@ -251,9 +275,10 @@ __global__ void __launch_bounds__(256, rows_waves(FMT, HDP)) aos_kv_rows_kernel(
   }
 
   const float cs = p.scale * LOG2E;
+  const bool marking = FMT == AOS_KV_BF16 && *p.b.nonfinite != 0;
   while (u < u1) {
-    Work x = work_of<R>(p, seq_at(p.b, s));
-    while (x.rts == 0 && s + 1 < p.b.n_seqs) x = work_of<R>(p, seq_at(p.b, ++s));
+    Work x = work_of<R>(p, few, seq_at(p.b, s));
+    while (x.rts == 0 && s + 1 < p.b.n_seqs) x = work_of<R>(p, few, seq_at(p.b, ++s));
     if (x.rts == 0) return; /* (never: u < total, so a later sequence has units) */
     const int seg = (u - base) / x.nt, j = u - base - seg * x.nt; /* which (head, row tile), and its tile */
     const int h = seg / x.rts, rt = seg - h * x.rts;
@@ -292,6 +317,9 @@ __global__ void __launch_bounds__(256, rows_waves(FMT, HDP)) aos_kv_rows_kernel(
 #pragma unroll
       for (int d = 0; d < DB; ++d) o[b][d] = f32x4{};
     }
+
+    OddMarks<NB * DB * 4> marks;
+    if constexpr (FMT == AOS_KV_BF16) marks.clear();
 
     const int mine = (n - wave + 3) / 4; /* tiles of this wave: j + wave, j + wave + 4, ... */
     for (int i0 = 0; i0 < mine; i0 += 64) {
@@ -381,17 +409,42 @@ __global__ void __launch_bounds__(256, rows_waves(FMT, HDP)) aos_kv_rows_kernel(
                                pack_bf16(sc[b][2 * t + 1][2], sc[b][2 * t + 1][3])};
           }
         }
-        bool odd = false;
         if constexpr (FMT == AOS_KV_BF16) {
-          if (edge) {
+          if (marking && edge) { /* uniform */
 #pragma unroll
-            for (int d = 0; d < DB; ++d)
+            for (int d = 0; d < DB; ++d) {
+              uint32_t any = 0;
 #pragma unroll
-              for (int k = 0; k < Tile<FMT, HDP>::VW; ++k) odd = odd || odd2(tl.v[d][k]);
-            odd = __ballot(odd) != 0;
+              for (int k = 0; k < 8; ++k) any |= odd2(tl.v[d][k]) ? 1u : 0u;
+              if (__ballot(any != 0) == 0) continue;
+#pragma unroll
+              for (int cls = 0; cls < 3; ++cls)
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                  f32x4 c = {};
+#pragma unroll
+                  for (int t = 0; t < 2; ++t) {
+                    u32x4 a, sf;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                      a[k] = odd_part(tl.v[d][4 * t + k], cls);
+                      sf[k] = (seen[b] >> (8 * t + 2 * k) & 1 ? 0x3f80u : 0u) |
+                              (seen[b] >> (8 * t + 2 * k + 1) & 1 ? 0x3f800000u : 0u);
+                    }
+                    c = mfma16(a, sf, c);
+                  }
+#pragma unroll
+                  for (int k = 0; k < 4; ++k) {
+                    const int e = (b * DB + d) * 4 + k;
+                    marks.bit[cls][e / 32] |= c[k] > 0.0f ? 1u << (e % 32) : 0u;
+                  }
+                }
+#pragma unroll
+              for (int k = 0; k < 8; ++k) tl.v[d][k] = odd_part(tl.v[d][k], -1);
+            }
           }
         }
-        if (!odd) {
+        {
 #pragma unroll
           for (int d = 0; d < DB; ++d) {
             if constexpr (FMT != AOS_KV_BF16) {
@@ -419,44 +472,18 @@ __global__ void __launch_bounds__(256, rows_waves(FMT, HDP)) aos_kv_rows_kernel(
               for (int b = 0; b < NB; ++b) o[b][d] = mfma16(a, pf[b][t], o[b][d]);
             }
           }
-        } else if constexpr (FMT == AOS_KV_BF16) {
-          /* An infinity or a NaN among the values of a tile that some row sees only in part: its product with a
-           * probability of zero would reach rows that do not see it. The finite values go through the product; of
-           * the others, each row counts those that it sees. */
-          u32x4 sf[NB][2];
-#pragma unroll
-          for (int b = 0; b < NB; ++b)
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-              for (int k = 0; k < 4; ++k)
-                sf[b][t][k] = (seen[b] >> (8 * t + 2 * k) & 1 ? 0x3f80u : 0u) |
-                              (seen[b] >> (8 * t + 2 * k + 1) & 1 ? 0x3f800000u : 0u);
-#pragma unroll
-          for (int d = 0; d < DB; ++d)
-#pragma unroll 1
-            for (int cls = -1; cls < 3; ++cls) {
-              f32x4 c[NB];
-#pragma unroll
-              for (int b = 0; b < NB; ++b) c[b] = cls < 0 ? o[b][d] : f32x4{};
-#pragma unroll
-              for (int t = 0; t < 2; ++t) {
-                u32x4 a;
-#pragma unroll
-                for (int k = 0; k < 4; ++k) a[k] = odd_part(tl.v[d][4 * t + k], cls);
-#pragma unroll
-                for (int b = 0; b < NB; ++b) c[b] = mfma16(a, cls < 0 ? pf[b][t] : sf[b][t], c[b]);
-              }
-#pragma unroll
-              for (int b = 0; b < NB; ++b)
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                  o[b][d][k] = cls < 0 ? c[b][k] : c[b][k] > 0.0f ? o[b][d][k] + odd_value(cls) : o[b][d][k];
-            }
         }
         if (i + 1 < cnt) tl.load_v(next, lane);
       }
     }
+
+    if (marking)
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) o[b][d][k] = marks.apply((b * DB + d) * 4 + k, o[b][d][k]);
 
     /* the waves' pieces: one maximum, then their sums two by two */
     const bool many = n > 1;
@@ -477,8 +504,8 @@ __global__ void __launch_bounds__(256, rows_waves(FMT, HDP)) aos_kv_rows_kernel(
         const float ms = safe_max(top);
         float sum = 0.0f;
 #pragma unroll
-        for (int v = 0; v < 4; ++v) sum = sum + mls[v][1][b][lane] * ex2(mls[v][0][b][lane] - ms);
-        const float f = ex2(m[b] - ms);
+        for (int v = 0; v < 4; ++v) sum = sum + mls[v][1][b][lane] * piece_weight(mls[v][0][b][lane], ms);
+        const float f = piece_weight(m[b], ms);
 #pragma unroll
         for (int d = 0; d < DB; ++d)
 #pragma unroll
@@ -559,14 +586,14 @@ __global__ void __launch_bounds__(256, rows_waves(FMT, HDP)) aos_kv_rows_kernel(
           const float ms = safe_max(top);
           float sum = 0.0f;
           for (int k = quad; k < np; k += 4)
-            sum = sum + aos_collect(p.part + slot(k) + 32 * b + 16 + col) * ex2(aos_collect(p.part + slot(k) + 32 * b + col) - ms);
+            sum = sum + aos_collect(p.part + slot(k) + 32 * b + 16 + col) * piece_weight(aos_collect(p.part + slot(k) + 32 * b + col), ms);
           sum = quad_sum(sum);
           if (16 * b + col < nrows)
             for (int d = wave; d < DB; d += 4) {
               f32x4 acc = {};
 #pragma unroll 4
               for (int k = 0; k < np; ++k) {
-                const float f = ex2(aos_collect(p.part + slot(k) + 32 * b + col) - ms);
+                const float f = piece_weight(aos_collect(p.part + slot(k) + 32 * b + col), ms);
                 const f32x4 y = __builtin_bit_cast(
                     f32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, (slot(k) + 32 * NB + ((b * DB + d) * 64 + lane) * 4) * 4, 0, SC1));
                 acc = acc + y * f;
@@ -585,17 +612,512 @@ __global__ void __launch_bounds__(256, rows_waves(FMT, HDP)) aos_kv_rows_kernel(
   }
 }
 
-constexpr int ROWS_WGS = 512;
+/* ---- many rows: tiles of 128, keys and values through LDS ------------------------------------- */
+
+/* Four waves of 32 rows walk a row tile's positions 64 at a time. A tile of the cache goes to LDS once for all of
+ * them, as bfloat16 in the cache's own order (a bfloat16 tile as it lies, straight from memory; quantised ones
+ * through registers), while the one before it is worked on: two stages, 64 KB for 128 dimensions, two workgroups a
+ * CU, so that one's exponentials run under the other's matrix instructions.
+ *
+ * S^T = K . Q^T and O^T = V^T . P^T by v_mfma_f32_32x32x16_bf16. Row 16 s + 8 a + 4 c + i of a block of 32 keys is
+ * position 16 c + 8 s + 4 a + i, which puts the 16 consecutive positions 16 c ..+15 on half c of the lanes, register
+ * by register: what the value pieces hold, so the probabilities never cross lanes here either.
+ *
+ * The running maximum of a row follows its scores only once they pass it by 2^8 (probabilities up to 256, exact
+ * powers of two apart from what the true maximum would give): the accumulators are hardly ever rescaled.
+ *
+ * The workgroups share all (key/value head, row tile, position tile) evenly; where a row tile is cut, its pieces meet
+ * as in the kernel above. Neighbouring shares, which read the same keys, go to one XCD. */
+constexpr int TR = 128;         /* rows of a row tile */
+constexpr float SLACK = 8.0f;   /* log2 */
+constexpr int tiles_per_cu(int hdp) { return hdp == 256 ? 1 : 2; }
+
+template <int HDP>
+constexpr int tile_part_floats() { /* of a piece: maxima and sums [4 waves][2][32], then the accumulators */
+  return 4 * 64 + TR * HDP;
+}
+
+__device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ float half_max(float x) { /* with the lane 32 away */
+  const uint32_t u = __builtin_bit_cast(uint32_t, x);
+  const auto a = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return fmaxf(__builtin_bit_cast(float, (uint32_t)a[0]), __builtin_bit_cast(float, (uint32_t)a[1]));
+}
+__device__ __forceinline__ float half_sum(float x) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, x);
+  const auto a = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return __builtin_bit_cast(float, (uint32_t)a[0]) + __builtin_bit_cast(float, (uint32_t)a[1]);
+}
+
+/* Eight codes of one dimension, each position with its own scale byte (of words s0, s1), as bfloat16. */
+template <int FMT>
+__device__ __forceinline__ u32x4 decode8_scaled(const uint32_t *w, uint32_t s0, uint32_t s1) {
+  float x[8];
+  if constexpr (FMT == AOS_KV_MXFP8) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const f32x2 a = __builtin_bit_cast(f32x2, __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w[i], 1.0f, false));
+      const f32x2 b = __builtin_bit_cast(f32x2, __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w[i], 1.0f, true));
+      x[4 * i] = a[0];
+      x[4 * i + 1] = a[1];
+      x[4 * i + 2] = b[0];
+      x[4 * i + 3] = b[1];
+    }
+  } else {
+    const f32x2 a = __builtin_bit_cast(f32x2, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[0], 1.0f, 0));
+    const f32x2 b = __builtin_bit_cast(f32x2, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[0], 1.0f, 1));
+    const f32x2 c = __builtin_bit_cast(f32x2, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[0], 1.0f, 2));
+    const f32x2 d = __builtin_bit_cast(f32x2, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[0], 1.0f, 3));
+    x[0] = a[0], x[1] = a[1], x[2] = b[0], x[3] = b[1], x[4] = c[0], x[5] = c[1], x[6] = d[0], x[7] = d[1];
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = x[i] * byte_scale(i < 4 ? s0 : s1, i & 3);
+  return u32x4{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7])};
+}
+
+/* A tile on its way to LDS (keys at `dst`, values TILE * HDP * 2 bytes after them). fetch() starts it, put() (of the
+ * quantised formats) writes what fetch() loaded; the caller waits and synchronises. */
+template <int FMT, int HDP>
+struct Stage {
+  static constexpr int KU = HDP * bits<FMT>() / 128 * TILE / 256; /* key units of a thread */
+  static constexpr int VU = 4 * HDP / 256;                        /* value units of a thread */
+  static constexpr int VW = bits<FMT>() / 2;
+  static constexpr bool Q = FMT != AOS_KV_BF16;
+  u32x4 k[Q ? (KU ? KU : 1) : 1];
+  uint32_t v[Q ? VU : 1][Q ? VW : 1];
+  u32x4 vs[Q ? VU : 1];
+  uint32_t ks[Q ? (KU ? KU : 1) : 1];
+
+  __device__ __forceinline__ void fetch(const unsigned char *t, unsigned char *dst, int tid) {
+    if constexpr (!Q) {
+      const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+      constexpr int N = 4 * TILE * HDP / 1024 / 4;
+      const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void *)t, (short)0, 4 * TILE * HDP, 0x00020000);
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(
+            rs, (__attribute__((address_space(3))) void *)(dst + (4 * i + wave) * 1024), 16, lane * 16, (4 * i + wave) * 1024, 0, 0);
+    } else {
+#pragma unroll
+      for (int i = 0; i < (KU ? KU : 1); ++i) {
+        const int c = tid + 256 * i, pos = c & 63, u = c >> 6;
+        if (KU == 0 && u >= HDP * bits<FMT>() / 128) break;
+        k[i] = aos_gld16(t + (u * TILE + pos) * 16);
+        ks[i] = *(const __attribute__((address_space(1))) unsigned char *)(t + ks_off<FMT, HDP>() +
+                                                                          (u * (128 / bits<FMT>()) / 32) * TILE + ks_index(pos));
+      }
+#pragma unroll
+      for (int i = 0; i < VU; ++i) {
+        const int c = tid + 256 * i, d = c % HDP, u = c / HDP;
+        const unsigned char *g = t + v_off<FMT, HDP>() + c * (4 * VW);
+        if constexpr (FMT == AOS_KV_MXFP8) {
+          const u32x4 w = aos_gld16(g);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[i][j % VW] = w[j];
+        } else {
+          const u32x2 w = *(const __attribute__((address_space(1))) u32x2 *)g;
+          v[i][0] = w.x;
+          v[i][1] = w.y;
+        }
+        vs[i] = aos_gld16(t + vs_off<FMT, HDP>() + (d >> 5) * TILE + 16 * u);
+      }
+    }
+  }
+  __device__ __forceinline__ void put(unsigned char *dst, int tid) {
+    if constexpr (Q) {
+#pragma unroll
+      for (int i = 0; i < (KU ? KU : 1); ++i) {
+        const int c = tid + 256 * i, pos = c & 63, u = c >> 6;
+        if (KU == 0 && u >= HDP * bits<FMT>() / 128) break;
+        constexpr int PER = 16 / bits<FMT>(); /* 16-byte bfloat16 units of a unit of codes */
+        uint32_t w[4] = {k[i][0], k[i][1], k[i][2], k[i][3]};
+#pragma unroll
+        for (int j = 0; j < PER; ++j)
+          *(u32x4 *)(dst + ((u * PER + j) * TILE + pos) * 16) = decode8<FMT>(&w[j * (4 / PER)], byte_scale(ks[i], 0));
+      }
+#pragma unroll
+      for (int i = 0; i < VU; ++i) {
+        const int c = tid + 256 * i, d = c % HDP, u = c / HDP;
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          *(u32x4 *)(dst + TILE * HDP * 2 + ((2 * u + j) * HDP + d) * 16) =
+              decode8_scaled<FMT>(&v[i][j * VW / 2], vs[i][2 * j], vs[i][2 * j + 1]);
+      }
+    }
+  }
+};
+
+/* Row tile slots of a batch: sequence s has its row tiles from slot_base(s) on, fewer than the next one's base. */
+__device__ __forceinline__ int slot_base(int start, int g, int s) { return (int)((long long)start * g / TR) + s; }
+
+/* A row tile: rows r0 .. r0 + rows - 1 of its sequence and the position tiles t0 .. t0 + nt - 1 that they see (at least
+ * one). nt 0: no such row tile, or one of a sequence of few rows. */
+struct RowTile {
+  Seq q;
+  int s, r0, rows, t0, nt;
+};
+__device__ __forceinline__ RowTile row_tile(const aos_kv_attn_params &p, int few, int slot) {
+  const int g = p.nh / p.b.nkv;
+  RowTile o = {};
+  int lo = 0, hi = p.b.n_seqs; /* the last sequence whose slots begin at or before `slot` */
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (slot_base(p.b.starts[mid], g, mid) <= slot) lo = mid; else hi = mid;
+  }
+  o.s = lo;
+  o.q = seq_at(p.b, lo);
+  const int all = o.q.count * g, r = slot - slot_base(o.q.row0, g, lo);
+  o.r0 = r * TR;
+  if (all <= few || r < 0 || o.r0 >= all) return o;
+  o.rows = all - o.r0 < TR ? all - o.r0 : TR;
+  const int p0 = o.q.len - o.q.count;
+  const int first = p0 + o.r0 / g, last = p0 + (o.r0 + o.rows - 1) / g;
+  const int low = p.window > 0 && first - p.window + 1 > 0 ? first - p.window + 1 : 0;
+  o.t0 = low / TILE;
+  o.nt = (last < 0 ? 0 : last / TILE) - o.t0 + 1;
+  return o;
+}
 
 template <int FMT, int HDP>
-int rows(const aos_kv_attn_params *p, const aos_launch_ctx *ctx) {
-  AOS_LAUNCH(ctx, (aos_kv_rows_kernel<FMT, HDP, 1>), dim3(ROWS_WGS), dim3(256), 0, *p, 8);
+__global__ void __launch_bounds__(256, tiles_per_cu(HDP)) aos_kv_tiles_kernel(aos_kv_attn_params p, int few, int slots,
+                                                                             int min_share) {
+  constexpr int KS = HDP / 16, DB = HDP / 32, STAGE = 4 * TILE * HDP;
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  __shared__ int scan[4], found[2];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 31, half = lane >> 5;
+  const int g = p.nh / p.b.nkv;
+  const int G = gridDim.x, w = (int)(blockIdx.x % 8) * (G / 8) + (int)(blockIdx.x / 8);
+
+  /* units of a key/value head (each thread a run of slots), this workgroup's share, and where it begins */
+  const int per = (slots + 255) / 256, first = tid * per, end = first + per < slots ? first + per : slots;
+  int sum = 0;
+  for (int x = first; x < end; ++x) sum += row_tile(p, few, x).nt;
+  const int upto = wave_scan(sum, lane);
+  if (lane == 63) scan[wave] = upto;
+  __syncthreads();
+  int before = upto - sum, N = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (i < wave) before += scan[i];
+    N += scan[i];
+  }
+  const int total = N * p.b.nkv;
+  int share = (total + G - 1) / G;
+  if (share < min_share) share = min_share;
+  int u = w * share;
+  if (u >= total) return; /* uniform */
+  const int u1 = u + share < total ? u + share : total;
+  int h = u / N;
+  {
+    int v = u - h * N - before;
+    if (v >= 0 && v < sum)
+      for (int x = first; x < end; ++x) {
+        const int nt = row_tile(p, few, x).nt;
+        if (v < nt) {
+          found[0] = x;
+          found[1] = v;
+          break;
+        }
+        v -= nt;
+      }
+  }
+  __syncthreads();
+  int slot = __builtin_amdgcn_readfirstlane(found[0]), j = __builtin_amdgcn_readfirstlane(found[1]);
+
+  /* (a scale of zero stays above it, so that what a row does not see keeps -infinity) */
+  const float cs = fmaxf(fabsf(p.scale) * LOG2E, 1.17549435e-38f);
+  const uint32_t flip = p.scale < 0.0f ? 0x80008000u : 0u; /* a negative scale: negated queries */
+  const bool marking = *p.b.nonfinite != 0;
+  while (u < u1) {
+    RowTile x = row_tile(p, few, slot);
+    if (x.nt == 0) { /* (the next slot, or the next head's first) */
+      if (++slot >= slots) {
+        slot = 0;
+        if (++h >= p.b.nkv) return; /* (never: u < total) */
+      }
+      continue;
+    }
+    const int n = x.nt - j < u1 - u ? x.nt - j : u1 - u;
+    const int p0 = x.q.len - x.q.count;
+    const int s = __builtin_amdgcn_readfirstlane(x.s);
+
+    /* this lane's row, and the wave's rows' positions: first and last, and what they all see */
+    const int wr = 32 * wave, nrows = x.rows - wr;
+    const int rr = wr + col < x.rows ? wr + col : x.rows - 1, row = x.r0 + rr;
+    const int t = row / g, hh = h * g + row - t * g;
+    const int hi = p0 + t, lo = p.window > 0 && hi - p.window + 1 > 0 ? hi - p.window + 1 : 0;
+    const int wfirst = x.r0 + (wr < x.rows ? wr : x.rows - 1), wlast = x.r0 + (wr + 31 < x.rows ? wr + 31 : x.rows - 1);
+    const int hi_min = p0 + wfirst / g, hi_max = p0 + wlast / g;
+    const int lo_min = p.window > 0 && hi_min - p.window + 1 > 0 ? hi_min - p.window + 1 : 0;
+    const int lo_max = p.window > 0 && hi_max - p.window + 1 > 0 ? hi_max - p.window + 1 : 0;
+
+    const int last_at = p0 + (x.r0 + x.rows - 1) / g; /* what every row of the tile sees: from wg_lo to wg_hi */
+    const int wg_hi = p0 + x.r0 / g;
+    const int wg_lo = p.window > 0 && last_at - p.window + 1 > 0 ? last_at - p.window + 1 : 0;
+
+    u32x4 qf[KS];
+    {
+      const uint16_t *qr = p.q + (long long)(x.q.row0 + t) * p.q_ld + hh * p.b.hd;
+#pragma unroll
+      for (int e = 0; e < KS; ++e) {
+        const int d = half * (HDP / 2) + 8 * e;
+        qf[e] = d < p.b.hd ? aos_gld16(qr + d) : u32x4{};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) qf[e][i] ^= flip;
+      }
+    }
+    f32x16 o[DB];
+#pragma unroll
+    for (int d = 0; d < DB; ++d) o[d] = f32x16{};
+    float m = NINF, l = 0.0f; /* l: this lane's half of the row's sum */
+
+    OddMarks<DB * 16> marks;
+    marks.clear();
+    /* values: step k takes the 8 positions 32 (k / 2) + 16 half + 8 (k % 2) ..+7 */
+    auto va = [&](const unsigned char *vt, int k, int d) {
+      return *(const u32x4 *)(vt + ((4 * (k >> 1) + 2 * half + (k & 1)) * HDP + 32 * d + col) * 16);
+    };
+    const int tile0 = x.t0 + j;
+    int pages = -1; /* of the 64 tiles from i & ~63 on, one a lane */
+    auto page = [&](int i) { /* of tile i, for i in order; -1 where it cannot be read */
+      if ((i & 63) == 0) {
+        const int pos = (tile0 + i + lane) * TILE;
+        pages = i + lane < n && pos < x.q.len ? page_of(p.b, s, pos) : -1;
+      }
+      return __builtin_amdgcn_readlane(pages, i & 63);
+    };
+    Stage<FMT, HDP> st;
+    int pg = page(0);
+    st.fetch(tile_ptr<FMT, HDP>(p.b, pg < 0 ? 0 : pg, h, tile0 * TILE), smem, tid);
+    st.put(smem, tid);
+    for (int i = 0; i < n; ++i) {
+      const unsigned char *kt = smem + (i & 1) * STAGE, *vt = kt + TILE * HDP * 2;
+      unsigned char *other = smem + ((i + 1) & 1) * STAGE;
+      aos_mem_wait(); /* tile i */
+      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); /* and every wave is past tile i - 1 */
+      const bool there = pg >= 0;
+      if (i + 1 < n) {
+        pg = page(i + 1);
+        st.fetch(tile_ptr<FMT, HDP>(p.b, pg < 0 ? 0 : pg, h, (tile0 + i + 1) * TILE), other, tid);
+      }
+      const int k0 = (tile0 + i) * TILE;
+      if (marking && (k0 < wg_lo || k0 + TILE - 1 > wg_hi)) { /* uniform over the workgroup */
+        u32x4 *vw = (u32x4 *)(kt + TILE * HDP * 2);
+        bool odd = false;
+#pragma unroll
+        for (int c = 0; c < TILE * HDP / 8 / 256; ++c) {
+          const u32x4 a = vw[tid + 256 * c];
+          odd = odd || odd2(a[0]) || odd2(a[1]) || odd2(a[2]) || odd2(a[3]);
+        }
+        if (__syncthreads_or(odd ? 1 : 0)) {
+          if (there)
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+              for (int cls = 0; cls < 3; ++cls) {
+                f32x16 c = {};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                  u32x4 sf;
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) {
+                    const int at = k0 + 32 * (k >> 1) + 16 * half + 8 * (k & 1) + 2 * e;
+                    sf[e] = (at >= lo && at <= hi ? 0x3f80u : 0u) | (at + 1 >= lo && at + 1 <= hi ? 0x3f800000u : 0u);
+                  }
+                  aos_compiler_barrier();
+                  c = mfma32(odd_part(va(vt, k, d), cls), sf, c);
+                }
+#pragma unroll
+                for (int v = 0; v < 16; ++v) marks.bit[cls][d / 2] |= c[v] > 0.0f ? 1u << (16 * (d % 2) + v) : 0u;
+              }
+          __syncthreads();
+#pragma unroll
+          for (int c = 0; c < TILE * HDP / 8 / 256; ++c) vw[tid + 256 * c] = odd_part(vw[tid + 256 * c], -1);
+          __syncthreads();
+        }
+      }
+      if (there && k0 <= hi_max && k0 + TILE > lo_min && nrows > 0) { /* uniform: some row of the wave sees some of it */
+        const bool edge = k0 < lo_max || k0 + TILE - 1 > hi_min;
+        f32x16 sc[2] = {f32x16{}, f32x16{}};
+        {
+          const int pos = ((col & 4) << 2) | ((col & 16) >> 1) | ((col & 8) >> 1) | (col & 3);
+          const unsigned char *kb = kt + (half * KS * TILE + pos) * 16;
+#pragma unroll
+          for (int e = 0; e < KS; ++e) {
+            sc[0] = mfma32(*(const u32x4 *)(kb + e * TILE * 16), qf[e], sc[0]);
+            sc[1] = mfma32(*(const u32x4 *)(kb + e * TILE * 16 + 512), qf[e], sc[1]);
+          }
+        }
+        if (edge) {
+          const int at = k0 + 16 * half;
+#pragma unroll
+          for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int v = 0; v < 16; ++v)
+              if (at + 32 * b + v < lo || at + 32 * b + v > hi) sc[b][v] = NINF;
+        }
+        float mx = NINF;
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int v = 0; v < 16; ++v) mx = fmaxf(mx, sc[b][v]);
+        mx = half_max(mx) * cs;
+        if (__ballot(mx > m + SLACK)) {
+          const float top = fmaxf(m, mx), alpha = ex2(m - safe_max(top));
+          l = l * alpha;
+#pragma unroll
+          for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) o[d][v] = o[d][v] * alpha;
+          m = top;
+        }
+        const float ms = safe_max(m);
+        u32x4 pf[4];
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int v = 0; v < 16; v += 2) {
+            const float e0 = ex2(fmaf(sc[b][v], cs, -ms)), e1 = ex2(fmaf(sc[b][v + 1], cs, -ms));
+            l = l + e0;
+            l = l + e1;
+            pf[2 * b + v / 8][v / 2 % 4] = pack_bf16(e0, e1);
+          }
+        {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int d = 0; d < DB; ++d) o[d] = mfma32(va(vt, k, d), pf[k], o[d]);
+        }
+      }
+      if (i + 1 < n) st.put(other, tid);
+    }
+    if (marking)
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) o[d][v] = marks.apply(16 * d + v, o[d][v]);
+    l = half_sum(l);
+
+    uint16_t *orow = p.out + (long long)(x.q.row0 + t) * p.out_ld + hh * p.b.hd;
+    auto put = [&](int d, int q, f32x4 y, float inv) { /* dimensions 32 d + 8 q + 4 half ..+3 */
+      const int at = 32 * d + 8 * q + 4 * half;
+      if (col < nrows && at < p.b.hd)
+        *(u32x2 *)(orow + at) = u32x2{pack_bf16(y[0] * inv, y[1] * inv), pack_bf16(y[2] * inv, y[3] * inv)};
+    };
+    if (n == x.nt) {
+      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          put(d, q, f32x4{o[d][4 * q], o[d][4 * q + 1], o[d][4 * q + 2], o[d][4 * q + 3]}, inv);
+    } else {
+      constexpr int PF = tile_part_floats<HDP>();
+      const int g0 = u - j, w0 = g0 / share, w1 = (g0 + x.nt - 1) / share;
+      const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void *)p.part, (short)0, 0x7fffffff, 0x00020000);
+      if (nrows > 0) {
+        const int at = (2 * w + (j > 0 ? 0 : 1)) * PF;
+        if (half == 0) {
+          aos_publish(p.part + at + 64 * wave + col, m);
+          aos_publish(p.part + at + 64 * wave + 32 + col, l);
+        }
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const f32x4 y = {o[d][4 * q], o[d][4 * q + 1], o[d][4 * q + 2], o[d][4 * q + 3]};
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, y), rs,
+                                                   (at + 256 + (((wave * DB + d) * 4 + q) * 64 + lane) * 4) * 4, 0, SC1);
+          }
+      }
+      aos_mem_wait();
+      __syncthreads();
+      if (tid == 0) {
+        const uint32_t old = aos_arrive(p.counters + w0);
+        if (old == (uint32_t)(w1 - w0)) aos_reset(p.counters + w0);
+        found[0] = old == (uint32_t)(w1 - w0) ? 1 : 0;
+      }
+      __syncthreads();
+      if (found[0] && nrows > 0) {
+        const int np = w1 - w0 + 1;
+        auto part = [&](int k) { return (k == 0 ? 2 * w0 + 1 : 2 * (w0 + k)) * PF; };
+        float top = NINF;
+        for (int k = 0; k < np; ++k) top = fmaxf(top, aos_collect(p.part + part(k) + 64 * wave + col));
+        const float ms = safe_max(top);
+        float all = 0.0f;
+#pragma unroll
+        for (int d = 0; d < DB; ++d) o[d] = f32x16{};
+        for (int k = 0; k < np; ++k) {
+          const float f = piece_weight(aos_collect(p.part + part(k) + 64 * wave + col), ms);
+          all = all + aos_collect(p.part + part(k) + 64 * wave + 32 + col) * f;
+#pragma unroll
+          for (int d = 0; d < DB; ++d) {
+            f32x4 y[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              y[q] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                                                   rs, (part(k) + 256 + (((wave * DB + d) * 4 + q) * 64 + lane) * 4) * 4, 0, SC1));
+#pragma unroll
+            for (int v = 0; v < 16; ++v) o[d][v] = o[d][v] + y[v >> 2][v & 3] * f;
+          }
+        }
+        const float inv = all == 0.0f ? 0.0f : 1.0f / all;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            put(d, q, f32x4{o[d][4 * q], o[d][4 * q + 1], o[d][4 * q + 2], o[d][4 * q + 3]}, inv);
+      }
+    }
+    __syncthreads(); /* the stages and found[] are free again */
+    u += n;
+    j = 0;
+    if (++slot >= slots) {
+      slot = 0;
+      ++h;
+    }
+  }
+}
+
+constexpr int ROWS_WGS = 512;
+constexpr int ROWS_FEW = 16; /* a sequence of up to this many rows is the first kernel's, in any batch */
+
+template <int FMT, int HDP>
+int attend(const aos_kv_attn_params *p, const aos_launch_ctx *ctx) {
+  const long long g = p->nh / p->b.nkv;
+  if (p->b.max_new * g > ROWS_FEW) {
+    static int ready[64]; /* (by device: the kernel's LDS size has been allowed) */
+    int dev = 0;
+    hipError_t e = hipGetDevice(&dev);
+    if (e != hipSuccess) return (int)e;
+    if (dev < 0 || dev >= 64 || !ready[dev]) {
+      e = hipFuncSetAttribute((const void *)aos_kv_tiles_kernel<FMT, HDP>, hipFuncAttributeMaxDynamicSharedMemorySize,
+                              8 * TILE * HDP);
+      if (e != hipSuccess) return (int)e;
+      if (dev >= 0 && dev < 64) ready[dev] = 1;
+    }
+    const long long slots = (long long)p->b.n_tokens * g / TR + p->b.n_seqs;
+    if (slots > (1 << 24)) return (int)hipErrorInvalidValue;
+    AOS_LAUNCH(ctx, (aos_kv_tiles_kernel<FMT, HDP>), dim3(256 * tiles_per_cu(HDP)), dim3(256), 8 * TILE * HDP, *p,
+               ROWS_FEW, (int)slots, 4);
+    if ((e = hipGetLastError()) != hipSuccess) return (int)e;
+    if (p->b.n_seqs == 1) return 0;
+  }
+  AOS_LAUNCH(ctx, (aos_kv_rows_kernel<FMT, HDP, 1>), dim3(ROWS_WGS), dim3(256), 0, *p, ROWS_FEW, 8);
   return (int)hipGetLastError();
 }
 
 }  // namespace
 
-size_t aos_kv_part_floats(int hdp) { return (size_t)2 * AOS_KV_MAX_WGS * (32 + 16 * hdp); }
+/* the largest launch's pieces, two for each workgroup */
+size_t aos_kv_part_floats(int hdp) {
+  const size_t rows = 2 * (size_t)ROWS_WGS * (32 + 16 * hdp);
+  const size_t tiles = 2 * (size_t)256 * (hdp == 256 ? 1 : 2) * (256 + TR * hdp);
+  return rows > tiles ? rows : tiles;
+}
 
 #define KV_DISPATCH(fn, fmt, hdp, ...)                                       \
   ((hdp) == 64 ? ((fmt) == AOS_KV_BF16    ? fn<AOS_KV_BF16, 64>(__VA_ARGS__)    \
@@ -609,5 +1131,5 @@ size_t aos_kv_part_floats(int hdp) { return (size_t)2 * AOS_KV_MAX_WGS * (32 + 1
                                              : fn<AOS_KV_MXFP4, 256>(__VA_ARGS__)))
 
 extern "C" int aos_launch_kv_attention(const aos_kv_attn_params *p, const aos_launch_ctx *ctx) {
-  return KV_DISPATCH(rows, p->b.format, p->b.hdp, p, ctx);
+  return KV_DISPATCH(attend, p->b.format, p->b.hdp, p, ctx);
 }
