@@ -110,6 +110,11 @@ struct OddMarks {
 #pragma unroll
       for (int i = 0; i < (N + 31) / 32; ++i) bit[c][i] = 0u;
   }
+  __device__ __forceinline__ void set(int cls, int i, uint32_t bits) { /* cls need not be constant */
+    bit[0][i] |= cls == 0 ? bits : 0u;
+    bit[1][i] |= cls == 1 ? bits : 0u;
+    bit[2][i] |= cls == 2 ? bits : 0u;
+  }
   __device__ __forceinline__ float apply(int i, float x) const {
     if (bit[0][i / 32] >> (i % 32) & 1) x = x + __builtin_inff();
     if (bit[1][i / 32] >> (i % 32) & 1) x = x - __builtin_inff();
@@ -417,7 +422,7 @@ __global__ void __launch_bounds__(256, rows_waves(FMT, HDP)) aos_kv_rows_kernel(
 #pragma unroll
               for (int k = 0; k < 8; ++k) any |= odd2(tl.v[d][k]) ? 1u : 0u;
               if (__ballot(any != 0) == 0) continue;
-#pragma unroll
+#pragma unroll 1
               for (int cls = 0; cls < 3; ++cls)
 #pragma unroll
                 for (int b = 0; b < NB; ++b) {
@@ -436,7 +441,7 @@ __global__ void __launch_bounds__(256, rows_waves(FMT, HDP)) aos_kv_rows_kernel(
 #pragma unroll
                   for (int k = 0; k < 4; ++k) {
                     const int e = (b * DB + d) * 4 + k;
-                    marks.bit[cls][e / 32] |= c[k] > 0.0f ? 1u << (e % 32) : 0u;
+                    marks.set(cls, e / 32, c[k] > 0.0f ? 1u << (e % 32) : 0u);
                   }
                 }
 #pragma unroll
@@ -752,27 +757,52 @@ struct Stage {
 /* Row tile slots of a batch: sequence s has its row tiles from slot_base(s) on, fewer than the next one's base. */
 __device__ __forceinline__ int slot_base(int start, int g, int s) { return (int)((long long)start * g / TR) + s; }
 
+/* Where a walk over the slots is: sequence s, which has the slots base .. next - 1. */
+struct Cursor {
+  Seq q;
+  int s, base, next;
+};
+__device__ __forceinline__ void open(const aos_kv_batch &b, int g, int s, Cursor &c) {
+  const int r0 = b.starts[s], r1 = b.starts[s + 1];
+  c.s = s;
+  c.q = seq_of(b, r0, r1, b.lens[s]);
+  c.base = slot_base(r0, g, s);
+  c.next = s + 1 < b.n_seqs ? slot_base(r1, g, s + 1) : 0x7fffffff;
+}
+__device__ __forceinline__ void seek(const aos_kv_batch &b, int g, int slot, Cursor &c) {
+  int lo = 0, hi = b.n_seqs; /* the last sequence whose slots begin at or before `slot` */
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (slot_base(b.starts[mid], g, mid) <= slot)
+      lo = mid;
+    else
+      hi = mid;
+  }
+  open(b, g, lo, c);
+}
+
+/* (for a wave whose lanes all hold the same: kept in scalar registers) */
+__device__ __forceinline__ void uniform(Cursor &c) {
+  c.q.row0 = __builtin_amdgcn_readfirstlane(c.q.row0);
+  c.q.count = __builtin_amdgcn_readfirstlane(c.q.count);
+  c.q.len = __builtin_amdgcn_readfirstlane(c.q.len);
+  c.s = __builtin_amdgcn_readfirstlane(c.s);
+  c.base = __builtin_amdgcn_readfirstlane(c.base);
+  c.next = __builtin_amdgcn_readfirstlane(c.next);
+}
+
 /* A row tile: rows r0 .. r0 + rows - 1 of its sequence and the position tiles t0 .. t0 + nt - 1 that they see (at least
  * one). nt 0: no such row tile, or one of a sequence of few rows. */
 struct RowTile {
-  Seq q;
-  int s, r0, rows, t0, nt;
+  int r0, rows, t0, nt;
 };
-__device__ __forceinline__ RowTile row_tile(const aos_kv_attn_params &p, int few, int slot) {
-  const int g = p.nh / p.b.nkv;
+__device__ __forceinline__ RowTile row_tile(const aos_kv_attn_params &p, int g, int few, const Cursor &c, int slot) {
   RowTile o = {};
-  int lo = 0, hi = p.b.n_seqs; /* the last sequence whose slots begin at or before `slot` */
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (slot_base(p.b.starts[mid], g, mid) <= slot) lo = mid; else hi = mid;
-  }
-  o.s = lo;
-  o.q = seq_at(p.b, lo);
-  const int all = o.q.count * g, r = slot - slot_base(o.q.row0, g, lo);
+  const int all = c.q.count * g, r = slot - c.base;
   o.r0 = r * TR;
   if (all <= few || r < 0 || o.r0 >= all) return o;
   o.rows = all - o.r0 < TR ? all - o.r0 : TR;
-  const int p0 = o.q.len - o.q.count;
+  const int p0 = c.q.len - c.q.count;
   const int first = p0 + o.r0 / g, last = p0 + (o.r0 + o.rows - 1) / g;
   const int low = p.window > 0 && first - p.window + 1 > 0 ? first - p.window + 1 : 0;
   o.t0 = low / TILE;
@@ -780,21 +810,33 @@ __device__ __forceinline__ RowTile row_tile(const aos_kv_attn_params &p, int few
   return o;
 }
 
-template <int FMT, int HDP>
-__global__ void __launch_bounds__(256, tiles_per_cu(HDP)) aos_kv_tiles_kernel(aos_kv_attn_params p, int few, int slots,
-                                                                             int min_share) {
-  constexpr int KS = HDP / 16, DB = HDP / 32, STAGE = 4 * TILE * HDP;
+/* Shares are of weights: a row tile's position tiles and SETUP for its beginning and end (its queries, its first tile's
+ * latency, its output), so that many short row tiles make a share of their own. A border that would cut fewer than
+ * SNAP tiles off a row tile moves to the row tile's end. */
+constexpr int SETUP = 3, SNAP = 3;
+
+template <int FMT, int HDP, bool MARK>
+__device__ __forceinline__ void tiles_body(const aos_kv_attn_params &p, int few, int slots, int min_share) {
+  constexpr int KS = HDP / 16, DB = HDP / 32, STAGE = 4 * TILE * HDP, AHEAD = HDP == 256 ? 4 : 8;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-  __shared__ int scan[4], found[2];
+  __shared__ int scan[4], found[4], joins;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 31, half = lane >> 5;
   const int g = p.nh / p.b.nkv;
   const int G = gridDim.x, w = (int)(blockIdx.x % 8) * (G / 8) + (int)(blockIdx.x / 8);
 
-  /* units of a key/value head (each thread a run of slots), this workgroup's share, and where it begins */
+  /* weights of a key/value head (each thread a run of slots), this workgroup's share, and its two borders */
   const int per = (slots + 255) / 256, first = tid * per, end = first + per < slots ? first + per : slots;
+  Cursor cur;
   int sum = 0;
-  for (int x = first; x < end; ++x) sum += row_tile(p, few, x).nt;
+  if (first < end) {
+    seek(p.b, g, first, cur);
+    for (int x = first; x < end; ++x) {
+      while (x >= cur.next) open(p.b, g, cur.s + 1, cur);
+      const int nt = row_tile(p, g, few, cur, x).nt;
+      sum += nt ? nt + SETUP : 0;
+    }
+  }
   const int upto = wave_scan(sum, lane);
   if (lane == 63) scan[wave] = upto;
   __syncthreads();
@@ -807,42 +849,59 @@ __global__ void __launch_bounds__(256, tiles_per_cu(HDP)) aos_kv_tiles_kernel(ao
   const int total = N * p.b.nkv;
   int share = (total + G - 1) / G;
   if (share < min_share) share = min_share;
-  int u = w * share;
-  if (u >= total) return; /* uniform */
-  const int u1 = u + share < total ? u + share : total;
-  int h = u / N;
-  {
-    int v = u - h * N - before;
-    if (v >= 0 && v < sum)
+  if (w * share >= total) return; /* uniform */
+  int h = w * share / N, h1 = p.b.nkv;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int at = (w + i) * share;
+    if (at >= total) {
+      if (tid == 0) found[2] = found[3] = 0;
+      break;
+    }
+    const int hh = at / N;
+    if (i) h1 = hh;
+    int v = at - hh * N - before;
+    if (v >= 0 && v < sum) {
+      seek(p.b, g, first, cur);
       for (int x = first; x < end; ++x) {
-        const int nt = row_tile(p, few, x).nt;
-        if (v < nt) {
-          found[0] = x;
-          found[1] = v;
+        while (x >= cur.next) open(p.b, g, cur.s + 1, cur);
+        const int nt = row_tile(p, g, few, cur, x).nt, weight = nt ? nt + SETUP : 0;
+        if (v < weight) {
+          const int j = v - SETUP;
+          found[2 * i] = nt - j < SNAP ? x + 1 : x;
+          found[2 * i + 1] = j < SNAP || nt - j < SNAP ? 0 : j;
           break;
         }
-        v -= nt;
+        v -= weight;
       }
+    }
   }
   __syncthreads();
   int slot = __builtin_amdgcn_readfirstlane(found[0]), j = __builtin_amdgcn_readfirstlane(found[1]);
-
+  const int slot1 = __builtin_amdgcn_readfirstlane(found[2]), j1 = __builtin_amdgcn_readfirstlane(found[3]);
+  seek(p.b, g, slot < slots ? slot : 0, cur);
+  uniform(cur);
   /* (a scale of zero stays above it, so that what a row does not see keeps -infinity) */
   const float cs = fmaxf(fabsf(p.scale) * LOG2E, 1.17549435e-38f);
   const uint32_t flip = p.scale < 0.0f ? 0x80008000u : 0u; /* a negative scale: negated queries */
-  const bool marking = *p.b.nonfinite != 0;
-  while (u < u1) {
-    RowTile x = row_tile(p, few, slot);
-    if (x.nt == 0) { /* (the next slot, or the next head's first) */
-      if (++slot >= slots) {
-        slot = 0;
-        if (++h >= p.b.nkv) return; /* (never: u < total) */
-      }
-      continue;
+  int pages = -1, pages_s = -1, pages_t = 0; /* pages of 64 tiles from pages_t on of a sequence, one a lane */
+  for (;; ++slot, j = 0) {
+    if (slot >= slots) {
+      if (++h >= p.b.nkv) break;
+      slot = 0;
+      seek(p.b, g, 0, cur);
+      uniform(cur);
     }
-    const int n = x.nt - j < u1 - u ? x.nt - j : u1 - u;
-    const int p0 = x.q.len - x.q.count;
-    const int s = __builtin_amdgcn_readfirstlane(x.s);
+    if (h > h1 || (h == h1 && slot >= slot1 && (slot > slot1 || j1 == 0))) break;
+    while (slot >= cur.next) {
+      open(p.b, g, cur.s + 1, cur);
+      uniform(cur);
+    }
+    const RowTile x = row_tile(p, g, few, cur, slot);
+    if (x.nt == 0) continue;
+    const int je = h == h1 && slot == slot1 ? j1 : x.nt; /* its tiles j .. je - 1 are this workgroup's */
+    const int n = je - j;
+    const int p0 = cur.q.len - cur.q.count;
 
     /* this lane's row, and the wave's rows' positions: first and last, and what they all see */
     const int wr = 32 * wave, nrows = x.rows - wr;
@@ -860,7 +919,7 @@ __global__ void __launch_bounds__(256, tiles_per_cu(HDP)) aos_kv_tiles_kernel(ao
 
     u32x4 qf[KS];
     {
-      const uint16_t *qr = p.q + (long long)(x.q.row0 + t) * p.q_ld + hh * p.b.hd;
+      const uint16_t *qr = p.q + (long long)(cur.q.row0 + t) * p.q_ld + hh * p.b.hd;
 #pragma unroll
       for (int e = 0; e < KS; ++e) {
         const int d = half * (HDP / 2) + 8 * e;
@@ -881,13 +940,15 @@ __global__ void __launch_bounds__(256, tiles_per_cu(HDP)) aos_kv_tiles_kernel(ao
       return *(const u32x4 *)(vt + ((4 * (k >> 1) + 2 * half + (k & 1)) * HDP + 32 * d + col) * 16);
     };
     const int tile0 = x.t0 + j;
-    int pages = -1; /* of the 64 tiles from i & ~63 on, one a lane */
-    auto page = [&](int i) { /* of tile i, for i in order; -1 where it cannot be read */
-      if ((i & 63) == 0) {
-        const int pos = (tile0 + i + lane) * TILE;
-        pages = i + lane < n && pos < x.q.len ? page_of(p.b, s, pos) : -1;
+    auto page = [&](int i) { /* of tile i; -1 where it cannot be read */
+      const int t = tile0 + i;
+      if (cur.s != pages_s || (t & ~63) != pages_t) { /* uniform */
+        pages_s = cur.s;
+        pages_t = t & ~63;
+        const int pos = (pages_t + lane) * TILE;
+        pages = pos < cur.q.len ? page_of(p.b, cur.s, pos) : -1;
       }
-      return __builtin_amdgcn_readlane(pages, i & 63);
+      return __builtin_amdgcn_readlane(pages, t & 63);
     };
     Stage<FMT, HDP> st;
     int pg = page(0);
@@ -904,7 +965,7 @@ __global__ void __launch_bounds__(256, tiles_per_cu(HDP)) aos_kv_tiles_kernel(ao
         st.fetch(tile_ptr<FMT, HDP>(p.b, pg < 0 ? 0 : pg, h, (tile0 + i + 1) * TILE), other, tid);
       }
       const int k0 = (tile0 + i) * TILE;
-      if (marking && (k0 < wg_lo || k0 + TILE - 1 > wg_hi)) { /* uniform over the workgroup */
+      if (MARK && (k0 < wg_lo || k0 + TILE - 1 > wg_hi)) { /* uniform over the workgroup */
         u32x4 *vw = (u32x4 *)(kt + TILE * HDP * 2);
         bool odd = false;
 #pragma unroll
@@ -916,7 +977,7 @@ __global__ void __launch_bounds__(256, tiles_per_cu(HDP)) aos_kv_tiles_kernel(ao
           if (there)
 #pragma unroll
             for (int d = 0; d < DB; ++d)
-#pragma unroll
+#pragma unroll 1
               for (int cls = 0; cls < 3; ++cls) {
                 f32x16 c = {};
 #pragma unroll
@@ -931,7 +992,7 @@ __global__ void __launch_bounds__(256, tiles_per_cu(HDP)) aos_kv_tiles_kernel(ao
                   c = mfma32(odd_part(va(vt, k, d), cls), sf, c);
                 }
 #pragma unroll
-                for (int v = 0; v < 16; ++v) marks.bit[cls][d / 2] |= c[v] > 0.0f ? 1u << (16 * (d % 2) + v) : 0u;
+                for (int v = 0; v < 16; ++v) marks.set(cls, d / 2, c[v] > 0.0f ? 1u << (16 * (d % 2) + v) : 0u);
               }
           __syncthreads();
 #pragma unroll
@@ -941,16 +1002,28 @@ __global__ void __launch_bounds__(256, tiles_per_cu(HDP)) aos_kv_tiles_kernel(ao
       }
       if (there && k0 <= hi_max && k0 + TILE > lo_min && nrows > 0) { /* uniform: some row of the wave sees some of it */
         const bool edge = k0 < lo_max || k0 + TILE - 1 > hi_min;
+        /* LDS reads run AHEAD matrix instructions before their use (the values' first ones before the softmax): left
+         * to itself the compiler reads each fragment right before the instruction that waits for it */
         f32x16 sc[2] = {f32x16{}, f32x16{}};
         {
           const int pos = ((col & 4) << 2) | ((col & 16) >> 1) | ((col & 8) >> 1) | (col & 3);
           const unsigned char *kb = kt + (half * KS * TILE + pos) * 16;
+          auto ka = [&](int i) { return *(const u32x4 *)(kb + (i >> 1) * TILE * 16 + 512 * (i & 1)); };
+          u32x4 kf[AHEAD];
 #pragma unroll
-          for (int e = 0; e < KS; ++e) {
-            sc[0] = mfma32(*(const u32x4 *)(kb + e * TILE * 16), qf[e], sc[0]);
-            sc[1] = mfma32(*(const u32x4 *)(kb + e * TILE * 16 + 512), qf[e], sc[1]);
+          for (int i = 0; i < AHEAD; ++i) kf[i] = ka(i);
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int i = 0; i < 2 * KS; ++i) {
+            sc[i & 1] = mfma32(kf[i % AHEAD], qf[i >> 1], sc[i & 1]);
+            if (i + AHEAD < 2 * KS) kf[i % AHEAD] = ka(i + AHEAD);
+            __builtin_amdgcn_sched_barrier(0);
           }
         }
+        u32x4 vf[AHEAD];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) vf[i] = va(vt, i / DB, i % DB);
+        __builtin_amdgcn_sched_barrier(0);
         if (edge) {
           const int at = k0 + 16 * half;
 #pragma unroll
@@ -985,23 +1058,24 @@ __global__ void __launch_bounds__(256, tiles_per_cu(HDP)) aos_kv_tiles_kernel(ao
             l = l + e1;
             pf[2 * b + v / 8][v / 2 % 4] = pack_bf16(e0, e1);
           }
-        {
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-#pragma unroll
-            for (int d = 0; d < DB; ++d) o[d] = mfma32(va(vt, k, d), pf[k], o[d]);
+        for (int i = 0; i < 4 * DB; ++i) {
+          o[i % DB] = mfma32(vf[i % AHEAD], pf[i / DB], o[i % DB]);
+          if (i + AHEAD < 4 * DB) vf[i % AHEAD] = va(vt, (i + AHEAD) / DB, (i + AHEAD) % DB);
+          __builtin_amdgcn_sched_barrier(0);
         }
       }
       if (i + 1 < n) st.put(other, tid);
     }
-    if (marking)
+    if (MARK)
 #pragma unroll
       for (int d = 0; d < DB; ++d)
 #pragma unroll
         for (int v = 0; v < 16; ++v) o[d][v] = marks.apply(16 * d + v, o[d][v]);
     l = half_sum(l);
 
-    uint16_t *orow = p.out + (long long)(x.q.row0 + t) * p.out_ld + hh * p.b.hd;
+    uint16_t *orow = p.out + (long long)(cur.q.row0 + t) * p.out_ld + hh * p.b.hd;
     auto put = [&](int d, int q, f32x4 y, float inv) { /* dimensions 32 d + 8 q + 4 half ..+3 */
       const int at = 32 * d + 8 * q + 4 * half;
       if (col < nrows && at < p.b.hd)
@@ -1016,7 +1090,9 @@ __global__ void __launch_bounds__(256, tiles_per_cu(HDP)) aos_kv_tiles_kernel(ao
           put(d, q, f32x4{o[d][4 * q], o[d][4 * q + 1], o[d][4 * q + 2], o[d][4 * q + 3]}, inv);
     } else {
       constexpr int PF = tile_part_floats<HDP>();
-      const int g0 = u - j, w0 = g0 / share, w1 = (g0 + x.nt - 1) / share;
+      /* the row tile's place among the weights, and the borders wf .. wl that cut it */
+      const int place = (j > 0 ? w * share - j : (w + 1) * share - je) - SETUP;
+      const int wf = (place + SETUP + SNAP + share - 1) / share, wl = (place + SETUP + x.nt - SNAP) / share;
       const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void *)p.part, (short)0, 0x7fffffff, 0x00020000);
       if (nrows > 0) {
         const int at = (2 * w + (j > 0 ? 0 : 1)) * PF;
@@ -1036,14 +1112,14 @@ __global__ void __launch_bounds__(256, tiles_per_cu(HDP)) aos_kv_tiles_kernel(ao
       aos_mem_wait();
       __syncthreads();
       if (tid == 0) {
-        const uint32_t old = aos_arrive(p.counters + w0);
-        if (old == (uint32_t)(w1 - w0)) aos_reset(p.counters + w0);
-        found[0] = old == (uint32_t)(w1 - w0) ? 1 : 0;
+        const uint32_t old = aos_arrive(p.counters + wf);
+        if (old == (uint32_t)(wl - wf + 1)) aos_reset(p.counters + wf);
+        joins = old == (uint32_t)(wl - wf + 1) ? 1 : 0;
       }
       __syncthreads();
-      if (found[0] && nrows > 0) {
-        const int np = w1 - w0 + 1;
-        auto part = [&](int k) { return (k == 0 ? 2 * w0 + 1 : 2 * (w0 + k)) * PF; };
+      if (joins && nrows > 0) {
+        const int np = wl - wf + 2;
+        auto part = [&](int k) { return (k == 0 ? 2 * wf - 1 : 2 * (wf + k - 1)) * PF; };
         float top = NINF;
         for (int k = 0; k < np; ++k) top = fmaxf(top, aos_collect(p.part + part(k) + 64 * wave + col));
         const float ms = safe_max(top);
@@ -1051,18 +1127,20 @@ __global__ void __launch_bounds__(256, tiles_per_cu(HDP)) aos_kv_tiles_kernel(ao
 #pragma unroll
         for (int d = 0; d < DB; ++d) o[d] = f32x16{};
         for (int k = 0; k < np; ++k) {
+          f32x4 y[DB][4]; /* (all in flight together) */
+#pragma unroll
+          for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              y[d][q] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                                                      rs, (part(k) + 256 + (((wave * DB + d) * 4 + q) * 64 + lane) * 4) * 4, 0, SC1));
+          __builtin_amdgcn_sched_barrier(0);
           const float f = piece_weight(aos_collect(p.part + part(k) + 64 * wave + col), ms);
           all = all + aos_collect(p.part + part(k) + 64 * wave + 32 + col) * f;
 #pragma unroll
-          for (int d = 0; d < DB; ++d) {
-            f32x4 y[4];
+          for (int d = 0; d < DB; ++d)
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
-              y[q] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(
-                                                   rs, (part(k) + 256 + (((wave * DB + d) * 4 + q) * 64 + lane) * 4) * 4, 0, SC1));
-#pragma unroll
-            for (int v = 0; v < 16; ++v) o[d][v] = o[d][v] + y[v >> 2][v & 3] * f;
-          }
+            for (int v = 0; v < 16; ++v) o[d][v] = o[d][v] + y[d][v >> 2][v & 3] * f;
         }
         const float inv = all == 0.0f ? 0.0f : 1.0f / all;
 #pragma unroll
@@ -1072,14 +1150,18 @@ __global__ void __launch_bounds__(256, tiles_per_cu(HDP)) aos_kv_tiles_kernel(ao
             put(d, q, f32x4{o[d][4 * q], o[d][4 * q + 1], o[d][4 * q + 2], o[d][4 * q + 3]}, inv);
       }
     }
-    __syncthreads(); /* the stages and found[] are free again */
-    u += n;
-    j = 0;
-    if (++slot >= slots) {
-      slot = 0;
-      ++h;
-    }
+    __syncthreads(); /* the stages and `joins` are free again */
   }
+}
+
+/* two bodies, so that the registers of the rare one (infinities or NaNs in the cache) stay out of the other's way */
+template <int FMT, int HDP>
+__global__ void __launch_bounds__(256, tiles_per_cu(HDP)) aos_kv_tiles_kernel(aos_kv_attn_params p, int few, int slots,
+                                                                             int min_share) {
+  if (*p.b.nonfinite)
+    tiles_body<FMT, HDP, true>(p, few, slots, min_share);
+  else
+    tiles_body<FMT, HDP, false>(p, few, slots, min_share);
 }
 
 constexpr int ROWS_WGS = 512;
@@ -1100,9 +1182,9 @@ int attend(const aos_kv_attn_params *p, const aos_launch_ctx *ctx) {
       if (dev >= 0 && dev < 64) ready[dev] = 1;
     }
     const long long slots = (long long)p->b.n_tokens * g / TR + p->b.n_seqs;
-    if (slots > (1 << 24)) return (int)hipErrorInvalidValue;
+    if (slots * (p->b.max_len / TILE + 1 + SETUP) * p->b.nkv > 0x7fffffffll - 0x1000000) return (int)hipErrorInvalidValue;
     AOS_LAUNCH(ctx, (aos_kv_tiles_kernel<FMT, HDP>), dim3(256 * tiles_per_cu(HDP)), dim3(256), 8 * TILE * HDP, *p,
-               ROWS_FEW, (int)slots, 4);
+               ROWS_FEW, (int)slots, 8);
     if ((e = hipGetLastError()) != hipSuccess) return (int)e;
     if (p->b.n_seqs == 1) return 0;
   }
