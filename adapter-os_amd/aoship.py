@@ -773,7 +773,9 @@ class KVCache:
         if not self.h:
             raise AosError(f"aoship_kv_cache_new: {last_error()}")
         self.num_kv_heads, self.head_dim, self.page_size = num_kv_heads, head_dim, page_size
-        self._rows = _KVRows()
+        import torch
+
+        self._rows, self._scale, self._dtypes = _KVRows(), head_dim ** -0.5, (torch.bfloat16, torch.int16)
 
     def set_rope(self, cosines=None, sines=None) -> None:
         """Host float32 [positions, head_dim / 2]; None for both turns the rotation off."""
@@ -796,65 +798,71 @@ class KVCache:
             raise AosError(f"aoship_kv_cache_faults: {last_error()}")
         return f
 
-    def _batch(self, batch: KVBatch, *rows):
-        """The batch for calls over these row tensors, which have the same number of rows."""
-        n = rows[0].shape[0]
-        for t in rows:
-            if t.dim() != 3 or t.shape[0] != n or t.shape[2] != self.head_dim or t.element_size() != 2 \
-                    or t.is_floating_point() and str(t.dtype) != "torch.bfloat16" or not t.is_cuda \
-                    or t.numel() and (t.stride(2) != 1 or t.shape[1] > 1 and t.stride(1) != self.head_dim):
-                raise AosError("KVCache: rows must be device bfloat16 tensors [tokens, heads, head_dim] of one length")
-        if batch.width * self.page_size < batch.c.max_len:
+    def _batch(self, batch: KVBatch, n: int):
+        """The batch for a call over n rows."""
+        c = batch.c
+        if batch.width * self.page_size < c.max_len:
             raise AosError("KVCache: the page table is too narrow for max_len")
-        batch.c.n_tokens = n
-        return C.byref(batch.c)
+        c.n_tokens = n
+        return C.byref(c)
 
-    @staticmethod
-    def _stride(t) -> int:
-        return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
-
-    def _kv_heads(self, *rows) -> None:
-        if any(t.shape[1] != self.num_kv_heads for t in rows):
-            raise AosError(f"KVCache: k and v rows must have {self.num_kv_heads} heads")
+    def _row(self, t, n: int, heads: int = 0) -> tuple[int, int]:
+        """(pointer, row stride) of a row tensor [n, heads, head_dim], checked (heads 0: any)."""
+        shape, stride = t.shape, t.stride()
+        hd = self.head_dim
+        if len(shape) != 3 or shape[0] != n or shape[2] != hd or heads and shape[1] != heads \
+                or t.dtype not in self._dtypes or not t.is_cuda \
+                or t.numel() and (stride[2] != 1 or shape[1] > 1 and stride[1] != hd):
+            raise AosError(f"KVCache: rows must be device bfloat16 tensors [{n}, {heads or 'heads'}, {hd}], the heads of "
+                           "a row side by side")
+        return t.data_ptr(), stride[0] if n > 1 else shape[1] * hd
 
     def append(self, layer: int, batch: KVBatch, k, v, q=None, q_out=None, q_bias=None, k_bias=None,
                v_bias=None) -> None:
         """Biases (device float32 [heads, head_dim]) and rotary embedding of the new rows; k and v go into the pages,
         q to q_out."""
-        if (q is None) != (q_out is None) or q is not None and q.shape != q_out.shape:
-            raise AosError("KVCache.append: q and q_out come together, with the same shape")
-        b = self._batch(batch, k, v) if q is None else self._batch(batch, k, v, q, q_out)
-        self._kv_heads(k, v)
-        for t, heads in ((q_bias, 0 if q is None else q.shape[1]), (k_bias, k.shape[1]), (v_bias, v.shape[1])):
-            if t is not None and (str(t.dtype) != "torch.float32" or t.numel() != heads * self.head_dim
-                                  or not t.is_contiguous() or not t.is_cuda):
-                raise AosError("KVCache.append: biases must be device float32 [heads, head_dim]")
-        r = self._rows
-        r.k, r.v, r.k_stride, r.v_stride = k.data_ptr(), v.data_ptr(), self._stride(k), self._stride(v)
-        r.q = r.q_out = None
-        r.num_heads = 0
-        if q is not None:
-            r.q, r.q_stride, r.num_heads = q.data_ptr(), self._stride(q), q.shape[1]
-            r.q_out, r.q_out_stride = q_out.data_ptr(), self._stride(q_out)
-        r.q_bias, r.k_bias, r.v_bias = _ptr(q_bias), _ptr(k_bias), _ptr(v_bias)
-        _check(lib().aoship_kv_append(self.h, layer, b, C.byref(r)), "aoship_kv_append")
+        if (q is None) != (q_out is None):
+            raise AosError("KVCache.append: q and q_out come together")
+        r, nkv, n = self._rows, self.num_kv_heads, k.shape[0]
+        r.k, r.k_stride = self._row(k, n, nkv)
+        r.v, r.v_stride = self._row(v, n, nkv)
+        if q is None:
+            nh, r.q, r.q_out = 0, None, None
+        else:
+            r.q, r.q_stride = self._row(q, n)
+            nh = q.shape[1]
+            r.q_out, r.q_out_stride = self._row(q_out, n, nh)
+        r.num_heads = nh
+        r.q_bias = None if q_bias is None else self._bias(q_bias, nh)
+        r.k_bias = None if k_bias is None else self._bias(k_bias, nkv)
+        r.v_bias = None if v_bias is None else self._bias(v_bias, nkv)
+        if _lib.aoship_kv_append(self.h, layer, self._batch(batch, n), C.byref(r)):
+            raise AosError(f"aoship_kv_append: {last_error()}")
+
+    def _bias(self, t, heads: int) -> int:
+        if str(t.dtype) != "torch.float32" or t.numel() != heads * self.head_dim or not t.is_contiguous() \
+                or not t.is_cuda:
+            raise AosError("KVCache.append: biases must be device float32 [heads, head_dim]")
+        return t.data_ptr()
 
     def read(self, layer: int, batch: KVBatch, k, v) -> None:
         """The values that the cache holds of the batch's new rows, into k and v."""
-        b = self._batch(batch, k, v)
-        self._kv_heads(k, v)
-        _check(lib().aoship_kv_read(self.h, layer, b, k.data_ptr(), self._stride(k), v.data_ptr(), self._stride(v)),
-               "aoship_kv_read")
+        n = k.shape[0]
+        kp, ks = self._row(k, n, self.num_kv_heads)
+        vp, vs = self._row(v, n, self.num_kv_heads)
+        if _lib.aoship_kv_read(self.h, layer, self._batch(batch, n), kp, ks, vp, vs):
+            raise AosError(f"aoship_kv_read: {last_error()}")
 
     def attention(self, layer: int, batch: KVBatch, q, out, scale: float | None = None, window: int = 0) -> None:
         """Causal attention of the batch's new rows (appended before) over their sequences; scale defaults to
         head_dim ** -0.5, window 0 is none."""
-        b = self._batch(batch, q, out)
-        if q.shape != out.shape:
-            raise AosError("KVCache.attention: q and out must have the same shape")
-        _check(lib().aoship_kv_attention(self.h, layer, b, q.data_ptr(), self._stride(q), q.shape[1],
-                                         self.head_dim ** -0.5 if scale is None else scale, window, out.data_ptr(),
-                                         self._stride(out)), "aoship_kv_attention")
+        n = q.shape[0]
+        qp, qs = self._row(q, n)
+        nh = q.shape[1]
+        op, os_ = self._row(out, n, nh)
+        if _lib.aoship_kv_attention(self.h, layer, self._batch(batch, n), qp, qs, nh,
+                                    self._scale if scale is None else scale, window, op, os_):
+            raise AosError(f"aoship_kv_attention: {last_error()}")
 
     def __del__(self):
         if getattr(self, "h", None) and _lib is not None:

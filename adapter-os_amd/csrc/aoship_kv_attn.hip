@@ -656,30 +656,27 @@ __device__ __forceinline__ float half_sum(float x) {
   return __builtin_bit_cast(float, (uint32_t)a[0]) + __builtin_bit_cast(float, (uint32_t)a[1]);
 }
 
-/* Eight codes of one dimension, each position with its own scale byte (of words s0, s1), as bfloat16. */
+/* Four positions of two dimensions (a word of 8-bit codes each, or the low halves of words of 4-bit ones) as bfloat16
+ * pairs of positions {dimension 0: 01, 23, dimension 1: 01, 23}: the codes of a position side by side, so that one
+ * conversion applies its scale to both, then the positions side by side. */
 template <int FMT>
-__device__ __forceinline__ u32x4 decode8_scaled(const uint32_t *w, uint32_t s0, uint32_t s1) {
-  float x[8];
+__device__ __forceinline__ u32x4 decode4x2(uint32_t w0, uint32_t w1, const float *scale) {
+  uint32_t x[4];
   if constexpr (FMT == AOS_KV_MXFP8) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const f32x2 a = __builtin_bit_cast(f32x2, __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w[i], 1.0f, false));
-      const f32x2 b = __builtin_bit_cast(f32x2, __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w[i], 1.0f, true));
-      x[4 * i] = a[0];
-      x[4 * i + 1] = a[1];
-      x[4 * i + 2] = b[0];
-      x[4 * i + 3] = b[1];
-    }
-  } else {
-    const f32x2 a = __builtin_bit_cast(f32x2, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[0], 1.0f, 0));
-    const f32x2 b = __builtin_bit_cast(f32x2, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[0], 1.0f, 1));
-    const f32x2 c = __builtin_bit_cast(f32x2, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[0], 1.0f, 2));
-    const f32x2 d = __builtin_bit_cast(f32x2, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[0], 1.0f, 3));
-    x[0] = a[0], x[1] = a[1], x[2] = b[0], x[3] = b[1], x[4] = c[0], x[5] = c[1], x[6] = d[0], x[7] = d[1];
+    const uint32_t lo = __builtin_amdgcn_perm(w1, w0, 0x05010400u), hi = __builtin_amdgcn_perm(w1, w0, 0x07030602u);
+    x[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale[0], false));
+    x[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale[1], true));
+    x[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale[2], false));
+    x[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale[3], true));
+  } else { /* nibbles of positions 0 .. 3: even ones (position 0, 2) and odd ones (1, 3), a byte a position */
+    const uint32_t even = (w0 & 0x0f0fu) | ((w1 << 4) & 0xf0f0u), odd = ((w0 >> 4) & 0x0f0fu) | (w1 & 0xf0f0u);
+    x[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(even, scale[0], 0));
+    x[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(odd, scale[1], 0));
+    x[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(even, scale[2], 1));
+    x[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(odd, scale[3], 1));
   }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = x[i] * byte_scale(i < 4 ? s0 : s1, i & 3);
-  return u32x4{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7])};
+  return u32x4{__builtin_amdgcn_perm(x[1], x[0], 0x05040100u), __builtin_amdgcn_perm(x[3], x[2], 0x05040100u),
+               __builtin_amdgcn_perm(x[1], x[0], 0x07060302u), __builtin_amdgcn_perm(x[3], x[2], 0x07060302u)};
 }
 
 /* A tile on its way to LDS (keys at `dst`, values TILE * HDP * 2 bytes after them). fetch() starts it, put() (of the
@@ -687,12 +684,19 @@ __device__ __forceinline__ u32x4 decode8_scaled(const uint32_t *w, uint32_t s0, 
 template <int FMT, int HDP>
 struct Stage {
   static constexpr int KU = HDP * bits<FMT>() / 128 * TILE / 256; /* key units of a thread */
-  static constexpr int VU = 4 * HDP / 256;                        /* value units of a thread */
+  static constexpr int VPAIRS = 4 * HDP / 2; /* pairs of value units: dimensions d and d + 16 of a block of 32 */
+  static constexpr int VP = (VPAIRS + 255) / 256;
   static constexpr int VW = bits<FMT>() / 2;
+  static __device__ __forceinline__ bool has(int tid, int i) { return tid + 256 * i < VPAIRS; }
+  static __device__ __forceinline__ int unit(int tid, int i) { return (tid + 256 * i) / (HDP / 2); }
+  static __device__ __forceinline__ int dim(int tid, int i) {
+    const int c = (tid + 256 * i) % (HDP / 2);
+    return (c & ~15) * 2 + (c & 15);
+  }
   static constexpr bool Q = FMT != AOS_KV_BF16;
   u32x4 k[Q ? (KU ? KU : 1) : 1];
-  uint32_t v[Q ? VU : 1][Q ? VW : 1];
-  u32x4 vs[Q ? VU : 1];
+  uint32_t v[Q ? VP : 1][2][Q ? VW : 1];
+  u32x4 vs[Q ? VP : 1];
   uint32_t ks[Q ? (KU ? KU : 1) : 1];
 
   __device__ __forceinline__ void fetch(const unsigned char *t, unsigned char *dst, int tid) {
@@ -714,17 +718,21 @@ struct Stage {
                                                                           (u * (128 / bits<FMT>()) / 32) * TILE + ks_index(pos));
       }
 #pragma unroll
-      for (int i = 0; i < VU; ++i) {
-        const int c = tid + 256 * i, d = c % HDP, u = c / HDP;
-        const unsigned char *g = t + v_off<FMT, HDP>() + c * (4 * VW);
-        if constexpr (FMT == AOS_KV_MXFP8) {
-          const u32x4 w = aos_gld16(g);
+      for (int i = 0; i < VP; ++i) {
+        if (!has(tid, i)) break;
+        const int d = dim(tid, i), u = unit(tid, i);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) v[i][j % VW] = w[j];
-        } else {
-          const u32x2 w = *(const __attribute__((address_space(1))) u32x2 *)g;
-          v[i][0] = w.x;
-          v[i][1] = w.y;
+        for (int e = 0; e < 2; ++e) {
+          const unsigned char *g = t + v_off<FMT, HDP>() + (u * HDP + d + 16 * e) * (4 * VW);
+          if constexpr (FMT == AOS_KV_MXFP8) {
+            const u32x4 w = aos_gld16(g);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[i][e][j % VW] = w[j];
+          } else {
+            const u32x2 w = *(const __attribute__((address_space(1))) u32x2 *)g;
+            v[i][e][0] = w.x;
+            v[i][e][1] = w.y;
+          }
         }
         vs[i] = aos_gld16(t + vs_off<FMT, HDP>() + (d >> 5) * TILE + 16 * u);
       }
@@ -743,12 +751,25 @@ struct Stage {
           *(u32x4 *)(dst + ((u * PER + j) * TILE + pos) * 16) = decode8<FMT>(&w[j * (4 / PER)], byte_scale(ks[i], 0));
       }
 #pragma unroll
-      for (int i = 0; i < VU; ++i) {
-        const int c = tid + 256 * i, d = c % HDP, u = c / HDP;
+      for (int i = 0; i < VP; ++i) {
+        if (!has(tid, i)) break;
+        const int d = dim(tid, i), u = unit(tid, i);
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
-          *(u32x4 *)(dst + TILE * HDP * 2 + ((2 * u + j) * HDP + d) * 16) =
-              decode8_scaled<FMT>(&v[i][j * VW / 2], vs[i][2 * j], vs[i][2 * j + 1]);
+        for (int j = 0; j < 2; ++j) {
+          u32x4 r[2];
+#pragma unroll
+          for (int k = 0; k < 2; ++k) { /* positions 8 j + 4 k ..+3 */
+            float sc[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sc[e] = byte_scale(vs[i][2 * j + k], e);
+            const uint32_t w0 = FMT == AOS_KV_MXFP8 ? v[i][0][(2 * j + k) % VW] : v[i][0][j % VW] >> (16 * k);
+            const uint32_t w1 = FMT == AOS_KV_MXFP8 ? v[i][1][(2 * j + k) % VW] : v[i][1][j % VW] >> (16 * k);
+            const u32x4 x = decode4x2<FMT>(w0, w1, sc);
+            r[0][2 * k] = x[0], r[0][2 * k + 1] = x[1], r[1][2 * k] = x[2], r[1][2 * k + 1] = x[3];
+          }
+#pragma unroll
+          for (int e = 0; e < 2; ++e) *(u32x4 *)(dst + TILE * HDP * 2 + ((2 * u + j) * HDP + d + 16 * e) * 16) = r[e];
+        }
       }
     }
   }
@@ -820,6 +841,7 @@ __device__ __forceinline__ void tiles_body(const aos_kv_attn_params &p, int few,
   constexpr int KS = HDP / 16, DB = HDP / 32, STAGE = 4 * TILE * HDP, AHEAD = HDP == 256 ? 4 : 8;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   __shared__ int scan[4], found[4], joins;
+  __shared__ Cursor at_first;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 31, half = lane >> 5;
   const int g = p.nh / p.b.nkv;
@@ -827,10 +849,11 @@ __device__ __forceinline__ void tiles_body(const aos_kv_attn_params &p, int few,
 
   /* weights of a key/value head (each thread a run of slots), this workgroup's share, and its two borders */
   const int per = (slots + 255) / 256, first = tid * per, end = first + per < slots ? first + per : slots;
-  Cursor cur;
+  Cursor own = {}, cur; /* own: where this thread's run begins */
   int sum = 0;
   if (first < end) {
-    seek(p.b, g, first, cur);
+    seek(p.b, g, first, own);
+    cur = own;
     for (int x = first; x < end; ++x) {
       while (x >= cur.next) open(p.b, g, cur.s + 1, cur);
       const int nt = row_tile(p, g, few, cur, x).nt;
@@ -862,12 +885,13 @@ __device__ __forceinline__ void tiles_body(const aos_kv_attn_params &p, int few,
     if (i) h1 = hh;
     int v = at - hh * N - before;
     if (v >= 0 && v < sum) {
-      seek(p.b, g, first, cur);
+      cur = own;
       for (int x = first; x < end; ++x) {
         while (x >= cur.next) open(p.b, g, cur.s + 1, cur);
         const int nt = row_tile(p, g, few, cur, x).nt, weight = nt ? nt + SETUP : 0;
         if (v < weight) {
           const int j = v - SETUP;
+          if (i == 0) at_first = cur;
           found[2 * i] = nt - j < SNAP ? x + 1 : x;
           found[2 * i + 1] = j < SNAP || nt - j < SNAP ? 0 : j;
           break;
@@ -879,7 +903,7 @@ __device__ __forceinline__ void tiles_body(const aos_kv_attn_params &p, int few,
   __syncthreads();
   int slot = __builtin_amdgcn_readfirstlane(found[0]), j = __builtin_amdgcn_readfirstlane(found[1]);
   const int slot1 = __builtin_amdgcn_readfirstlane(found[2]), j1 = __builtin_amdgcn_readfirstlane(found[3]);
-  seek(p.b, g, slot < slots ? slot : 0, cur);
+  cur = at_first;
   uniform(cur);
   /* (a scale of zero stays above it, so that what a row does not see keeps -infinity) */
   const float cs = fmaxf(fabsf(p.scale) * LOG2E, 1.17549435e-38f);
@@ -917,17 +941,6 @@ __device__ __forceinline__ void tiles_body(const aos_kv_attn_params &p, int few,
     const int wg_hi = p0 + x.r0 / g;
     const int wg_lo = p.window > 0 && last_at - p.window + 1 > 0 ? last_at - p.window + 1 : 0;
 
-    u32x4 qf[KS];
-    {
-      const uint16_t *qr = p.q + (long long)(cur.q.row0 + t) * p.q_ld + hh * p.b.hd;
-#pragma unroll
-      for (int e = 0; e < KS; ++e) {
-        const int d = half * (HDP / 2) + 8 * e;
-        qf[e] = d < p.b.hd ? aos_gld16(qr + d) : u32x4{};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) qf[e][i] ^= flip;
-      }
-    }
     f32x16 o[DB];
 #pragma unroll
     for (int d = 0; d < DB; ++d) o[d] = f32x16{};
@@ -953,6 +966,17 @@ __device__ __forceinline__ void tiles_body(const aos_kv_attn_params &p, int few,
     Stage<FMT, HDP> st;
     int pg = page(0);
     st.fetch(tile_ptr<FMT, HDP>(p.b, pg < 0 ? 0 : pg, h, tile0 * TILE), smem, tid);
+    u32x4 qf[KS];
+    {
+      const uint16_t *qr = p.q + (long long)(cur.q.row0 + t) * p.q_ld + hh * p.b.hd;
+#pragma unroll
+      for (int e = 0; e < KS; ++e) {
+        const int d = half * (HDP / 2) + 8 * e;
+        qf[e] = d < p.b.hd ? aos_gld16(qr + d) : u32x4{};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) qf[e][i] ^= flip;
+      }
+    }
     st.put(smem, tid);
     for (int i = 0; i < n; ++i) {
       const unsigned char *kt = smem + (i & 1) * STAGE, *vt = kt + TILE * HDP * 2;
