@@ -13,6 +13,8 @@
 #include "aoship_kv.h"
 #include <hip/hip_ext.h>
 
+#include <type_traits>
+
 using namespace kv;
 
 namespace {
@@ -23,6 +25,9 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 constexpr int SC1 = 16; /* buffer cache policy: device-coherent (sc1) */
 constexpr float LOG2E = 1.44269504f;
 constexpr float NINF = -__builtin_inff();
+/* The running maximum of a row follows its scores only once they pass it by 2^SLACK (probabilities up to 256, an exact
+ * power of two from what the true maximum would give): the accumulators are hardly ever rescaled. */
+constexpr float SLACK = 8.0f;
 
 __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
@@ -72,9 +77,23 @@ __device__ __forceinline__ u32x4 decode8(const uint32_t *w, float scale) {
                  __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[0], scale, 3))};
   }
 }
-/* scale byte j of a word as its power of two; 255 gives infinity, which times its zero codes is NaN */
-__device__ __forceinline__ float byte_scale(uint32_t w, int j) {
-  return __builtin_bit_cast(float, (j == 3 ? w >> 1 : j == 2 ? w << 7 : j == 1 ? w << 15 : w << 23) & 0x7f800000u);
+/* Scale byte j of a word as its power of two; 255 gives infinity, which times its zero codes is NaN. One instruction
+ * that selects the byte and shifts it (the compiler makes two of it: 64 more of a 4-bit tile's about 650). */
+template <int J>
+__device__ __forceinline__ float byte_scale(uint32_t w) {
+  uint32_t r;
+  if constexpr (J == 0)
+    asm("v_lshlrev_b32_sdwa %0, %1, %2 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:DWORD src1_sel:BYTE_0" : "=v"(r) : "v"(23), "v"(w));
+  else if constexpr (J == 1)
+    asm("v_lshlrev_b32_sdwa %0, %1, %2 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:DWORD src1_sel:BYTE_1" : "=v"(r) : "v"(23), "v"(w));
+  else if constexpr (J == 2)
+    asm("v_lshlrev_b32_sdwa %0, %1, %2 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:DWORD src1_sel:BYTE_2" : "=v"(r) : "v"(23), "v"(w));
+  else
+    asm("v_lshlrev_b32_sdwa %0, %1, %2 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:DWORD src1_sel:BYTE_3" : "=v"(r) : "v"(23), "v"(w));
+  return __builtin_bit_cast(float, r);
+}
+__device__ __forceinline__ float byte_scale(uint32_t w, int j) { /* (j constant once unrolled) */
+  return j == 0 ? byte_scale<0>(w) : j == 1 ? byte_scale<1>(w) : j == 2 ? byte_scale<2>(w) : byte_scale<3>(w);
 }
 
 /* Infinities and NaNs among the values. In a tile that a row sees only in part, the product of such a value with a
@@ -157,6 +176,11 @@ __device__ __forceinline__ int wave_scan(int x, int lane) { /* inclusive sum ove
   return x;
 }
 
+/* Shares are of weights: a row tile's position tiles and, for its beginning and end (its queries, its first tile's
+ * latency, the joining of its waves, its output), as many more as they take the time of. A border that would cut fewer
+ * than SNAP tiles off a row tile moves to the row tile's end. */
+constexpr int SNAP = 3;
+
 /* ---- few rows: 16 to a wave, the cache streamed through registers ------------------------------ */
 
 /* A workgroup takes an even share of all (sequence, key/value head, row tile, tile of positions); its four waves
@@ -238,56 +262,89 @@ constexpr int part_floats() { /* of a piece: maxima and sums [NB][2][16], then t
   return NB * (32 + 16 * HDP);
 }
 
-/* waves per SIMD that the registers of a tile in flight and the accumulators leave room for */
-constexpr int rows_waves(int fmt, int hdp) { return hdp == 256 || (fmt == AOS_KV_BF16 && hdp == 128) ? 1 : 2; }
+template <int HDP, int NB>
+struct RowsShared {
+  float red[2][NB * HDP / 4][64]; /* accumulators of two waves */
+  float mls[4][2][NB][64];        /* the waves' maxima and sums */
+  uint32_t last;
+};
 
-template <int FMT, int HDP, int NB>
-__global__ void __launch_bounds__(256, rows_waves(FMT, HDP)) aos_kv_rows_kernel(aos_kv_attn_params p, int few, int min_share) {
+constexpr int ROWS_SETUP = 5; /* weight of a row tile beside its position tiles */
+
+/* LEAN: a tile's keys and values are loaded as their turn comes, not a tile ahead (half the registers) */
+
+template <int FMT, int HDP, int NB, bool MARK, bool LEAN>
+__device__ __forceinline__ void rows_body(const aos_kv_attn_params &p, int few, int min_share, RowsShared<HDP, NB> &sh) {
   constexpr int R = 16 * NB, DB = HDP / 16, KS = HDP / 32, W8 = bits<FMT>() / 4; /* W8: words of 8 codes */
-  __shared__ float red[2][NB * DB * 4][64];
-  __shared__ float mls[4][2][NB][64];
-  __shared__ uint32_t last_word;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, quad = lane >> 4;
   const int G = gridDim.x, w = blockIdx.x;
   const int g = p.nh / p.b.nkv;
 
-  /* all units, this workgroup's share [u0, u1) of them, and the sequence that u0 falls in */
-  auto units = [&](int s) {
-    if (s >= p.b.n_seqs) return 0;
-    const Work x = work_of<R>(p, few, seq_at(p.b, s));
-    return p.b.nkv * x.rts * x.nt;
+  /* The sequences go by 64 at a time, one a lane: all weights, this workgroup's share [u, u1) of them, and the
+   * sequence that u falls in. */
+  int c0 = 0; /* the first sequence that the lanes hold */
+  Seq held;
+  auto hold = [&](int s0) {
+    c0 = s0;
+    held = s0 + lane < p.b.n_seqs ? seq_at(p.b, s0 + lane) : Seq{0, 0, 0};
+    const Work x = work_of<R>(p, few, held);
+    return p.b.nkv * x.rts * (x.nt + ROWS_SETUP);
   };
-  int total = 0;
-  for (int s0 = 0; s0 < p.b.n_seqs; s0 += 64)
-    total += __builtin_amdgcn_readlane(wave_scan(units(s0 + lane), lane), 63);
+  int mine = hold(0), upto = wave_scan(mine, lane);
+  int total = __builtin_amdgcn_readlane(upto, 63);
+  for (int s0 = 64; s0 < p.b.n_seqs; s0 += 64) total += __builtin_amdgcn_readlane(wave_scan(hold(s0), lane), 63);
   int share = (total + G - 1) / G;
   if (share < min_share) share = min_share;
-  int u = w * share;
+  const int u = w * share;
   if (u >= total) return;
   const int u1 = u + share < total ? u + share : total;
-  int s = 0, base = 0; /* base: units before sequence s */
-  for (int s0 = 0, before = 0; s0 < p.b.n_seqs; s0 += 64) {
-    const int mine = units(s0 + lane), upto = before + wave_scan(mine, lane);
-    const uint64_t past = __ballot(upto > u);
-    if (past) {
-      const int l = __builtin_ctzll(past);
-      s = s0 + l;
-      base = __builtin_amdgcn_readlane(upto - mine, l);
-      break;
-    }
-    before = __builtin_amdgcn_readlane(upto, 63);
+  int base = 0; /* weights before sequence s */
+  if (c0) {
+    mine = hold(0);
+    upto = wave_scan(mine, lane);
+  }
+  while (__builtin_amdgcn_readlane(upto, 63) + base <= u) { /* (u < total) */
+    base += __builtin_amdgcn_readlane(upto, 63);
+    mine = hold(c0 + 64);
+    upto = wave_scan(mine, lane);
+  }
+  int s;
+  {
+    const int l = __builtin_ctzll(__ballot(upto + base > u));
+    s = c0 + l;
+    base += __builtin_amdgcn_readlane(upto - mine, l);
   }
 
-  const float cs = p.scale * LOG2E;
-  const bool marking = FMT == AOS_KV_BF16 && *p.b.nonfinite != 0;
-  while (u < u1) {
-    Work x = work_of<R>(p, few, seq_at(p.b, s));
-    while (x.rts == 0 && s + 1 < p.b.n_seqs) x = work_of<R>(p, few, seq_at(p.b, ++s));
-    if (x.rts == 0) return; /* (never: u < total, so a later sequence has units) */
-    const int seg = (u - base) / x.nt, j = u - base - seg * x.nt; /* which (head, row tile), and its tile */
-    const int h = seg / x.rts, rt = seg - h * x.rts;
-    const int n = x.nt - j < u1 - u ? x.nt - j : u1 - u;
+  /* (a scale of zero stays above it, so that what a row does not see keeps -infinity) */
+  const float cs = fmaxf(fabsf(p.scale) * LOG2E, 1.17549435e-38f);
+  const uint32_t flip = p.scale < 0.0f ? 0x80008000u : 0u; /* a negative scale: negated queries */
+  for (int place = -1, seg = 0; place < u1;) { /* place: where row tile seg of sequence s begins among the weights */
+    if (s >= c0 + 64) (void)hold(s);
+    Seq sq;
+    sq.row0 = __builtin_amdgcn_readlane(held.row0, s - c0);
+    sq.count = __builtin_amdgcn_readlane(held.count, s - c0);
+    sq.len = __builtin_amdgcn_readlane(held.len, s - c0);
+    const Work x = work_of<R>(p, few, sq);
+    const int weight = x.nt + ROWS_SETUP;
+    if (place < 0) { /* the first: the border may be anywhere in it */
+      seg = (u - base) / weight;
+      place = base + seg * weight;
+    }
+    if (seg >= p.b.nkv * x.rts) { /* the next sequence's */
+      if (++s >= p.b.n_seqs) break;
+      seg = 0;
+      continue;
+    }
+    auto cut = [&](int at) { /* the tile before which a border at weight `at` cuts this row tile */
+      const int t = at - place - ROWS_SETUP;
+      return t < SNAP ? 0 : x.nt - t < SNAP ? x.nt : t;
+    };
+    const int j = u > place ? cut(u) : 0, je = u1 < place + weight ? cut(u1) : x.nt, n = je - j;
+    const int h = seg / x.rts, rt = seg - h * x.rts, at0 = place;
+    ++seg;
+    place += weight;
+    if (n <= 0) continue;
     const int r0 = rt * R, nrows = x.rows - r0 < R ? x.rows - r0 : R;
     const int p0 = x.q.len - x.q.count; /* position of the sequence's first new token */
 
@@ -307,6 +364,8 @@ __global__ void __launch_bounds__(256, rows_waves(FMT, HDP)) aos_kv_rows_kernel(
       for (int e = 0; e < KS; ++e) {
         const int d = quad * (HDP / 4) + 8 * e;
         qf[b][e] = d < p.b.hd && 16 * b + col < nrows ? aos_gld16(qr + d) : u32x4{};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) qf[b][e][i] ^= flip;
       }
     }
     const int t_first = r0 / g, t_last = (r0 + nrows - 1) / g;
@@ -324,7 +383,7 @@ __global__ void __launch_bounds__(256, rows_waves(FMT, HDP)) aos_kv_rows_kernel(
     }
 
     OddMarks<NB * DB * 4> marks;
-    if constexpr (FMT == AOS_KV_BF16) marks.clear();
+    if constexpr (MARK) marks.clear();
 
     const int mine = (n - wave + 3) / 4; /* tiles of this wave: j + wave, j + wave + 4, ... */
     for (int i0 = 0; i0 < mine; i0 += 64) {
@@ -342,13 +401,14 @@ __global__ void __launch_bounds__(256, rows_waves(FMT, HDP)) aos_kv_rows_kernel(
       };
       {
         const unsigned char *t = ptr(0);
-        tl.load_k(t, lane);
-        tl.load_v(t, lane);
+        if (!LEAN) tl.load_k(t, lane);
+        if (!LEAN) tl.load_v(t, lane);
       }
       for (int i = 0; i < cnt; ++i) {
         const int tb = (x.t0 + j + wave + 4 * (i0 + i)) * TILE;
         const bool there = __builtin_amdgcn_readlane(pg, i) >= 0;
-        const unsigned char *next = ptr(i + 1 < cnt ? i + 1 : i);
+        const unsigned char *next = ptr(i + 1 < cnt ? i + 1 : i), *here = ptr(i);
+        if (LEAN) tl.load_k(here, lane);
         f32x4 sc[NB][4];
 #pragma unroll
         for (int b = 0; b < NB; ++b)
@@ -363,65 +423,63 @@ __global__ void __launch_bounds__(256, rows_waves(FMT, HDP)) aos_kv_rows_kernel(
 #pragma unroll
             for (int b = 0; b < NB; ++b) sc[b][k] = mfma16(a, qf[b][e], sc[b][k]);
           }
-        if (i + 1 < cnt) tl.load_k(next, lane);
+        if (!LEAN && i + 1 < cnt) tl.load_k(next, lane);
+        if (LEAN) tl.load_v(here, lane);
 
         const bool edge = !there || tb < lo_max || tb + TILE - 1 > hi_min; /* uniform */
-        uint32_t seen[NB]; /* bit 4 b + i: the row sees position 16 quad + 4 b + i of the tile */
+        /* most tiles need no masks: two copies where the registers allow it, else one that asks as it goes */
+        auto work = [&](auto copy) {
+          constexpr int COPY = decltype(copy)::value; /* 0: without masks, 1: with them, 2: either */
+          const bool masks = COPY == 1 || (COPY == 2 && edge);
+          uint32_t seen[NB]; /* bit 4 b + i: the row sees position 16 quad + 4 b + i of the tile */
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-          seen[b] = 0xffffu;
-          if (edge) {
-            const int at = tb + 16 * quad;
-            seen[b] = 0;
+          for (int b = 0; b < NB; ++b) {
+            seen[b] = 0xffffu;
+            if (masks) {
+              const int at = tb + 16 * quad;
+              seen[b] = 0;
 #pragma unroll
-            for (int k = 0; k < 16; ++k)
-              if (there && at + k >= lo[b] && at + k <= hi[b]) seen[b] |= 1u << k;
+              for (int k = 0; k < 16; ++k)
+                if (there && at + k >= lo[b] && at + k <= hi[b]) seen[b] |= 1u << k;
+            }
           }
-        }
-        u32x4 pf[NB][2]; /* probabilities: operand of the second product */
+          u32x4 pf[NB][2]; /* probabilities: operand of the second product */
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-          float mx = m[b];
+          for (int b = 0; b < NB; ++b) {
+            float mx = NINF;
 #pragma unroll
-          for (int k = 0; k < 16; ++k) {
-            float y = sc[b][k >> 2][k & 3] * cs;
-            if (edge && !(seen[b] >> k & 1)) y = NINF;
-            sc[b][k >> 2][k & 3] = y;
-            mx = fmaxf(mx, y);
+            for (int k = 0; k < 16; ++k) {
+              if (masks && !(seen[b] >> k & 1)) sc[b][k >> 2][k & 3] = NINF;
+              mx = fmaxf(mx, sc[b][k >> 2][k & 3]);
+            }
+            mx = quad_max(mx) * cs;
+            if (__ballot(mx > m[b] + SLACK)) {
+              const float top = fmaxf(m[b], mx), alpha = ex2(m[b] - safe_max(top));
+              l[b] = l[b] * alpha;
+#pragma unroll
+              for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) o[b][d][k] = o[b][d][k] * alpha;
+              m[b] = top;
+            }
+            const float ms = safe_max(m[b]);
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+              const float e = ex2(fmaf(sc[b][k >> 2][k & 3], cs, -ms));
+              l[b] = l[b] + e;
+              sc[b][k >> 2][k & 3] = e;
+            }
+            if constexpr (FMT == AOS_KV_BF16) {
+#pragma unroll
+              for (int t = 0; t < 2; ++t)
+                pf[b][t] = u32x4{pack_bf16(sc[b][2 * t][0], sc[b][2 * t][1]), pack_bf16(sc[b][2 * t][2], sc[b][2 * t][3]),
+                                 pack_bf16(sc[b][2 * t + 1][0], sc[b][2 * t + 1][1]),
+                                 pack_bf16(sc[b][2 * t + 1][2], sc[b][2 * t + 1][3])};
+            }
           }
-          mx = quad_max(mx);
-          if (__ballot(mx > m[b])) {
-            const float alpha = ex2(m[b] - safe_max(mx));
-            l[b] = l[b] * alpha;
-#pragma unroll
-            for (int d = 0; d < DB; ++d)
-#pragma unroll
-              for (int k = 0; k < 4; ++k) o[b][d][k] = o[b][d][k] * alpha;
-            m[b] = mx;
-          }
-          const float ms = safe_max(m[b]);
-#pragma unroll
-          for (int k = 0; k < 16; ++k) {
-            const float e = ex2(sc[b][k >> 2][k & 3] - ms);
-            l[b] = l[b] + e;
-            sc[b][k >> 2][k & 3] = e;
-          }
-          if constexpr (FMT == AOS_KV_BF16) {
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-              pf[b][t] = u32x4{pack_bf16(sc[b][2 * t][0], sc[b][2 * t][1]), pack_bf16(sc[b][2 * t][2], sc[b][2 * t][3]),
-                               pack_bf16(sc[b][2 * t + 1][0], sc[b][2 * t + 1][1]),
-                               pack_bf16(sc[b][2 * t + 1][2], sc[b][2 * t + 1][3])};
-          }
-        }
-        if constexpr (FMT == AOS_KV_BF16) {
-          if (marking && edge) { /* uniform */
+          if (MARK && masks) {
 #pragma unroll
             for (int d = 0; d < DB; ++d) {
-              uint32_t any = 0;
-#pragma unroll
-              for (int k = 0; k < 8; ++k) any |= odd2(tl.v[d][k]) ? 1u : 0u;
-              if (__ballot(any != 0) == 0) continue;
 #pragma unroll 1
               for (int cls = 0; cls < 3; ++cls)
 #pragma unroll
@@ -432,7 +490,7 @@ __global__ void __launch_bounds__(256, rows_waves(FMT, HDP)) aos_kv_rows_kernel(
                     u32x4 a, sf;
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
-                      a[k] = odd_part(tl.v[d][4 * t + k], cls);
+                      a[k] = odd_part(tl.v[d][(4 * t + k) % Tile<FMT, HDP>::VW], cls);
                       sf[k] = (seen[b] >> (8 * t + 2 * k) & 1 ? 0x3f80u : 0u) |
                               (seen[b] >> (8 * t + 2 * k + 1) & 1 ? 0x3f800000u : 0u);
                     }
@@ -445,11 +503,9 @@ __global__ void __launch_bounds__(256, rows_waves(FMT, HDP)) aos_kv_rows_kernel(
                   }
                 }
 #pragma unroll
-              for (int k = 0; k < 8; ++k) tl.v[d][k] = odd_part(tl.v[d][k], -1);
+              for (int k = 0; k < Tile<FMT, HDP>::VW; ++k) tl.v[d][k] = odd_part(tl.v[d][k], -1);
             }
           }
-        }
-        {
 #pragma unroll
           for (int d = 0; d < DB; ++d) {
             if constexpr (FMT != AOS_KV_BF16) {
@@ -463,7 +519,7 @@ __global__ void __launch_bounds__(256, rows_waves(FMT, HDP)) aos_kv_rows_kernel(
                     for (int k = 0; k < 8; ++k) {
                       y[k] = sc[b][2 * t + (k >> 2)][k & 3] * byte_scale(tl.vs[d / 2][2 * t + (k >> 2)], k & 3);
                       /* (a scale that is not a number, of a position that the row does not see) */
-                      if (edge && !(seen[b] >> (8 * t + k) & 1)) y[k] = 0.0f;
+                      if (masks) y[k] = seen[b] >> (8 * t + k) & 1 ? y[k] : 0.0f;
                     }
                     pf[b][t] = u32x4{pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]), pack_bf16(y[4], y[5]),
                                      pack_bf16(y[6], y[7])};
@@ -477,12 +533,18 @@ __global__ void __launch_bounds__(256, rows_waves(FMT, HDP)) aos_kv_rows_kernel(
               for (int b = 0; b < NB; ++b) o[b][d] = mfma16(a, pf[b][t], o[b][d]);
             }
           }
-        }
-        if (i + 1 < cnt) tl.load_v(next, lane);
+        };
+        if constexpr (FMT == AOS_KV_BF16 || NB > 1 || HDP == 256)
+          work(std::integral_constant<int, 2>{});
+        else if (edge)
+          work(std::integral_constant<int, 1>{});
+        else
+          work(std::integral_constant<int, 0>{});
+        if (!LEAN && i + 1 < cnt) tl.load_v(next, lane);
       }
     }
 
-    if (marking)
+    if constexpr (MARK)
 #pragma unroll
       for (int b = 0; b < NB; ++b)
 #pragma unroll
@@ -490,26 +552,23 @@ __global__ void __launch_bounds__(256, rows_waves(FMT, HDP)) aos_kv_rows_kernel(
 #pragma unroll
           for (int k = 0; k < 4; ++k) o[b][d][k] = marks.apply((b * DB + d) * 4 + k, o[b][d][k]);
 
-    /* the waves' pieces: one maximum, then their sums two by two */
-    const bool many = n > 1;
-#pragma unroll
-    for (int b = 0; b < NB; ++b) l[b] = quad_sum(l[b]);
-    if (many) {
+    /* the waves' pieces into wave 0's: one maximum, then their sums two by two */
+    auto join_waves = [&]() {
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
-        mls[wave][0][b][lane] = m[b];
-        mls[wave][1][b][lane] = l[b];
+        sh.mls[wave][0][b][lane] = m[b];
+        sh.mls[wave][1][b][lane] = l[b];
       }
       __syncthreads();
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
         float top = NINF;
 #pragma unroll
-        for (int v = 0; v < 4; ++v) top = fmaxf(top, mls[v][0][b][lane]);
+        for (int v = 0; v < 4; ++v) top = fmaxf(top, sh.mls[v][0][b][lane]);
         const float ms = safe_max(top);
         float sum = 0.0f;
 #pragma unroll
-        for (int v = 0; v < 4; ++v) sum = sum + mls[v][1][b][lane] * piece_weight(mls[v][0][b][lane], ms);
+        for (int v = 0; v < 4; ++v) sum = sum + sh.mls[v][1][b][lane] * piece_weight(sh.mls[v][0][b][lane], ms);
         const float f = piece_weight(m[b], ms);
 #pragma unroll
         for (int d = 0; d < DB; ++d)
@@ -518,6 +577,7 @@ __global__ void __launch_bounds__(256, rows_waves(FMT, HDP)) aos_kv_rows_kernel(
         m[b] = top;
         l[b] = sum;
       }
+#pragma unroll
       for (int half = 2; half >= 1; half >>= 1) {
         if (wave >= half && wave < 2 * half)
 #pragma unroll
@@ -525,7 +585,7 @@ __global__ void __launch_bounds__(256, rows_waves(FMT, HDP)) aos_kv_rows_kernel(
 #pragma unroll
             for (int d = 0; d < DB; ++d)
 #pragma unroll
-              for (int k = 0; k < 4; ++k) red[wave - half][(b * DB + d) * 4 + k][lane] = o[b][d][k];
+              for (int k = 0; k < 4; ++k) sh.red[wave - half][(b * DB + d) * 4 + k][lane] = o[b][d][k];
         __syncthreads();
         if (wave < half)
 #pragma unroll
@@ -533,10 +593,13 @@ __global__ void __launch_bounds__(256, rows_waves(FMT, HDP)) aos_kv_rows_kernel(
 #pragma unroll
             for (int d = 0; d < DB; ++d)
 #pragma unroll
-              for (int k = 0; k < 4; ++k) o[b][d][k] = o[b][d][k] + red[wave][(b * DB + d) * 4 + k][lane];
+              for (int k = 0; k < 4; ++k) o[b][d][k] = o[b][d][k] + sh.red[wave][(b * DB + d) * 4 + k][lane];
         __syncthreads();
       }
-    }
+    };
+#pragma unroll
+    for (int b = 0; b < NB; ++b) l[b] = quad_sum(l[b]);
+    if (n > 1) join_waves(); /* (one tile is wave 0's) */
 
     auto put = [&](int b, int d, f32x4 y, float sum) {
       const float inv = sum == 0.0f ? 0.0f : 1.0f / sum; /* a row that sees nothing: zeros */
@@ -544,17 +607,13 @@ __global__ void __launch_bounds__(256, rows_waves(FMT, HDP)) aos_kv_rows_kernel(
       if (16 * b + col < nrows && at < p.b.hd)
         *(u32x2 *)(p.out + orow[b] + at) = u32x2{pack_bf16(y[0] * inv, y[1] * inv), pack_bf16(y[2] * inv, y[3] * inv)};
     };
-    if (n == x.nt) {
-      if (wave == 0)
-#pragma unroll
-        for (int b = 0; b < NB; ++b)
-#pragma unroll
-          for (int d = 0; d < DB; ++d) put(b, d, o[b][d], l[b]);
-    } else {
-      /* a cut row tile: its pieces lie in the slots of workgroups w0 .. w1 (2 w: the piece that w begins with, 2 w + 1:
-       * the one that it ends with), and the last to arrive joins them in that order */
-      constexpr int PF = part_floats<HDP, NB>();
-      const int g0 = u - j, w0 = g0 / share, w1 = (g0 + x.nt - 1) / share;
+    bool done = n == x.nt;
+    if (!done) {
+      /* a cut row tile: borders wf .. wl cut it, its pieces lie in slots of workgroups wf - 1 .. wl (2 w: the piece that w
+       * begins with, 2 w + 1: the one that it ends with), and the last to arrive joins them: each of its waves every
+       * fourth, several in flight */
+      constexpr int PF = part_floats<HDP, NB>(), FLY = 4 / NB;
+      const int wf = (at0 + ROWS_SETUP + SNAP + share - 1) / share, wl = (at0 + ROWS_SETUP + x.nt - SNAP) / share;
       const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void *)p.part, (short)0, 0x7fffffff, 0x00020000);
       if (wave == 0) {
         const int slot = (2 * w + (j > 0 ? 0 : 1)) * PF;
@@ -573,48 +632,91 @@ __global__ void __launch_bounds__(256, rows_waves(FMT, HDP)) aos_kv_rows_kernel(
                                                      (slot + 32 * NB + ((b * DB + d) * 64 + lane) * 4) * 4, 0, SC1);
         aos_mem_wait();
         if (lane == 0) {
-          const uint32_t old = aos_arrive(p.counters + w0);
-          if (old == (uint32_t)(w1 - w0)) aos_reset(p.counters + w0);
-          last_word = old == (uint32_t)(w1 - w0) ? 1u : 0u;
+          const uint32_t old = aos_arrive(p.counters + wf);
+          if (old == (uint32_t)(wl - wf + 1)) aos_reset(p.counters + wf);
+          sh.last = old == (uint32_t)(wl - wf + 1) ? 1u : 0u;
         }
       }
       __syncthreads();
-      const bool last = last_word != 0;
-      if (last) {
-        const int np = w1 - w0 + 1;
-        auto slot = [&](int k) { return (k == 0 ? 2 * w0 + 1 : 2 * (w0 + k)) * PF; };
+      done = sh.last != 0;
+      if (done) {
+        const int np = wl - wf + 2;
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-          float top = NINF;
-          for (int k = quad; k < np; k += 4) top = fmaxf(top, aos_collect(p.part + slot(k) + 32 * b + col));
-          top = quad_max(top);
-          const float ms = safe_max(top);
-          float sum = 0.0f;
-          for (int k = quad; k < np; k += 4)
-            sum = sum + aos_collect(p.part + slot(k) + 32 * b + 16 + col) * piece_weight(aos_collect(p.part + slot(k) + 32 * b + col), ms);
-          sum = quad_sum(sum);
-          if (16 * b + col < nrows)
-            for (int d = wave; d < DB; d += 4) {
-              f32x4 acc = {};
-#pragma unroll 4
-              for (int k = 0; k < np; ++k) {
-                const float f = piece_weight(aos_collect(p.part + slot(k) + 32 * b + col), ms);
-                const f32x4 y = __builtin_bit_cast(
-                    f32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, (slot(k) + 32 * NB + ((b * DB + d) * 64 + lane) * 4) * 4, 0, SC1));
-                acc = acc + y * f;
-              }
-              put(b, d, acc, sum);
-            }
+          m[b] = NINF;
+          l[b] = 0.0f;
+#pragma unroll
+          for (int d = 0; d < DB; ++d) o[b][d] = f32x4{};
         }
+        for (int k0 = wave; k0 < np; k0 += 4 * FLY) {
+          float pm[FLY][NB], pl[FLY][NB];
+          f32x4 y[FLY][NB][DB];
+#pragma unroll
+          for (int i = 0; i < FLY; ++i) {
+            const int k = k0 + 4 * i < np ? k0 + 4 * i : k0; /* (past the end: the first again, with no weight) */
+            const int slot = (k == 0 ? 2 * wf - 1 : 2 * (wf + k - 1)) * PF;
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+              pm[i][b] = aos_collect(p.part + slot + 32 * b + col);
+              pl[i][b] = aos_collect(p.part + slot + 32 * b + 16 + col);
+#pragma unroll
+              for (int d = 0; d < DB; ++d)
+                y[i][b][d] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                                                           rs, (slot + 32 * NB + ((b * DB + d) * 64 + lane) * 4) * 4, 0, SC1));
+            }
+          }
+#pragma unroll
+          for (int b = 0; b < NB; ++b) {
+            float top = m[b];
+#pragma unroll
+            for (int i = 0; i < FLY; ++i) top = fmaxf(top, pm[i][b]);
+            const float ms = safe_max(top), f0 = piece_weight(m[b], ms);
+            l[b] = l[b] * f0;
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[b][d][e] = o[b][d][e] * f0;
+#pragma unroll
+            for (int i = 0; i < FLY; ++i) {
+              if (k0 + 4 * i >= np) continue; /* uniform */
+              const float f = piece_weight(pm[i][b], ms);
+              l[b] = l[b] + pl[i][b] * f;
+#pragma unroll
+              for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[b][d][e] = o[b][d][e] + y[i][b][d][e] * f;
+            }
+            m[b] = top;
+          }
+        }
+        join_waves();
       }
-      __syncthreads(); /* last_word and the reduction's memory are free again */
+      __syncthreads(); /* sh.last is free again */
     }
-    u += n;
-    if (u - base >= p.b.nkv * x.rts * x.nt) {
-      base += p.b.nkv * x.rts * x.nt;
-      ++s;
+    if (done && wave == 0)
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int d = 0; d < DB; ++d) put(b, d, o[b][d], l[b]);
+  }
+}
+
+/* waves per SIMD that the registers of a tile in flight and the accumulators leave room for */
+constexpr int rows_waves(int fmt, int hdp, int nb) {
+  return nb > 1 || hdp == 256 || (fmt == AOS_KV_BF16 && hdp == 128) ? 1 : 2;
+}
+
+/* two bodies, so that the registers of the rare one (infinities or NaNs in the cache) stay out of the other's way */
+template <int FMT, int HDP, int NB>
+__global__ void __launch_bounds__(256, rows_waves(FMT, HDP, NB)) aos_kv_rows_kernel(aos_kv_attn_params p, int few, int min_share) {
+  __shared__ RowsShared<HDP, NB> sh;
+  if constexpr (FMT == AOS_KV_BF16) {
+    if (*p.b.nonfinite) {
+      rows_body<FMT, HDP, NB, true, FMT == AOS_KV_BF16 && HDP == 256>(p, few, min_share, sh);
+      return;
     }
   }
+  rows_body<FMT, HDP, NB, false, FMT == AOS_KV_BF16 && HDP == 256>(p, few, min_share, sh);
 }
 
 /* ---- many rows: tiles of 128, keys and values through LDS ------------------------------------- */
@@ -628,13 +730,9 @@ __global__ void __launch_bounds__(256, rows_waves(FMT, HDP)) aos_kv_rows_kernel(
  * position 16 c + 8 s + 4 a + i, which puts the 16 consecutive positions 16 c ..+15 on half c of the lanes, register
  * by register: what the value pieces hold, so the probabilities never cross lanes here either.
  *
- * The running maximum of a row follows its scores only once they pass it by 2^8 (probabilities up to 256, exact
- * powers of two apart from what the true maximum would give): the accumulators are hardly ever rescaled.
- *
  * The workgroups share all (key/value head, row tile, position tile) evenly; where a row tile is cut, its pieces meet
  * as in the kernel above. Neighbouring shares, which read the same keys, go to one XCD. */
 constexpr int TR = 128;         /* rows of a row tile */
-constexpr float SLACK = 8.0f;   /* log2 */
 constexpr int tiles_per_cu(int hdp) { return hdp == 256 ? 1 : 2; }
 
 template <int HDP>
@@ -831,17 +929,17 @@ __device__ __forceinline__ RowTile row_tile(const aos_kv_attn_params &p, int g, 
   return o;
 }
 
-/* Shares are of weights: a row tile's position tiles and SETUP for its beginning and end (its queries, its first tile's
- * latency, its output), so that many short row tiles make a share of their own. A border that would cut fewer than
- * SNAP tiles off a row tile moves to the row tile's end. */
-constexpr int SETUP = 3, SNAP = 3;
+constexpr int SETUP = 3; /* weight of a row tile beside its position tiles */
+
+struct TilesShared {
+  int scan[4], found[4], joins;
+  Cursor at_first;
+};
 
 template <int FMT, int HDP, bool MARK>
-__device__ __forceinline__ void tiles_body(const aos_kv_attn_params &p, int few, int slots, int min_share) {
+__device__ __forceinline__ void tiles_body(const aos_kv_attn_params &p, int few, int slots, int min_share, TilesShared &sh) {
   constexpr int KS = HDP / 16, DB = HDP / 32, STAGE = 4 * TILE * HDP, AHEAD = HDP == 256 ? 4 : 8;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-  __shared__ int scan[4], found[4], joins;
-  __shared__ Cursor at_first;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 31, half = lane >> 5;
   const int g = p.nh / p.b.nkv;
@@ -861,13 +959,13 @@ __device__ __forceinline__ void tiles_body(const aos_kv_attn_params &p, int few,
     }
   }
   const int upto = wave_scan(sum, lane);
-  if (lane == 63) scan[wave] = upto;
+  if (lane == 63) sh.scan[wave] = upto;
   __syncthreads();
   int before = upto - sum, N = 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    if (i < wave) before += scan[i];
-    N += scan[i];
+    if (i < wave) before += sh.scan[i];
+    N += sh.scan[i];
   }
   const int total = N * p.b.nkv;
   int share = (total + G - 1) / G;
@@ -878,7 +976,7 @@ __device__ __forceinline__ void tiles_body(const aos_kv_attn_params &p, int few,
   for (int i = 0; i < 2; ++i) {
     const int at = (w + i) * share;
     if (at >= total) {
-      if (tid == 0) found[2] = found[3] = 0;
+      if (tid == 0) sh.found[2] = sh.found[3] = 0;
       break;
     }
     const int hh = at / N;
@@ -891,9 +989,9 @@ __device__ __forceinline__ void tiles_body(const aos_kv_attn_params &p, int few,
         const int nt = row_tile(p, g, few, cur, x).nt, weight = nt ? nt + SETUP : 0;
         if (v < weight) {
           const int j = v - SETUP;
-          if (i == 0) at_first = cur;
-          found[2 * i] = nt - j < SNAP ? x + 1 : x;
-          found[2 * i + 1] = j < SNAP || nt - j < SNAP ? 0 : j;
+          if (i == 0) sh.at_first = cur;
+          sh.found[2 * i] = nt - j < SNAP ? x + 1 : x;
+          sh.found[2 * i + 1] = j < SNAP || nt - j < SNAP ? 0 : j;
           break;
         }
         v -= weight;
@@ -901,13 +999,12 @@ __device__ __forceinline__ void tiles_body(const aos_kv_attn_params &p, int few,
     }
   }
   __syncthreads();
-  int slot = __builtin_amdgcn_readfirstlane(found[0]), j = __builtin_amdgcn_readfirstlane(found[1]);
-  const int slot1 = __builtin_amdgcn_readfirstlane(found[2]), j1 = __builtin_amdgcn_readfirstlane(found[3]);
-  cur = at_first;
+  int slot = __builtin_amdgcn_readfirstlane(sh.found[0]), j = __builtin_amdgcn_readfirstlane(sh.found[1]);
+  const int slot1 = __builtin_amdgcn_readfirstlane(sh.found[2]), j1 = __builtin_amdgcn_readfirstlane(sh.found[3]);
+  cur = sh.at_first;
   uniform(cur);
-  /* (a scale of zero stays above it, so that what a row does not see keeps -infinity) */
   const float cs = fmaxf(fabsf(p.scale) * LOG2E, 1.17549435e-38f);
-  const uint32_t flip = p.scale < 0.0f ? 0x80008000u : 0u; /* a negative scale: negated queries */
+  const uint32_t flip = p.scale < 0.0f ? 0x80008000u : 0u; /* (both as above) */
   int pages = -1, pages_s = -1, pages_t = 0; /* pages of 64 tiles from pages_t on of a sequence, one a lane */
   for (;; ++slot, j = 0) {
     if (slot >= slots) {
@@ -1138,10 +1235,10 @@ __device__ __forceinline__ void tiles_body(const aos_kv_attn_params &p, int few,
       if (tid == 0) {
         const uint32_t old = aos_arrive(p.counters + wf);
         if (old == (uint32_t)(wl - wf + 1)) aos_reset(p.counters + wf);
-        joins = old == (uint32_t)(wl - wf + 1) ? 1 : 0;
+        sh.joins = old == (uint32_t)(wl - wf + 1) ? 1 : 0;
       }
       __syncthreads();
-      if (joins && nrows > 0) {
+      if (sh.joins && nrows > 0) {
         const int np = wl - wf + 2;
         auto part = [&](int k) { return (k == 0 ? 2 * wf - 1 : 2 * (wf + k - 1)) * PF; };
         float top = NINF;
@@ -1178,50 +1275,80 @@ __device__ __forceinline__ void tiles_body(const aos_kv_attn_params &p, int few,
   }
 }
 
-/* two bodies, so that the registers of the rare one (infinities or NaNs in the cache) stay out of the other's way */
+/* two bodies, as above */
 template <int FMT, int HDP>
 __global__ void __launch_bounds__(256, tiles_per_cu(HDP)) aos_kv_tiles_kernel(aos_kv_attn_params p, int few, int slots,
                                                                              int min_share) {
+  __shared__ TilesShared sh;
   if (*p.b.nonfinite)
-    tiles_body<FMT, HDP, true>(p, few, slots, min_share);
+    tiles_body<FMT, HDP, true>(p, few, slots, min_share, sh);
   else
-    tiles_body<FMT, HDP, false>(p, few, slots, min_share);
+    tiles_body<FMT, HDP, false>(p, few, slots, min_share, sh);
 }
 
-constexpr int ROWS_WGS = 512;
-constexpr int ROWS_FEW = 16; /* a sequence of up to this many rows is the first kernel's, in any batch */
+/* least weight of a workgroup of the first kernel: two tiles a wave, one or so where a tile has several row blocks to
+ * work on */
+constexpr int rows_share(int nb) { return nb > 2 ? 5 : 8 + ROWS_SETUP; }
+constexpr int TILES_SHARE = 8;
+
+/* Workgroups of the first kernel: as many as keep memory busy, which is one a CU where a tile is 16 KB or more (32
+ * streams of up to 8191, 8 bits: 69 us with 256, 74 with 512; 64 of up to 16001, 16 bits: 230 and 236) and two where it
+ * is less (24 of 32768, 4 bits: 147 and 122). */
+template <int FMT, int HDP>
+constexpr int rows_wgs() {
+  return tile_bytes<FMT, HDP>() >= 16384 ? 256 : 512;
+}
+
+template <int FMT, int HDP, int NB>
+int launch_rows(const aos_kv_attn_params *p, const aos_launch_ctx *ctx) { /* sequences of up to 16 NB rows */
+  /* no more workgroups than shares */
+  const long long weights = (long long)p->b.n_seqs * p->b.nkv * (p->b.max_len / TILE + 1 + ROWS_SETUP);
+  const long long wgs = (weights + rows_share(NB) - 1) / rows_share(NB), most = rows_wgs<FMT, HDP>();
+  AOS_LAUNCH(ctx, (aos_kv_rows_kernel<FMT, HDP, NB>), dim3(wgs < most ? (int)wgs : (int)most), dim3(256), 0, *p, 16 * NB,
+             rows_share(NB));
+  return (int)hipGetLastError();
+}
 
 template <int FMT, int HDP>
 int attend(const aos_kv_attn_params *p, const aos_launch_ctx *ctx) {
-  const long long g = p->nh / p->b.nkv;
-  if (p->b.max_new * g > ROWS_FEW) {
-    static int ready[64]; /* (by device: the kernel's LDS size has been allowed) */
-    int dev = 0;
-    hipError_t e = hipGetDevice(&dev);
-    if (e != hipSuccess) return (int)e;
-    if (dev < 0 || dev >= 64 || !ready[dev]) {
-      e = hipFuncSetAttribute((const void *)aos_kv_tiles_kernel<FMT, HDP>, hipFuncAttributeMaxDynamicSharedMemorySize,
-                              8 * TILE * HDP);
-      if (e != hipSuccess) return (int)e;
-      if (dev >= 0 && dev < 64) ready[dev] = 1;
-    }
-    const long long slots = (long long)p->b.n_tokens * g / TR + p->b.n_seqs;
-    if (slots * (p->b.max_len / TILE + 1 + SETUP) * p->b.nkv > 0x7fffffffll - 0x1000000) return (int)hipErrorInvalidValue;
-    AOS_LAUNCH(ctx, (aos_kv_tiles_kernel<FMT, HDP>), dim3(256 * tiles_per_cu(HDP)), dim3(256), 8 * TILE * HDP, *p,
-               ROWS_FEW, (int)slots, 8);
-    if ((e = hipGetLastError()) != hipSuccess) return (int)e;
-    if (p->b.n_seqs == 1) return 0;
+  const long long g = p->nh / p->b.nkv, rows = p->b.max_new * g;
+  /* weights are counted in 32 bits */
+  const long long slots = (long long)p->b.n_tokens * g / TR + p->b.n_seqs;
+  const long long per = p->b.max_len / TILE + 1 + (SETUP > ROWS_SETUP ? SETUP : ROWS_SETUP);
+  if (slots * per * p->b.nkv > 0x7f000000ll) return (int)hipErrorInvalidValue;
+  if (rows <= 16) return launch_rows<FMT, HDP, 1>(p, ctx);
+  if constexpr (HDP <= 128)
+    if (rows <= 32) return launch_rows<FMT, HDP, 2>(p, ctx);
+  if constexpr (HDP == 64) { /* (the registers of wider heads do not hold more) */
+    if (rows <= 48) return launch_rows<FMT, HDP, 3>(p, ctx);
+    if (rows <= 64) return launch_rows<FMT, HDP, 4>(p, ctx);
   }
-  AOS_LAUNCH(ctx, (aos_kv_rows_kernel<FMT, HDP, 1>), dim3(ROWS_WGS), dim3(256), 0, *p, ROWS_FEW, 8);
-  return (int)hipGetLastError();
+  static int ready[64]; /* (by device: the kernel's LDS size has been allowed) */
+  int dev = 0;
+  hipError_t e = hipGetDevice(&dev);
+  if (e != hipSuccess) return (int)e;
+  if (dev < 0 || dev >= 64 || !ready[dev]) {
+    e = hipFuncSetAttribute((const void *)aos_kv_tiles_kernel<FMT, HDP>, hipFuncAttributeMaxDynamicSharedMemorySize,
+                            8 * TILE * HDP);
+    if (e != hipSuccess) return (int)e;
+    if (dev >= 0 && dev < 64) ready[dev] = 1;
+  }
+  /* among several sequences, those of up to 16 rows (decoding streams among prompts) are the first kernel's. (Both
+   * bodies in one launch, half of the workgroups streaming the few rows' cache while the others multiply, spills the
+   * tile loop's registers: chunk of 512 over 15872 at 8 bits 319 us for 200, mixed batch of 32 179 for 127.) */
+  const int few = p->b.n_seqs == 1 ? 0 : 16;
+  AOS_LAUNCH(ctx, (aos_kv_tiles_kernel<FMT, HDP>), dim3(256 * tiles_per_cu(HDP)), dim3(256), 8 * TILE * HDP, *p, few,
+             (int)slots, TILES_SHARE);
+  if ((e = hipGetLastError()) != hipSuccess || !few) return (int)e;
+  return launch_rows<FMT, HDP, 1>(p, ctx);
 }
 
 }  // namespace
 
-/* the largest launch's pieces, two for each workgroup */
+/* pieces, two for each workgroup of the larger launch */
 size_t aos_kv_part_floats(int hdp) {
-  const size_t rows = 2 * (size_t)ROWS_WGS * (32 + 16 * hdp);
-  const size_t tiles = 2 * (size_t)256 * (hdp == 256 ? 1 : 2) * (256 + TR * hdp);
+  const size_t rows = 2 * 512 * (size_t)(hdp == 64 ? 4 : 2) * (32 + 16 * hdp);
+  const size_t tiles = 2 * 256 * (size_t)(hdp == 256 ? 1 : 2) * (256 + TR * hdp);
   return rows > tiles ? rows : tiles;
 }
 
