@@ -776,6 +776,7 @@ class KVCache:
         import torch
 
         self._rows, self._scale, self._dtypes = _KVRows(), head_dim ** -0.5, (torch.bfloat16, torch.int16)
+        self._device = _initialised
 
     def set_rope(self, cosines=None, sines=None) -> None:
         """Host float32 [positions, head_dim / 2]; None for both turns the rotation off."""
@@ -801,6 +802,8 @@ class KVCache:
     def _batch(self, batch: KVBatch, n: int):
         """The batch for a call over n rows."""
         c = batch.c
+        if batch.lens.get_device() != self._device:
+            raise AosError("KVCache: the batch is on another device than the cache")
         if batch.width * self.page_size < c.max_len:
             raise AosError("KVCache: the page table is too narrow for max_len")
         c.n_tokens = n
@@ -811,7 +814,7 @@ class KVCache:
         shape, stride = t.shape, t.stride()
         hd = self.head_dim
         if len(shape) != 3 or shape[0] != n or shape[2] != hd or heads and shape[1] != heads \
-                or t.dtype not in self._dtypes or not t.is_cuda \
+                or t.dtype not in self._dtypes or t.get_device() != self._device \
                 or t.numel() and (stride[2] != 1 or shape[1] > 1 and stride[1] != hd):
             raise AosError(f"KVCache: rows must be device bfloat16 tensors [{n}, {heads or 'heads'}, {hd}], the heads of "
                            "a row side by side")
@@ -841,7 +844,7 @@ class KVCache:
 
     def _bias(self, t, heads: int) -> int:
         if str(t.dtype) != "torch.float32" or t.numel() != heads * self.head_dim or not t.is_contiguous() \
-                or not t.is_cuda:
+                or t.get_device() != self._device:
             raise AosError("KVCache.append: biases must be device float32 [heads, head_dim]")
         return t.data_ptr()
 

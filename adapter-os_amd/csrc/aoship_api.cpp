@@ -3480,6 +3480,10 @@ extern "C" aoship_kv_cache_t *aoship_kv_cache_new(const aoship_kv_config_t *c) {
     return nullptr;
   }
   if (ensure_device()) return nullptr;
+  if (const int e = aos_kv_attention_prepare(c->format, hdp)) {
+    set_err(std::string("aoship_kv_cache_new: ") + hipGetErrorString((hipError_t)e));
+    return nullptr;
+  }
   auto *m = new (std::nothrow) aoship_kv_cache();
   if (!m) {
     set_err("aoship_kv_cache_new: out of host memory");
@@ -3549,8 +3553,8 @@ static int kv_batch_check(const char *what, const aoship_kv_config_t &c, int lay
   if (!b) return bad("null batch");
   if (layer < 0 || layer >= c.num_layers) return bad("layer out of range");
   if (b->n_seqs < 0 || b->n_tokens < 0 || b->max_new < 0 || b->max_len < 0) return bad("negative size in the batch");
-  if (b->max_len > (1 << 30) || b->n_seqs > (1 << 24) || b->n_tokens > (1 << 28))
-    return bad("batch too large (2^30 positions, 2^24 sequences, 2^28 rows)");
+  if (b->max_len > (1 << 30) || b->n_seqs > (1 << 20) || b->n_tokens > (1 << 26))
+    return bad("batch too large (2^30 positions, 2^20 sequences, 2^26 rows)");
   if (b->n_seqs == 0 || b->n_tokens == 0 || b->max_new == 0) return 1;
   if (!b->starts || !b->lens || (!b->pages && b->max_len > 0)) return bad("null array in the batch");
   if ((uintptr_t)b->starts % 4 || (uintptr_t)b->lens % 4 || (uintptr_t)b->pages % 4)
@@ -3636,6 +3640,14 @@ static int kv_attention_check(const aoship_kv_config_t &c, int layer, const aosh
   if (!kv_rows_ok(q, q_stride, qw) || !kv_rows_ok(out, out_stride, qw))
     return set_err(what + ": rows must be non-NULL, 16-byte aligned, with strides of at least a row and multiples of 8");
   if (q == out) return set_err(what + ": out must not be q");
+  aos_kv_batch size;
+  memset(&size, 0, sizeof(size));
+  size.nkv = c.num_kv_heads;
+  size.n_seqs = batch->n_seqs;
+  size.n_tokens = batch->n_tokens;
+  size.max_new = batch->max_new;
+  size.max_len = batch->max_len;
+  if (!aos_kv_attention_fits(&size, num_heads)) return set_err(what + ": rows times positions of the batch too large");
   return 0;
 }
 
@@ -3707,7 +3719,7 @@ extern "C" int aoship_kv_attention(aoship_kv_cache_t *m, int layer, const aoship
   p.q_ld = q_stride;
   p.out_ld = out_stride;
   p.nh = num_heads;
-  p.window = window;
+  p.window = window < batch->max_len ? window : 0; /* (a window of everything is none) */
   p.scale = scale;
   p.part = m->part.as<float>();
   p.counters = m->counters.as<uint32_t>();

@@ -717,6 +717,8 @@ extern "C" {
 int aos_launch_kv_append(const aos_kv_append_params *p, const aos_launch_ctx *ctx);
 int aos_launch_kv_read(const aos_kv_read_params *p, const aos_launch_ctx *ctx);
 int aos_launch_kv_attention(const aos_kv_attn_params *p, const aos_launch_ctx *ctx);
+int aos_kv_attention_prepare(int format, int hdp); /* once on a device before attention launches of this kind */
+int aos_kv_attention_fits(const aos_kv_batch *b, int nh); /* 1: a launch can count this batch's work */
 size_t aos_kv_part_floats(int hdp); /* workspace of an attention launch over a cache of this padded head_dim */
 size_t aos_kv_tile_bytes(int format, int hdp);
 int aos_launch_route(const aos_route_params *p, const aos_launch_ctx *ctx);

@@ -1312,10 +1312,8 @@ int launch_rows(const aos_kv_attn_params *p, const aos_launch_ctx *ctx) { /* seq
 template <int FMT, int HDP>
 int attend(const aos_kv_attn_params *p, const aos_launch_ctx *ctx) {
   const long long g = p->nh / p->b.nkv, rows = p->b.max_new * g;
-  /* weights are counted in 32 bits */
   const long long slots = (long long)p->b.n_tokens * g / TR + p->b.n_seqs;
-  const long long per = p->b.max_len / TILE + 1 + (SETUP > ROWS_SETUP ? SETUP : ROWS_SETUP);
-  if (slots * per * p->b.nkv > 0x7f000000ll) return (int)hipErrorInvalidValue;
+  if (!aos_kv_attention_fits(&p->b, p->nh)) return (int)hipErrorInvalidValue;
   if (rows <= 16) return launch_rows<FMT, HDP, 1>(p, ctx);
   if constexpr (HDP <= 128)
     if (rows <= 32) return launch_rows<FMT, HDP, 2>(p, ctx);
@@ -1323,27 +1321,32 @@ int attend(const aos_kv_attn_params *p, const aos_launch_ctx *ctx) {
     if (rows <= 48) return launch_rows<FMT, HDP, 3>(p, ctx);
     if (rows <= 64) return launch_rows<FMT, HDP, 4>(p, ctx);
   }
-  static int ready[64]; /* (by device: the kernel's LDS size has been allowed) */
-  int dev = 0;
-  hipError_t e = hipGetDevice(&dev);
-  if (e != hipSuccess) return (int)e;
-  if (dev < 0 || dev >= 64 || !ready[dev]) {
-    e = hipFuncSetAttribute((const void *)aos_kv_tiles_kernel<FMT, HDP>, hipFuncAttributeMaxDynamicSharedMemorySize,
-                            8 * TILE * HDP);
-    if (e != hipSuccess) return (int)e;
-    if (dev >= 0 && dev < 64) ready[dev] = 1;
-  }
   /* among several sequences, those of up to 16 rows (decoding streams among prompts) are the first kernel's. (Both
    * bodies in one launch, half of the workgroups streaming the few rows' cache while the others multiply, spills the
    * tile loop's registers: chunk of 512 over 15872 at 8 bits 319 us for 200, mixed batch of 32 179 for 127.) */
   const int few = p->b.n_seqs == 1 ? 0 : 16;
   AOS_LAUNCH(ctx, (aos_kv_tiles_kernel<FMT, HDP>), dim3(256 * tiles_per_cu(HDP)), dim3(256), 8 * TILE * HDP, *p, few,
              (int)slots, TILES_SHARE);
-  if ((e = hipGetLastError()) != hipSuccess || !few) return (int)e;
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess || !few) return (int)e;
   return launch_rows<FMT, HDP, 1>(p, ctx);
 }
 
+/* what a launch needs of the device beforehand: the second kernel's LDS size allowed */
+template <int FMT, int HDP>
+int prepare() {
+  return (int)hipFuncSetAttribute((const void *)aos_kv_tiles_kernel<FMT, HDP>, hipFuncAttributeMaxDynamicSharedMemorySize,
+                                  8 * TILE * HDP);
+}
+
 }  // namespace
+
+/* rows of a sequence and weights of a batch are counted in 32 bits */
+int aos_kv_attention_fits(const aos_kv_batch *b, int nh) {
+  const long long g = nh / b->nkv, slots = (long long)b->n_tokens * g / TR + b->n_seqs;
+  const long long per = b->max_len / TILE + 1 + (SETUP > ROWS_SETUP ? SETUP : ROWS_SETUP);
+  return b->max_new * g <= (1ll << 30) && slots <= (1ll << 30) && slots * per <= 0x7f000000ll / b->nkv;
+}
 
 /* pieces, two for each workgroup of the larger launch */
 size_t aos_kv_part_floats(int hdp) {
@@ -1366,3 +1369,5 @@ size_t aos_kv_part_floats(int hdp) {
 extern "C" int aos_launch_kv_attention(const aos_kv_attn_params *p, const aos_launch_ctx *ctx) {
   return KV_DISPATCH(attend, p->b.format, p->b.hdp, p, ctx);
 }
+
+extern "C" int aos_kv_attention_prepare(int format, int hdp) { return KV_DISPATCH(prepare, format, hdp); }

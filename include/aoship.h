@@ -386,13 +386,14 @@ typedef struct {
   int num_layers, num_kv_heads, head_dim, page_size, num_pages, format;
 } aoship_kv_config_t;
 
-/* The pages (zeros at first) and the attention's workspace, allocated here: no call below allocates, and all of
- * them can be captured into a graph. NULL on error. */
+/* The pages (zeros at first) and the attention's workspace (17 to 68 MB) are allocated here: append, read and attention
+ * allocate nothing and can be captured into a graph, which can be replayed any number of times. Like calls, the replays
+ * of graphs that hold one cache's calls are serialised by the caller (they share its workspace). NULL on error. */
 aoship_kv_cache_t *aoship_kv_cache_new(const aoship_kv_config_t *config);
 void aoship_kv_cache_free(aoship_kv_cache_t *cache);
 
 /* Rotary embedding of aoship_kv_append: cosines and sines [positions][head_dim / 2] (host, copied); NULL for both:
- * none, as at first. Synchronises the device. Returns 0 / -1. */
+ * none, as at first. Synchronises the device; graphs captured before hold the old tables, which are gone. Returns 0 / -1. */
 int aoship_kv_cache_set_rope(aoship_kv_cache_t *cache, const float *cosines, const float *sines, int positions);
 
 /* Stream (hipStream_t) for this cache's launches; NULL = null stream. Returns 0 / -1. */
@@ -400,8 +401,9 @@ int aoship_kv_cache_set_stream(aoship_kv_cache_t *cache, void *stream);
 
 /* What the launches found wrong in the device arrays of their batches since the last call (and clears it):
  * a combination of the bits below, 0 for nothing, -1 on error. Synchronises the device. Such a sequence is left
- * out whole (BATCH: starts that fall or pass n_tokens, more new rows than max_new, a length outside 0..max_len), or
- * the positions of such a page are (PAGE): not written, read as zeros, not attended to. */
+ * out whole, its rows of the outputs left as they are (BATCH: starts that fall or pass n_tokens, more new rows than
+ * max_new, a length outside 0..max_len; where starts does not ascend, others may be left out with it), or the positions
+ * of such a page are (PAGE): not written, read as zeros, not attended to. */
 #define AOSHIP_KV_FAULT_BATCH 1
 #define AOSHIP_KV_FAULT_PAGE 2
 int aoship_kv_cache_faults(aoship_kv_cache_t *cache);
@@ -410,8 +412,8 @@ int aoship_kv_cache_faults(aoship_kv_cache_t *cache);
  * tokens (none is fine) and holds lens[s] positions, the new ones the last of them; position i is in page
  * pages[s * page_stride + i / page_size]. Rows past starts[n_seqs] are left as they are. With fewer positions than
  * rows (a sequence padded in front), the first rows have no position: append and read skip them (their outputs are
- * left as they are) and attention gives zeros. Pages may be shared by sequences that only read them; a page that
- * two sequences of one append write holds the rows of either. starts, lens and pages are device arrays, read by the
+ * left as they are) and attention gives zeros. Pages may be shared by sequences that only read them; where two
+ * sequences of one append write into the same 16 positions of a page, what these hold is unspecified. starts, lens and pages are device arrays, read by the
  * launch; n_tokens, max_new and max_len are bounds that it is made for (so that a captured launch can be replayed
  * with other contents within them): rows of the arrays, most new rows and most positions of a sequence. */
 typedef struct {
@@ -449,7 +451,8 @@ int aoship_kv_read(aoship_kv_cache_t *cache, int layer, const aoship_kv_batch_t 
 /* Attention of the new rows (already appended) over their sequences: o = sum_j softmax_j(scale q . k_j) v_j over the
  * positions j up to the row's own p, and past p - window (0: all); query heads share key/value heads in
  * consecutive groups. A row that sees nothing gives zeros. q, out: device rows of num_heads * head_dim (out must
- * not overlap q). Asynchronous. Returns 0 / -1. */
+ * not overlap q). An infinity or a NaN reaches the rows that see its position and no others; once one has been appended
+ * to a cache's values, attention over it takes somewhat longer. Asynchronous. Returns 0 / -1. */
 int aoship_kv_attention(aoship_kv_cache_t *cache, int layer, const aoship_kv_batch_t *batch, const aoship_bf16_t *q,
                         int64_t q_stride, int num_heads, float scale, int window, aoship_bf16_t *out,
                         int64_t out_stride);

@@ -106,6 +106,74 @@ def test_rows_that_see_nothing(hip, fmt, new, lens):
     assert (got[:new[0] - lens[0]] == 0).all() and (got[-new[2]:] == 0).all()
 
 
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 30, 80, 79])
+def test_windows_past_everything(hip, window):
+    """Windows as long as the sequence or longer, with rows in front that have no position."""
+    new, lens = [12, 90, 1], [7, 80, 80]
+    pool, q, seqs = _setup(hip, "bf16", 4, 2, 64, 64, new, lens)
+    _check(_run(pool, q, new, lens, window), seqs, new, 64 ** -0.5, window)
+
+
+@pytest.mark.parametrize("fmt,new", [("bf16", 1), ("bf16", 20), ("mxfp8", 1), ("mxfp8", 20)])
+def test_far_pages(hip, fmt, new):
+    """Pages whose offset passes 32 bits, in the last layer of a cache of more than 4 GB a layer."""
+    import torch
+
+    rng = np.random.default_rng(1)
+    nh, nkv, hd, L, page = 8, 8, 128, 300, 256
+    row = 2 * nkv * (hd * 2 if fmt == "bf16" else hd + hd // 32)
+    n = (1 << 32) // (row * page) + 8
+    cache = hip.KVCache(2, nkv, hd, page, n, fmt)
+    pages = torch.tensor([[n - 1, n - 3]], dtype=torch.int32).cuda()
+    k, v = (P.bf16(rng.standard_normal((L, nkv, hd))) for _ in range(2))
+    q = P.bf16(rng.standard_normal((new, nh, hd)))
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32).cuda()  # noqa: E731
+    cache.append(1, hip.KVBatch(i32(0, L), i32(L), pages, L, L), P.to_gpu(k), P.to_gpu(v))
+    out = torch.empty((new, nh, hd), dtype=torch.bfloat16, device="cuda")
+    cache.attention(1, hip.KVBatch(i32(0, new), i32(L), pages, new, L), P.to_gpu(q), out)
+    _check(P.to_cpu(out), [(q, P.quantised(k, fmt), P.quantised(v, fmt))], [new], hd ** -0.5)
+    back = [torch.empty((L, nkv, hd), dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    cache.read(1, hip.KVBatch(i32(0, L), i32(L), pages, L, L), *back)
+    assert np.array_equal(P.to_cpu(back[0]), P.quantised(k, fmt)) and np.array_equal(P.to_cpu(back[1]), P.quantised(v, fmt))
+    assert cache.faults() == 0
+
+
+@pytest.mark.parametrize("new", [1, 3, 30])
+def test_two_caches_at_once(hip, new):
+    """Two caches' calls on two streams at the same time: each has its own workspace."""
+    import torch
+
+    lens = [3000 + new, 5000 + new]
+    made = [_setup(hip, f, 8, 1, 128, 64, [new] * 2, lens, seed=i) for i, f in enumerate(("mxfp8", "bf16"))]
+    streams = [torch.cuda.Stream() for _ in made]
+    outs, runs = [], []
+    for (pool, q, _), st in zip(made, streams):
+        outs.append(torch.empty(q.shape, dtype=torch.bfloat16, device="cuda"))
+        runs.append((pool, pool.batch([new] * 2, lens), P.to_gpu(q), outs[-1]))
+        pool.cache.set_stream(st.cuda_stream)
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for pool, batch, q, out in runs:
+            pool.cache.attention(0, batch, q, out)
+    torch.cuda.synchronize()
+    for (_, _, seqs), out in zip(made, outs):
+        _check(P.to_cpu(out), seqs, [new] * 2, 128 ** -0.5)
+
+
+def test_pages_shared_by_readers(hip):
+    """Sequences with a common prefix read the same pages."""
+    import torch
+
+    new, L, nh, hd = [1, 1, 60], 190, 4, 64
+    pool, q, seqs = _setup(hip, "mxfp8", nh, 2, hd, 64, [1], [L])
+    pool.pages = pool.pages.expand(3, -1).contiguous()
+    rng = np.random.default_rng(8)
+    q = P.bf16(rng.standard_normal((62, nh, hd)))
+    _, k, v = seqs[0]
+    lens = [130, L, 128]
+    _check(_run(pool, q, new, lens), [(q[:1], k[:130], v[:130]), (q[1:2], k, v), (q[2:], k[:128], v[:128])], new, hd ** -0.5)
+
+
 @pytest.mark.parametrize("fmt", P.FORMATS)
 @pytest.mark.parametrize("new", [1, 4, 90])
 def test_infinities_and_nans(hip, fmt, new):

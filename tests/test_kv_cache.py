@@ -60,7 +60,7 @@ def test_good_calls_pass():
 BAD_BATCHES = [dict(n_seqs=-1), dict(n_tokens=-1), dict(max_new=-1), dict(max_len=-1), dict(max_len=641),
                dict(starts=None), dict(lens=None), dict(pages=None), dict(starts=ALIGNED + 2), dict(pages=ALIGNED + 1),
                dict(page_stride=9), dict(page_stride=-1), dict(max_len=(1 << 30) + 1, page_stride=1 << 25),
-               dict(n_seqs=(1 << 24) + 1), dict(n_tokens=(1 << 28) + 1)]
+               dict(n_seqs=(1 << 20) + 1), dict(n_tokens=(1 << 26) + 1)]
 
 
 @pytest.mark.parametrize("kw", BAD_BATCHES, ids=lambda k: "-".join(k))
@@ -98,6 +98,15 @@ def test_other_refusals():
     assert _attention(nh=6) == -1 and _attention(nh=0) == -1 and _attention(window=-1) == -1
     assert _attention(scale=float("nan")) == -1 and _attention(scale=float("inf")) == -1
     assert _attention(out=ALIGNED) == -1 and _attention(out=None) == -1 and _attention(os=1020) == -1
+
+
+def test_batches_whose_work_cannot_be_counted():
+    big = dict(max_len=1 << 30, page_stride=1 << 24)
+    assert _attention(batch=_batch(n_seqs=1, n_tokens=1, max_new=1, **big)) == 0
+    assert _attention(batch=_batch(n_seqs=64, n_tokens=64, max_new=1, **big)) == -1 and "too large" in aoship.last_error()
+    assert _append(batch=_batch(n_seqs=64, n_tokens=64, max_new=1, **big)) == 0  # (attention only)
+    assert _attention(batch=_batch(n_seqs=1, n_tokens=1 << 20, max_new=1 << 20, max_len=1 << 20, page_stride=1 << 14)) == 0
+    assert _attention(batch=_batch(n_seqs=1, n_tokens=1 << 26, max_new=1 << 26, max_len=1 << 26, page_stride=1 << 20)) == -1
 
 
 def test_shapes_that_a_cache_refuses():
