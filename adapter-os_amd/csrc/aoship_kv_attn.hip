@@ -929,7 +929,7 @@ __device__ __forceinline__ RowTile row_tile(const aos_kv_attn_params &p, int g, 
   return o;
 }
 
-constexpr int SETUP = 3; /* weight of a row tile beside its position tiles */
+constexpr int SETUP = 4; /* weight of a row tile beside its position tiles */
 
 struct TilesShared {
   int scan[4], found[4], joins;
@@ -1286,10 +1286,11 @@ __global__ void __launch_bounds__(256, tiles_per_cu(HDP)) aos_kv_tiles_kernel(ao
     tiles_body<FMT, HDP, false>(p, few, slots, min_share, sh);
 }
 
-/* least weight of a workgroup of the first kernel: two tiles a wave, one or so where a tile has several row blocks to
- * work on */
-constexpr int rows_share(int nb) { return nb > 2 ? 5 : 8 + ROWS_SETUP; }
-constexpr int TILES_SHARE = 8;
+/* Least weight of a workgroup of the first kernel: a whole row tile where the batch's longest sequence has few position
+ * tiles, else one or two tiles a wave (28 heads of 128 over 4, one token: 512 positions 9.0 us whole and 11.5 cut, 1280
+ * positions 12.3 and 12.6; 2000 positions 14.3 us in shares of 13 and 12.9 in shares of 6). */
+constexpr int rows_share(int nb, int tiles) { return tiles <= 24 / nb ? tiles + ROWS_SETUP : 6; }
+constexpr int TILES_SHARE = 6; /* (prompt of 300, 28 heads of 128: 24 us, 29 with 8, 31 with 12) */
 
 /* Workgroups of the first kernel: as many as keep memory busy, which is one a CU where a tile is 16 KB or more (32
  * streams of up to 8191, 8 bits: 69 us with 256, 74 with 512; 64 of up to 16001, 16 bits: 230 and 236) and two where it
@@ -1302,10 +1303,11 @@ constexpr int rows_wgs() {
 template <int FMT, int HDP, int NB>
 int launch_rows(const aos_kv_attn_params *p, const aos_launch_ctx *ctx) { /* sequences of up to 16 NB rows */
   /* no more workgroups than shares */
-  const long long weights = (long long)p->b.n_seqs * p->b.nkv * (p->b.max_len / TILE + 1 + ROWS_SETUP);
-  const long long wgs = (weights + rows_share(NB) - 1) / rows_share(NB), most = rows_wgs<FMT, HDP>();
+  const int tiles = (p->b.max_len + TILE - 1) / TILE, share = rows_share(NB, tiles);
+  const long long weights = (long long)p->b.n_seqs * p->b.nkv * (tiles + 1 + ROWS_SETUP);
+  const long long wgs = (weights + share - 1) / share, most = rows_wgs<FMT, HDP>();
   AOS_LAUNCH(ctx, (aos_kv_rows_kernel<FMT, HDP, NB>), dim3(wgs < most ? (int)wgs : (int)most), dim3(256), 0, *p, 16 * NB,
-             rows_share(NB));
+             share);
   return (int)hipGetLastError();
 }
 
