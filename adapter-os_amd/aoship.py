@@ -167,6 +167,8 @@ def lib():
         L.aoship_internal_layer_set_gemv_geometry.argtypes = [_P, C.c_int, C.c_int, C.c_int]
         L.aoship_internal_layer_set_mlp1.restype = C.c_int
         L.aoship_internal_layer_set_mlp1.argtypes = [_P, C.c_int]
+        L.aoship_internal_kv_cache_set_small_batches.restype = C.c_int
+        L.aoship_internal_kv_cache_set_small_batches.argtypes = [_P, C.c_int]
         L.aoship_internal_set_spin_limit.restype = C.c_int
         L.aoship_internal_set_spin_limit.argtypes = [C.c_uint32]
         _lib = L
@@ -798,6 +800,11 @@ class KVCache:
         if f < 0:
             raise AosError(f"aoship_kv_cache_faults: {last_error()}")
         return f
+
+    def set_small_batches(self, on: bool) -> None:
+        """Diagnostic: False has attention take the kernels of large batches at any size."""
+        _check(lib().aoship_internal_kv_cache_set_small_batches(self.h, 1 if on else 0),
+               "aoship_internal_kv_cache_set_small_batches")
 
     def _batch(self, batch: KVBatch, n: int):
         """The batch for a call over n rows."""

@@ -706,6 +706,7 @@ typedef struct {
   long long q_ld, out_ld;
   int nh, window; /* window 0: none */
   float scale;
+  int no_small;       /* diagnostic: no batch counts as small */
   float *part;        /* pieces of cut row tiles (aos_kv_part_floats) */
   uint32_t *counters; /* [AOS_KV_MAX_WGS], zero between launches */
 } aos_kv_attn_params;

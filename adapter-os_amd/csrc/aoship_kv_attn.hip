@@ -77,23 +77,11 @@ __device__ __forceinline__ u32x4 decode8(const uint32_t *w, float scale) {
                  __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[0], scale, 3))};
   }
 }
-/* Scale byte j of a word as its power of two; 255 gives infinity, which times its zero codes is NaN. One instruction
- * that selects the byte and shifts it (the compiler makes two of it: 64 more of a 4-bit tile's about 650). */
-template <int J>
-__device__ __forceinline__ float byte_scale(uint32_t w) {
-  uint32_t r;
-  if constexpr (J == 0)
-    asm("v_lshlrev_b32_sdwa %0, %1, %2 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:DWORD src1_sel:BYTE_0" : "=v"(r) : "v"(23), "v"(w));
-  else if constexpr (J == 1)
-    asm("v_lshlrev_b32_sdwa %0, %1, %2 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:DWORD src1_sel:BYTE_1" : "=v"(r) : "v"(23), "v"(w));
-  else if constexpr (J == 2)
-    asm("v_lshlrev_b32_sdwa %0, %1, %2 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:DWORD src1_sel:BYTE_2" : "=v"(r) : "v"(23), "v"(w));
-  else
-    asm("v_lshlrev_b32_sdwa %0, %1, %2 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:DWORD src1_sel:BYTE_3" : "=v"(r) : "v"(23), "v"(w));
-  return __builtin_bit_cast(float, r);
-}
-__device__ __forceinline__ float byte_scale(uint32_t w, int j) { /* (j constant once unrolled) */
-  return j == 0 ? byte_scale<0>(w) : j == 1 ? byte_scale<1>(w) : j == 2 ? byte_scale<2>(w) : byte_scale<3>(w);
+/* Scale byte j of a word (constant once unrolled) as its power of two; 255 gives infinity, which times its zero codes is
+ * NaN. Plain operations, two where one that selects a byte would do (24 streams of 32768 at 4 bits: 126 us and 124): beside matrix instructions the compiler
+ * places wait states for what it knows, not for an asm statement. */
+__device__ __forceinline__ float byte_scale(uint32_t w, int j) {
+  return __builtin_bit_cast(float, (w >> 8 * j & 255u) << 23);
 }
 
 /* Infinities and NaNs among the values. In a tile that a row sees only in part, the product of such a value with a
@@ -369,7 +357,7 @@ __device__ __forceinline__ void rows_body(const aos_kv_attn_params &p, int few, 
       }
     }
     const int t_first = r0 / g, t_last = (r0 + nrows - 1) / g;
-    const int hi_min = p0 + t_first;
+    const int hi_min = p0 + t_first, hi_max = p0 + t_last;
     const int lo_max = p.window > 0 && p0 + t_last - p.window + 1 > 0 ? p0 + t_last - p.window + 1 : 0;
 
     f32x4 o[NB][DB];
@@ -385,7 +373,8 @@ __device__ __forceinline__ void rows_body(const aos_kv_attn_params &p, int few, 
     OddMarks<NB * DB * 4> marks;
     if constexpr (MARK) marks.clear();
 
-    const int mine = (n - wave + 3) / 4; /* tiles of this wave: j + wave, j + wave + 4, ... */
+    /* tiles of this wave: j + wave, j + wave + 4, ..., up to the last that the row tile sees */
+    const int sees = hi_max / TILE - x.t0 + 1 - j, mine = ((sees < n && hi_max >= 0 ? sees : n) - wave + 3) / 4;
     for (int i0 = 0; i0 < mine; i0 += 64) {
       const int cnt = mine - i0 < 64 ? mine - i0 : 64;
       /* the pages of the next 64 tiles, one a lane */
@@ -1301,28 +1290,35 @@ constexpr int rows_wgs() {
 }
 
 template <int FMT, int HDP, int NB>
-int launch_rows(const aos_kv_attn_params *p, const aos_launch_ctx *ctx) { /* sequences of up to 16 NB rows */
-  /* no more workgroups than shares */
+int launch_rows(const aos_kv_attn_params *p, const aos_launch_ctx *ctx, int few) { /* sequences of up to `few` rows */
   const int tiles = (p->b.max_len + TILE - 1) / TILE, share = rows_share(NB, tiles);
-  const long long weights = (long long)p->b.n_seqs * p->b.nkv * (tiles + 1 + ROWS_SETUP);
+  /* no more workgroups than shares */
+  const long long rts = (long long)p->b.n_tokens * (p->nh / p->b.nkv) / (16 * NB) + p->b.n_seqs;
+  const long long weights = rts * p->b.nkv * (tiles + 1 + ROWS_SETUP);
   const long long wgs = (weights + share - 1) / share, most = rows_wgs<FMT, HDP>();
-  AOS_LAUNCH(ctx, (aos_kv_rows_kernel<FMT, HDP, NB>), dim3(wgs < most ? (int)wgs : (int)most), dim3(256), 0, *p, 16 * NB,
+  AOS_LAUNCH(ctx, (aos_kv_rows_kernel<FMT, HDP, NB>), dim3(wgs < most ? (int)wgs : (int)most), dim3(256), 0, *p, few,
              share);
   return (int)hipGetLastError();
 }
+
+/* Up to so many (16-row block, key/value head, position tile) of a batch, and bytes of cache read for them, every sequence
+ * goes to the first kernel in blocks of 16 rows, each reading the cache for itself: small batches gain more from many
+ * workgroups than they lose by reading again. Rows of 16, and in blocks that share a tile or in the second kernel: 12
+ * streams x 5 tokens of 7 rows over 2000, heads of 64: 14.3 us and 17.4; 8 x 8 x 7 over 1000, heads of 128: 17 and 28; a
+ * prompt of 300 x 7: 22 and 24; 4 x 100 x 3 over 600, 4 bits: 25 and 33. Beyond: a prompt of 420 x 7: 29 and 24; 8 x 4 x 7
+ * over 8000: 48 and 34; 32 x 8 x 7 over 8000, heads of 64: 81 and 40. */
+constexpr long long SMALL_UNITS = 12288, SMALL_BYTES = 160000000;
 
 template <int FMT, int HDP>
 int attend(const aos_kv_attn_params *p, const aos_launch_ctx *ctx) {
   const long long g = p->nh / p->b.nkv, rows = p->b.max_new * g;
   const long long slots = (long long)p->b.n_tokens * g / TR + p->b.n_seqs;
   if (!aos_kv_attention_fits(&p->b, p->nh)) return (int)hipErrorInvalidValue;
-  if (rows <= 16) return launch_rows<FMT, HDP, 1>(p, ctx);
-  if constexpr (HDP <= 128)
-    if (rows <= 32) return launch_rows<FMT, HDP, 2>(p, ctx);
-  if constexpr (HDP == 64) { /* (the registers of wider heads do not hold more) */
-    if (rows <= 48) return launch_rows<FMT, HDP, 3>(p, ctx);
-    if (rows <= 64) return launch_rows<FMT, HDP, 4>(p, ctx);
-  }
+  const long long units = ((long long)p->b.n_tokens * g / 16 + p->b.n_seqs) * p->b.nkv * ((p->b.max_len + TILE - 1) / TILE);
+  if (rows <= 16 || (!p->no_small && units <= SMALL_UNITS && units * tile_bytes<FMT, HDP>() <= SMALL_BYTES))
+    return launch_rows<FMT, HDP, 1>(p, ctx, 0x7fffffff);
+  if constexpr (HDP <= 128) /* (the registers of wider heads do not hold two blocks) */
+    if (rows <= 32) return launch_rows<FMT, HDP, 2>(p, ctx, 32);
   /* among several sequences, those of up to 16 rows (decoding streams among prompts) are the first kernel's. (Both
    * bodies in one launch, half of the workgroups streaming the few rows' cache while the others multiply, spills the
    * tile loop's registers: chunk of 512 over 15872 at 8 bits 319 us for 200, mixed batch of 32 179 for 127.) */
@@ -1331,7 +1327,7 @@ int attend(const aos_kv_attn_params *p, const aos_launch_ctx *ctx) {
              (int)slots, TILES_SHARE);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || !few) return (int)e;
-  return launch_rows<FMT, HDP, 1>(p, ctx);
+  return launch_rows<FMT, HDP, 1>(p, ctx, few);
 }
 
 /* what a launch needs of the device beforehand: the second kernel's LDS size allowed */
@@ -1352,7 +1348,7 @@ int aos_kv_attention_fits(const aos_kv_batch *b, int nh) {
 
 /* pieces, two for each workgroup of the larger launch */
 size_t aos_kv_part_floats(int hdp) {
-  const size_t rows = 2 * 512 * (size_t)(hdp == 64 ? 4 : 2) * (32 + 16 * hdp);
+  const size_t rows = 2 * 512 * 2 * (size_t)(32 + 16 * hdp);
   const size_t tiles = 2 * 256 * (size_t)(hdp == 256 ? 1 : 2) * (256 + TR * hdp);
   return rows > tiles ? rows : tiles;
 }

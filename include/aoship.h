@@ -386,7 +386,7 @@ typedef struct {
   int num_layers, num_kv_heads, head_dim, page_size, num_pages, format;
 } aoship_kv_config_t;
 
-/* The pages (zeros at first) and the attention's workspace (17 to 68 MB) are allocated here: append, read and attention
+/* The pages (zeros at first) and the attention's workspace (35 to 68 MB) are allocated here: append, read and attention
  * allocate nothing and can be captured into a graph, which can be replayed any number of times. Like calls, the replays
  * of graphs that hold one cache's calls are serialised by the caller (they share its workspace). NULL on error. */
 aoship_kv_cache_t *aoship_kv_cache_new(const aoship_kv_config_t *config);

@@ -8,6 +8,18 @@ import kv_plain as P
 pytestmark = pytest.mark.gpu
 
 
+@pytest.fixture(autouse=True, params=[True, False], ids=["small", "large"])
+def kernels(request, hip, monkeypatch):
+    """Every test with the kernels that its sizes choose, and with those of large batches."""
+    if not request.param:
+        class Large(hip.KVCache):
+            def __init__(self, *a):
+                super().__init__(*a)
+                self.set_small_batches(False)
+
+        monkeypatch.setattr(hip, "KVCache", Large)
+
+
 def _setup(hip, fmt, nh, nkv, hd, page, new, lens, seed=0, sharp=1.0, poison=None):
     """A cache of sequences whose rows are random, and queries for their last `new` positions."""
     rng = np.random.default_rng(seed)
@@ -76,7 +88,19 @@ def test_chunks(hip, fmt, nh, nkv, hd, page, window):
 
 
 @pytest.mark.parametrize("fmt", P.FORMATS)
-@pytest.mark.parametrize("new,lens", [([1], [9001]), ([5], [20011]), ([300], [3001]), ([700], [700]), ([1, 1], [64, 40000])])
+@pytest.mark.parametrize("nh,nkv,hd,page", [(14, 2, 64, 64), (28, 4, 128, 128), (6, 1, 80, 64), (12, 2, 256, 64)])
+@pytest.mark.parametrize("window", [0, 33])
+def test_drafted(hip, fmt, nh, nkv, hd, page, window):
+    """Up to 28 rows a sequence: one and two blocks of a matrix instruction's columns, the second in part or empty."""
+    new = [4, 1, 3, 0, 2, 4]
+    lens = [70, 1, 3, 9, 700, 64]
+    pool, q, seqs = _setup(hip, fmt, nh, nkv, hd, page, new, lens, seed=hd + window)
+    _check(_run(pool, q, new, lens, window), seqs, new, hd ** -0.5, window)
+
+
+@pytest.mark.parametrize("fmt", P.FORMATS)
+@pytest.mark.parametrize("new,lens", [([1], [9001]), ([3], [30001]), ([5], [20011]), ([300], [3001]), ([700], [700]),
+                                      ([1, 1], [64, 40000])])
 def test_long(hip, fmt, new, lens):
     """Row tiles that many workgroups share, and uneven lengths."""
     pool, q, seqs = _setup(hip, fmt, 7, 1, 128, 256, new, lens, seed=lens[-1], sharp=3.0)
@@ -97,7 +121,7 @@ def test_many_sequences(hip, n, new):
 
 
 @pytest.mark.parametrize("fmt", P.FORMATS)
-@pytest.mark.parametrize("new,lens", [([6, 4, 1], [2, 0, 0]), ([40, 90, 3], [10, 70, 0])])
+@pytest.mark.parametrize("new,lens", [([6, 4, 1], [2, 0, 0]), ([12, 16, 2], [9, 3, 0]), ([40, 90, 3], [10, 70, 0])])
 def test_rows_that_see_nothing(hip, fmt, new, lens):
     """Sequences padded in front, and rows of a sequence without positions: zeros."""
     pool, q, seqs = _setup(hip, fmt, 4, 2, 128, 64, new, lens)
@@ -175,7 +199,7 @@ def test_pages_shared_by_readers(hip):
 
 
 @pytest.mark.parametrize("fmt", P.FORMATS)
-@pytest.mark.parametrize("new", [1, 4, 90])
+@pytest.mark.parametrize("new", [1, 4, 14, 90])
 def test_infinities_and_nans(hip, fmt, new):
     """Visible ones reach the rows that see them, by the formula; those of later positions, of positions left of the
     window and of stale rows in a page reach nobody."""
@@ -233,7 +257,7 @@ def test_bad_pages_and_rows(hip):
     reported and neighbours are served."""
     import torch
 
-    for new in ([1, 1, 1], [1, 100, 40]):
+    for new in ([1, 1, 1], [1, 12, 9], [1, 100, 40]):
         lens, nh, hd = [70, 200, 90], 4, 64
         pool, q, seqs = _setup(hip, "bf16", nh, 2, hd, 64, new, lens)
         pool.pages[1, 1] = 10 ** 7
