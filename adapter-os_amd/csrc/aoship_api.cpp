@@ -3501,6 +3501,13 @@ extern "C" aoship_kv_cache_t *aoship_kv_cache_new(const aoship_kv_config_t *c) {
     delete m;
     return nullptr;
   }
+  /* (the first launch may be on a stream that does not wait for the null stream's fills) */
+  const hipError_t done = hipDeviceSynchronize();
+  if (done != hipSuccess) {
+    set_err(std::string("aoship_kv_cache_new: ") + hipGetErrorString(done));
+    delete m;
+    return nullptr;
+  }
   return m;
 }
 
@@ -3529,6 +3536,7 @@ extern "C" int aoship_kv_cache_set_rope(aoship_kv_cache_t *m, const float *cosin
   if (m->rope.alloc(2 * table, false)) return -1;
   HIP_OR_FAIL(hipMemcpy(m->rope.p, cosines, table, hipMemcpyHostToDevice), "hipMemcpy H2D");
   HIP_OR_FAIL(hipMemcpy(m->rope.as<unsigned char>() + table, sines, table, hipMemcpyHostToDevice), "hipMemcpy H2D");
+  HIP_OR_FAIL(hipDeviceSynchronize(), "hipDeviceSynchronize");
   m->rope_positions = positions;
   return 0;
 }
@@ -3544,7 +3552,10 @@ extern "C" int aoship_kv_cache_faults(aoship_kv_cache_t *m) {
   HIP_OR_FAIL(hipDeviceSynchronize(), "hipDeviceSynchronize");
   uint32_t f = 0;
   HIP_OR_FAIL(hipMemcpy(&f, m->faults.p, sizeof(f), hipMemcpyDeviceToHost), "hipMemcpy D2H");
-  if (f) HIP_OR_FAIL(hipMemset(m->faults.p, 0, sizeof(f)), "hipMemset");
+  if (f) {
+    HIP_OR_FAIL(hipMemset(m->faults.p, 0, sizeof(f)), "hipMemset");
+    HIP_OR_FAIL(hipDeviceSynchronize(), "hipDeviceSynchronize");
+  }
   return (int)f;
 }
 

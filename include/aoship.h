@@ -393,7 +393,8 @@ aoship_kv_cache_t *aoship_kv_cache_new(const aoship_kv_config_t *config);
 void aoship_kv_cache_free(aoship_kv_cache_t *cache);
 
 /* Rotary embedding of aoship_kv_append: cosines and sines [positions][head_dim / 2] (host, copied); NULL for both:
- * none, as at first. Synchronises the device; graphs captured before hold the old tables, which are gone. Returns 0 / -1. */
+ * none, as at first. Synchronises the device; graphs captured before hold the old tables, which are gone.
+ * Returns 0 / -1. */
 int aoship_kv_cache_set_rope(aoship_kv_cache_t *cache, const float *cosines, const float *sines, int positions);
 
 /* Stream (hipStream_t) for this cache's launches; NULL = null stream. Returns 0 / -1. */
@@ -413,9 +414,10 @@ int aoship_kv_cache_faults(aoship_kv_cache_t *cache);
  * pages[s * page_stride + i / page_size]. Rows past starts[n_seqs] are left as they are. With fewer positions than
  * rows (a sequence padded in front), the first rows have no position: append and read skip them (their outputs are
  * left as they are) and attention gives zeros. Pages may be shared by sequences that only read them; where two
- * sequences of one append write into the same 16 positions of a page, what these hold is unspecified. starts, lens and pages are device arrays, read by the
- * launch; n_tokens, max_new and max_len are bounds that it is made for (so that a captured launch can be replayed
- * with other contents within them): rows of the arrays, most new rows and most positions of a sequence. */
+ * sequences of one append write into the same 16 positions of a page, what these hold is unspecified. starts, lens and
+ * pages are device arrays, read by the launch; n_tokens, max_new and max_len are bounds that it is made for (so that a
+ * captured launch can be replayed with other contents within them): rows of the arrays, most new rows and most positions
+ * of a sequence. */
 typedef struct {
   int n_seqs, n_tokens, max_new, max_len;
   const int32_t *starts; /* [n_seqs + 1] */

@@ -236,3 +236,32 @@ def test_binding_refuses_wrong_tensors(hip):
     pool.cache.set_rope()
     pool.cache.append(0, b, ok, ok)
     assert pool.cache.faults() == 0
+
+
+def test_a_new_cache_on_another_stream(hip):
+    """The first append to a large cache, on a stream that does not wait for the null stream, is not undone by the pages'
+    first zeros; the same with the rotary tables."""
+    import torch
+
+    rng = np.random.default_rng(4)
+    nkv, hd, n = 8, 128, 200
+    x = [P.bf16(rng.standard_normal((n, nkv, hd))) for _ in range(2)]
+    k, v = map(P.to_gpu, x)
+    back = [torch.zeros_like(k) for _ in range(2)]
+    i32 = lambda *a: torch.tensor(a, dtype=torch.int32).cuda()  # noqa: E731
+    side = torch.cuda.Stream()
+    pages = 8 * (1 << 30) // (2 * nkv * hd * 2 * 256)
+    batch = hip.KVBatch(i32(0, n), i32(n), i32(pages - 1).view(1, 1), n, n)
+    torch.cuda.synchronize()
+    cache = hip.KVCache(1, nkv, hd, 256, pages, "bf16")
+    cache.set_stream(side.cuda_stream)
+    cache.append(0, batch, k, v)
+    torch.cuda.synchronize()
+    cache.read(0, batch, *back)
+    torch.cuda.synchronize()
+    assert all(np.array_equal(P.to_cpu(b), y) for b, y in zip(back, x))
+    cache.set_rope(-np.ones((n, hd // 2), np.float32), np.zeros((n, hd // 2), np.float32))
+    cache.append(0, batch, k, v)
+    cache.read(0, batch, *back)
+    torch.cuda.synchronize()
+    assert np.array_equal(P.to_cpu(back[0]), -x[0]) and np.array_equal(P.to_cpu(back[1]), x[1])
