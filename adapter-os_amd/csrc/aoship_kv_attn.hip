@@ -78,8 +78,8 @@ __device__ __forceinline__ u32x4 decode8(const uint32_t *w, float scale) {
   }
 }
 /* Scale byte j of a word (constant once unrolled) as its power of two; 255 gives infinity, which times its zero codes is
- * NaN. Plain operations, two where one that selects a byte would do (24 streams of 32768 at 4 bits: 126 us and 124): beside matrix instructions the compiler
- * places wait states for what it knows, not for an asm statement. */
+ * NaN. Plain operations, two where one that selects a byte would do (24 streams of 32768 at 4 bits: 126 us and 124):
+ * beside matrix instructions the compiler places wait states for what it knows, not for an asm statement. */
 __device__ __forceinline__ float byte_scale(uint32_t w, int j) {
   return __builtin_bit_cast(float, (w >> 8 * j & 255u) << 23);
 }
@@ -177,7 +177,13 @@ constexpr int SNAP = 3;
  * the row 4 j + i of block b is made position 16 j + 4 b + i, so a lane's scores are the 16 consecutive positions
  * 16 quad ..+15, which is what the value units hold: the probabilities never cross lanes. Probabilities are rounded
  * to bfloat16 for the second product (half a unit of 8 bits each, like the output's own rounding); sums are float32.
- * In the quantised formats the value scales multiply the probabilities (exactly: powers of two). */
+ * In the quantised formats the value scales multiply the probabilities (exactly: powers of two).
+ *
+ * Bound by reading the cache once, by latency where that is little. Keys and values go straight to registers, the next
+ * tile's on their way while one is worked on: a tile is used by one workgroup's one or two matrix instructions a block,
+ * which LDS would not speed up. 64 streams of up to 16001 positions, 28/4 heads of 128: 16 bits 228 us, 5.7 TB/s; 32 of up
+ * to 8191, 24/8 heads, 8 bits: 73 us, 4.6 TB/s; 24 of 32768, 40/8 heads, 4 bits: 122 us, 4.7 TB/s (a decoded tile is some
+ * 470 vector instructions). */
 template <int FMT, int HDP>
 struct Tile { /* a tile's keys and values in registers */
   static constexpr int KW = HDP * bits<FMT>() / 128; /* words of a key row's quarter */
@@ -720,7 +726,11 @@ __global__ void __launch_bounds__(256, rows_waves(FMT, HDP, NB)) aos_kv_rows_ker
  * by register: what the value pieces hold, so the probabilities never cross lanes here either.
  *
  * The workgroups share all (key/value head, row tile, position tile) evenly; where a row tile is cut, its pieces meet
- * as in the kernel above. Neighbouring shares, which read the same keys, go to one XCD. */
+ * as in the kernel above. Neighbouring shares, which read the same keys, go to one XCD.
+ *
+ * Bound by the matrix cores. Prompt of 4076 tokens, 28/4 heads of 128, 16 bits: 141 us, 850 TFLOP/s (long prompts 1000, a
+ * large library product 1140 on the same card); 512 tokens over 15872, 40/8 heads, 8 bits: 200 us, 850 TFLOP/s. With
+ * fragments read from LDS just before each matrix instruction 200 us for 151, with row tiles dealt whole 210. */
 constexpr int TR = 128;         /* rows of a row tile */
 constexpr int tiles_per_cu(int hdp) { return hdp == 256 ? 1 : 2; }
 
