@@ -777,7 +777,8 @@ class KVCache:
         self.num_kv_heads, self.head_dim, self.page_size = num_kv_heads, head_dim, page_size
         import torch
 
-        self._rows, self._scale, self._dtypes = _KVRows(), head_dim ** -0.5, (torch.bfloat16, torch.int16)
+        self._rows, self._scale = _KVRows(), head_dim ** -0.5
+        self._dtypes, self._f32 = (torch.bfloat16, torch.int16), torch.float32
         self._device = _initialised
 
     def set_rope(self, cosines=None, sines=None) -> None:
@@ -818,11 +819,10 @@ class KVCache:
 
     def _row(self, t, n: int, heads: int = 0) -> tuple[int, int]:
         """(pointer, row stride) of a row tensor [n, heads, head_dim], checked (heads 0: any)."""
-        shape, stride = t.shape, t.stride()
-        hd = self.head_dim
-        if len(shape) != 3 or shape[0] != n or shape[2] != hd or heads and shape[1] != heads \
-                or t.dtype not in self._dtypes or t.get_device() != self._device \
-                or t.numel() and (stride[2] != 1 or shape[1] > 1 and stride[1] != hd):
+        hd, shape, stride = self.head_dim, t.shape, t.stride()
+        if len(shape) != 3 or shape != (n, heads or shape[1], hd) or t.dtype not in self._dtypes \
+                or t.get_device() != self._device \
+                or stride[1:] != (hd, 1) and t.numel() and (stride[2] != 1 or shape[1] > 1 and stride[1] != hd):
             raise AosError(f"KVCache: rows must be device bfloat16 tensors [{n}, {heads or 'heads'}, {hd}], the heads of "
                            "a row side by side")
         return t.data_ptr(), stride[0] if n > 1 else shape[1] * hd
@@ -841,7 +841,7 @@ class KVCache:
         else:
             r.q, r.q_stride = self._row(q, n)
             nh = q.shape[1]
-            r.q_out, r.q_out_stride = self._row(q_out, n, nh)
+            r.q_out, r.q_out_stride = (r.q, r.q_stride) if q_out is q else self._row(q_out, n, nh)
         r.num_heads = nh
         r.q_bias = None if q_bias is None else self._bias(q_bias, nh)
         r.k_bias = None if k_bias is None else self._bias(k_bias, nkv)
@@ -850,7 +850,7 @@ class KVCache:
             raise AosError(f"aoship_kv_append: {last_error()}")
 
     def _bias(self, t, heads: int) -> int:
-        if str(t.dtype) != "torch.float32" or t.numel() != heads * self.head_dim or not t.is_contiguous() \
+        if t.dtype is not self._f32 or t.numel() != heads * self.head_dim or not t.is_contiguous() \
                 or t.get_device() != self._device:
             raise AosError("KVCache.append: biases must be device float32 [heads, head_dim]")
         return t.data_ptr()
