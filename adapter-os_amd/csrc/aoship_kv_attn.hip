@@ -25,6 +25,9 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 constexpr int SC1 = 16; /* buffer cache policy: device-coherent (sc1) */
 constexpr float LOG2E = 1.44269504f;
 constexpr float NINF = -__builtin_inff();
+/* Running maximum of a row that has seen positions, whose scores were all minus infinity: its sum of zero makes it NaN,
+ * that of a row that has seen nothing (NINF) zeros. */
+constexpr float LEAST = -3.40282347e38f;
 /* The running maximum of a row follows its scores only once they pass it by 2^SLACK (probabilities up to 256, an exact
  * power of two from what the true maximum would give): the accumulators are hardly ever rescaled. */
 constexpr float SLACK = 8.0f;
@@ -56,6 +59,9 @@ __device__ __forceinline__ float quad_sum(float x) {
   const uint32_t v = __builtin_bit_cast(uint32_t, y);
   const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
   return __builtin_bit_cast(float, (uint32_t)b[0]) + __builtin_bit_cast(float, (uint32_t)b[1]);
+}
+__device__ __forceinline__ float inverse(float sum, float m) {
+  return sum != 0.0f ? 1.0f / sum : m == NINF ? 0.0f : __builtin_nanf("");
 }
 /* exponent base of a running maximum: a row that has seen nothing yet keeps its zero sum free of inf - inf */
 __device__ __forceinline__ float safe_max(float m) { return m == NINF ? 0.0f : m; }
@@ -448,6 +454,7 @@ __device__ __forceinline__ void rows_body(const aos_kv_attn_params &p, int few, 
               mx = fmaxf(mx, sc[b][k >> 2][k & 3]);
             }
             mx = quad_max(mx) * cs;
+            if (!masks || (there && lo[b] < tb + TILE && hi[b] >= tb)) mx = fmaxf(mx, LEAST);
             if (__ballot(mx > m[b] + SLACK)) {
               const float top = fmaxf(m[b], mx), alpha = ex2(m[b] - safe_max(top));
               l[b] = l[b] * alpha;
@@ -596,8 +603,7 @@ __device__ __forceinline__ void rows_body(const aos_kv_attn_params &p, int few, 
     for (int b = 0; b < NB; ++b) l[b] = quad_sum(l[b]);
     if (n > 1) join_waves(); /* (one tile is wave 0's) */
 
-    auto put = [&](int b, int d, f32x4 y, float sum) {
-      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum; /* a row that sees nothing: zeros */
+    auto put = [&](int b, int d, f32x4 y, float inv) {
       const int at = 16 * d + 4 * quad;
       if (16 * b + col < nrows && at < p.b.hd)
         *(u32x2 *)(p.out + orow[b] + at) = u32x2{pack_bf16(y[0] * inv, y[1] * inv), pack_bf16(y[2] * inv, y[3] * inv)};
@@ -690,9 +696,11 @@ __device__ __forceinline__ void rows_body(const aos_kv_attn_params &p, int few, 
     }
     if (done && wave == 0)
 #pragma unroll
-      for (int b = 0; b < NB; ++b)
+      for (int b = 0; b < NB; ++b) {
+        const float inv = inverse(l[b], m[b]);
 #pragma unroll
-        for (int d = 0; d < DB; ++d) put(b, d, o[b][d], l[b]);
+        for (int d = 0; d < DB; ++d) put(b, d, o[b][d], inv);
+      }
   }
 }
 
@@ -1158,6 +1166,7 @@ __device__ __forceinline__ void tiles_body(const aos_kv_attn_params &p, int few,
 #pragma unroll
           for (int v = 0; v < 16; ++v) mx = fmaxf(mx, sc[b][v]);
         mx = half_max(mx) * cs;
+        if (!edge || (lo < k0 + TILE && hi >= k0)) mx = fmaxf(mx, LEAST);
         if (__ballot(mx > m + SLACK)) {
           const float top = fmaxf(m, mx), alpha = ex2(m - safe_max(top));
           l = l * alpha;
@@ -1202,7 +1211,7 @@ __device__ __forceinline__ void tiles_body(const aos_kv_attn_params &p, int few,
         *(u32x2 *)(orow + at) = u32x2{pack_bf16(y[0] * inv, y[1] * inv), pack_bf16(y[2] * inv, y[3] * inv)};
     };
     if (n == x.nt) {
-      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+      const float inv = inverse(l, m);
 #pragma unroll
       for (int d = 0; d < DB; ++d)
 #pragma unroll
@@ -1262,7 +1271,7 @@ __device__ __forceinline__ void tiles_body(const aos_kv_attn_params &p, int few,
 #pragma unroll
             for (int v = 0; v < 16; ++v) o[d][v] = o[d][v] + y[d][v >> 2][v & 3] * f;
         }
-        const float inv = all == 0.0f ? 0.0f : 1.0f / all;
+        const float inv = inverse(all, top);
 #pragma unroll
         for (int d = 0; d < DB; ++d)
 #pragma unroll

@@ -229,6 +229,22 @@ def test_infinities_and_nans(hip, fmt, new):
         assert (np.abs(got - o)[fin] <= P.attention_bound(q, k[:L], a, o, hd ** -0.5)[fin]).all()
 
 
+@pytest.mark.parametrize("nh,nkv,hd", [(4, 2, 64), (14, 2, 128), (2, 1, 256)])
+def test_infinite_scores(hip, nh, nkv, hd):
+    """Scores of plus infinity make their rows NaN, and so do scores of minus infinity where a row sees no others."""
+    new, lens = [1, 70, 1, 1, 3, 40], [1, 70, 200, 300, 700, 700]
+
+    def poison(k, v):
+        k[0, :, 0] = np.inf             # the only position of the first sequence
+        k[1, :, 0] = -np.inf            # the first position of the second
+        k[71 + 150:71 + 200, :, 1] = np.inf   # the last positions of the third
+        k[271:, :, 2] = np.inf          # every position of the others
+        k[1271 + 600, :, 2] = 1.0       # but one
+
+    pool, q, seqs = _setup(hip, "bf16", nh, nkv, hd, 64, new, lens, seed=hd, poison=poison)
+    _check(_run(pool, q, new, lens), seqs, new, hd ** -0.5)
+
+
 @pytest.mark.parametrize("sharp,scale", [(60.0, None), (1.0, 0.0), (2.0, -0.3)])
 def test_scores_of_any_size(hip, sharp, scale):
     """Scores of hundreds (the running maximum moves far), a scale of zero, a negative one."""
