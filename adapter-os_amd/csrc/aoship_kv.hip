@@ -198,7 +198,8 @@ __global__ void __launch_bounds__(256) aos_kv_append_kernel(aos_kv_append_params
       const uint32_t byte = scale_byte<FMT>(block_top(x));
       if (is_v) {
         vsc[blk][t] = byte;
-        if (byte == 255u) *p.b.nonfinite = 1u;
+        /* (also a scale whose largest code stands for 2^128) */
+        if (byte >= (FMT == AOS_KV_MXFP8 ? 247u : 253u)) *p.b.nonfinite = 1u;
         if (fresh) tile[vs_off<FMT, HDP>() + blk * TILE + tp + t] = (unsigned char)byte;
         continue;
       }

@@ -229,6 +229,20 @@ def test_infinities_and_nans(hip, fmt, new):
         assert (np.abs(got - o)[fin] <= P.attention_bound(q, k[:L], a, o, hd ** -0.5)[fin]).all()
 
 
+@pytest.mark.parametrize("fmt", P.FORMATS)
+@pytest.mark.parametrize("new", [2, 12, 90])
+def test_largest_values(hip, fmt, new):
+    """A value whose code stands for 2^128 is an infinity to the row that sees it, and nothing to the others."""
+    def poison(k, v):
+        v[229, 1, 40] = P.bf16([3.3895e38])[0]
+        k[229] = 0.0
+
+    pool, q, seqs = _setup(hip, fmt, 4, 2, 64, 64, [new], [230], poison=poison)
+    got = _run(pool, q, [new], [230])
+    o, a = P.attention(*seqs[0], 64 ** -0.5)
+    assert (np.abs(got - o)[:-1] <= P.attention_bound(seqs[0][0], seqs[0][1], a, o, 64 ** -0.5)[:-1]).all()
+
+
 @pytest.mark.parametrize("nh,nkv,hd", [(4, 2, 64), (14, 2, 128), (2, 1, 256)])
 def test_infinite_scores(hip, nh, nkv, hd):
     """Scores of plus infinity make their rows NaN, and so do scores of minus infinity where a row sees no others."""
