@@ -188,8 +188,8 @@ constexpr int SNAP = 3;
  * Bound by reading the cache once, by latency where that is little. Keys and values go straight to registers, the next
  * tile's on their way while one is worked on: a tile is used by one workgroup's one or two matrix instructions a block,
  * which LDS would not speed up. 64 streams of up to 16001 positions, 28/4 heads of 128: 16 bits 228 us, 5.7 TB/s; 32 of up
- * to 8191, 24/8 heads, 8 bits: 73 us, 4.6 TB/s; 24 of 32768, 40/8 heads, 4 bits: 122 us, 4.7 TB/s (a decoded tile is some
- * 470 vector instructions). */
+ * to 8191, 24/8 heads, 8 bits: 73 us, 4.6 TB/s; 24 of 32768, 40/8 heads, 4 bits: 122 us, 4.7 TB/s (a quarter fewer of a
+ * decoded tile's 470 vector instructions: 1%). */
 template <int FMT, int HDP>
 struct Tile { /* a tile's keys and values in registers */
   static constexpr int KW = HDP * bits<FMT>() / 128; /* words of a key row's quarter */
