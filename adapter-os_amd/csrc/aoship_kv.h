@@ -75,9 +75,18 @@ struct Seq {
   int row0, count, len;
 };
 
+/* notes a fault in the cache's word (on the host, where tests walk a batch, in an ordinary one) */
+__host__ __device__ __forceinline__ void note(uint32_t *faults, uint32_t bits) {
+#ifdef __HIP_DEVICE_COMPILE__
+  __hip_atomic_fetch_or(faults, bits, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+#else
+  *faults |= bits;
+#endif
+}
+
 /* What the caller's device arrays say of sequence s, refused (no rows, the fault noted) where it does not fit the
  * sizes that the launch was made for: nothing below indexes with a value that was not checked here. */
-__device__ __forceinline__ Seq seq_of(const aos_kv_batch &b, int r0, int r1, int len) {
+__host__ __device__ __forceinline__ Seq seq_of(const aos_kv_batch &b, int r0, int r1, int len) {
   Seq q;
   q.row0 = r0;
   q.count = r1 - r0;
@@ -85,7 +94,7 @@ __device__ __forceinline__ Seq seq_of(const aos_kv_batch &b, int r0, int r1, int
   const bool ok = r0 >= 0 && r1 >= r0 && r1 <= b.n_tokens && r1 - r0 <= b.max_new && len >= 0 && len <= b.max_len;
   if (!ok) {
     q.row0 = q.count = q.len = 0;
-    __hip_atomic_fetch_or(b.faults, AOS_KV_FAULT_BATCH, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    note(b.faults, AOS_KV_FAULT_BATCH);
   }
   return q;
 }
@@ -97,7 +106,7 @@ __device__ __forceinline__ Seq seq_at(const aos_kv_batch &b, int s) {
 __device__ __forceinline__ int page_of(const aos_kv_batch &b, int s, int pos) {
   const int page = b.pages[(long long)s * b.stride + (pos >> b.page_shift)];
   if ((unsigned)page < (unsigned)b.num_pages) return page;
-  __hip_atomic_fetch_or(b.faults, AOS_KV_FAULT_PAGE, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  note(b.faults, AOS_KV_FAULT_PAGE);
   return -1;
 }
 

@@ -881,21 +881,21 @@ struct Stage {
 };
 
 /* Row tile slots of a batch: sequence s has its row tiles from slot_base(s) on, fewer than the next one's base. */
-__device__ __forceinline__ int slot_base(int start, int g, int s) { return (int)((long long)start * g / TR) + s; }
+__host__ __device__ __forceinline__ int slot_base(int start, int g, int s) { return (int)((long long)start * g / TR) + s; }
 
 /* Where a walk over the slots is: sequence s, which has the slots base .. next - 1. */
 struct Cursor {
   Seq q;
   int s, base, next;
 };
-__device__ __forceinline__ void open(const aos_kv_batch &b, int g, int s, Cursor &c) {
+__host__ __device__ __forceinline__ void open(const aos_kv_batch &b, int g, int s, Cursor &c) {
   const int r0 = b.starts[s], r1 = b.starts[s + 1];
   c.s = s;
   c.q = seq_of(b, r0, r1, b.lens[s]);
   c.base = slot_base(r0, g, s);
   c.next = s + 1 < b.n_seqs ? slot_base(r1, g, s + 1) : 0x7fffffff;
 }
-__device__ __forceinline__ void seek(const aos_kv_batch &b, int g, int slot, Cursor &c) {
+__host__ __device__ __forceinline__ void seek(const aos_kv_batch &b, int g, int slot, Cursor &c) {
   int lo = 0, hi = b.n_seqs; /* the last sequence whose slots begin at or before `slot` */
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
@@ -908,13 +908,15 @@ __device__ __forceinline__ void seek(const aos_kv_batch &b, int g, int slot, Cur
 }
 
 /* (for a wave whose lanes all hold the same: kept in scalar registers) */
-__device__ __forceinline__ void uniform(Cursor &c) {
+__host__ __device__ __forceinline__ void uniform(Cursor &c) {
+#ifdef __HIP_DEVICE_COMPILE__
   c.q.row0 = __builtin_amdgcn_readfirstlane(c.q.row0);
   c.q.count = __builtin_amdgcn_readfirstlane(c.q.count);
   c.q.len = __builtin_amdgcn_readfirstlane(c.q.len);
   c.s = __builtin_amdgcn_readfirstlane(c.s);
   c.base = __builtin_amdgcn_readfirstlane(c.base);
   c.next = __builtin_amdgcn_readfirstlane(c.next);
+#endif
 }
 
 /* A row tile: rows r0 .. r0 + rows - 1 of its sequence and the position tiles t0 .. t0 + nt - 1 that they see (at least
@@ -922,11 +924,11 @@ __device__ __forceinline__ void uniform(Cursor &c) {
 struct RowTile {
   int r0, rows, t0, nt;
 };
-__device__ __forceinline__ RowTile row_tile(const aos_kv_attn_params &p, int g, int few, const Cursor &c, int slot) {
+__host__ __device__ __forceinline__ RowTile row_tile(const aos_kv_attn_params &p, int g, int few, const Cursor &c, int slot) {
   RowTile o = {};
   const int all = c.q.count * g, r = slot - c.base;
+  if (all <= few || r < 0 || r > (all - 1) / TR) return o; /* (slots times TR may pass 32 bits) */
   o.r0 = r * TR;
-  if (all <= few || r < 0 || o.r0 >= all) return o;
   o.rows = all - o.r0 < TR ? all - o.r0 : TR;
   const int p0 = c.q.len - c.q.count;
   const int first = p0 + o.r0 / g, last = p0 + (o.r0 + o.rows - 1) / g;
@@ -937,6 +939,65 @@ __device__ __forceinline__ RowTile row_tile(const aos_kv_attn_params &p, int g, 
 }
 
 constexpr int SETUP = 4; /* weight of a row tile beside its position tiles */
+
+/* The weights of a key/value head are counted in runs of slots, each from a cursor at the run's first slot on: a run's sum,
+ * and where a border at weight v of it falls: a slot and the position tile of its row tile that the border cuts off (0:
+ * the border is at the row tile's beginning). */
+__host__ __device__ __forceinline__ int run_weight(const aos_kv_attn_params &p, int g, int few, Cursor c, int first, int end) {
+  int sum = 0;
+  for (int x = first; x < end; ++x) {
+    while (x >= c.next) open(p.b, g, c.s + 1, c);
+    const int nt = row_tile(p, g, few, c, x).nt;
+    sum += nt ? nt + SETUP : 0;
+  }
+  return sum;
+}
+__host__ __device__ __forceinline__ void run_border(const aos_kv_attn_params &p, int g, int few, Cursor &c, int first,
+                                                    int end, int v, int &slot, int &j) {
+  for (int x = first; x < end; ++x) {
+    while (x >= c.next) open(p.b, g, c.s + 1, c);
+    const int nt = row_tile(p, g, few, c, x).nt, weight = nt ? nt + SETUP : 0;
+    if (v < weight) {
+      const int t = v - SETUP;
+      slot = nt - t < SNAP ? x + 1 : x;
+      j = t < SNAP || nt - t < SNAP ? 0 : t;
+      return;
+    }
+    v -= weight;
+  }
+}
+
+/* A workgroup's walk: at position tile j of head h's slot, up to position tile j1 of head h1's slot1. */
+struct Walk {
+  int h, slot, j, h1, slot1, j1;
+};
+/* Goes on to the next row tile, from the slot that the walk is at; false where its share ends. */
+__host__ __device__ __forceinline__ bool next_row_tile(const aos_kv_attn_params &p, int g, int few, int slots, Walk &k,
+                                                       Cursor &c, RowTile &x) {
+  for (;; ++k.slot, k.j = 0) {
+    if (k.slot >= slots) {
+      if (++k.h >= p.b.nkv) return false;
+      k.slot = 0;
+      seek(p.b, g, 0, c);
+      uniform(c);
+    }
+    if (k.h > k.h1 || (k.h == k.h1 && k.slot >= k.slot1 && (k.slot > k.slot1 || k.j1 == 0))) return false;
+    while (k.slot >= c.next) {
+      open(p.b, g, c.s + 1, c);
+      uniform(c);
+    }
+    x = row_tile(p, g, few, c, k.slot);
+    if (x.nt) return true;
+  }
+}
+/* Borders wf .. wl cut the row tile of nt position tiles of which workgroup w has j .. je - 1 (not all). */
+struct Cuts {
+  int wf, wl;
+};
+__host__ __device__ __forceinline__ Cuts cuts_of(int w, int share, int j, int je, int nt) {
+  const int place = (j > 0 ? w * share - j : (w + 1) * share - je) - SETUP; /* the row tile's place among the weights */
+  return Cuts{(place + SETUP + SNAP + share - 1) / share, (place + SETUP + nt - SNAP) / share};
+}
 
 struct TilesShared {
   int scan[4], found[4], joins;
@@ -958,12 +1019,7 @@ __device__ __forceinline__ void tiles_body(const aos_kv_attn_params &p, int few,
   int sum = 0;
   if (first < end) {
     seek(p.b, g, first, own);
-    cur = own;
-    for (int x = first; x < end; ++x) {
-      while (x >= cur.next) open(p.b, g, cur.s + 1, cur);
-      const int nt = row_tile(p, g, few, cur, x).nt;
-      sum += nt ? nt + SETUP : 0;
-    }
+    sum = run_weight(p, g, few, own, first, end);
   }
   const int upto = wave_scan(sum, lane);
   if (lane == 63) sh.scan[wave] = upto;
@@ -978,56 +1034,39 @@ __device__ __forceinline__ void tiles_body(const aos_kv_attn_params &p, int few,
   int share = (total + G - 1) / G;
   if (share < min_share) share = min_share;
   if (w * share >= total) return; /* uniform */
-  int h = w * share / N, h1 = p.b.nkv;
+  Walk walk;
+  walk.h = w * share / N;
+  walk.h1 = p.b.nkv;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    const int at = (w + i) * share;
-    if (at >= total) {
+    const int border = (w + i) * share;
+    if (border >= total) {
       if (tid == 0) sh.found[2] = sh.found[3] = 0;
       break;
     }
-    const int hh = at / N;
-    if (i) h1 = hh;
-    int v = at - hh * N - before;
+    const int hh = border / N, v = border - hh * N - before;
+    if (i) walk.h1 = hh;
     if (v >= 0 && v < sum) {
       cur = own;
-      for (int x = first; x < end; ++x) {
-        while (x >= cur.next) open(p.b, g, cur.s + 1, cur);
-        const int nt = row_tile(p, g, few, cur, x).nt, weight = nt ? nt + SETUP : 0;
-        if (v < weight) {
-          const int j = v - SETUP;
-          if (i == 0) sh.at_first = cur;
-          sh.found[2 * i] = nt - j < SNAP ? x + 1 : x;
-          sh.found[2 * i + 1] = j < SNAP || nt - j < SNAP ? 0 : j;
-          break;
-        }
-        v -= weight;
-      }
+      run_border(p, g, few, cur, first, end, v, sh.found[2 * i], sh.found[2 * i + 1]);
+      if (i == 0) sh.at_first = cur;
     }
   }
   __syncthreads();
-  int slot = __builtin_amdgcn_readfirstlane(sh.found[0]), j = __builtin_amdgcn_readfirstlane(sh.found[1]);
-  const int slot1 = __builtin_amdgcn_readfirstlane(sh.found[2]), j1 = __builtin_amdgcn_readfirstlane(sh.found[3]);
+  walk.slot = __builtin_amdgcn_readfirstlane(sh.found[0]);
+  walk.j = __builtin_amdgcn_readfirstlane(sh.found[1]);
+  walk.slot1 = __builtin_amdgcn_readfirstlane(sh.found[2]);
+  walk.j1 = __builtin_amdgcn_readfirstlane(sh.found[3]);
   cur = sh.at_first;
   uniform(cur);
   const float cs = fmaxf(fabsf(p.scale) * LOG2E, 1.17549435e-38f);
   const uint32_t flip = p.scale < 0.0f ? 0x80008000u : 0u; /* (both as above) */
   int pages = -1, pages_s = -1, pages_t = 0; /* pages of 64 tiles from pages_t on of a sequence, one a lane */
-  for (;; ++slot, j = 0) {
-    if (slot >= slots) {
-      if (++h >= p.b.nkv) break;
-      slot = 0;
-      seek(p.b, g, 0, cur);
-      uniform(cur);
-    }
-    if (h > h1 || (h == h1 && slot >= slot1 && (slot > slot1 || j1 == 0))) break;
-    while (slot >= cur.next) {
-      open(p.b, g, cur.s + 1, cur);
-      uniform(cur);
-    }
-    const RowTile x = row_tile(p, g, few, cur, slot);
-    if (x.nt == 0) continue;
-    const int je = h == h1 && slot == slot1 ? j1 : x.nt; /* its tiles j .. je - 1 are this workgroup's */
+  for (;; ++walk.slot, walk.j = 0) {
+    RowTile x;
+    if (!next_row_tile(p, g, few, slots, walk, cur, x)) break;
+    const int h = walk.h, j = walk.j;
+    const int je = h == walk.h1 && walk.slot == walk.slot1 ? walk.j1 : x.nt; /* its tiles j .. je - 1 are this workgroup's */
     const int n = je - j;
     const int p0 = cur.q.len - cur.q.count;
 
@@ -1219,9 +1258,8 @@ __device__ __forceinline__ void tiles_body(const aos_kv_attn_params &p, int few,
           put(d, q, f32x4{o[d][4 * q], o[d][4 * q + 1], o[d][4 * q + 2], o[d][4 * q + 3]}, inv);
     } else {
       constexpr int PF = tile_part_floats<HDP>();
-      /* the row tile's place among the weights, and the borders wf .. wl that cut it */
-      const int place = (j > 0 ? w * share - j : (w + 1) * share - je) - SETUP;
-      const int wf = (place + SETUP + SNAP + share - 1) / share, wl = (place + SETUP + x.nt - SNAP) / share;
+      const Cuts cuts = cuts_of(w, share, j, je, x.nt);
+      const int wf = cuts.wf, wl = cuts.wl;
       const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void *)p.part, (short)0, 0x7fffffff, 0x00020000);
       if (nrows > 0) {
         const int at = (2 * w + (j > 0 ? 0 : 1)) * PF;
@@ -1388,3 +1426,65 @@ extern "C" int aos_launch_kv_attention(const aos_kv_attn_params *p, const aos_la
 }
 
 extern "C" int aos_kv_attention_prepare(int format, int hdp) { return KV_DISPATCH(prepare, format, hdp); }
+
+/* Diagnostic, for tests without a device: the pieces of row tiles that the G workgroups of the second kernel take of a
+ * batch (starts and lens: host arrays), walked as it walks them: rows of {workgroup, head, sequence, first row, rows, first
+ * position tile, position tiles, j, je, wf, wl} (the last two -1 where the row tile is whole). Returns their number (at
+ * most cap are written), or -1 where the kernel takes the batch for one that does not fit. */
+extern "C" int aoship_internal_kv_tile_pieces(int nh, int nkv, int window, int n_seqs, int n_tokens, int max_new, int max_len,
+                                              const int32_t *starts, const int32_t *lens, int few, int G, int min_share,
+                                              int (*out)[11], int cap) {
+  uint32_t faults = 0;
+  aos_kv_attn_params p = {};
+  p.b.nkv = nkv;
+  p.b.starts = starts;
+  p.b.lens = lens;
+  p.b.n_seqs = n_seqs;
+  p.b.n_tokens = n_tokens;
+  p.b.max_new = max_new;
+  p.b.max_len = max_len;
+  p.b.faults = &faults;
+  p.nh = nh;
+  p.window = window;
+  const int g = nh / nkv, slots = (int)((long long)n_tokens * g / TR) + n_seqs, per = (slots + 255) / 256;
+  Cursor own[256] = {};
+  int before[257] = {};
+  for (int t = 0; t < 256; ++t) {
+    const int first = t * per, end = first + per < slots ? first + per : slots;
+    int sum = 0;
+    if (first < end) {
+      seek(p.b, g, first, own[t]);
+      sum = run_weight(p, g, few, own[t], first, end);
+    }
+    before[t + 1] = before[t] + sum;
+  }
+  const int N = before[256], total = N * nkv;
+  int share = (total + G - 1) / G, n = 0;
+  if (share < min_share) share = min_share;
+  for (int w = 0; w < G && w * share < total; ++w) {
+    Walk walk = {w * share / N, 0, 0, nkv, 0, 0};
+    Cursor cur = {};
+    for (int i = 0; i < 2 && (w + i) * share < total; ++i) {
+      const int hh = (w + i) * share / N, v = (w + i) * share - hh * N;
+      int t = 0;
+      while (v >= before[t + 1]) ++t;
+      const int first = t * per, end = first + per < slots ? first + per : slots;
+      Cursor c = own[t];
+      run_border(p, g, few, c, first, end, v - before[t], i ? walk.slot1 : walk.slot, i ? walk.j1 : walk.j);
+      if (i)
+        walk.h1 = hh;
+      else
+        cur = c;
+    }
+    RowTile x;
+    for (; next_row_tile(p, g, few, slots, walk, cur, x); ++walk.slot, walk.j = 0) {
+      const int je = walk.h == walk.h1 && walk.slot == walk.slot1 ? walk.j1 : x.nt;
+      Cuts cuts = {-1, -1};
+      if (je - walk.j != x.nt) cuts = cuts_of(w, share, walk.j, je, x.nt);
+      const int row[11] = {w, walk.h, cur.s, x.r0, x.rows, x.t0, x.nt, walk.j, je, cuts.wf, cuts.wl};
+      for (int i = 0; n < cap && i < 11; ++i) out[n][i] = row[i];
+      ++n;
+    }
+  }
+  return n;
+}

@@ -192,3 +192,82 @@ def test_plain_quantiser():
                     best = near[0] if len(near) == 1 else near[near % 2 == 0][0]  # ties to the even code
                     assert abs(got[r, b + i]) == codes[best] * 2.0 ** e
                     assert got[r, b + i] == 0 or np.sign(got[r, b + i]) == np.sign(v)
+
+
+# ---- the row tiles that the second attention kernel's workgroups share ----
+
+
+def _pieces(nh, nkv, starts, lens, n_tokens, max_new, max_len, window=0, few=0, G=512, min_share=6, cap=1 << 16):
+    """The kernel's walk over a batch, as rows of (workgroup, head, sequence, first row, rows, first position tile,
+    position tiles, j, je, wf, wl), or None where it refuses the batch."""
+    starts, lens = np.asarray(starts, np.int32), np.asarray(lens, np.int32)
+    out = np.zeros((cap, 11), np.int32)
+    f = _fn("aoship_internal_kv_tile_pieces", [I, I, I, I, I, I, I, V, V, I, I, I, V, I])
+    n = f(nh, nkv, window, len(lens), n_tokens, max_new, max_len, starts.ctypes.data, lens.ctypes.data, few, G,
+          min_share, out.ctypes.data, cap)
+    assert n <= cap
+    return None if n < 0 else out[:n]
+
+
+def _row_tiles(nh, nkv, starts, lens, window, few):
+    """(head, sequence, first row, rows, first position tile, position tiles) of the sequences that fit, by definition"""
+    g, found = nh // nkv, []
+    for s, n in enumerate(lens):
+        count = starts[s + 1] - starts[s]
+        if count * g <= few:
+            continue
+        for r0 in range(0, count * g, 128):
+            rows = min(128, count * g - r0)
+            first, last = n - count + r0 // g, n - count + (r0 + rows - 1) // g
+            t0 = max(0, first - window + 1) // 64 if window else 0
+            found += [(h, s, r0, rows, t0, max(0, last) // 64 - t0 + 1) for h in range(nkv)]
+    return sorted(found)
+
+
+def _check_pieces(got, want):
+    """Every row tile's position tiles are taken once, and each piece of a cut one expects the arrivals that come."""
+    tiles = {}
+    for w, h, s, r0, rows, t0, nt, j, je, wf, wl in got.tolist():
+        tiles.setdefault((h, s, r0, rows, t0, nt), []).append((j, je, w, wf, wl))
+    assert sorted(tiles) == want
+    borders = set()
+    for (_, _, _, _, _, nt), parts in tiles.items():
+        parts.sort()
+        assert [a for a, *_ in parts] == [0] + [b for _, b, *_ in parts[:-1]] and parts[-1][1] == nt
+        if len(parts) == 1:
+            assert parts[0][3:] == (-1, -1)
+            continue
+        wf, wl = parts[0][3:]
+        assert all(p[3:] == (wf, wl) for p in parts) and len(parts) == wl - wf + 2
+        assert [p[2] for p in parts] == list(range(wf - 1, wl + 1))  # their slots of the workspace
+        assert not borders & set(range(wf, wl + 1))
+        borders |= set(range(wf, wl + 1))
+
+
+@pytest.mark.parametrize("seed", range(40))
+def test_workgroups_share_row_tiles(seed):
+    """Random batches: no rows, few, many, padding in front, windows, rows behind the last sequence, a sequence that
+    does not fit."""
+    rng = np.random.default_rng(seed)
+    n, nkv, g = int(rng.integers(1, 40)), int(rng.integers(1, 5)), int(rng.choice([1, 3, 7, 16]))
+    new = rng.integers(0, int(rng.choice([3, 40, 700])) + 1, n)
+    lens = np.maximum(0, new + rng.integers(0, 5000, n) * rng.integers(0, 2, n) - (rng.random(n) < 0.1) * 30)
+    starts, few = np.concatenate([[0], np.cumsum(new)]), int(rng.choice([0, 16]))
+    window, most = int(rng.choice([0, 1, 300, 2048])), max(1, int(new.max()))
+    T, max_len, fits = int(starts[-1] + rng.integers(0, 30)), int(lens.max()) + 1, list(lens)
+    if rng.random() < 0.3:
+        bad = int(rng.integers(0, n))
+        lens[bad], fits[bad] = max_len + 5, None
+    got = _pieces(g * nkv, nkv, starts, lens, T, most, max_len, window, few, G=int(rng.choice([256, 512])))
+    want = [t for t in _row_tiles(g * nkv, nkv, starts, lens, window, few) if fits[t[1]] is not None]
+    _check_pieces(got, want)
+
+
+def test_row_tiles_of_more_rows_than_32_bits_count():
+    """A batch made for 60 000 000 rows of 40 heads that holds one sequence of 1000: its row tiles and no others."""
+    b = _batch(n_seqs=1, n_tokens=60000000, max_new=1000, max_len=1000, page_stride=16)
+    cfg = aoship._KVConfig(1, 1, 128, 64, 100, 0)
+    f = _fn("aoship_internal_kv_attention_check", [V, I, V, V, C.c_int64, I, C.c_float, I, V, C.c_int64])
+    assert f(C.byref(cfg), 0, C.byref(b), ALIGNED, 5120, 40, 0.1, 0, 2 * ALIGNED, 5120) == 0
+    got = _pieces(40, 1, [0, 1000], [1000], 60000000, 1000, 1000)
+    _check_pieces(got, _row_tiles(40, 1, [0, 1000], [1000], 0, 0))
