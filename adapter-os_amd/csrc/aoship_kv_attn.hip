@@ -880,8 +880,20 @@ struct Stage {
   }
 };
 
-/* Row tile slots of a batch: sequence s has its row tiles from slot_base(s) on, fewer than the next one's base. */
-__host__ __device__ __forceinline__ int slot_base(int start, int g, int s) { return (int)((long long)start * g / TR) + s; }
+/* Row tile slots of a batch: sequence s, whose rows begin at `start`, has its row tiles from slot_base() on, fewer than the
+ * next one's base. Starts outside the batch's rows (of sequences that do not fit) count as its ends, so that the bases
+ * ascend wherever the starts do; the kernel takes no batch whose starts fall: which sequence a slot belongs to would depend
+ * on where a walk comes from, and workgroups that share a row tile would expect other arrivals than come. */
+__host__ __device__ __forceinline__ int slot_base(const aos_kv_batch &b, int start, int g, int s) {
+  start = start < 0 ? 0 : start > b.n_tokens ? b.n_tokens : start;
+  return (int)((long long)start * g / TR) + s;
+}
+/* whether the starts of every n-th sequence from the first-th on fall */
+__host__ __device__ __forceinline__ bool starts_fall(const aos_kv_batch &b, int first, int n) {
+  bool fall = false;
+  for (int s = first; s < b.n_seqs; s += n) fall |= b.starts[s + 1] < b.starts[s];
+  return fall;
+}
 
 /* Where a walk over the slots is: sequence s, which has the slots base .. next - 1. */
 struct Cursor {
@@ -892,14 +904,14 @@ __host__ __device__ __forceinline__ void open(const aos_kv_batch &b, int g, int 
   const int r0 = b.starts[s], r1 = b.starts[s + 1];
   c.s = s;
   c.q = seq_of(b, r0, r1, b.lens[s]);
-  c.base = slot_base(r0, g, s);
-  c.next = s + 1 < b.n_seqs ? slot_base(r1, g, s + 1) : 0x7fffffff;
+  c.base = slot_base(b, r0, g, s);
+  c.next = s + 1 < b.n_seqs ? slot_base(b, r1, g, s + 1) : 0x7fffffff;
 }
 __host__ __device__ __forceinline__ void seek(const aos_kv_batch &b, int g, int slot, Cursor &c) {
   int lo = 0, hi = b.n_seqs; /* the last sequence whose slots begin at or before `slot` */
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
-    if (slot_base(b.starts[mid], g, mid) <= slot)
+    if (slot_base(b, b.starts[mid], g, mid) <= slot)
       lo = mid;
     else
       hi = mid;
@@ -1023,7 +1035,10 @@ __device__ __forceinline__ void tiles_body(const aos_kv_attn_params &p, int few,
   }
   const int upto = wave_scan(sum, lane);
   if (lane == 63) sh.scan[wave] = upto;
-  __syncthreads();
+  if (__syncthreads_or(starts_fall(p.b, tid, 256) ? 1 : 0)) {
+    if (tid == 0) note(p.b.faults, AOS_KV_FAULT_BATCH);
+    return;
+  }
   int before = upto - sum, N = 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -1447,6 +1462,7 @@ extern "C" int aoship_internal_kv_tile_pieces(int nh, int nkv, int window, int n
   p.nh = nh;
   p.window = window;
   const int g = nh / nkv, slots = (int)((long long)n_tokens * g / TR) + n_seqs, per = (slots + 255) / 256;
+  if (starts_fall(p.b, 0, 1)) return -1;
   Cursor own[256] = {};
   int before[257] = {};
   for (int t = 0; t < 256; ++t) {

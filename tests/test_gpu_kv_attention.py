@@ -407,3 +407,16 @@ def test_a_layer_as_it_is_served(hip, fmt):
         layer.proj_forward("o_proj", out.view(T, nh * hd), rings, again)
         assert torch.isfinite(y).all() and torch.equal(y, again)
     assert pool.cache.faults() == 0
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "mxfp8"])
+def test_starts_that_fall(hip, fmt):
+    """Noted, no row written, and the cache's next calls are right: workgroups that share a row tile count their
+    arrivals in words that stay with the cache."""
+    new, lens, nh, hd = [700, 300, 100], [900, 400, 300], 28, 64
+    pool, q, seqs = _setup(hip, fmt, nh, 4, hd, 64, new, lens)
+    for starts in ([0, 700, 300, 1100], [700, 0, 400, 900]):
+        got = _run(pool, q, new, lens, starts=starts, max_new=1100)
+        assert pool.cache.faults() == hip.KV_FAULT_BATCH and (got == 7).all()
+        _check(_run(pool, q, new, lens), seqs, new, hd ** -0.5)
+        assert pool.cache.faults() == 0

@@ -210,11 +210,11 @@ def _pieces(nh, nkv, starts, lens, n_tokens, max_new, max_len, window=0, few=0, 
 
 
 def _row_tiles(nh, nkv, starts, lens, window, few):
-    """(head, sequence, first row, rows, first position tile, position tiles) of the sequences that fit, by definition"""
+    """(head, sequence, first row, rows, first position tile, position tiles) of the sequences that fit (None: those that do not), by definition"""
     g, found = nh // nkv, []
     for s, n in enumerate(lens):
         count = starts[s + 1] - starts[s]
-        if count * g <= few:
+        if n is None or count * g <= few:
             continue
         for r0 in range(0, count * g, 128):
             rows = min(128, count * g - r0)
@@ -259,8 +259,7 @@ def test_workgroups_share_row_tiles(seed):
         bad = int(rng.integers(0, n))
         lens[bad], fits[bad] = max_len + 5, None
     got = _pieces(g * nkv, nkv, starts, lens, T, most, max_len, window, few, G=int(rng.choice([256, 512])))
-    want = [t for t in _row_tiles(g * nkv, nkv, starts, lens, window, few) if fits[t[1]] is not None]
-    _check_pieces(got, want)
+    _check_pieces(got, _row_tiles(g * nkv, nkv, starts, fits, window, few))
 
 
 def test_row_tiles_of_more_rows_than_32_bits_count():
@@ -271,3 +270,26 @@ def test_row_tiles_of_more_rows_than_32_bits_count():
     assert f(C.byref(cfg), 0, C.byref(b), ALIGNED, 5120, 40, 0.1, 0, 2 * ALIGNED, 5120) == 0
     got = _pieces(40, 1, [0, 1000], [1000], 60000000, 1000, 1000)
     _check_pieces(got, _row_tiles(40, 1, [0, 1000], [1000], 0, 0))
+
+
+FALLING = [([1330, 210, 160, 610, 870], [3200, 3500, 3000, 800], 1500), ([0, 700, 300, 1000], [900, 900, 900], 1000),
+           ([500, 0, 400], [600, 600], 500)]
+
+
+@pytest.mark.parametrize("starts,lens,T", FALLING)
+def test_starts_that_fall_are_refused_whole(starts, lens, T):
+    """Which sequence a slot of row tiles belongs to would depend on where a walk comes from: workgroups that share a
+    row tile would expect other arrivals than come."""
+    assert _pieces(28, 4, starts, lens, T, T, 4000) is None
+
+
+@pytest.mark.parametrize("starts,good", [([-2 ** 31, -2 ** 30, -9, 0, 400, 900, 950], [3, 4, 5]),
+                                         ([0, 400, 900, 2 ** 30, 2 ** 31 - 1, 2 ** 31 - 1, 2 ** 31 - 1], [0, 1]),
+                                         ([-5, 300, 300, 340, 2000, 2000, 2000], [1, 2]),
+                                         ([-2 ** 31, -10 ** 8, 0, 400, 900, 950, 950], [2, 3, 4, 5])])
+@pytest.mark.parametrize("g", [7, 4096])
+def test_starts_outside_the_rows_leave_the_others(starts, good, g):
+    """Ascending starts of which some are no rows of the batch: those sequences are left out, the others served."""
+    lens = [500, 610, 600, 700, 900, 64]
+    got = _pieces(2 * g, 2, starts, lens, 1000, 1000, 1000)
+    _check_pieces(got, _row_tiles(2 * g, 2, starts, [n if s in good else None for s, n in enumerate(lens)], 0, 0))
