@@ -102,12 +102,18 @@ __device__ __forceinline__ Seq seq_at(const aos_kv_batch &b, int s) {
   return seq_of(b, b.starts[s], b.starts[s + 1], b.lens[s]);
 }
 
-/* The page that holds a position (0 <= pos < max_len, which the table covers), or -1. */
-__device__ __forceinline__ int page_of(const aos_kv_batch &b, int s, int pos) {
-  const int page = b.pages[(long long)s * b.stride + (pos >> b.page_shift)];
+/* What the table says of the page that holds a position (0 <= pos < max_len, which the table covers). */
+__device__ __forceinline__ int page_entry(const aos_kv_batch &b, int s, int pos) {
+  return b.pages[(long long)s * b.stride + (pos >> b.page_shift)];
+}
+/* The page of a position that a launch reads or writes, or -1 where the table's entry is none. */
+__device__ __forceinline__ int page_checked(const aos_kv_batch &b, int page) {
   if ((unsigned)page < (unsigned)b.num_pages) return page;
   note(b.faults, AOS_KV_FAULT_PAGE);
   return -1;
+}
+__device__ __forceinline__ int page_of(const aos_kv_batch &b, int s, int pos) {
+  return page_checked(b, page_entry(b, s, pos));
 }
 
 /* Blocks of 16 positions, aligned in their sequence, that a batch's new rows can touch: sequence s has its blocks

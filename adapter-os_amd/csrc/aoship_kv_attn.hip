@@ -1076,7 +1076,9 @@ __device__ __forceinline__ void tiles_body(const aos_kv_attn_params &p, int few,
   uniform(cur);
   const float cs = fmaxf(fabsf(p.scale) * LOG2E, 1.17549435e-38f);
   const uint32_t flip = p.scale < 0.0f ? 0x80008000u : 0u; /* (both as above) */
-  int pages = -1, pages_s = -1, pages_t = 0; /* pages of 64 tiles from pages_t on of a sequence, one a lane */
+  /* the table's entries for 64 tiles from pages_t on of a sequence, one a lane; checked only as a tile's turn comes: what no
+   * row sees (left of a window) may be no page any more */
+  int pages = -1, pages_s = -1, pages_t = 0;
   for (;; ++walk.slot, walk.j = 0) {
     RowTile x;
     if (!next_row_tile(p, g, few, slots, walk, cur, x)) break;
@@ -1117,9 +1119,10 @@ __device__ __forceinline__ void tiles_body(const aos_kv_attn_params &p, int few,
         pages_s = cur.s;
         pages_t = t & ~63;
         const int pos = (pages_t + lane) * TILE;
-        pages = pos < cur.q.len ? page_of(p.b, cur.s, pos) : -1;
+        pages = pos < cur.q.len ? page_entry(p.b, cur.s, pos) : -1;
       }
-      return __builtin_amdgcn_readlane(pages, t & 63);
+      const int page = __builtin_amdgcn_readlane(pages, t & 63);
+      return t * TILE < cur.q.len ? page_checked(p.b, page) : -1; /* (tile 0 of a sequence without positions) */
     };
     Stage<FMT, HDP> st;
     int pg = page(0);

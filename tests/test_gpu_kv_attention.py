@@ -420,3 +420,18 @@ def test_starts_that_fall(hip, fmt):
         assert pool.cache.faults() == hip.KV_FAULT_BATCH and (got == 7).all()
         _check(_run(pool, q, new, lens), seqs, new, hd ** -0.5)
         assert pool.cache.faults() == 0
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "mxfp4"])
+@pytest.mark.parametrize("new", [1, 3, 14, 90, 700])
+def test_pages_left_of_every_window(hip, fmt, new):
+    """Pages taken back (-1 in the table) since no row sees them any more are no fault; a page that one does see is."""
+    L, window, nh, hd = 5000, 300, 4, 64
+    pool, q, seqs = _setup(hip, fmt, nh, 2, hd, 64, [new], [L])
+    gone = (L - new - window + 1) // 64
+    pool.pages[0, :gone] = -1
+    _check(_run(pool, q, [new], [L], window), seqs, [new], hd ** -0.5, window)
+    assert pool.cache.faults() == 0
+    pool.pages[0, gone] = -1
+    _run(pool, q, [new], [L], window)
+    assert pool.cache.faults() == hip.KV_FAULT_PAGE
