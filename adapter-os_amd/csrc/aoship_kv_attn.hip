@@ -135,9 +135,18 @@ struct OddMarks {
     return x;
   }
 };
-/* weight of a piece whose maximum is m in a sum whose maximum is ms: kept off zero, which an infinity would turn into
- * a NaN */
-__device__ __forceinline__ float piece_weight(float m, float ms) { return fmaxf(ex2(m - ms), 1.17549435e-38f); }
+/* Weight of a piece whose maximum is m in a sum whose maximum is ms. Zero would turn an infinity that the row sees into a
+ * NaN, and a weight kept at 2^-126 would let values near 2^128 count: where there are infinities (MARK), a weight below
+ * that is 2^-126 twice, which leaves less than 2^-123 of anything finite. */
+template <bool MARK>
+struct Weight {
+  float f, g;
+  __device__ __forceinline__ Weight(float m, float ms) : f(ex2(m - ms)), g(1.0f) {
+    constexpr float TINY = 1.17549435e-38f;
+    if (MARK && f < TINY) f = g = TINY;
+  }
+  __device__ __forceinline__ float operator()(float x) const { return MARK ? x * f * g : x * f; }
+};
 
 /* ---- sharing the work ------------------------------------------------------------------------ */
 
@@ -570,12 +579,12 @@ __device__ __forceinline__ void rows_body(const aos_kv_attn_params &p, int few, 
         const float ms = safe_max(top);
         float sum = 0.0f;
 #pragma unroll
-        for (int v = 0; v < 4; ++v) sum = sum + sh.mls[v][1][b][lane] * piece_weight(sh.mls[v][0][b][lane], ms);
-        const float f = piece_weight(m[b], ms);
+        for (int v = 0; v < 4; ++v) sum = sum + Weight<MARK>(sh.mls[v][0][b][lane], ms)(sh.mls[v][1][b][lane]);
+        const Weight<MARK> f(m[b], ms);
 #pragma unroll
         for (int d = 0; d < DB; ++d)
 #pragma unroll
-          for (int k = 0; k < 4; ++k) o[b][d][k] = o[b][d][k] * f;
+          for (int k = 0; k < 4; ++k) o[b][d][k] = f(o[b][d][k]);
         m[b] = top;
         l[b] = sum;
       }
@@ -671,21 +680,22 @@ __device__ __forceinline__ void rows_body(const aos_kv_attn_params &p, int few, 
             float top = m[b];
 #pragma unroll
             for (int i = 0; i < FLY; ++i) top = fmaxf(top, pm[i][b]);
-            const float ms = safe_max(top), f0 = piece_weight(m[b], ms);
-            l[b] = l[b] * f0;
+            const float ms = safe_max(top);
+            const Weight<MARK> f0(m[b], ms);
+            l[b] = f0(l[b]);
 #pragma unroll
             for (int d = 0; d < DB; ++d)
 #pragma unroll
-              for (int e = 0; e < 4; ++e) o[b][d][e] = o[b][d][e] * f0;
+              for (int e = 0; e < 4; ++e) o[b][d][e] = f0(o[b][d][e]);
 #pragma unroll
             for (int i = 0; i < FLY; ++i) {
               if (k0 + 4 * i >= np) continue; /* uniform */
-              const float f = piece_weight(pm[i][b], ms);
-              l[b] = l[b] + pl[i][b] * f;
+              const Weight<MARK> f(pm[i][b], ms);
+              l[b] = l[b] + f(pl[i][b]);
 #pragma unroll
               for (int d = 0; d < DB; ++d)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) o[b][d][e] = o[b][d][e] + y[i][b][d][e] * f;
+                for (int e = 0; e < 4; ++e) o[b][d][e] = o[b][d][e] + f(y[i][b][d][e]);
             }
             m[b] = top;
           }
@@ -1320,12 +1330,12 @@ __device__ __forceinline__ void tiles_body(const aos_kv_attn_params &p, int few,
               y[d][q] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(
                                                       rs, (part(k) + 256 + (((wave * DB + d) * 4 + q) * 64 + lane) * 4) * 4, 0, SC1));
           __builtin_amdgcn_sched_barrier(0);
-          const float f = piece_weight(aos_collect(p.part + part(k) + 64 * wave + col), ms);
-          all = all + aos_collect(p.part + part(k) + 64 * wave + 32 + col) * f;
+          const Weight<MARK> f(aos_collect(p.part + part(k) + 64 * wave + col), ms);
+          all = all + f(aos_collect(p.part + part(k) + 64 * wave + 32 + col));
 #pragma unroll
           for (int d = 0; d < DB; ++d)
 #pragma unroll
-            for (int v = 0; v < 16; ++v) o[d][v] = o[d][v] + y[d][v >> 2][v & 3] * f;
+            for (int v = 0; v < 16; ++v) o[d][v] = o[d][v] + f(y[d][v >> 2][v & 3]);
         }
         const float inv = inverse(all, top);
 #pragma unroll

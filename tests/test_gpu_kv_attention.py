@@ -435,3 +435,25 @@ def test_pages_left_of_every_window(hip, fmt, new):
     pool.pages[0, gone] = -1
     _run(pool, q, [new], [L], window)
     assert pool.cache.faults() == hip.KV_FAULT_PAGE
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "mxfp8"])
+@pytest.mark.parametrize("new", [1, 7, 300])
+@pytest.mark.parametrize("odd", [False, True])
+def test_large_values_far_below_the_maximum(hip, fmt, new, odd):
+    """A long run of positions whose scores lie hundreds below the others' counts for nothing, however large its values
+    (odd: also in a cache that has held an infinity). Their scores are all the same and their probabilities beside each
+    other 1: 2000 of them times 2^116 stay below 2^127."""
+    L, nh, hd = 6000, 4, 128
+
+    def poison(k, v):
+        k[:2000] = 0.0
+        k[:2000, :, 0] = -256.0
+        v[:2000] = 2.0 ** 116
+        if odd:
+            v[L] = np.inf
+
+    pool, q, seqs = _setup(hip, fmt, nh, 1, hd, 64, [new], [L + 1], poison=poison)
+    q[:, :, 0] = 16.0  # (-4096 / sqrt(128) = -362 of a score)
+    _, k, v = seqs[0]
+    _check(_run(pool, q, [new], [L], max_len=L + 1), [(q, k[:L], v[:L])], [new], hd ** -0.5)
