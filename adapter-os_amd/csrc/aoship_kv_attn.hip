@@ -1028,7 +1028,14 @@ struct TilesShared {
 
 template <int FMT, int HDP, bool MARK>
 __device__ __forceinline__ void tiles_body(const aos_kv_attn_params &p, int few, int slots, int min_share, TilesShared &sh) {
-  constexpr int KS = HDP / 16, DB = HDP / 32, STAGE = 4 * TILE * HDP, AHEAD = HDP == 256 ? 4 : 8;
+  constexpr int KS = HDP / 16, DB = HDP / 32, STAGE = 4 * TILE * HDP;
+  /* What keeps the kernel within a wave's registers (workgroups hand pieces to each other: the build refuses private memory
+   * here): fragments read ahead, blocks of 32 dimensions of a piece in flight as it is joined, and, for infinities in wide
+   * quantised heads, the queries read again for each tile and 8-bit tiles fetched in their turn (for other caches that
+   * would be 204 us for 127: 512 tokens over 8000, 16/2 heads of 256, 8 bits). */
+  constexpr int AHEAD = MARK ? 2 : HDP == 256 ? 4 : 8;
+  constexpr int FLY = MARK ? 1 : HDP == 256 ? 2 : FMT == AOS_KV_MXFP8 ? DB / 2 : DB;
+  constexpr bool AGAIN = MARK && HDP == 256 && FMT != AOS_KV_BF16, LATE = AGAIN && FMT == AOS_KV_MXFP8;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 31, half = lane >> 5;
@@ -1138,7 +1145,7 @@ __device__ __forceinline__ void tiles_body(const aos_kv_attn_params &p, int few,
     int pg = page(0);
     st.fetch(tile_ptr<FMT, HDP>(p.b, pg < 0 ? 0 : pg, h, tile0 * TILE), smem, tid);
     u32x4 qf[KS];
-    {
+    auto load_queries = [&]() {
       const uint16_t *qr = p.q + (long long)(cur.q.row0 + t) * p.q_ld + hh * p.b.hd;
 #pragma unroll
       for (int e = 0; e < KS; ++e) {
@@ -1147,7 +1154,8 @@ __device__ __forceinline__ void tiles_body(const aos_kv_attn_params &p, int few,
 #pragma unroll
         for (int i = 0; i < 4; ++i) qf[e][i] ^= flip;
       }
-    }
+    };
+    if (!AGAIN) load_queries();
     st.put(smem, tid);
     for (int i = 0; i < n; ++i) {
       const unsigned char *kt = smem + (i & 1) * STAGE, *vt = kt + TILE * HDP * 2;
@@ -1157,7 +1165,7 @@ __device__ __forceinline__ void tiles_body(const aos_kv_attn_params &p, int few,
       const bool there = pg >= 0;
       if (i + 1 < n) {
         pg = page(i + 1);
-        st.fetch(tile_ptr<FMT, HDP>(p.b, pg < 0 ? 0 : pg, h, (tile0 + i + 1) * TILE), other, tid);
+        if (!LATE) st.fetch(tile_ptr<FMT, HDP>(p.b, pg < 0 ? 0 : pg, h, (tile0 + i + 1) * TILE), other, tid);
       }
       const int k0 = (tile0 + i) * TILE;
       if (MARK && (k0 < wg_lo || k0 + TILE - 1 > wg_hi)) { /* uniform over the workgroup */
@@ -1196,6 +1204,7 @@ __device__ __forceinline__ void tiles_body(const aos_kv_attn_params &p, int few,
         }
       }
       if (there && k0 <= hi_max && k0 + TILE > lo_min && nrows > 0) { /* uniform: some row of the wave sees some of it */
+        if (AGAIN) load_queries();
         const bool edge = k0 < lo_max || k0 + TILE - 1 > hi_min;
         /* LDS reads run AHEAD matrix instructions before their use (the values' first ones before the softmax): left
          * to itself the compiler reads each fragment right before the instruction that waits for it */
@@ -1262,6 +1271,7 @@ __device__ __forceinline__ void tiles_body(const aos_kv_attn_params &p, int few,
           __builtin_amdgcn_sched_barrier(0);
         }
       }
+      if (LATE && i + 1 < n) st.fetch(tile_ptr<FMT, HDP>(p.b, pg < 0 ? 0 : pg, h, (tile0 + i + 1) * TILE), other, tid);
       if (i + 1 < n) st.put(other, tid);
     }
     if (MARK)
@@ -1322,20 +1332,25 @@ __device__ __forceinline__ void tiles_body(const aos_kv_attn_params &p, int few,
 #pragma unroll
         for (int d = 0; d < DB; ++d) o[d] = f32x16{};
         for (int k = 0; k < np; ++k) {
-          f32x4 y[DB][4]; /* (all in flight together) */
-#pragma unroll
-          for (int d = 0; d < DB; ++d)
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-              y[d][q] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(
-                                                      rs, (part(k) + 256 + (((wave * DB + d) * 4 + q) * 64 + lane) * 4) * 4, 0, SC1));
-          __builtin_amdgcn_sched_barrier(0);
           const Weight<MARK> f(aos_collect(p.part + part(k) + 64 * wave + col), ms);
           all = all + f(aos_collect(p.part + part(k) + 64 * wave + 32 + col));
 #pragma unroll
-          for (int d = 0; d < DB; ++d)
+          for (int d0 = 0; d0 < DB; d0 += FLY) {
+            f32x4 y[FLY][4]; /* (all in flight together) */
 #pragma unroll
-            for (int v = 0; v < 16; ++v) o[d][v] = o[d][v] + f(y[d][v >> 2][v & 3]);
+            for (int d = 0; d < FLY; ++d)
+#pragma unroll
+              for (int q = 0; q < 4; ++q)
+                y[d][q] = __builtin_bit_cast(
+                    f32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                               rs, (part(k) + 256 + (((wave * DB + d0 + d) * 4 + q) * 64 + lane) * 4) * 4, 0, SC1));
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int d = 0; d < FLY; ++d)
+#pragma unroll
+              for (int v = 0; v < 16; ++v) o[d0 + d][v] = o[d0 + d][v] + f(y[d][v >> 2][v & 3]);
+            __builtin_amdgcn_sched_barrier(0);
+          }
         }
         const float inv = inverse(all, top);
 #pragma unroll

@@ -33,3 +33,12 @@ def test_guard_rejects_scratch_in_handoff_kernels():
 def test_guard_ignores_other_kernels():
     b = _build_module()
     b._check_resources("x.hip", _remarks("_ZN12_GLOBAL__N_116aos_route_kernelILb1EEEv16aos_route_params", 8))
+
+
+def test_guard_rejects_scratch_in_the_paged_attention():
+    b = _build_module()
+    for k in ("_ZN12_GLOBAL__N_118aos_kv_rows_kernelILi1ELi128ELi1EEEv18aos_kv_attn_paramsii",
+              "_ZN12_GLOBAL__N_119aos_kv_tiles_kernelILi1ELi128EEEv18aos_kv_attn_paramsiii"):
+        with pytest.raises(SystemExit):
+            b._check_resources("x.hip", _remarks(k, 12))
+        b._check_resources("x.hip", _remarks(k, 0))

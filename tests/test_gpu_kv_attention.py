@@ -457,3 +457,36 @@ def test_large_values_far_below_the_maximum(hip, fmt, new, odd):
     q[:, :, 0] = 16.0  # (-4096 / sqrt(128) = -362 of a score)
     _, k, v = seqs[0]
     _check(_run(pool, q, [new], [L], max_len=L + 1), [(q, k[:L], v[:L])], [new], hd ** -0.5)
+
+
+@pytest.mark.parametrize("fmt", P.FORMATS)
+@pytest.mark.parametrize("hd", [80, 128, 256])
+@pytest.mark.parametrize("new", [1, 4, 14, 90])
+def test_infinities_and_nans_in_wide_heads(hip, fmt, hd, new):
+    """As above, in dimensions of every block, and over enough positions that workgroups share a row tile: the
+    marked elements are more than a word of bits there."""
+    nh, nkv, L, window = 4, 2, 900, 700
+    first = L - new
+    dims = [d for d in (0, 5, 33, 63, 79, 95, 127, 128, 191, 255) if d < hd]
+
+    def poison(k, v):
+        for i, d in enumerate(dims):
+            v[first + new // 2, 0, d] = (np.inf, -np.inf, np.nan)[i % 3]  # seen by the second half of the new rows
+            v[first - 100 - 40 * i, 1, d] = (-np.inf, np.nan, np.inf)[i % 3]  # seen by all
+        v[first - 333, 1, dims[-1]] = -np.inf  # (meets a plus infinity of the same dimension, or not)
+        v[L - 1, 1, 1] = np.nan                # seen by the last row only
+        v[:first - window + 1] = np.nan        # left of every window
+        v[L:] = -np.inf                        # (stale rows)
+        k[L:] = np.nan
+
+    pool, q, seqs = _setup(hip, fmt, nh, nkv, hd, 64, [new], [L + 20], poison=poison)
+    _, k, v = seqs[0]
+    got = _run(pool, q, [new], [L], window=window, max_len=960)
+    if fmt == "bf16":
+        _check(got, [(q, k[:L], v[:L])], [new], hd ** -0.5, window)
+    else:
+        o, a = P.attention(q, k[:L], v[:L], hd ** -0.5, window)
+        assert np.array_equal(np.isnan(got), ~np.isfinite(o))
+        fin = np.isfinite(o)
+        assert (np.abs(got - o)[fin] <= P.attention_bound(q, k[:L], a, o, hd ** -0.5)[fin]).all()
+    assert np.array_equal(got, _run(pool, q, [new], [L], window=window, max_len=960), equal_nan=True)
