@@ -737,7 +737,7 @@ class _KVBatch(C.Structure):
 class _KVRows(C.Structure):
     _fields_ = [("q", _P), ("k", _P), ("v", _P), ("q_stride", C.c_int64), ("k_stride", C.c_int64),
                 ("v_stride", C.c_int64), ("q_bias", _P), ("k_bias", _P), ("v_bias", _P), ("q_out", _P),
-                ("q_out_stride", C.c_int64), ("num_heads", C.c_int)]
+                ("q_out_stride", C.c_int64), ("num_heads", C.c_int), ("rotated", C.c_int)]
 
 
 class KVBatch:
@@ -828,9 +828,9 @@ class KVCache:
         return t.data_ptr(), stride[0] if n > 1 else shape[1] * hd
 
     def append(self, layer: int, batch: KVBatch, k, v, q=None, q_out=None, q_bias=None, k_bias=None,
-               v_bias=None) -> None:
+               v_bias=None, rotated: bool = False) -> None:
         """Biases (device float32 [heads, head_dim]) and rotary embedding of the new rows; k and v go into the pages,
-        q to q_out."""
+        q to q_out. rotated: the rows are rotated already (rows that read returned, written again)."""
         if (q is None) != (q_out is None):
             raise AosError("KVCache.append: q and q_out come together")
         r, nkv, n = self._rows, self.num_kv_heads, k.shape[0]
@@ -842,7 +842,7 @@ class KVCache:
             r.q, r.q_stride = self._row(q, n)
             nh = q.shape[1]
             r.q_out, r.q_out_stride = (r.q, r.q_stride) if q_out is q else self._row(q_out, n, nh)
-        r.num_heads = nh
+        r.num_heads, r.rotated = nh, rotated
         r.q_bias = None if q_bias is None else self._bias(q_bias, nh)
         r.k_bias = None if k_bias is None else self._bias(k_bias, nkv)
         r.v_bias = None if v_bias is None else self._bias(v_bias, nkv)

@@ -3621,7 +3621,7 @@ static int kv_append_check(const aoship_kv_config_t &c, int rope_positions, int 
     return set_err(what + ": biases must be 16-byte aligned");
   if (r->q && r->q_out == r->q && r->q_out_stride != r->q_stride)
     return set_err(what + ": q_out in the place of q needs its stride");
-  if (rope_positions && batch->max_len > rope_positions)
+  if (rope_positions && !r->rotated && batch->max_len > rope_positions)
     return set_err(what + ": max_len passes the rotary tables (" + std::to_string(rope_positions) + " positions)");
   return 0;
 }
@@ -3695,8 +3695,8 @@ extern "C" int aoship_kv_append(aoship_kv_cache_t *m, int layer, const aoship_kv
   p.qb = r->q_bias;
   p.kb = r->k_bias;
   p.vb = r->v_bias;
-  p.cosines = m->rope_positions ? m->rope.as<float>() : nullptr;
-  p.sines = m->rope_positions ? p.cosines + (size_t)m->rope_positions * (size_t)(m->cfg.head_dim / 2) : nullptr;
+  p.cosines = m->rope_positions && !r->rotated ? m->rope.as<float>() : nullptr;
+  p.sines = p.cosines ? p.cosines + (size_t)m->rope_positions * (size_t)(m->cfg.head_dim / 2) : nullptr;
   p.q_out = r->q_out;
   p.nh = r->num_heads;
   const aos_launch_ctx ctx = {m->stream, nullptr, nullptr};

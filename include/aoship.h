@@ -429,7 +429,9 @@ typedef struct {
 /* Rows of a call (device): row t at q + t * q_stride (elements, multiples of 8; pointers 16-byte aligned), its heads
  * head_dim apart, so that the projections' outputs and slices of a joint one both serve. Biases are device float32
  * [heads * head_dim] or NULL. q, q_out and num_heads (a multiple of num_kv_heads) are 0 where there are no queries;
- * q_out may be q. */
+ * q_out may be q. `rotated` is 0, or nonzero where the rows are rotated already, as those that aoship_kv_read returned
+ * are: append then rotates none of them (biases are still added), so that a sequence read back can be written again,
+ * to other pages or another cache, and holds what it held (but for a block that reads back with an infinity: NaN). */
 typedef struct {
   const aoship_bf16_t *q, *k, *v;
   int64_t q_stride, k_stride, v_stride;
@@ -437,6 +439,7 @@ typedef struct {
   aoship_bf16_t *q_out;
   int64_t q_out_stride;
   int num_heads;
+  int rotated;
 } aoship_kv_rows_t;
 
 /* Biases and rotary embedding of the new rows (float32; (a, b) -> (a c - b s, a s + b c) over the halves of a query

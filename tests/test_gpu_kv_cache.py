@@ -265,3 +265,36 @@ def test_a_new_cache_on_another_stream(hip):
     cache.read(0, batch, *back)
     torch.cuda.synchronize()
     assert np.array_equal(P.to_cpu(back[0]), -x[0]) and np.array_equal(P.to_cpu(back[1]), x[1])
+
+
+@pytest.mark.parametrize("fmt", P.FORMATS)
+def test_there_and_back_again(hip, fmt):
+    """Streams read out of a cache with rotary tables and written to other pages hold, and attend to, what they did."""
+    import torch
+
+    rng = np.random.default_rng(6)
+    nh, nkv, hd, lens = 4, 2, 128, [70, 1, 200]
+    T = sum(lens)
+    pool = P.Pool(hip, lens, nkv, hd, 64, fmt)
+    other = P.Pool(hip, lens, nkv, hd, 128, fmt, seed=1)
+    cos, sin = (f(np.arange(200)[:, None] * 3.0 ** -np.arange(hd // 2)).astype(np.float32) for f in (np.cos, np.sin))
+    for p in (pool, other):
+        p.cache.set_rope(cos, sin)
+    q, k, v = (P.to_gpu(_rows(rng, T, h, hd)) for h in (nh, nkv, nkv))
+    turned = torch.empty_like(q)
+    pool.cache.append(0, pool.batch(lens, lens), k, v, q=q, q_out=turned)
+    held = [torch.empty_like(k) for _ in range(2)]
+    pool.cache.read(0, pool.batch(lens, lens), *held)
+    again, back = torch.empty_like(q), [torch.empty_like(k) for _ in range(2)]
+    other.cache.append(0, other.batch(lens, lens), *held, q=turned, q_out=again, rotated=True)
+    other.cache.read(0, other.batch(lens, lens), *back)
+    assert torch.equal(turned.view(torch.int16), again.view(torch.int16))
+    out = [torch.empty_like(q) for _ in range(2)]
+    for p, o in zip((pool, other), out):
+        p.cache.attention(0, p.batch(lens, lens), turned, o)
+        assert p.cache.faults() == 0
+    for a, b in zip((*held, out[0]), (*back, out[1])):
+        assert torch.equal(a.view(torch.int16), b.view(torch.int16))
+    pool.cache.append(0, pool.batch(lens, lens), k, v)  # (the next call rotates again)
+    pool.cache.read(0, pool.batch(lens, lens), *back)
+    assert torch.equal(held[0].view(torch.int16), back[0].view(torch.int16))

@@ -293,3 +293,8 @@ def test_starts_outside_the_rows_leave_the_others(starts, good, g):
     lens = [500, 610, 600, 700, 900, 64]
     got = _pieces(2 * g, 2, starts, lens, 1000, 1000, 1000)
     _check_pieces(got, _row_tiles(2 * g, 2, starts, [n if s in good else None for s, n in enumerate(lens)], 0, 0))
+
+
+def test_rotated_rows_need_no_tables():
+    assert C.sizeof(aoship._KVRows) == 96
+    assert _append(rope=639) == -1 and _append(rope=639, rows=_rows(rotated=1)) == 0
