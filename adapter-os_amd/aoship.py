@@ -751,6 +751,8 @@ class KVBatch:
         for t, dims in ((starts, 1), (lens, 1), (pages, 2)):
             if t.dtype != torch.int32 or t.dim() != dims or not t.is_cuda or (t.numel() and t.stride(-1) != 1):
                 raise AosError("KVBatch: starts, lens [n] and pages [n, stride] must be device int32 tensors")
+        if starts.get_device() != lens.get_device() or pages.get_device() != lens.get_device():
+            raise AosError("KVBatch: starts, lens and pages must be on one device")
         n = lens.numel()
         if starts.numel() != n + 1 or pages.shape[0] != n:
             raise AosError("KVBatch: starts must have one entry more than lens, pages a row for each")

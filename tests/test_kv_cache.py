@@ -298,3 +298,34 @@ def test_starts_outside_the_rows_leave_the_others(starts, good, g):
 def test_rotated_rows_need_no_tables():
     assert C.sizeof(aoship._KVRows) == 96
     assert _append(rope=639) == -1 and _append(rope=639, rows=_rows(rotated=1)) == 0
+
+
+class _Tensor:
+    """What KVBatch looks at of an int32 tensor on a device."""
+
+    def __init__(self, device, *shape):
+        import torch
+
+        self.dtype, self.is_cuda, self.shape, self.device = torch.int32, True, shape, device
+
+    def dim(self):
+        return len(self.shape)
+
+    def numel(self):
+        return int(np.prod(self.shape))
+
+    def stride(self, i):
+        return 1 if i in (-1, len(self.shape) - 1) else self.shape[-1]
+
+    def data_ptr(self):
+        return ALIGNED
+
+    def get_device(self):
+        return self.device
+
+
+def test_a_batch_is_on_one_device():
+    aoship.KVBatch(_Tensor(1, 4), _Tensor(1, 3), _Tensor(1, 3, 8), 5, 500)
+    for devices in ((0, 1, 1), (1, 0, 1), (1, 1, 0)):
+        with pytest.raises(aoship.AosError, match="device"):
+            aoship.KVBatch(*(_Tensor(d, *s) for d, s in zip(devices, ((4,), (3,), (3, 8)))), 5, 500)
