@@ -34,10 +34,14 @@ static int set_err(const std::string &s) {
   return -1;
 }
 
+/* (the runtime keeps a failed call's error until it is asked for: the next launch would be reported as failed) */
 #define HIP_OR_FAIL(expr, what)                                                        \
   do {                                                                                 \
     hipError_t e_ = (expr);                                                            \
-    if (e_ != hipSuccess) return set_err(std::string(what) + ": " + hipGetErrorString(e_)); \
+    if (e_ != hipSuccess) {                                                            \
+      (void)hipGetLastError();                                                         \
+      return set_err(std::string(what) + ": " + hipGetErrorString(e_));                \
+    }                                                                                  \
   } while (0)
 
 extern "C" const char *aoship_get_last_error(void) { return g_last_error.c_str(); }
@@ -720,6 +724,7 @@ extern "C" aoship_layer_t *aoship_layer_new(int layer_idx, int group_size, int b
   }
   void *wh = nullptr;
   if (hipHostMalloc(&wh, 256, hipHostMallocCoherent | hipHostMallocMapped) != hipSuccess) {
+    (void)hipGetLastError();
     set_err("aoship_layer_new: hipHostMalloc failed");
     delete l;
     return nullptr;

@@ -298,3 +298,28 @@ def test_there_and_back_again(hip, fmt):
     pool.cache.append(0, pool.batch(lens, lens), k, v)  # (the next call rotates again)
     pool.cache.read(0, pool.batch(lens, lens), *back)
     assert torch.equal(held[0].view(torch.int16), back[0].view(torch.int16))
+
+
+def _turned(hip, fails):
+    """A cache whose tables negate the keys; what `fails` does to it is refused, and its calls are as before."""
+    import torch
+
+    hd, n = 256, 20
+    pool = P.Pool(hip, [n], 1, hd, 64, "bf16")
+    x = P.bf16(np.random.default_rng(0).standard_normal((n, 1, hd)))
+    k, batch = P.to_gpu(x), pool.batch([n], [n])
+    back = [torch.empty_like(k) for _ in range(2)]
+    zeros = np.zeros((n, hd // 2), np.float32)
+    pool.cache.set_rope(zeros - 1, zeros)
+    with pytest.raises(hip.AosError, match="out of memory"):
+        fails(pool.cache)
+    pool.cache.append(0, batch, k, k)
+    pool.cache.read(0, batch, *back)
+    _same(P.to_cpu(back[0]), -x)
+    _same(P.to_cpu(back[1]), x)
+    assert pool.cache.faults() == 0
+
+
+def test_a_cache_that_does_not_fit(hip):
+    """Its failed allocation is no later call's error."""
+    _turned(hip, lambda cache: hip.KVCache(1, 8, 128, 256, 2000000, "bf16"))
