@@ -3533,16 +3533,16 @@ extern "C" int aoship_kv_cache_set_rope(aoship_kv_cache_t *m, const float *cosin
   if (!m || (!cosines != !sines) || (cosines && positions < 1))
     return set_err("aoship_kv_cache_set_rope: null cache, one table without the other, or no positions");
   if (kv_check(m, "aoship_kv_cache_set_rope")) return -1;
+  DevBuf rope; /* (a call that fails leaves the old tables) */
+  if (cosines) {
+    const size_t table = (size_t)positions * (size_t)(m->cfg.head_dim / 2) * sizeof(float);
+    if (rope.alloc(2 * table, false)) return -1;
+    HIP_OR_FAIL(hipMemcpy(rope.p, cosines, table, hipMemcpyHostToDevice), "hipMemcpy H2D");
+    HIP_OR_FAIL(hipMemcpy(rope.as<unsigned char>() + table, sines, table, hipMemcpyHostToDevice), "hipMemcpy H2D");
+  }
   HIP_OR_FAIL(hipDeviceSynchronize(), "hipDeviceSynchronize"); /* (a launch may still read the old tables) */
-  m->rope_positions = 0;
-  m->rope.release();
-  if (!cosines) return 0;
-  const size_t table = (size_t)positions * (size_t)(m->cfg.head_dim / 2) * sizeof(float);
-  if (m->rope.alloc(2 * table, false)) return -1;
-  HIP_OR_FAIL(hipMemcpy(m->rope.p, cosines, table, hipMemcpyHostToDevice), "hipMemcpy H2D");
-  HIP_OR_FAIL(hipMemcpy(m->rope.as<unsigned char>() + table, sines, table, hipMemcpyHostToDevice), "hipMemcpy H2D");
-  HIP_OR_FAIL(hipDeviceSynchronize(), "hipDeviceSynchronize");
-  m->rope_positions = positions;
+  m->rope = std::move(rope);
+  m->rope_positions = cosines ? positions : 0;
   return 0;
 }
 

@@ -393,7 +393,8 @@ aoship_kv_cache_t *aoship_kv_cache_new(const aoship_kv_config_t *config);
 void aoship_kv_cache_free(aoship_kv_cache_t *cache);
 
 /* Rotary embedding of aoship_kv_append: cosines and sines [positions][head_dim / 2] (host, copied); NULL for both:
- * none, as at first. Synchronises the device; graphs captured before hold the old tables, which are gone.
+ * none, as at first. Synchronises the device; graphs captured before hold the old tables, which are gone. A call that
+ * fails leaves the tables that were set.
  * Returns 0 / -1. */
 int aoship_kv_cache_set_rope(aoship_kv_cache_t *cache, const float *cosines, const float *sines, int positions);
 

@@ -323,3 +323,13 @@ def _turned(hip, fails):
 def test_a_cache_that_does_not_fit(hip):
     """Its failed allocation is no later call's error."""
     _turned(hip, lambda cache: hip.KVCache(1, 8, 128, 256, 2000000, "bf16"))
+
+
+def test_tables_that_do_not_fit(hip):
+    """The tables that were set stay."""
+    def fails(cache):
+        few = np.zeros((1, 128), np.float32)  # (not read: the allocation comes first)
+        if hip.lib().aoship_kv_cache_set_rope(cache.h, few.ctypes.data, few.ctypes.data, 2 ** 31 - 1):
+            raise hip.AosError(hip.last_error())
+
+    _turned(hip, fails)
