@@ -458,8 +458,10 @@ int aoship_kv_read(aoship_kv_cache_t *cache, int layer, const aoship_kv_batch_t 
  * positions j up to the row's own p, and past p - window (0: all); query heads share key/value heads in
  * consecutive groups. A row that sees nothing gives zeros. q, out: device rows of num_heads * head_dim (out must
  * not overlap q). Probabilities times values are summed in float32 before the division by their sum: magnitudes above
- * some 2^90 can come out as infinities or NaN. An infinity or a NaN reaches the rows that see its position and no others; once one has been appended
- * to a cache's values, attention over it takes somewhat longer. Asynchronous. Returns 0 / -1. */
+ * some 2^90 can come out as infinities or NaN. An infinity or a NaN reaches the rows that see its position and no others;
+ * a quantised value whose code stands for 2^128 (aoship_kv_read: infinity) counts as an infinity or as that number. Once
+ * an infinity or a NaN has been appended to a cache's values, attention over it takes somewhat longer. Asynchronous.
+ * Returns 0 / -1. */
 int aoship_kv_attention(aoship_kv_cache_t *cache, int layer, const aoship_kv_batch_t *batch, const aoship_bf16_t *q,
                         int64_t q_stride, int num_heads, float scale, int window, aoship_bf16_t *out,
                         int64_t out_stride);

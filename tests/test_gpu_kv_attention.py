@@ -490,3 +490,24 @@ def test_infinities_and_nans_in_wide_heads(hip, fmt, hd, new):
         fin = np.isfinite(o)
         assert (np.abs(got - o)[fin] <= P.attention_bound(q, k[:L], a, o, hd ** -0.5)[fin]).all()
     assert np.array_equal(got, _run(pool, q, [new], [L], window=window, max_len=960), equal_nan=True)
+
+
+@pytest.mark.parametrize("fmt", ["mxfp8", "mxfp4"])
+@pytest.mark.parametrize("new", [2, 12, 90])
+def test_largest_values_where_they_are_seen(hip, fmt, new):
+    """The row that sees a value whose code stands for 2^128 takes it as that number or as infinity, the rest of its
+    dimensions and the other heads as they are."""
+    def poison(k, v):
+        v[229, 1, 40] = P.bf16([3.3895e38])[0]
+        k[229] = 0.0
+
+    pool, q, seqs = _setup(hip, fmt, 4, 2, 64, 64, [new], [230], poison=poison)
+    got = _run(pool, q, [new], [230])[-1]
+    q, k, v = seqs[0]
+    assert np.isinf(v).sum() == 1
+    v = np.where(np.isinf(v), 2.0 ** 128, v)
+    o, a = P.attention(q[-1:], k, v, 64 ** -0.5)
+    near = np.abs(got - o[0]) <= P.attention_bound(q, k, a, o, 64 ** -0.5)[0]
+    top = np.zeros_like(near)
+    top[2:, 40] = True
+    assert (near | (top & (got == np.inf))).all()
