@@ -3662,7 +3662,7 @@ static int kv_attention_check(const aoship_kv_config_t &c, int layer, const aosh
   size.nkv = c.num_kv_heads;
   size.n_seqs = batch->n_seqs;
   size.n_tokens = batch->n_tokens;
-  size.max_new = batch->max_new;
+  size.max_new = batch->max_new < batch->n_tokens ? batch->max_new : batch->n_tokens;
   size.max_len = batch->max_len;
   if (!aos_kv_attention_fits(&size, num_heads)) return set_err(what + ": rows times positions of the batch too large");
   return 0;

@@ -329,3 +329,9 @@ def test_a_batch_is_on_one_device():
     for devices in ((0, 1, 1), (1, 0, 1), (1, 1, 0)):
         with pytest.raises(aoship.AosError, match="device"):
             aoship.KVBatch(*(_Tensor(d, *s) for d, s in zip(devices, ((4,), (3,), (3, 8)))), 5, 500)
+
+
+def test_bounds_beyond_the_rows():
+    """max_new bounds a sequence's rows: any number past n_tokens bounds them as n_tokens does."""
+    assert _attention(batch=_batch(max_new=2 ** 31 - 1)) == 0
+    assert _read(batch=_batch(max_new=2 ** 31 - 1)) == 0 and _append(batch=_batch(max_new=2 ** 31 - 1)) == 0
