@@ -3651,7 +3651,8 @@ static int kv_attention_check(const aoship_kv_config_t &c, int layer, const aosh
   if (num_heads < 1 || num_heads % c.num_kv_heads || num_heads > 65536)
     return set_err(what + ": num_heads must be a multiple of num_kv_heads");
   if (window < 0) return set_err(what + ": negative window");
-  if (!std::isfinite(scale)) return set_err(what + ": scale must be finite");
+  if (!std::isfinite(scale * 1.44269504f)) /* (the kernels' scores are powers of two) */
+    return set_err(what + ": scale must be finite, and so must scale * log2(e)");
   if (empty) return 1;
   const long long qw = (long long)num_heads * c.head_dim;
   if (!kv_rows_ok(q, q_stride, qw) || !kv_rows_ok(out, out_stride, qw))

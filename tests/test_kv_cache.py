@@ -335,3 +335,10 @@ def test_bounds_beyond_the_rows():
     """max_new bounds a sequence's rows: any number past n_tokens bounds them as n_tokens does."""
     assert _attention(batch=_batch(max_new=2 ** 31 - 1)) == 0
     assert _read(batch=_batch(max_new=2 ** 31 - 1)) == 0 and _append(batch=_batch(max_new=2 ** 31 - 1)) == 0
+
+
+def test_scales_that_overflow():
+    """Scores are taken in powers of two: a scale whose product with log2 e is no float32 would make every score NaN."""
+    for s in (2.4e38, -2.4e38, 3.4e38):
+        assert _attention(scale=s) == -1 and "scale" in aoship.last_error()
+    assert _attention(scale=2.3e38) == 0 and _attention(scale=-2.3e38) == 0
