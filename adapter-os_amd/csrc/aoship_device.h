@@ -42,7 +42,9 @@ __device__ __forceinline__ f32x16 aos_mfma32(u32x4 a, u32x4 b, f32x16 c) {
  * used wherever fewer than 16 result registers are read. Operand holds are used in the one-token
  * MLP launch, where (2) was measured; in the streaming GEMV and shrink loops they would keep 32-48
  * more registers live (three waves per SIMD to two, the 7B gate/up GEMV 25 to 34 us), and those
- * kernels' outputs are checked run to run and against the oracle by the GPU tests instead. */
+ * kernels' outputs are checked run to run and against the oracle by the GPU tests instead. So are those
+ * of the attention over the paged cache, which reads all of its results and whose registers are full
+ * (aoship_kv_attn.hip). */
 __device__ __forceinline__ void aos_mfma_hold(const f32x16 &t) {
   float u = t[0];
   asm volatile("" : "+v"(u) : "v"(t));

@@ -8,6 +8,11 @@
  * in one pass over the tiles of 64 positions with the running m and sum in float32. The new tokens of a sequence
  * and the query heads that share a key/value head are one list of rows (token, head), so a tile is read once for
  * all of them.
+ *
+ * Matrix instructions' registers (aoship_device.h): every accumulator register is read, so results need no hold. Operands,
+ * some of which vector instructions have just converted, are not held until the results are read: that would take
+ * registers which the kernels do not have (256 of 256 and no private memory). The tests check the outputs with the whole
+ * chip multiplying and converting at once, in every format, against float64 and run to run, bit for bit.
  */
 #include "aoship_internal.h"
 #include "aoship_kv.h"

@@ -511,3 +511,44 @@ def test_largest_values_where_they_are_seen(hip, fmt, new):
     top = np.zeros_like(near)
     top[2:, 40] = True
     assert (near | (top & (got == np.inf))).all()
+
+
+@pytest.mark.parametrize("fmt", P.FORMATS)
+@pytest.mark.parametrize("new,count", [(1, 96), (4, 64), (400, 5)])
+@pytest.mark.parametrize("odd", [False, True])
+def test_with_the_chip_full(hip, fmt, new, count, odd):
+    """Waves that convert and multiply side by side on every SIMD: float64 of what the cache holds, and the same bits
+    each time (odd: the bodies for caches that have held an infinity)."""
+    import torch
+
+    nh, nkv, hd = 28, 4, 128
+    rng = np.random.default_rng(count)
+    lens = [int(n) for n in rng.integers(1200, 2500, count)]
+    pool = P.Pool(hip, [*lens, 1], nkv, hd, 64, fmt)
+    gen = torch.Generator(device="cuda").manual_seed(count)
+    k, v = (torch.randn((sum(lens), nkv, hd), generator=gen, device="cuda").bfloat16() for _ in range(2))
+    q = torch.randn((count * new, nh, hd), generator=gen, device="cuda").bfloat16()
+    pool.cache.append(0, pool.batch([*lens, 0], [*lens, 0]), k, v)
+    if odd:  # (in a page of a sequence that is not among the others)
+        bad = torch.full((1, nkv, hd), float("inf"), dtype=torch.bfloat16, device="cuda")
+        pool.cache.append(0, pool.batch([0] * count + [1], [0] * count + [1]), bad, bad)
+    pool.cache.read(0, pool.batch([*lens, 0], [*lens, 0]), k, v)
+    batch = pool.batch([new] * count + [0], [*lens, 0])
+    outs = [torch.empty_like(q) for _ in range(6)]
+    for out in outs:
+        pool.cache.attention(0, batch, q, out)
+    assert pool.cache.faults() == 0
+    assert all(torch.equal(out.view(torch.int16), outs[0].view(torch.int16)) for out in outs)
+    at = 0
+    for s, n in enumerate(lens):
+        ks, vs = (x[at:at + n].double().transpose(0, 1).contiguous() for x in (k, v))
+        at += n
+        rows = slice(s * new, (s + 1) * new)
+        qs = q[rows].double().view(new, nkv, -1, hd).permute(1, 0, 2, 3).reshape(nkv, -1, hd)
+        sc = torch.matmul(qs, ks.transpose(1, 2).contiguous()) * hd ** -0.5
+        hidden = torch.arange(n, device="cuda") > (n - new + torch.arange(new, device="cuda"))[:, None]
+        p = torch.softmax(sc.view(nkv, new, -1, n).masked_fill(hidden[None, :, None], float("-inf")).flatten(1, 2), -1)
+        o, a = torch.matmul(p, vs), torch.matmul(p, vs.abs())
+        d = (hd + 4) * 2.0 ** -24 * hd ** -0.5 * qs.abs().sum(-1).max() * ks.abs().max()  # (as attention_bound)
+        got = outs[0][rows].double().view(new, nkv, -1, hd).permute(1, 0, 2, 3).reshape(nkv, -1, hd)
+        assert ((got - o).abs() <= 2.0 ** -8 * o.abs() + (2.0 ** -8 + 2.2 * d + 2.0 ** -14) * a + 1e-30).all()
