@@ -202,8 +202,9 @@ constexpr int SNAP = 3;
  * Bound by reading the cache once, by latency where that is little. Keys and values go straight to registers, the next
  * tile's on their way while one is worked on: a tile is used by one workgroup's one or two matrix instructions a block,
  * which LDS would not speed up. 64 streams of up to 16001 positions, 28/4 heads of 128: 16 bits 228 us, 5.7 TB/s; 32 of up
- * to 8191, 24/8 heads, 8 bits: 73 us, 4.6 TB/s; 24 of 32768, 40/8 heads, 4 bits: 122 us, 4.7 TB/s (a quarter fewer of a
- * decoded tile's 470 vector instructions: 1%). */
+ * to 8191, 24/8 heads, 8 bits: 73 us, 4.6 TB/s; 24 of 32768, 40/8 heads, 4 bits: 122 us, 4.7 TB/s. The quantised ones wait
+ * half of the waves' time with half as many bytes on their way (67 KB a CU for 128): not memory's limit, which 16 bits
+ * come nearer, nor the vector instructions' (a quarter fewer of a decoded tile's 470: 1%). */
 template <int FMT, int HDP>
 struct Tile { /* a tile's keys and values in registers */
   static constexpr int KW = HDP * bits<FMT>() / 128; /* words of a key row's quarter */
@@ -751,9 +752,10 @@ __global__ void __launch_bounds__(256, rows_waves(FMT, HDP, NB)) aos_kv_rows_ker
  * The workgroups share all (key/value head, row tile, position tile) evenly; where a row tile is cut, its pieces meet
  * as in the kernel above. Neighbouring shares, which read the same keys, go to one XCD.
  *
- * Bound by the matrix cores. Prompt of 4076 tokens, 28/4 heads of 128, 16 bits: 141 us, 850 TFLOP/s (long prompts 1000, a
- * large library product 1140 on the same card); 512 tokens over 15872, 40/8 heads, 8 bits: 200 us, 850 TFLOP/s. With
- * fragments read from LDS just before each matrix instruction 200 us for 151, with row tiles dealt whole 210. */
+ * Bound by the matrix cores. Prompt of 4076 tokens, 28/4 heads of 128, 16 bits: 142 us, 840 TFLOP/s (16304 tokens 1890 us,
+ * 1010; a large library product 1140 on the same card); 512 tokens over 15872, 40/8 heads, 8 bits: 202 us, 830 TFLOP/s.
+ * Other cards took up to 155 and 215 us. With fragments read from LDS just before each matrix instruction 200 us for 151,
+ * with row tiles dealt whole 210. */
 constexpr int TR = 128;         /* rows of a row tile */
 constexpr int tiles_per_cu(int hdp) { return hdp == 256 ? 1 : 2; }
 

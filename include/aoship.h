@@ -457,11 +457,16 @@ int aoship_kv_read(aoship_kv_cache_t *cache, int layer, const aoship_kv_batch_t 
 /* Attention of the new rows (already appended) over their sequences: o = sum_j softmax_j(scale q . k_j) v_j over the
  * positions j up to the row's own p, and past p - window (0: all); query heads share key/value heads in
  * consecutive groups. A row that sees nothing gives zeros. q, out: device rows of num_heads * head_dim (out must
- * not overlap q). Probabilities times values are summed in float32 before the division by their sum: magnitudes above
- * some 2^90 can come out as infinities or NaN. An infinity or a NaN reaches the rows that see its position and no others;
- * a quantised value whose code stands for 2^128 (aoship_kv_read: infinity) counts as an infinity or as that number. Once
- * an infinity or a NaN has been appended to a cache's values, attention over it takes somewhat longer. Asynchronous.
- * Returns 0 / -1. */
+ * not overlap q). Scores, probabilities and sums are float32; each probability is rounded to bfloat16 (by at most 2^-8 of
+ * it, beside its exact sum) where it multiplies a value, and the result at the end. Probabilities times values are summed
+ * before the division by their sum: magnitudes above some 2^90 can come out as infinities or NaN. The order of these sums
+ * follows from the whole batch (its sequences' rows and lengths, and the device): the same call gives the same bits each
+ * time, but a sequence among other neighbours may differ in its last bits.
+ * An infinity or a NaN reaches the rows that see its position and no others (an infinity whose probability rounds to zero,
+ * as NaN or as itself); a quantised value whose code stands for 2^128 (aoship_kv_read: infinity) counts as an infinity or
+ * as that number. Once an infinity or a NaN has been appended to a cache's values, attention over that cache takes longer
+ * until it is freed (0 to 20%; few rows at 16 bits up to 1.6 times, many rows over quantised heads wider than 128 1.7
+ * times). Asynchronous. Returns 0 / -1. */
 int aoship_kv_attention(aoship_kv_cache_t *cache, int layer, const aoship_kv_batch_t *batch, const aoship_bf16_t *q,
                         int64_t q_stride, int num_heads, float scale, int window, aoship_bf16_t *out,
                         int64_t out_stride);
