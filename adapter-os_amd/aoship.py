@@ -84,6 +84,11 @@ _SIGS = {
     "aoship_model_reset_cache": (C.c_int, [_P]),
     "aoship_model_cache_len": (C.c_int, [_P]),
     "aoship_model_forward": (C.c_int, [_P, _P, C.c_int, C.c_int, _P, _P]),
+    "aoship_model_score": (C.c_int, [_P, _P, C.c_int, C.c_int, _P, _P, _P, _P]),
+    "aoship_logprobs_new": (_P, []),
+    "aoship_logprobs_free": (None, [_P]),
+    "aoship_logprobs_set_stream": (C.c_int, [_P, _P]),
+    "aoship_logprobs": (C.c_int, [_P, _P, C.c_int, C.c_int, C.c_int, C.c_int64, _P, _P]),
     "aoship_kv_cache_new": (_P, [_P]),
     "aoship_kv_cache_free": (None, [_P]),
     "aoship_kv_cache_set_rope": (C.c_int, [_P, _P, _P, C.c_int]),
@@ -712,11 +717,77 @@ class Model:
         _check(lib().aoship_model_forward(self.h, _ptr(ids), T, off, _ptr(rings), _ptr(logits)),
                "aoship_model_forward")
 
+    def score(self, ids, rings, targets=None, logprob=None, entropy=None, rank=None, top_ids=None, top_logprobs=None,
+              logits=None, position_offset: int | None = None) -> None:
+        """forward() with, for every token, what the model gives after it: the log probability and the rank of
+        targets [T], the entropy and the most probable tokens (outputs as of LogProbs). logits: device float32 [vocab]
+        for the last token's, or None."""
+        T = ids.numel()
+        out, tp = _logprobs_out("Model.score", T, targets, logprob, entropy, rank, top_ids, top_logprobs)
+        off = self.cache_len() if position_offset is None else position_offset
+        _check(lib().aoship_model_score(self.h, _ptr(ids), T, off, _ptr(rings), tp, C.byref(out), _ptr(logits)),
+               "aoship_model_score")
+
     def __del__(self):
         if getattr(self, "h", None) and _lib is not None:
             for layer in getattr(self, "layers", []):
                 layer.h = None
             _lib.aoship_model_free(self.h)
+            self.h = None
+
+
+LOGPROBS_MAX_TOP = 32
+
+
+class _LogProbsOut(C.Structure):
+    """aoship_logprobs_out_t"""
+    _fields_ = [("logprob", _P), ("rank", _P), ("entropy", _P), ("top_ids", _P), ("top_logprobs", _P), ("n_top", C.c_int)]
+
+
+def _logprobs_out(what: str, T: int, targets, logprob, entropy, rank, top_ids, top_logprobs):
+    """(the outputs' struct, the targets' pointer), checked: device tensors of T rows, contiguous."""
+    import torch
+
+    n = next((t.shape[-1] for t in (top_ids, top_logprobs) if t is not None and t.dim() == 2), 0)
+    for t, kind, shape in ((targets, torch.int32, (T,)), (logprob, torch.float32, (T,)), (entropy, torch.float32, (T,)),
+                           (rank, torch.int32, (T,)), (top_ids, torch.int32, (T, n)), (top_logprobs, torch.float32, (T, n))):
+        if t is not None and (t.dtype != kind or tuple(t.shape) != shape or not t.is_contiguous()
+                              or t.get_device() != _initialised):
+            raise AosError(f"{what}: targets and rank [T], logprob and entropy [T], top_ids and top_logprobs [T, n] must be "
+                           "contiguous int32 and float32 tensors on the device")
+    return _LogProbsOut(_ptr(logprob), _ptr(rank), _ptr(entropy), _ptr(top_ids), _ptr(top_logprobs), n), _ptr(targets)
+
+
+class LogProbs:
+    """aoship_logprobs_t: log probabilities, ranks, entropies and most probable tokens of rows of logits."""
+
+    def __init__(self):
+        self.h = lib().aoship_logprobs_new()
+        if not self.h:
+            raise AosError(f"aoship_logprobs_new: {last_error()}")
+
+    def set_stream(self, stream_ptr) -> None:
+        _check(lib().aoship_logprobs_set_stream(self.h, stream_ptr), "aoship_logprobs_set_stream")
+
+    def __call__(self, logits, targets=None, logprob=None, entropy=None, rank=None, top_ids=None,
+                 top_logprobs=None) -> None:
+        """logits: device float32 or bfloat16 [T, vocab] (rows may be set apart); targets: device int32 [T]. Outputs, each
+        may be None: logprob, entropy float32 [T], rank int32 [T], top_ids int32 and top_logprobs float32 [T, n]."""
+        import torch
+
+        if logits.dim() != 2 or logits.dtype not in (torch.float32, torch.bfloat16) \
+                or logits.get_device() != _initialised or (logits.shape[1] > 1 and logits.stride(1) != 1):
+            raise AosError("LogProbs: logits must be a float32 or bfloat16 tensor [T, vocab] on the device, the logits of a "
+                           "row side by side")
+        T, vocab = logits.shape
+        out, tp = _logprobs_out("LogProbs", T, targets, logprob, entropy, rank, top_ids, top_logprobs)
+        if _lib.aoship_logprobs(self.h, logits.data_ptr(), logits.dtype is torch.bfloat16, T, vocab,
+                                logits.stride(0) if T > 1 else vocab, tp, C.byref(out)):
+            raise AosError(f"aoship_logprobs: {last_error()}")
+
+    def __del__(self):
+        if getattr(self, "h", None) and _lib is not None:
+            _lib.aoship_logprobs_free(self.h)
             self.h = None
 
 

@@ -50,6 +50,7 @@ SOURCES = [
     "aoship_gemm.hip",
     "aoship_model.hip",
     "aoship_liquid.hip",
+    "aoship_logprobs.hip",
     "aoship_mlp1.hip",
     "aoship_kv.hip",
     "aoship_kv_attn.hip",

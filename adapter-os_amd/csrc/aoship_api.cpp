@@ -3077,6 +3077,7 @@ struct aoship_model {
   bool emb_set = false;
   Q4Mat lm;
   DevBuf lm_part, lm_ctr;
+  DevBuf score; /* aoship_model_score: pieces of rows, then logits of up to 32 rows */
   DevBuf attn_ctr; /* [ws_T][num_heads] split arrivals, zero between launches */
   std::vector<DevBuf> norm_in, norm_post, bias; /* bias: [layer * 3 + {q,k,v}] */
   DevBuf norm_final;
@@ -3315,17 +3316,58 @@ extern "C" int aoship_model_reserve(aoship_model_t *m, int max_tokens) {
   return 0;
 }
 
-extern "C" int aoship_model_forward(aoship_model_t *m, const int32_t *ids, int T, int position_offset,
-                                    const aoship_ring_t *rings, float *logits) {
-  if (!m || !ids || !rings || !logits) return set_err("aoship_model_forward: null argument");
+static int model_norm(const aoship_model *m, const uint16_t *add, const DevBuf &wt, int rows, float *hid, uint16_t *out) {
+  const aos_launch_ctx ctx = {m->stream, nullptr, nullptr};
+  aos_norm_params np;
+  np.hidden = hid;
+  np.add = add;
+  np.w = wt.as<float>();
+  np.eps = m->cfg.rms_eps;
+  np.T = rows;
+  np.H = m->cfg.hidden;
+  np.out = out;
+  return launch_err(aos_launch_norm(&np, &ctx), "rms norm");
+}
+
+/* logits [rows][vocab] of normalised rows (at most 32) */
+static int model_head(aoship_model *m, const uint16_t *x, int rows, float *logits) {
+  const aos_launch_ctx ctx = {m->stream, nullptr, nullptr};
+  aos_gemv_params g;
+  memset(&g, 0, sizeof(g));
+  g.w0 = m->lm.dev();
+  g.x = x;
+  g.T = rows;
+  g.yf = logits;
+  g.zero_row = m->layers[0]->zeros.as<uint16_t>();
+  if (rows == 1)
+    gemv_geometry(m->lm.RB, m->lm.G, 1, false, false, g);
+  else
+    gemv_launch_geometry(GV_PROJ, m->lm.RB, m->lm.G, rows, 0, 0, 0, 0, g);
+  if (g.ks > 1) {
+    const size_t part = (size_t)m->lm.RB * g.ks * nv_for(rows) * 64 * 4;
+    if (m->lm_part.bytes < part && m->lm_part.alloc(part, false)) return -1;
+    if (m->lm_ctr.bytes < (size_t)m->lm.RB * 4) {
+      if (m->lm_ctr.alloc((size_t)m->lm.RB * 4, true)) return -1;
+      HIP_OR_FAIL(hipDeviceSynchronize(), "hipDeviceSynchronize"); /* (the stream need not wait for the fill) */
+    }
+    g.part = m->lm_part.as<float>();
+    g.counters = m->lm_ctr.as<uint32_t>();
+  }
+  return launch_err(aos_launch_gemv(&g, 0, &ctx), "lm head");
+}
+
+/* Everything of a forward before the final norm: checks, workspace, embedding and layers. The rows' last MLP outputs are in
+ * w.y, to be added to w.hidden. */
+static int model_layers(const char *what, aoship_model_t *m, const int32_t *ids, int T, int position_offset,
+                        const aoship_ring_t *rings, ModelWs &w) {
   const aoship_model_config_t &c = m->cfg;
-  if (T < 1) return set_err("aoship_model_forward: T must be positive");
+  if (T < 1) return set_err(std::string(what) + ": T must be positive");
   if (position_offset != m->cache_len)
-    return set_err("aoship_model_forward: position_offset must equal the cache length (" +
+    return set_err(std::string(what) + ": position_offset must equal the cache length (" +
                    std::to_string(m->cache_len) + ")");
-  if (position_offset + T > c.max_seq) return set_err("aoship_model_forward: the KV cache is full");
-  if (!m->emb_set) return set_err("aoship_model_forward: embedding not set");
-  if (!m->lm.valid) return set_err("aoship_model_forward: LM head not set");
+  if (position_offset + T > c.max_seq) return set_err(std::string(what) + ": the KV cache is full");
+  if (!m->emb_set) return set_err(std::string(what) + ": embedding not set");
+  if (!m->lm.valid) return set_err(std::string(what) + ": LM head not set");
   for (auto *l : m->layers)
     if (check_no_timeout(l)) return -1;
   if (ensure_device()) return -1;
@@ -3335,7 +3377,7 @@ extern "C" int aoship_model_forward(aoship_model_t *m, const int32_t *ids, int T
     if (m->ws.alloc(bytes, false) || m->attn_ctr.alloc((size_t)T * c.num_heads * 4, true)) return -1;
     m->ws_T = T;
   }
-  const ModelWs w = model_ws(c, T, m->ws.p);
+  w = model_ws(c, T, m->ws.p);
   aos_launch_ctx ctx = {m->stream, nullptr, nullptr};
   const int hd = c.head_dim, nh = c.num_heads, nkv = c.num_kv_heads;
 
@@ -3354,15 +3396,7 @@ extern "C" int aoship_model_forward(aoship_model_t *m, const int32_t *ids, int T
   if (launch_err(aos_launch_embed(&ep, &ctx), "embedding")) return -1;
 
   auto norm = [&](const uint16_t *add, const DevBuf &wt, int rows, float *hid, uint16_t *out) {
-    aos_norm_params np;
-    np.hidden = hid;
-    np.add = add;
-    np.w = wt.as<float>();
-    np.eps = c.rms_eps;
-    np.T = rows;
-    np.H = c.hidden;
-    np.out = out;
-    return launch_err(aos_launch_norm(&np, &ctx), "rms norm");
+    return model_norm(m, add, wt, rows, hid, out);
   };
   const size_t layer_cache = (size_t)nkv * c.max_seq * hd;
   for (int li = 0; li < c.num_layers; ++li) {
@@ -3424,25 +3458,153 @@ extern "C" int aoship_model_forward(aoship_model_t *m, const int32_t *ids, int T
     if (norm(w.y, m->norm_post[(size_t)li], T, w.hidden, w.normed)) return -1;
     if (aoship_mlp_forward(l, w.normed, T, rings, w.y)) return -1;
   }
+  return 0;
+}
+
+extern "C" int aoship_model_forward(aoship_model_t *m, const int32_t *ids, int T, int position_offset,
+                                    const aoship_ring_t *rings, float *logits) {
+  if (!m || !ids || !rings || !logits) return set_err("aoship_model_forward: null argument");
+  ModelWs w;
+  if (model_layers("aoship_model_forward", m, ids, T, position_offset, rings, w)) return -1;
   /* residual of the last MLP and the final norm, for the last token only */
-  const size_t lastH = (size_t)(T - 1) * c.hidden;
-  if (norm(w.y + lastH, m->norm_final, 1, w.hidden + lastH, w.normed + lastH)) return -1;
-  aos_gemv_params g;
-  memset(&g, 0, sizeof(g));
-  g.w0 = m->lm.dev();
-  g.x = w.normed + lastH;
-  g.T = 1;
-  g.yf = logits;
-  g.zero_row = m->layers[0]->zeros.as<uint16_t>();
-  gemv_geometry(m->lm.RB, m->lm.G, 1, false, false, g);
-  if (g.ks > 1) {
-    const size_t part = (size_t)m->lm.RB * g.ks * 64 * 4;
-    if (m->lm_part.bytes < part && m->lm_part.alloc(part, false)) return -1;
-    if (m->lm_ctr.bytes < (size_t)m->lm.RB * 4 && m->lm_ctr.alloc((size_t)m->lm.RB * 4, true)) return -1;
-    g.part = m->lm_part.as<float>();
-    g.counters = m->lm_ctr.as<uint32_t>();
+  const size_t last = (size_t)(T - 1) * m->cfg.hidden;
+  if (model_norm(m, w.y + last, m->norm_final, 1, w.hidden + last, w.normed + last)) return -1;
+  if (model_head(m, w.normed + last, 1, logits)) return -1;
+  m->cache_len += T;
+  return 0;
+}
+
+/* ------------------------------------------------------------------------------------------ */
+/* log probabilities                                                                           */
+/* ------------------------------------------------------------------------------------------ */
+
+static_assert(AOSHIP_LOGPROBS_MAX_TOP == AOS_LOGPROBS_MAX_TOP, "tops");
+
+struct aoship_logprobs_handle {
+  int device = 0;
+  DevBuf part;
+  hipStream_t stream = nullptr;
+};
+
+extern "C" aoship_logprobs_t *aoship_logprobs_new(void) {
+  if (ensure_device()) return nullptr;
+  auto *h = new (std::nothrow) aoship_logprobs_handle();
+  if (!h) {
+    set_err("aoship_logprobs_new: out of host memory");
+    return nullptr;
   }
-  if (launch_err(aos_launch_gemv(&g, 0, &ctx), "lm head")) return -1;
+  h->device = g_device;
+  if (h->part.alloc((size_t)AOS_LOGPROBS_WGS * AOS_LOGPROBS_PART * sizeof(float), false)) {
+    delete h;
+    return nullptr;
+  }
+  return h;
+}
+
+extern "C" void aoship_logprobs_free(aoship_logprobs_t *h) {
+  if (!h) return;
+  (void)hipDeviceSynchronize();
+  delete h;
+}
+
+extern "C" int aoship_logprobs_set_stream(aoship_logprobs_t *h, void *stream) {
+  if (!h) return set_err("aoship_logprobs_set_stream: null handle");
+  h->stream = (hipStream_t)stream;
+  return 0;
+}
+
+static int logprobs_out_check(const std::string &what, int vocab, const int32_t *targets, const aoship_logprobs_out_t *o) {
+  if (!o) return set_err(what + ": null outputs");
+  if (o->n_top < 0 || o->n_top > AOSHIP_LOGPROBS_MAX_TOP || o->n_top > vocab)
+    return set_err(what + ": n_top must be 0 to 32 and no more than the vocabulary");
+  if (!targets && (o->logprob || o->rank)) return set_err(what + ": log probabilities and ranks need targets");
+  if (o->n_top == 0 && (o->top_ids || o->top_logprobs)) return set_err(what + ": top_ids and top_logprobs need n_top");
+  for (const void *p : {(const void *)targets, (const void *)o->logprob, (const void *)o->rank, (const void *)o->entropy,
+                        (const void *)o->top_ids, (const void *)o->top_logprobs})
+    if ((uintptr_t)p % 4) return set_err(what + ": targets and outputs must be 4-byte aligned");
+  return 0;
+}
+
+static int logprobs_check(const void *logits, int bf16, int T, int vocab, int64_t stride, const int32_t *targets,
+                          const aoship_logprobs_out_t *o) {
+  const std::string what = "aoship_logprobs";
+  if (T < 0 || T > (1 << 26) || vocab < 1 || vocab > (1 << 30))
+    return set_err(what + ": 0 to 2^26 rows of 1 to 2^30 logits");
+  if (stride < vocab || stride >= (1ll << 40)) return set_err(what + ": stride must be at least vocab (and below 2^40)");
+  if (logprobs_out_check(what, vocab, targets, o)) return -1;
+  if (T == 0) return 1;
+  if (!logits || (uintptr_t)logits % (bf16 ? 2 : 4))
+    return set_err(what + ": logits must be non-NULL and aligned to their element size");
+  return 0;
+}
+
+static int logprobs_run(hipStream_t stream, float *part, const void *logits, int bf16, int T, int vocab, int64_t stride,
+                        const int32_t *targets, const aoship_logprobs_out_t *o, int first) {
+  aos_logprobs_params p;
+  memset(&p, 0, sizeof(p));
+  p.logits = logits;
+  p.ld = stride;
+  p.bf16 = bf16 ? 1 : 0;
+  p.T = T;
+  p.vocab = vocab;
+  p.n_top = o->top_ids || o->top_logprobs ? o->n_top : 0;
+  const size_t at = (size_t)first, tops = at * (size_t)o->n_top;
+  p.targets = targets ? targets + at : nullptr;
+  p.logprob = o->logprob ? o->logprob + at : nullptr;
+  p.entropy = o->entropy ? o->entropy + at : nullptr;
+  p.rank = o->rank ? o->rank + at : nullptr;
+  p.top_ids = o->top_ids ? o->top_ids + tops : nullptr;
+  p.top_logprobs = o->top_logprobs ? o->top_logprobs + tops : nullptr;
+  p.part = part;
+  aos_logprobs_shape(T, vocab, &p.slices, &p.span);
+  const aos_launch_ctx ctx = {stream, nullptr, nullptr};
+  return launch_err(aos_launch_logprobs(&p, &ctx), "log probabilities");
+}
+
+/* Diagnostics (no counterpart in the reference), for tests without a device: a call's checks (0 goes ahead, 1 has nothing
+ * to do, -1 is refused), and the slices that its rows are cut into. */
+extern "C" int aoship_internal_logprobs_check(const void *logits, int bf16, int T, int vocab, int64_t stride,
+                                              const int32_t *targets, const aoship_logprobs_out_t *o) {
+  return logprobs_check(logits, bf16, T, vocab, stride, targets, o);
+}
+extern "C" int aoship_internal_logprobs_shape(int T, int vocab, int *span) {
+  int slices;
+  aos_logprobs_shape(T, vocab, &slices, span);
+  return slices;
+}
+
+extern "C" int aoship_logprobs(aoship_logprobs_t *h, const void *logits, int bf16, int T, int vocab, int64_t stride,
+                               const int32_t *targets, const aoship_logprobs_out_t *out) {
+  if (!h) return set_err("aoship_logprobs: null handle");
+  if (h->device != g_device) return set_err("aoship_logprobs: the handle is on another device than aoship_init's");
+  const int rc = logprobs_check(logits, bf16, T, vocab, stride, targets, out);
+  if (rc) return rc < 0 ? -1 : 0;
+  if (ensure_device()) return -1;
+  return logprobs_run(h->stream, h->part.as<float>(), logits, bf16, T, vocab, stride, targets, out, 0);
+}
+
+extern "C" int aoship_model_score(aoship_model_t *m, const int32_t *ids, int T, int position_offset,
+                                  const aoship_ring_t *rings, const int32_t *targets, const aoship_logprobs_out_t *out,
+                                  float *logits) {
+  if (!m || !ids || !rings) return set_err("aoship_model_score: null argument");
+  const aoship_model_config_t &c = m->cfg;
+  if (logprobs_out_check("aoship_model_score", c.vocab, targets, out)) return -1;
+  if (ensure_device()) return -1;
+  /* logits of AOS_DECODE_MAX_T rows at a time: what one pass over the LM head's weights serves, and few enough to be read
+   * back from the caches */
+  const size_t part = (size_t)AOS_LOGPROBS_WGS * AOS_LOGPROBS_PART * sizeof(float);
+  const size_t rows = (size_t)(T < AOS_DECODE_MAX_T ? T : AOS_DECODE_MAX_T) * (size_t)c.vocab * sizeof(float);
+  if (T > 0 && m->score.bytes < part + rows && m->score.alloc(part + rows, false)) return -1;
+  ModelWs w;
+  if (model_layers("aoship_model_score", m, ids, T, position_offset, rings, w)) return -1;
+  if (model_norm(m, w.y, m->norm_final, T, w.hidden, w.normed)) return -1;
+  float *chunk = m->score.as<float>() + part / sizeof(float);
+  for (int t = 0; t < T; t += AOS_DECODE_MAX_T) {
+    const int n = T - t < AOS_DECODE_MAX_T ? T - t : AOS_DECODE_MAX_T;
+    if (model_head(m, w.normed + (size_t)t * c.hidden, n, chunk)) return -1;
+    if (logprobs_run(m->stream, m->score.as<float>(), chunk, 0, n, c.vocab, c.vocab, targets, out, t)) return -1;
+  }
+  if (logits && model_head(m, w.normed + (size_t)(T - 1) * c.hidden, 1, logits)) return -1;
   m->cache_len += T;
   return 0;
 }

@@ -711,10 +711,29 @@ typedef struct {
   uint32_t *counters; /* [AOS_KV_MAX_WGS], zero between launches */
 } aos_kv_attn_params;
 
+/* ---- log probabilities ---- */
+#define AOS_LOGPROBS_MAX_TOP 32
+#define AOS_LOGPROBS_WGS 2048         /* rows times slices where rows are cut: pieces of the workspace */
+#define AOS_LOGPROBS_MAX_SLICES 1024  /* of a row */
+#define AOS_LOGPROBS_PART (4 + 2 * AOS_LOGPROBS_MAX_TOP) /* floats of a piece: maximum, sums, count, keys */
+typedef struct {
+  const void *logits; /* [T] rows of vocab elements, ld elements apart */
+  long long ld;
+  int bf16, T, vocab, slices, span, n_top;
+  const int32_t *targets;       /* [T] or NULL */
+  float *logprob, *entropy;     /* [T] or NULL */
+  int32_t *rank;                /* [T] or NULL */
+  int32_t *top_ids;             /* [T][n_top] or NULL */
+  float *top_logprobs;          /* [T][n_top] or NULL */
+  float *part;                  /* [AOS_LOGPROBS_WGS][AOS_LOGPROBS_PART] */
+} aos_logprobs_params;
+
 #ifdef __cplusplus
 extern "C" {
 #endif
 /* Host-side launchers (return hipError_t as int). */
+int aos_launch_logprobs(const aos_logprobs_params *p, const aos_launch_ctx *ctx);
+void aos_logprobs_shape(int T, int vocab, int *slices, int *span);
 int aos_launch_kv_append(const aos_kv_append_params *p, const aos_launch_ctx *ctx);
 int aos_launch_kv_read(const aos_kv_read_params *p, const aos_launch_ctx *ctx);
 int aos_launch_kv_attention(const aos_kv_attn_params *p, const aos_launch_ctx *ctx);

@@ -363,6 +363,52 @@ int aoship_model_cache_len(const aoship_model_t *model);
 int aoship_model_forward(aoship_model_t *model, const int32_t *ids, int T, int position_offset,
                          const aoship_ring_t *rings, float *logits);
 
+/* ---- log probabilities of tokens ------------------------------------------------------------ */
+
+/* Of rows of logits (what aoship_model_forward gives for one token, or a program's own head for many): the log
+ * probability of a given token and its rank, the entropy, and the most probable tokens, in one pass (the reference's host
+ * samples from the logits that its step returns, crates/adapteros-lora-kernel-api/src/lib.rs:371). */
+#define AOSHIP_LOGPROBS_MAX_TOP 32
+
+/* The handle holds the workspace of rows that are cut into pieces (0.6 MB): calls allocate nothing and can be captured
+ * into a graph. Calls on one handle, replays among them, are serialised by the caller. NULL on error. */
+typedef struct aoship_logprobs_handle aoship_logprobs_t;
+aoship_logprobs_t *aoship_logprobs_new(void);
+void aoship_logprobs_free(aoship_logprobs_t *handle);
+/* Stream (hipStream_t) for this handle's launches; NULL = null stream. Returns 0 / -1. */
+int aoship_logprobs_set_stream(aoship_logprobs_t *handle, void *stream);
+
+/* Outputs (device, contiguous, 4-byte aligned); each but n_top may be NULL. With p_i = e^(x_i) / sum_j e^(x_j):
+ *   logprob, rank    [T]         ln p of the row's target, and how many tokens come before it; a target outside
+ *                                0 .. vocab - 1 is none: NaN and -1
+ *   entropy          [T]         - sum p_i ln p_i (nats)
+ *   top_ids, top_logprobs [T][n_top]  the n_top first tokens and their ln p
+ * Tokens are in the order of their logits, equal ones (as +0 and -0 are) in that of their numbers. Logits of minus
+ * infinity have probability zero. A row that holds a NaN or +infinity, or nothing above minus infinity, has no
+ * probabilities: NaN, ranks and ids -1. Sums are float32. */
+typedef struct {
+  float *logprob;
+  int32_t *rank;
+  float *entropy;
+  int32_t *top_ids;
+  float *top_logprobs;
+  int n_top; /* 0 .. AOSHIP_LOGPROBS_MAX_TOP, at most vocab */
+} aoship_logprobs_out_t;
+
+/* logits: device [T] rows of vocab float32 (bf16 0) or bfloat16 values, `stride` elements (at least vocab) apart, aligned to
+ * their element size; targets: device int32 [T], or NULL without logprob and rank. A repeated call gives the same
+ * bits. Asynchronous. Returns 0 / -1. */
+int aoship_logprobs(aoship_logprobs_t *handle, const void *logits, int bf16, int T, int vocab, int64_t stride,
+                    const int32_t *targets, const aoship_logprobs_out_t *out);
+
+/* aoship_model_forward with the log probabilities of all T tokens' successors: row t of the outputs is what the model
+ * gives after token t, targets[t] (device, or NULL) the token whose log probability is asked for there (the next one of the
+ * prompt, to score it). logits: device float32 [vocab] for the last token's logits, as aoship_model_forward gives them, or
+ * NULL. The cache is extended by the T tokens. Allocates on its first call, and the first with more tokens up to 32 (21 MB
+ * for 32 tokens of 152064). Asynchronous. Returns 0 / -1. */
+int aoship_model_score(aoship_model_t *model, const int32_t *ids, int T, int position_offset, const aoship_ring_t *rings,
+                       const int32_t *targets, const aoship_logprobs_out_t *out, float *logits);
+
 /* ---- paged key/value cache: many sequences, 16, 8 or 4 bits ---------------------------------- */
 
 /* The cache of aoship_model_t holds one sequence; a program that serves many keeps their keys and values in a
