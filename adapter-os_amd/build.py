@@ -59,11 +59,12 @@ SOURCES = [
 
 
 # Kernels whose workgroups hand data to each other within the launch (the fused decode launches, the
-# attention over the paged cache) must compile without a private stack: a non-inlined device function call in one of them (which
-# forced a stack frame and one wave per SIMD) gave wrong one-token results even where the call
-# was never taken. The build fails if one of them gets private memory.
+# attention over the paged cache, the log probabilities) must compile without a private stack: a
+# non-inlined device function call in one of them (which forced a stack frame and one wave per SIMD)
+# gave wrong one-token results even where the call was never taken. The build fails if one of them
+# gets private memory.
 NO_SCRATCH = ("aos_gemv_fused_kernel", "aos_route_gu_kernel", "aos_decode_mlp_kernel", "aos_mlp1_kernel",
-              "aos_kv_rows_kernel", "aos_kv_tiles_kernel")
+              "aos_kv_rows_kernel", "aos_kv_tiles_kernel", "aos_logprobs_kernel")
 RESOURCE_REMARKS = ["-Rpass-analysis=kernel-resource-usage"]
 
 

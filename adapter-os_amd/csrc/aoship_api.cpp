@@ -3077,7 +3077,7 @@ struct aoship_model {
   bool emb_set = false;
   Q4Mat lm;
   DevBuf lm_part, lm_ctr;
-  DevBuf score; /* aoship_model_score: pieces of rows, then logits of up to 32 rows */
+  DevBuf score; /* aoship_model_score: logprobs_ws, then logits of up to 32 rows */
   DevBuf attn_ctr; /* [ws_T][num_heads] split arrivals, zero between launches */
   std::vector<DevBuf> norm_in, norm_post, bias; /* bias: [layer * 3 + {q,k,v}] */
   DevBuf norm_final;
@@ -3486,6 +3486,17 @@ struct aoship_logprobs_handle {
   hipStream_t stream = nullptr;
 };
 
+/* a workspace with room for `more` bytes behind it; the first launch may be on a stream that does not wait for its fill */
+static int logprobs_ws(DevBuf &ws, size_t more) {
+  if (ws.alloc(AOS_LOGPROBS_WS + more, false)) return -1;
+  hipError_t e = hipMemset(ws.p, 0, AOS_LOGPROBS_WS);
+  if (e == hipSuccess) e = hipDeviceSynchronize();
+  if (e == hipSuccess) return 0;
+  (void)hipGetLastError();
+  ws.release();
+  return set_err(std::string("hipMemset: ") + hipGetErrorString(e));
+}
+
 extern "C" aoship_logprobs_t *aoship_logprobs_new(void) {
   if (ensure_device()) return nullptr;
   auto *h = new (std::nothrow) aoship_logprobs_handle();
@@ -3494,7 +3505,7 @@ extern "C" aoship_logprobs_t *aoship_logprobs_new(void) {
     return nullptr;
   }
   h->device = g_device;
-  if (h->part.alloc((size_t)AOS_LOGPROBS_WGS * AOS_LOGPROBS_PART * sizeof(float), false)) {
+  if (logprobs_ws(h->part, 0)) {
     delete h;
     return nullptr;
   }
@@ -3538,7 +3549,7 @@ static int logprobs_check(const void *logits, int bf16, int T, int vocab, int64_
   return 0;
 }
 
-static int logprobs_run(hipStream_t stream, float *part, const void *logits, int bf16, int T, int vocab, int64_t stride,
+static int logprobs_run(hipStream_t stream, const DevBuf &ws, const void *logits, int bf16, int T, int vocab, int64_t stride,
                         const int32_t *targets, const aoship_logprobs_out_t *o, int first) {
   aos_logprobs_params p;
   memset(&p, 0, sizeof(p));
@@ -3555,7 +3566,8 @@ static int logprobs_run(hipStream_t stream, float *part, const void *logits, int
   p.rank = o->rank ? o->rank + at : nullptr;
   p.top_ids = o->top_ids ? o->top_ids + tops : nullptr;
   p.top_logprobs = o->top_logprobs ? o->top_logprobs + tops : nullptr;
-  p.part = part;
+  p.part = ws.as<uint64_t>();
+  p.counters = (uint32_t *)(p.part + (size_t)AOS_LOGPROBS_WGS * AOS_LOGPROBS_PART);
   aos_logprobs_shape(T, vocab, &p.slices, &p.span);
   const aos_launch_ctx ctx = {stream, nullptr, nullptr};
   return launch_err(aos_launch_logprobs(&p, &ctx), "log probabilities");
@@ -3580,7 +3592,7 @@ extern "C" int aoship_logprobs(aoship_logprobs_t *h, const void *logits, int bf1
   const int rc = logprobs_check(logits, bf16, T, vocab, stride, targets, out);
   if (rc) return rc < 0 ? -1 : 0;
   if (ensure_device()) return -1;
-  return logprobs_run(h->stream, h->part.as<float>(), logits, bf16, T, vocab, stride, targets, out, 0);
+  return logprobs_run(h->stream, h->part, logits, bf16, T, vocab, stride, targets, out, 0);
 }
 
 extern "C" int aoship_model_score(aoship_model_t *m, const int32_t *ids, int T, int position_offset,
@@ -3592,17 +3604,16 @@ extern "C" int aoship_model_score(aoship_model_t *m, const int32_t *ids, int T, 
   if (ensure_device()) return -1;
   /* logits of AOS_DECODE_MAX_T rows at a time: what one pass over the LM head's weights serves, and few enough to be read
    * back from the caches */
-  const size_t part = (size_t)AOS_LOGPROBS_WGS * AOS_LOGPROBS_PART * sizeof(float);
   const size_t rows = (size_t)(T < AOS_DECODE_MAX_T ? T : AOS_DECODE_MAX_T) * (size_t)c.vocab * sizeof(float);
-  if (T > 0 && m->score.bytes < part + rows && m->score.alloc(part + rows, false)) return -1;
+  if (T > 0 && m->score.bytes < AOS_LOGPROBS_WS + rows && logprobs_ws(m->score, rows)) return -1;
   ModelWs w;
   if (model_layers("aoship_model_score", m, ids, T, position_offset, rings, w)) return -1;
   if (model_norm(m, w.y, m->norm_final, T, w.hidden, w.normed)) return -1;
-  float *chunk = m->score.as<float>() + part / sizeof(float);
+  float *chunk = m->score.as<float>() + AOS_LOGPROBS_WS / sizeof(float);
   for (int t = 0; t < T; t += AOS_DECODE_MAX_T) {
     const int n = T - t < AOS_DECODE_MAX_T ? T - t : AOS_DECODE_MAX_T;
     if (model_head(m, w.normed + (size_t)t * c.hidden, n, chunk)) return -1;
-    if (logprobs_run(m->stream, m->score.as<float>(), chunk, 0, n, c.vocab, c.vocab, targets, out, t)) return -1;
+    if (logprobs_run(m->stream, m->score, chunk, 0, n, c.vocab, c.vocab, targets, out, t)) return -1;
   }
   if (logits && model_head(m, w.normed + (size_t)(T - 1) * c.hidden, 1, logits)) return -1;
   m->cache_len += T;

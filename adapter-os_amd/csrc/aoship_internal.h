@@ -713,9 +713,10 @@ typedef struct {
 
 /* ---- log probabilities ---- */
 #define AOS_LOGPROBS_MAX_TOP 32
-#define AOS_LOGPROBS_WGS 2048         /* rows times slices where rows are cut: pieces of the workspace */
+#define AOS_LOGPROBS_WGS 1024         /* rows times slices where rows are cut: pieces of the workspace */
 #define AOS_LOGPROBS_MAX_SLICES 1024  /* of a row */
-#define AOS_LOGPROBS_PART (4 + 2 * AOS_LOGPROBS_MAX_TOP) /* floats of a piece: maximum, sums, count, keys */
+#define AOS_LOGPROBS_PART (2 + AOS_LOGPROBS_MAX_TOP) /* 64-bit words of a piece: maximum, sums, count, keys */
+#define AOS_LOGPROBS_WS ((size_t)AOS_LOGPROBS_WGS * (8 * AOS_LOGPROBS_PART + 4)) /* bytes of pieces and counters */
 typedef struct {
   const void *logits; /* [T] rows of vocab elements, ld elements apart */
   long long ld;
@@ -725,7 +726,8 @@ typedef struct {
   int32_t *rank;                /* [T] or NULL */
   int32_t *top_ids;             /* [T][n_top] or NULL */
   float *top_logprobs;          /* [T][n_top] or NULL */
-  float *part;                  /* [AOS_LOGPROBS_WGS][AOS_LOGPROBS_PART] */
+  uint64_t *part;               /* [AOS_LOGPROBS_WGS][AOS_LOGPROBS_PART] */
+  uint32_t *counters;           /* [AOS_LOGPROBS_WGS] arrivals of a row's slices, zero between launches */
 } aos_logprobs_params;
 
 #ifdef __cplusplus

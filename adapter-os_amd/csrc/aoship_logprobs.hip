@@ -11,9 +11,14 @@
  * The n largest without sorting anything long: a thread's 16-byte units of the row (every 256th) are four groups, of
  * each of which it keeps the largest value and the unit it is in. The n largest elements lie in the n groups whose
  * largest come first; these few groups are read again (from the L2), what is not before the last of their largest
- * goes to a list (about n entries), and an entry's place in the answer is the number of entries before it.
+ * goes to a list (about n entries), and an entry's place in the answer is the number of entries before it. The n groups
+ * are found in the same way: a bound that n of a wave's lanes reach, by bisection of the bits, then a list and places in it.
  *
- * Bound by reading the logits once.
+ * Few rows are cut into slices, whose pieces the row's last workgroup joins (a second launch cost 5 us more).
+ *
+ * Bound by reading the logits once, and nearly as much by the vector instructions (an exponential and nine others a logit):
+ * 4000 rows of 50257 bfloat16 99 us, 4.1 TB/s. Few rows by the latencies of the choice: 1 row of 152064 with 5 tokens 14
+ * us, 64 of 128256 with 20 24 us (taking the n one after the other from 64 lanes 72).
  */
 #include "aoship_device.h"
 #include "aoship_internal.h"
@@ -25,7 +30,7 @@ constexpr int NT = 256;         /* threads of a workgroup */
 constexpr int SEGS = 4;         /* groups of a thread */
 constexpr int LIST = 1024;      /* entries of the list */
 constexpr float LEAST = -3.40282347e38f;
-constexpr float LOG2E = 1.44269504f;
+constexpr float LOG2E = 1.44269504f, LN2 = 0.693147181f;
 constexpr uint32_t NONE = 0xffffffffu;
 
 /* order of candidates: by value (both zeros alike), then by index; 0 is no candidate */
@@ -40,29 +45,44 @@ __device__ __forceinline__ float key_value(uint64_t k) {
 }
 __device__ __forceinline__ uint32_t key_index(uint64_t k) { return ~(uint32_t)k; }
 
+/* largest of the wave's values, by data moves within the vector registers (lane 63 ends with all of them); uniform */
+__device__ __forceinline__ uint32_t wave_max32(uint32_t x) {
+  auto step = [&](uint32_t y) { x = y > x ? y : x; };
+  step((uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x111, 0xf, 0xf, false)); /* row_shr 1, 2, 4, 8 */
+  step((uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x112, 0xf, 0xf, false));
+  step((uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x114, 0xf, 0xf, false));
+  step((uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x118, 0xf, 0xf, false));
+  step((uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x142, 0xa, 0xf, false)); /* row_bcast 15, 31 */
+  step((uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x143, 0xc, 0xf, false));
+  return (uint32_t)__builtin_amdgcn_readlane((int)x, 63);
+}
+__device__ __forceinline__ uint64_t lane_key(uint64_t k, int lane) {
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(k >> 32), lane);
+  return ((uint64_t)hi << 32) | (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)k, lane);
+}
+/* largest key: the values first, the indices only where several lanes have the value */
 __device__ __forceinline__ uint64_t wave_max(uint64_t k) {
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const uint64_t o = aos_shfl64(k, (int)(threadIdx.x & 63) ^ d);
-    k = o > k ? o : k;
-  }
-  return k;
+  const uint32_t hi = wave_max32((uint32_t)(k >> 32));
+  const uint64_t tied = __ballot((uint32_t)(k >> 32) == hi);
+  if (tied & (tied - 1)) return ((uint64_t)hi << 32) | wave_max32((uint32_t)(k >> 32) == hi ? (uint32_t)k : 0u);
+  return lane_key(k, __builtin_ctzll(tied));
 }
 
-/* running maximum, sum and weighted sum */
+/* Running maximum m, sum l of 2^a and weighted sum s of 2^a a, a = (x - m) log2 e. (A maximum kept times log2 e would make a
+ * one fused operation, but overflows for logits past 2.3e38.) */
 struct Stat {
   float m, l, s;
   __device__ __forceinline__ void clear() { m = LEAST, l = 0.0f, s = 0.0f; }
   __device__ __forceinline__ void lift(float top) { /* to a maximum that is no less */
-    const float d = m - top, f = __builtin_amdgcn_exp2f(d * LOG2E);
+    const float d = (m - top) * LOG2E, f = __builtin_amdgcn_exp2f(d);
     s = f * (s + l * fmaxf(d, -200.0f)); /* (below that f is zero: no zero times infinity) */
     l = l * f;
     m = top;
   }
   __device__ __forceinline__ void add(float x) { /* x <= m */
-    const float d = x - m, e = __builtin_amdgcn_exp2f(d * LOG2E);
+    const float a = (x - m) * LOG2E, e = __builtin_amdgcn_exp2f(a);
     l = l + e;
-    s = s + e * fmaxf(d, -200.0f);
+    s = fmaf(e, fmaxf(a, -200.0f), s);
   }
   __device__ __forceinline__ void join(Stat o) {
     const float top = fmaxf(m, o.m);
@@ -73,58 +93,81 @@ struct Stat {
   }
 };
 
+constexpr int PAD = 32;
+
 struct Shared {
-  uint64_t list[LIST];
-  uint64_t wave[4][AOS_LOGPROBS_MAX_TOP];
+  uint64_t list[LIST + PAD];
+  uint64_t wave[4];
   uint64_t top[AOS_LOGPROBS_MAX_TOP];
   float stat[4][3];
   int before[4];
   uint32_t listed;
 };
 
-/* The n largest of all threads' four keys, in order, into sh.top (zeros where there are fewer). */
-__device__ __forceinline__ void largest(Shared &sh, uint64_t (&k)[4], int n) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  auto order = [](uint64_t &a, uint64_t &b) {
-    const uint64_t hi = a > b ? a : b, lo = a > b ? b : a;
-    a = hi;
-    b = lo;
-  };
-  order(k[0], k[1]);
-  order(k[2], k[3]);
-  order(k[0], k[2]);
-  order(k[1], k[3]);
-  order(k[1], k[2]);
-  for (int i = 0; i < n; ++i) {
-    const uint64_t best = wave_max(k[0]);
-    if (lane == 0) sh.wave[wave][i] = best;
-    if (k[0] == best) k[0] = k[1], k[1] = k[2], k[2] = k[3], k[3] = 0; /* (keys are distinct, zeros apart) */
-  }
+/* The n first of the list's entries, in order, into sh.top (zeros where there are fewer): each counts those before it. */
+__device__ __forceinline__ void rank_list(Shared &sh, int n) {
   __syncthreads();
-  if (wave == 0) {
-    uint64_t a = lane < n ? sh.wave[0][lane] : lane >= 32 && lane - 32 < n ? sh.wave[1][lane - 32] : 0;
-    uint64_t b = lane < n ? sh.wave[2][lane] : lane >= 32 && lane - 32 < n ? sh.wave[3][lane - 32] : 0;
-    order(a, b);
-    for (int i = 0; i < n; ++i) {
-      const uint64_t best = wave_max(a);
-      if (lane == 0) sh.top[i] = best;
-      if (a == best) a = b, b = 0;
-    }
+  const int count = (int)sh.listed, tid = threadIdx.x;
+  if (tid < n) sh.top[tid] = 0;
+  if (tid < PAD) sh.list[count + tid] = 0;
+  __syncthreads();
+  for (int i0 = 0; i0 < count; i0 += NT / 4) { /* four lanes an entry, each with every fourth of the others */
+    const int i = i0 + tid / 4;
+    const uint64_t mine = i < count ? sh.list[i] : 0;
+    int before = 0;
+    for (int j = tid % 4; j < count; j += PAD) /* (eight reads in flight together) */
+#pragma unroll
+      for (int k = 0; k < PAD; k += 4) before += sh.list[j + k] > mine ? 1 : 0;
+    before += __builtin_amdgcn_update_dpp(0, before, 0xb1, 0xf, 0xf, false); /* quad_perm 1 0 3 2 */
+    before += __builtin_amdgcn_update_dpp(0, before, 0x4e, 0xf, 0xf, false); /* 2 3 0 1 */
+    if (i < count && tid % 4 == 0 && before < n) sh.top[before] = mine;
   }
   __syncthreads();
 }
+__device__ __forceinline__ void push(Shared &sh, uint64_t k) {
+  const uint32_t at = atomicAdd(&sh.listed, 1u);
+  if (at < LIST) sh.list[at] = k;
+}
 
-/* The n first of the list's entries into sh.top: each entry counts those before it. */
-__device__ __forceinline__ void rank_list(Shared &sh, int n) {
-  const int count = (int)sh.listed;
-  if ((int)threadIdx.x < n) sh.top[threadIdx.x] = 0;
-  __syncthreads();
-  for (int i = threadIdx.x; i < count; i += NT) {
-    const uint64_t mine = sh.list[i];
-    int before = 0;
-    for (int j = 0; j < count; ++j) before += sh.list[j] > mine ? 1 : 0;
-    if (before < n) sh.top[before] = mine;
+/* A bound that exactly n of the wave's keys reach (0 where there are no n): the value's bits from the highest on, as far as
+ * it takes to part n from the others, the index's where values are alike. Uniform. */
+__device__ __forceinline__ uint64_t wave_nth(uint64_t k, int n) {
+  const uint32_t hi = (uint32_t)(k >> 32), lo = (uint32_t)k;
+  uint32_t v = 0;
+  for (uint32_t bit = 1u << 31; bit; bit >>= 1) {
+    const int c = (int)__popcll(__ballot(hi >= (v | bit)));
+    if (c < n) continue;
+    v |= bit;
+    if (c == n) return (uint64_t)v << 32;
   }
+  n -= (int)__popcll(__ballot(hi > v));
+  uint32_t i = 0;
+  for (uint32_t bit = 1u << 31; bit; bit >>= 1) {
+    const int c = (int)__popcll(__ballot(hi == v && lo >= (i | bit)));
+    if (c < n) continue;
+    i |= bit;
+    if (c == n) break;
+  }
+  return ((uint64_t)v << 32) | i;
+}
+
+/* The n largest of all threads' four keys (distinct, zeros for none), in order, into sh.top. Of a wave's lanes' largest the
+ * n-th is no more than the n-th of all keys: those from the largest such bound on are listed, about twice n. */
+__device__ __forceinline__ void largest(Shared &sh, const uint64_t (&k)[4], int n) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const uint64_t a = k[0] > k[1] ? k[0] : k[1], b = k[2] > k[3] ? k[2] : k[3], mine = a > b ? a : b;
+  const uint64_t bound = wave_nth(mine, n);
+  if (lane == 0) sh.wave[wave] = bound;
+  if (tid == 0) sh.listed = 0;
+  __syncthreads();
+  uint64_t from = 1;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) from = sh.wave[w] > from ? sh.wave[w] : from;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (k[i] >= from) push(sh, k[i]);
+  rank_list(sh, n);
+  if (tid == 0) sh.listed = 0;
   __syncthreads();
 }
 
@@ -144,22 +187,29 @@ __device__ __forceinline__ float element(const void *row, long long i) {
   return ((const float *)row)[i];
 }
 
+/* the next float32 under a finite one or +infinity */
+__device__ __forceinline__ float next_under(float x) {
+  const int u = (int)__builtin_bit_cast(uint32_t, x + 0.0f); /* (-0 as +0) */
+  return __builtin_bit_cast(float, (uint32_t)(u > 0 ? u - 1 : u == 0 ? (int)0x80000001 : u + 1));
+}
+
 /* what a workgroup writes of a row: the answer, or its slice's piece of it */
 __device__ __forceinline__ void answer(const aos_logprobs_params &p, Shared &sh, int row, Stat st, float xt, bool target,
                                        int before) {
   const int tid = threadIdx.x;
-  const float ln = logf(st.l), nan = __builtin_nanf("");
+  const float bits = log2f(st.l), nan = __builtin_nanf("");
   const bool ok = st.l > 0.0f; /* neither a NaN nor all minus infinity */
+  auto lnp = [&](float x) { return (x - st.m) - bits * LN2; };
   if (tid == 0) {
-    if (p.logprob) p.logprob[row] = ok && target ? xt - st.m - ln : nan;
+    if (p.logprob) p.logprob[row] = ok && target ? lnp(xt) : nan;
     if (p.rank) p.rank[row] = ok && target ? before : -1;
-    if (p.entropy) p.entropy[row] = ok ? ln - st.s / st.l : nan;
+    if (p.entropy) p.entropy[row] = ok ? (bits - st.s / st.l) * LN2 : nan;
   }
   if (tid < p.n_top) {
     const uint64_t k = sh.top[tid];
     const long long at = (long long)row * p.n_top + tid;
     if (p.top_ids) p.top_ids[at] = ok ? (int)key_index(k) : -1;
-    if (p.top_logprobs) p.top_logprobs[at] = ok ? key_value(k) - st.m - ln : nan;
+    if (p.top_logprobs) p.top_logprobs[at] = ok ? lnp(key_value(k)) : nan;
   }
 }
 
@@ -191,11 +241,28 @@ __device__ __forceinline__ void join_block(Shared &sh, Stat &st, int &before) {
   }
 }
 
+/* A slice's piece of its row, for the row's last workgroup (device-coherent: aoship_device.h). */
+__device__ __forceinline__ void publish(uint64_t *p, uint64_t v) {
+  __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ uint64_t collect(const uint64_t *p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  return __builtin_bit_cast(uint32_t, a) | ((uint64_t)__builtin_bit_cast(uint32_t, b) << 32);
+}
+__device__ __forceinline__ float low(uint64_t v) { return __builtin_bit_cast(float, (uint32_t)v); }
+__device__ __forceinline__ float high(uint64_t v) { return __builtin_bit_cast(float, (uint32_t)(v >> 32)); }
+__device__ __forceinline__ uint64_t slice_key(uint64_t k, int slice) {
+  return (k & 0xffffffff00000000ull) | (uint32_t)~(uint32_t)slice;
+}
+
 /* Grid: rows times slices. A workgroup's slice of its row: elements in front of the first 16-byte border and behind the
  * last, one a thread, and the units between. */
 template <bool BF16>
-__global__ void __launch_bounds__(NT) aos_logprobs_kernel(aos_logprobs_params p) {
+__global__ void __launch_bounds__(NT, 4) aos_logprobs_kernel(aos_logprobs_params p) {
   constexpr int N = Unit<BF16>::N, SIZE = 16 / N;
+  constexpr int FLY = 2; /* units of a thread on their way while as many are worked on */
   __shared__ Shared sh;
   const int tid = threadIdx.x;
   const int row = (int)(blockIdx.x / (uint32_t)p.slices), slice = (int)(blockIdx.x - (uint32_t)row * (uint32_t)p.slices);
@@ -210,51 +277,74 @@ __global__ void __launch_bounds__(NT) aos_logprobs_kernel(aos_logprobs_params p)
   const bool target = t >= 0 && t < p.vocab;
   const float xt = target ? element<BF16>(x, t) : 0.0f;
 
+  /* An element comes before the target if it is not <= edge: the target's logit, or behind it, where equal ones come first
+   * (the target's own unit counts as behind it and is put right below), the next number under it; a NaN under -infinity,
+   * so that everything comes before. */
+  const float under = xt == -__builtin_inff() ? __builtin_nanf("") : next_under(xt);
   Stat st;
   st.clear();
-  int before = 0;
+  int before = 0, counted = 0; /* a lane's own, the wave's */
   const int each = (units + NT - 1) / NT, per = (each + SEGS - 1) / SEGS; /* units of a thread, of a group */
+  const int full = units / NT;                                         /* units that every thread has */
   uint64_t key[SEGS];
-#pragma unroll
+#pragma unroll 1
   for (int g = 0; g < SEGS; ++g) {
     float best = __builtin_nanf("");
     uint32_t at = NONE;
-    for (int i0 = g * per; i0 < (g + 1) * per; i0 += 4) {
-      Unit<BF16> w[4];
-      int live = 0;
+    auto unit_max = [&](const Unit<BF16> &w, int u) {
+      float um = w[0];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int u = (i0 + j) * NT + tid;
-        const bool in = i0 + j < (g + 1) * per && u < units;
-        if (in) w[j].w = aos_gld16(body + (long long)u * 16);
-        live += in ? 1 : 0; /* (the first so many) */
-      }
-      float top = st.m;
+      for (int e = 1; e < N; ++e) um = fmaxf(um, w[e]);
+      if (!(um <= best)) best = um, at = (uint32_t)u;
+      return um;
+    };
+    const int i1 = (g + 1) * per < full ? (g + 1) * per : full;
+    int i = g * per;
+    Unit<BF16> w[FLY], next[FLY];
+    auto fetch = [&](Unit<BF16> (&x)[FLY], int from) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (j >= live) continue;
-        float um = w[j][0];
+      for (int j = 0; j < FLY; ++j) x[j].w = aos_gld16(body + (long long)((from + j) * NT + tid) * 16);
+    };
+    if (i + FLY <= i1) fetch(w, i);
+    for (; i + FLY <= i1; i += FLY) {
+      if (i + 2 * FLY <= i1) fetch(next, i + FLY);
+      float top = w[0][0];
 #pragma unroll
-        for (int e = 1; e < N; ++e) um = fmaxf(um, w[j][e]);
-        if (!(um <= best)) best = um, at = (uint32_t)((i0 + j) * NT + tid);
-        top = fmaxf(top, um);
-      }
-      st.lift(top);
+      for (int j = 0; j < FLY; ++j) top = fmaxf(top, unit_max(w[j], (i + j) * NT + tid));
+      st.lift(fmaxf(st.m, top));
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (j >= live) continue;
-        const int i = u0 + ((i0 + j) * NT + tid) * N;
-        const bool front = i + N <= t; /* (the unit that holds t: counted as behind it, put right below) */
+      for (int j = 0; j < FLY; ++j) {
+        const float edge = u0 + ((i + j) * NT + tid) * N + N <= t ? under : xt;
 #pragma unroll
         for (int e = 0; e < N; ++e) {
           const float v = w[j][e];
           st.add(v);
-          before += (v > xt) || (front && v == xt) ? 1 : 0;
+          counted += (int)__popcll(__ballot(!(v <= edge)));
         }
       }
+#pragma unroll
+      for (int j = 0; j < FLY; ++j) w[j] = next[j];
     }
-    key[g] = at == NONE ? 0 : key_of(best, at);
+    /* the group's last units, one at a time, and one that only some threads have */
+    for (; i < (g + 1) * per; ++i) {
+      const int u = i * NT + tid;
+      if (u >= units) break;
+      Unit<BF16> x;
+      x.w = aos_gld16(body + (long long)u * 16);
+      st.lift(fmaxf(st.m, unit_max(x, u)));
+      const float edge = u0 + u * N + N <= t ? under : xt;
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const float v = x[e];
+        st.add(v);
+        before += !(v <= edge) ? 1 : 0;
+      }
+    }
+    const uint64_t k = at == NONE ? 0 : key_of(best, at);
+#pragma unroll
+    for (int j = 0; j < SEGS; ++j) key[j] = j == g ? k : key[j];
   }
+  if ((tid & 63) == 0) before += counted;
   /* elements outside the units: at most 2 (N - 1), thread i has the i-th */
   const int odd = tid < head ? a0 + tid : tid - head < a1 - t0 ? t0 + tid - head : -1;
   uint64_t mine = 0;
@@ -270,34 +360,31 @@ __global__ void __launch_bounds__(NT) aos_logprobs_kernel(aos_logprobs_params p)
   join_block(sh, st, before);
   const int n = p.n_top;
   if (n > 0) {
-    if (tid == 0) sh.listed = 0;
     largest(sh, key, n);
     /* the last of the n groups' largest: nothing behind it (in value, then unit) is among the n */
     const uint64_t last = sh.top[n - 1];
+    const float least = last ? key_value(last) : -__builtin_inff();
     int groups = 0;
     while (groups < n && sh.top[groups]) ++groups;
-    auto wanted = [&](float v, uint32_t unit) { return key_of(v, unit) >= last; };
-    auto push = [&](uint64_t k) {
-      const uint32_t at = atomicAdd(&sh.listed, 1u);
-      if (at < LIST) sh.list[at] = k;
+    /* each unit of the groups, 16 lanes a group */
+    auto units_of_groups = [&](auto &&take) {
+      for (int gi = tid / 16; gi < groups; gi += NT / 16) {
+        const int u = (int)key_index(sh.top[gi]), th = u % NT, from = (u / NT) / per * per;
+        for (int i = from + tid % 16; i < from + per; i += 16) {
+          const int un = i * NT + th;
+          if (un >= units) break;
+          Unit<BF16> w;
+          w.w = aos_gld16(body + (long long)un * 16);
+          take(w, un);
+        }
+      }
     };
-    auto unit_of = [&](int q) { /* of the q-th unit of the groups; -1 past the row's end */
-      const int gi = q / per, i = q - gi * per;
-      const uint32_t u = key_index(sh.top[gi]);
-      const int th = (int)(u % NT), g = (int)(u / NT) / per;
-      const int un = (g * per + i) * NT + th;
-      return un < units ? un : -1;
-    };
-    for (int q = tid; q < groups * per; q += NT) {
-      const int un = unit_of(q);
-      if (un < 0) continue;
-      Unit<BF16> w;
-      w.w = aos_gld16(body + (long long)un * 16);
+    units_of_groups([&](const Unit<BF16> &w, int un) {
 #pragma unroll
       for (int e = 0; e < N; ++e)
-        if (wanted(w[e], (uint32_t)un)) push(key_of(w[e], (uint32_t)(u0 + un * N + e)));
-    }
-    if (mine) push(mine);
+        if (w[e] >= least && key_of(w[e], (uint32_t)un) >= last) push(sh, key_of(w[e], (uint32_t)(u0 + un * N + e)));
+    });
+    if (mine) push(sh, mine);
     __syncthreads();
     if (sh.listed <= LIST) {
       rank_list(sh, n);
@@ -307,23 +394,19 @@ __global__ void __launch_bounds__(NT) aos_logprobs_kernel(aos_logprobs_params p)
       uint64_t below = ~0ull, found = 0;
       for (int r = 0; r < n; ++r) {
         uint64_t best = mine < below ? mine : 0;
-        for (int q = tid; q < groups * per; q += NT) {
-          const int un = unit_of(q);
-          if (un < 0) continue;
-          Unit<BF16> w;
-          w.w = aos_gld16(body + (long long)un * 16);
+        units_of_groups([&](const Unit<BF16> &w, int un) {
 #pragma unroll
           for (int e = 0; e < N; ++e) {
             const uint64_t k = key_of(w[e], (uint32_t)(u0 + un * N + e));
             best = k < below && k > best ? k : best;
           }
-        }
+        });
         best = wave_max(best);
-        if ((tid & 63) == 0) sh.wave[tid >> 6][0] = best;
+        if ((tid & 63) == 0) sh.wave[tid >> 6] = best;
         __syncthreads();
         below = 0;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) below = sh.wave[w][0] > below ? sh.wave[w][0] : below;
+        for (int w = 0; w < 4; ++w) below = sh.wave[w] > below ? sh.wave[w] : below;
         if (tid == r) found = below;
         __syncthreads();
       }
@@ -335,77 +418,71 @@ __global__ void __launch_bounds__(NT) aos_logprobs_kernel(aos_logprobs_params p)
     answer(p, sh, row, st, xt, target, before);
     return;
   }
-  float *part = p.part + (size_t)blockIdx.x * AOS_LOGPROBS_PART;
+  uint64_t *part = p.part + (size_t)blockIdx.x * AOS_LOGPROBS_PART;
   if (tid == 0) {
-    part[0] = st.m;
-    part[1] = st.l;
-    part[2] = st.s;
-    ((int *)part)[3] = before;
+    publish(part, pair(st.m, st.l));
+    publish(part + 1, pair(st.s, __builtin_bit_cast(float, before)));
   }
-  if (tid < n) ((uint64_t *)(part + 4))[tid] = sh.top[tid];
-}
+  if (tid < n) publish(part + 2 + tid, sh.top[tid]);
+  aos_mem_wait();
+  __syncthreads();
+  if (tid == 0) {
+    const bool last = aos_arrive(p.counters + row) == (uint32_t)p.slices - 1u;
+    if (last) aos_reset(p.counters + row);
+    sh.listed = last ? 1u : 0u;
+  }
+  __syncthreads();
+  if (!sh.listed) return;
 
-/* Grid: rows. The slices' pieces joined: their n largest lie in the n slices whose largest come first. */
-template <bool BF16>
-__global__ void __launch_bounds__(NT) aos_logprobs_join_kernel(aos_logprobs_params p) {
-  __shared__ Shared sh;
-  const int tid = threadIdx.x, row = blockIdx.x, n = p.n_top;
-  const float *part = p.part + (size_t)row * p.slices * AOS_LOGPROBS_PART;
-  auto keys = [&](int slice) { return (const uint64_t *)(part + (size_t)slice * AOS_LOGPROBS_PART + 4); };
-  Stat st;
+  /* the row's last workgroup joins the slices' pieces: their n largest lie in the n slices whose largest come first */
+  part = p.part + (size_t)row * p.slices * AOS_LOGPROBS_PART;
   st.clear();
-  int before = 0;
-  uint64_t key[4];
+  before = 0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) { /* (at most 4 NT slices) */
+  for (int i = 0; i < SEGS; ++i) { /* (at most SEGS NT slices) */
     const int s = i * NT + tid;
     key[i] = 0;
     if (s < p.slices) {
-      const float *q = part + (size_t)s * AOS_LOGPROBS_PART;
-      st.join(Stat{q[0], q[1], q[2]});
-      before += ((const int *)q)[3];
-      /* a slice's rank among slices: its largest's value, then the slice */
-      if (n > 0 && keys(s)[0]) key[i] = (keys(s)[0] & 0xffffffff00000000ull) | (uint32_t)~(uint32_t)s;
+      const uint64_t *q = part + (size_t)s * AOS_LOGPROBS_PART;
+      const uint64_t ml = collect(q), sb = collect(q + 1), k = n > 0 ? collect(q + 2) : 0;
+      st.join(Stat{low(ml), high(ml), low(sb)});
+      before += __builtin_bit_cast(int, high(sb));
+      /* a slice's place among slices: its largest's value, then the slice */
+      if (k) key[i] = slice_key(k, s);
     }
   }
+  __syncthreads(); /* (sh.listed has been read) */
   join_block(sh, st, before);
   if (n > 0) {
-    if (tid == 0) sh.listed = 0;
     largest(sh, key, n);
     const uint64_t last = sh.top[n - 1];
-    for (int q = tid; q < n * n; q += NT) { /* (at most LIST) */
-      if (!sh.top[q / n]) continue;
-      const uint32_t s = key_index(sh.top[q / n]);
-      const uint64_t k = keys((int)s)[q % n];
-      if (k && ((k & 0xffffffff00000000ull) | (uint32_t)~s) >= last) sh.list[atomicAdd(&sh.listed, 1u)] = k;
+    for (int i = tid / 32; i < n && sh.top[i]; i += NT / 32) { /* (at most LIST keys) */
+      if (tid % 32 >= n) break;
+      const int s = (int)key_index(sh.top[i]);
+      const uint64_t k = collect(part + (size_t)s * AOS_LOGPROBS_PART + 2 + tid % 32);
+      if (k && slice_key(k, s) >= last) push(sh, k);
     }
-    __syncthreads();
     rank_list(sh, n);
   }
-  const char *x = (const char *)p.logits + (long long)row * p.ld * (BF16 ? 2 : 4);
-  const int t = p.targets ? p.targets[row] : -1;
-  const bool target = t >= 0 && t < p.vocab;
-  answer(p, sh, row, st, target ? element<BF16>(x, t) : 0.0f, target, before);
+  answer(p, sh, row, st, xt, target, before);
 }
 
 template <bool BF16>
 int launch(const aos_logprobs_params *p, const aos_launch_ctx *ctx) {
   AOS_LAUNCH(ctx, (aos_logprobs_kernel<BF16>), dim3((uint32_t)p->T * (uint32_t)p->slices), dim3(NT), 0, *p);
-  const hipError_t e = hipGetLastError();
-  if (e != hipSuccess || p->slices == 1) return (int)e;
-  AOS_LAUNCH(ctx, (aos_logprobs_join_kernel<BF16>), dim3(p->T), dim3(NT), 0, *p);
   return (int)hipGetLastError();
 }
 
 }  // namespace
 
 static_assert(AOS_LOGPROBS_MAX_TOP <= 32 && AOS_LOGPROBS_MAX_TOP * AOS_LOGPROBS_MAX_TOP <= LIST, "lists");
-static_assert(AOS_LOGPROBS_MAX_SLICES <= 4 * NT, "a thread takes four slices");
+static_assert(AOS_LOGPROBS_MAX_SLICES <= SEGS * NT, "a thread takes SEGS slices");
 
-/* Slices of a row: one where there are rows enough to fill the chip with a workgroup each (eight a CU), else as many as
- * do, of at least 2048 elements. */
+/* Slices of a row: as many as give the rows 512 workgroups, of at least 2048 elements. A workgroup's choice of candidates
+ * costs as much as reading some 10000 elements: 64 rows of 128256 with 20 of them 34 us in 2048 workgroups, 35 in 1024,
+ * 24 in 512, 25 in 256. */
 extern "C" void aos_logprobs_shape(int T, int vocab, int *slices, int *span) {
-  long long s = T > 0 ? AOS_LOGPROBS_WGS / T : 1;
+  long long s = T > 0 ? (512 + T - 1) / T : 1;
   if (s > vocab / 2048) s = vocab / 2048;
   if (s > AOS_LOGPROBS_MAX_SLICES) s = AOS_LOGPROBS_MAX_SLICES;
   if (s < 1) s = 1;

@@ -370,7 +370,7 @@ int aoship_model_forward(aoship_model_t *model, const int32_t *ids, int T, int p
  * samples from the logits that its step returns, crates/adapteros-lora-kernel-api/src/lib.rs:371). */
 #define AOSHIP_LOGPROBS_MAX_TOP 32
 
-/* The handle holds the workspace of rows that are cut into pieces (0.6 MB): calls allocate nothing and can be captured
+/* The handle holds the workspace of rows that are cut into pieces (0.3 MB): calls allocate nothing and can be captured
  * into a graph. Calls on one handle, replays among them, are serialised by the caller. NULL on error. */
 typedef struct aoship_logprobs_handle aoship_logprobs_t;
 aoship_logprobs_t *aoship_logprobs_new(void);
