@@ -92,9 +92,14 @@ _SIGS = {
     "aoship_kv_cache_new": (_P, [_P]),
     "aoship_kv_cache_free": (None, [_P]),
     "aoship_kv_cache_set_rope": (C.c_int, [_P, _P, _P, C.c_int]),
+    "aoship_kv_cache_set_rope_axes": (C.c_int, [_P, _P, C.c_int]),
     "aoship_kv_cache_set_stream": (C.c_int, [_P, _P]),
     "aoship_kv_cache_faults": (C.c_int, [_P]),
     "aoship_kv_append": (C.c_int, [_P, C.c_int, _P, _P]),
+    "aoship_kv_append_at": (C.c_int, [_P, C.c_int, _P, _P, _P, C.c_int64]),
+    "aoship_kv_weigh": (C.c_int, [_P, C.c_int, _P, _P, C.c_int64, C.c_int, C.c_float, C.c_int, _P]),
+    "aoship_kv_weigh_reserve": (C.c_int, [_P] + [C.c_int] * 5),
+    "aoship_kv_evict": (C.c_int, [_P, C.c_int, _P, _P]),
     "aoship_kv_read": (C.c_int, [_P, C.c_int, _P, _P, C.c_int64, _P, C.c_int64]),
     "aoship_kv_attention": (C.c_int, [_P, C.c_int, _P, _P, C.c_int64, C.c_int, C.c_float, C.c_int, _P, C.c_int64]),
 }
@@ -792,7 +797,7 @@ class LogProbs:
 
 
 KV_FORMATS = {"bf16": 0, "mxfp8": 1, "mxfp4": 2}
-KV_FAULT_BATCH, KV_FAULT_PAGE = 1, 2
+KV_FAULT_BATCH, KV_FAULT_PAGE, KV_FAULT_POSITION = 1, 2, 4
 
 
 class _KVConfig(C.Structure):
@@ -809,6 +814,20 @@ class _KVRows(C.Structure):
     _fields_ = [("q", _P), ("k", _P), ("v", _P), ("q_stride", C.c_int64), ("k_stride", C.c_int64),
                 ("v_stride", C.c_int64), ("q_bias", _P), ("k_bias", _P), ("v_bias", _P), ("q_out", _P),
                 ("q_out_stride", C.c_int64), ("num_heads", C.c_int), ("rotated", C.c_int)]
+
+
+class _KVWeights(C.Structure):
+    """aoship_kv_weights_t"""
+    _fields_ = [("prior", _P), ("prior_seq", C.c_int64), ("prior_head", C.c_int64), ("out", _P), ("out_seq", C.c_int64),
+                ("out_head", C.c_int64)]
+
+
+class _KVEvict(C.Structure):
+    """aoship_kv_evict_t"""
+    _fields_ = [("weights", _P), ("weights_seq", C.c_int64), ("weights_head", C.c_int64), ("keep", _P),
+                ("max_keep", C.c_int), ("first", C.c_int), ("recent", C.c_int), ("to_pages", _P), ("to_stride", C.c_int),
+                ("kept", _P), ("kept_seq", C.c_int64), ("kept_head", C.c_int64), ("weights_out", _P),
+                ("out_seq", C.c_int64), ("out_head", C.c_int64)]
 
 
 class KVBatch:
@@ -847,11 +866,11 @@ class KVCache:
         self.h = lib().aoship_kv_cache_new(C.byref(cfg))
         if not self.h:
             raise AosError(f"aoship_kv_cache_new: {last_error()}")
-        self.num_kv_heads, self.head_dim, self.page_size = num_kv_heads, head_dim, page_size
+        self.num_kv_heads, self.head_dim, self.page_size, self.n_axes = num_kv_heads, head_dim, page_size, 1
         import torch
 
         self._rows, self._scale = _KVRows(), head_dim ** -0.5
-        self._dtypes, self._f32 = (torch.bfloat16, torch.int16), torch.float32
+        self._dtypes, self._f32, self._i32 = (torch.bfloat16, torch.int16), torch.float32, torch.int32
         self._device = _initialised
 
     def set_rope(self, cosines=None, sines=None) -> None:
@@ -864,6 +883,20 @@ class KVCache:
             raise AosError("KVCache.set_rope: tables must be [positions, head_dim / 2]")
         _check(lib().aoship_kv_cache_set_rope(self.h, c.ctypes.data, s.ctypes.data, c.shape[0]),
                "aoship_kv_cache_set_rope")
+
+    def set_rope_axes(self, axes=None) -> None:
+        """The axis (0 .. 3) of each rotated pair, [head_dim / 2], whose position turns it where append is given positions;
+        None: all of them axis 0."""
+        if axes is None:
+            _check(lib().aoship_kv_cache_set_rope_axes(self.h, None, 0), "aoship_kv_cache_set_rope_axes")
+            self.n_axes = 1
+            return
+        a = np.asarray(axes)
+        if a.shape != (self.head_dim // 2,) or a.dtype.kind not in "iu" or a.min() < 0 or a.max() > 3:
+            raise AosError("KVCache.set_rope_axes: one axis, 0 to 3, for each of the head_dim / 2 pairs")
+        a, n = np.ascontiguousarray(a, dtype=np.uint8), int(a.max()) + 1
+        _check(lib().aoship_kv_cache_set_rope_axes(self.h, a.ctypes.data, n), "aoship_kv_cache_set_rope_axes")
+        self.n_axes = n
 
     def set_stream(self, stream_ptr) -> None:
         _check(lib().aoship_kv_cache_set_stream(self.h, stream_ptr), "aoship_kv_cache_set_stream")
@@ -901,9 +934,10 @@ class KVCache:
         return t.data_ptr(), stride[0] if n > 1 else shape[1] * hd
 
     def append(self, layer: int, batch: KVBatch, k, v, q=None, q_out=None, q_bias=None, k_bias=None,
-               v_bias=None, rotated: bool = False) -> None:
+               v_bias=None, rotated: bool = False, positions=None) -> None:
         """Biases (device float32 [heads, head_dim]) and rotary embedding of the new rows; k and v go into the pages,
-        q to q_out. rotated: the rows are rotated already (rows that read returned, written again)."""
+        q to q_out. rotated: the rows are rotated already (rows that read returned, written again). positions: device int32
+        [rows], or [axes, rows] with set_rope_axes, where the rows' rotary positions are not their places in the cache."""
         if (q is None) != (q_out is None):
             raise AosError("KVCache.append: q and q_out come together")
         r, nkv, n = self._rows, self.num_kv_heads, k.shape[0]
@@ -919,7 +953,16 @@ class KVCache:
         r.q_bias = None if q_bias is None else self._bias(q_bias, nh)
         r.k_bias = None if k_bias is None else self._bias(k_bias, nkv)
         r.v_bias = None if v_bias is None else self._bias(v_bias, nkv)
-        if _lib.aoship_kv_append(self.h, layer, self._batch(batch, n), C.byref(r)):
+        if positions is not None:
+            t = positions
+            if t.dtype is not self._i32 or t.get_device() != self._device or t.shape[-1] != n or t.dim() > 2 \
+                    or (t.shape[0] if t.dim() == 2 else 1) != self.n_axes or (n > 1 and t.stride(-1) != 1):
+                raise AosError(f"KVCache.append: positions must be device int32 [{self.n_axes}, {n}], those of an axis side "
+                               "by side")
+            ld = t.stride(0) if t.dim() == 2 and self.n_axes > 1 else n
+            if _lib.aoship_kv_append_at(self.h, layer, self._batch(batch, n), C.byref(r), t.data_ptr(), ld):
+                raise AosError(f"aoship_kv_append_at: {last_error()}")
+        elif _lib.aoship_kv_append(self.h, layer, self._batch(batch, n), C.byref(r)):
             raise AosError(f"aoship_kv_append: {last_error()}")
 
     def _bias(self, t, heads: int) -> int:
@@ -946,6 +989,59 @@ class KVCache:
         if _lib.aoship_kv_attention(self.h, layer, self._batch(batch, n), qp, qs, nh,
                                     self._scale if scale is None else scale, window, op, os_):
             raise AosError(f"aoship_kv_attention: {last_error()}")
+
+    def _table(self, what: str, t, n: int, width: int, kind) -> tuple[int, int, int]:
+        """(pointer, sequence stride, head stride) of a device tensor [n, num_kv_heads, at least width], checked."""
+        if t.dim() != 3 or t.dtype is not kind or t.get_device() != self._device or t.shape[0] != n \
+                or t.shape[1] != self.num_kv_heads or t.shape[2] < width or (t.shape[2] > 1 and t.stride(2) != 1):
+            raise AosError(f"KVCache.{what}: a device {str(kind)[6:]} tensor [{n}, {self.num_kv_heads}, {width} or more], the "
+                           "positions of a head side by side")
+        head = t.stride(1) if self.num_kv_heads > 1 else max(t.stride(1), t.shape[2])
+        return t.data_ptr(), t.stride(0) if n > 1 else self.num_kv_heads * head, head
+
+    def weigh(self, layer: int, batch: KVBatch, q, weights, scale: float | None = None, window: int = 0, prior=None) -> None:
+        """The attention weight of each cached position of the batch's sequences from the batch's rows (appended before),
+        into weights, device float32 [sequences, num_kv_heads, max_len or more]; added to those of prior (may be
+        weights itself) where given."""
+        n, c, w = q.shape[0], batch.c, _KVWeights()
+        qp, qs = self._row(q, n)
+        seqs = c.n_seqs
+        w.out, w.out_seq, w.out_head = self._table("weigh: weights", weights, seqs, c.max_len, self._f32)
+        if prior is not None:
+            w.prior, w.prior_seq, w.prior_head = self._table("weigh: prior", prior, seqs, c.max_len, self._f32)
+        if _lib.aoship_kv_weigh(self.h, layer, self._batch(batch, n), qp, qs, q.shape[1],
+                                self._scale if scale is None else scale, window, C.byref(w)):
+            raise AosError(f"aoship_kv_weigh: {last_error()}")
+
+    def reserve_weigh(self, num_heads: int, batch: KVBatch, rows: int) -> None:
+        """Sizes weigh's workspace for batches of up to this one's sizes, with up to `rows` rows."""
+        c = batch.c
+        _check(lib().aoship_kv_weigh_reserve(self.h, num_heads, c.n_seqs, rows, c.max_new, c.max_len),
+               "aoship_kv_weigh_reserve")
+
+    def evict(self, layer: int, batch: KVBatch, weights, keep, to_pages, kept, first: int = 0, recent: int = 0,
+              weights_out=None) -> None:
+        """Moves of each of the batch's sequences the first and the last (recent) positions and those of greatest weight
+        between, keep [sequences] (device int32) in all, to the pages of to_pages (device int32 [sequences, pages]); writes the
+        kept positions of each key/value head to kept, device int32 [sequences, num_kv_heads, most], and their weights
+        to weights_out."""
+        c, e = batch.c, _KVEvict()
+        n = c.n_seqs
+        for t, dims in ((keep, 1), (to_pages, 2)):
+            if t.dtype is not self._i32 or t.dim() != dims or t.shape[0] != n or t.get_device() != self._device \
+                    or (t.numel() and t.shape[-1] > 1 and t.stride(-1) != 1):
+                raise AosError("KVCache.evict: keep [n] and to_pages [n, pages] must be device int32 tensors")
+        e.weights, e.weights_seq, e.weights_head = self._table("evict: weights", weights, n, c.max_len, self._f32)
+        e.kept, e.kept_seq, e.kept_head = self._table("evict: kept", kept, n, 0, self._i32)
+        if weights_out is not None:
+            e.weights_out, e.out_seq, e.out_head = self._table("evict: weights_out", weights_out, n, c.max_len, self._f32)
+        e.keep, e.to_pages, e.to_stride = keep.data_ptr(), to_pages.data_ptr(), to_pages.shape[1]
+        if n > 1 and to_pages.stride(0) != to_pages.shape[1]:
+            e.to_stride = to_pages.stride(0)
+        e.max_keep = min(kept.shape[2], to_pages.shape[1] * self.page_size)
+        e.first, e.recent = first, recent
+        if _lib.aoship_kv_evict(self.h, layer, self._batch(batch, c.n_tokens), C.byref(e)):
+            raise AosError(f"aoship_kv_evict: {last_error()}")
 
     def __del__(self):
         if getattr(self, "h", None) and _lib is not None:

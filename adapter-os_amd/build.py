@@ -54,6 +54,8 @@ SOURCES = [
     "aoship_mlp1.hip",
     "aoship_kv.hip",
     "aoship_kv_attn.hip",
+    "aoship_kv_weigh.hip",
+    "aoship_kv_evict.hip",
     "aoship_api.cpp",
 ]
 

@@ -671,6 +671,8 @@ typedef struct {
 #define AOS_KV_MAX_HD 256
 #define AOS_KV_FAULT_BATCH 1u /* inconsistent rows or lengths of a sequence */
 #define AOS_KV_FAULT_PAGE 2u  /* a page outside the cache */
+#define AOS_KV_FAULT_POSITION 4u /* a position outside the rotary tables */
+#define AOS_KV_MAX_AXES 4
 typedef struct {
   unsigned char *pool; /* this layer's pages */
   int format, hd, hdp, nkv, page_shift /* log2 of a page's positions */, num_pages;
@@ -686,6 +688,10 @@ typedef struct {
   long long q_ld, k_ld, v_ld, out_ld;
   const float *qb, *kb, *vb; /* biases [heads][hd], NULL = none */
   const float *cosines, *sines; /* [position][hd / 2], NULL = no rotation */
+  const int32_t *at;            /* [axis][at_ld] rotary positions of the rows; NULL: those in their sequences */
+  long long at_ld;
+  const uint8_t *axes;          /* [hd / 8] axes of four pairs, two bits each; NULL: all 0 */
+  int rope_positions;
   uint16_t *q_out;
   int nh;
 } aos_kv_append_params;
@@ -695,6 +701,43 @@ typedef struct {
   uint16_t *k, *v; /* rows k_ld / v_ld elements apart */
   long long k_ld, v_ld;
 } aos_kv_read_params;
+
+/* Attention weights of cached positions (aoship_kv_weigh.hip). */
+#define AOS_KV_WEIGH_FEW 32
+#define AOS_KV_WEIGH_BLOCK 256
+#define AOS_KV_WEIGH_ROWS 1024
+#define AOS_KV_WEIGH_KEEP 1.0e9  /* bytes of kept scores at most: beyond, the keys are read twice instead */
+#define AOS_KV_WEIGH_MOST 6.4e10 /* bytes of workspace at most */
+typedef struct {
+  aos_kv_batch b;
+  const uint16_t *q;
+  long long q_ld;
+  int nh, window; /* window 0: none */
+  float scale;
+  int no_few;     /* diagnostic: no batch counts as one of few rows */
+  const float *prior; /* NULL: zeros */
+  float *w;           /* [sequence][head][position]; may be prior */
+  long long prior_seq, prior_head, w_seq, w_head;
+  /* aos_kv_weigh_shape: */
+  int few, rows, blocks, lpad, tiles, pieces, chunks;
+  /* aos_kv_weigh_parts: */
+  float *scores; /* few: [sequence][head][rows][lpad]; else the chunks' weights [sequence][head][chunks][lpad] */
+  float *part;   /* maxima and sums: few: [sequence][head][pieces][rows][2]; else [head][blocks][all rows][2] */
+  float *stat;   /* [head][all rows][2] maxima and inverse sums */
+} aos_kv_weigh_params;
+
+/* Shortening sequences to the positions of greatest weight (aoship_kv_evict.hip). */
+typedef struct {
+  aos_kv_batch b;       /* (starts unused) */
+  const float *weights; /* [sequence][head][position] */
+  float *w_out;         /* NULL, or the kept positions' weights, then zeros up to the old length */
+  long long w_seq, w_head, wo_seq, wo_head, kept_seq, kept_head;
+  const int32_t *keep;  /* [n_seqs] */
+  int max_keep, first, recent;
+  const int32_t *to;    /* [n_seqs][to_stride] pages */
+  int to_stride;
+  int32_t *kept;        /* [sequence][head][kept position] */
+} aos_kv_evict_params;
 
 /* Attention splits its work evenly over its workgroups, whatever sequence a share falls in; a row tile cut between
  * workgroups has its pieces in the slots of those workgroups (two each) and is joined by the last of them. */
@@ -739,6 +782,11 @@ void aos_logprobs_shape(int T, int vocab, int *slices, int *span);
 int aos_launch_kv_append(const aos_kv_append_params *p, const aos_launch_ctx *ctx);
 int aos_launch_kv_read(const aos_kv_read_params *p, const aos_launch_ctx *ctx);
 int aos_launch_kv_attention(const aos_kv_attn_params *p, const aos_launch_ctx *ctx);
+int aos_launch_kv_evict(const aos_kv_evict_params *p, const aos_launch_ctx *ctx);
+int aos_launch_kv_weigh(const aos_kv_weigh_params *p, const aos_launch_ctx *ctx);
+int aos_kv_weigh_shape(aos_kv_weigh_params *p, size_t *bytes); /* 0: a launch cannot count this batch's work */
+size_t aos_kv_weigh_most(const aos_kv_weigh_params *p);
+void aos_kv_weigh_parts(aos_kv_weigh_params *p, void *ws);
 int aos_kv_attention_prepare(int format, int hdp); /* once on a device before attention launches of this kind */
 int aos_kv_attention_fits(const aos_kv_batch *b, int nh); /* 1: a launch can count this batch's work */
 size_t aos_kv_part_floats(int hdp); /* workspace of an attention launch over a cache of this padded head_dim */

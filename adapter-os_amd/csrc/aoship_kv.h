@@ -102,6 +102,13 @@ __device__ __forceinline__ Seq seq_at(const aos_kv_batch &b, int s) {
   return seq_of(b, b.starts[s], b.starts[s + 1], b.lens[s]);
 }
 
+/* whether the starts of every n-th sequence from the first-th on fall */
+__host__ __device__ __forceinline__ bool starts_fall(const aos_kv_batch &b, int first, int n) {
+  bool fall = false;
+  for (int s = first; s < b.n_seqs; s += n) fall |= b.starts[s + 1] < b.starts[s];
+  return fall;
+}
+
 /* What the table says of the page that holds a position (0 <= pos < max_len, which the table covers). */
 __device__ __forceinline__ int page_entry(const aos_kv_batch &b, int s, int pos) {
   return b.pages[(long long)s * b.stride + (pos >> b.page_shift)];
@@ -114,6 +121,60 @@ __device__ __forceinline__ int page_checked(const aos_kv_batch &b, int page) {
 }
 __device__ __forceinline__ int page_of(const aos_kv_batch &b, int s, int pos) {
   return page_checked(b, page_entry(b, s, pos));
+}
+
+/* ---- what the attention and its weights share ------------------------------------------------- */
+
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+constexpr float LOG2E = 1.44269504f;
+constexpr float NINF = -__builtin_inff();
+/* Running maximum of a row that has seen positions, whose scores were all minus infinity: its sum of zero makes it NaN,
+ * that of a row that has seen nothing (NINF) zeros. */
+constexpr float LEAST = -3.40282347e38f;
+__device__ __forceinline__ float ex2(float x) { return __builtin_amdgcn_exp2f(x); }
+
+__device__ __forceinline__ float inverse(float sum, float m) {
+  return sum != 0.0f ? 1.0f / sum : m == NINF ? 0.0f : __builtin_nanf("");
+}
+/* exponent base of a running maximum: a row that has seen nothing yet keeps its zero sum free of inf - inf */
+__device__ __forceinline__ float safe_max(float m) { return m == NINF ? 0.0f : m; }
+
+/* eight consecutive codes (of W words each 8) as the bfloat16 operand of a matrix instruction */
+template <int FMT>
+__device__ __forceinline__ u32x4 decode8(const uint32_t *w, float scale) {
+  if constexpr (FMT == AOS_KV_BF16) {
+    return u32x4{w[0], w[1], w[2], w[3]};
+  } else if constexpr (FMT == AOS_KV_MXFP8) {
+    return u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[0], scale, false)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[0], scale, true)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[1], scale, false)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[1], scale, true))};
+  } else {
+    return u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[0], scale, 0)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[0], scale, 1)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[0], scale, 2)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[0], scale, 3))};
+  }
+}
+/* Scale byte j of a word (constant once unrolled) as its power of two; 255 gives infinity, which times its zero codes is
+ * NaN. Plain operations, two where one that selects a byte would do (24 streams of 32768 at 4 bits: 126 us and 124):
+ * beside matrix instructions the compiler places wait states for what it knows, not for an asm statement. */
+__device__ __forceinline__ float byte_scale(uint32_t w, int j) {
+  return __builtin_bit_cast(float, (w >> 8 * j & 255u) << 23);
+}
+
+__device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ float half_max(float x) { /* with the lane 32 away */
+  const uint32_t u = __builtin_bit_cast(uint32_t, x);
+  const auto a = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return fmaxf(__builtin_bit_cast(float, (uint32_t)a[0]), __builtin_bit_cast(float, (uint32_t)a[1]));
+}
+__device__ __forceinline__ float half_sum(float x) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, x);
+  const auto a = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return __builtin_bit_cast(float, (uint32_t)a[0]) + __builtin_bit_cast(float, (uint32_t)a[1]);
 }
 
 /* Blocks of 16 positions, aligned in their sequence, that a batch's new rows can touch: sequence s has its blocks

@@ -22,7 +22,6 @@ using namespace kv;
 
 namespace {
 
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef short s16x2 __attribute__((ext_vector_type(2)));
 
 constexpr int Q_HEADS = 8; /* query heads of a workgroup */
@@ -93,10 +92,44 @@ __device__ __forceinline__ uint32_t block_top(const uint16_t *p) {
   return m;
 }
 
+/* The cosines and sines of the pairs d .. d + 3 of a row: those of its position in the sequence, or (AT) of the positions
+ * that the caller gives it, one an axis, each pair with its axis's. A quad of pairs mostly has one axis: one load each. */
+template <bool AT>
+__device__ __forceinline__ void turn_of(const aos_kv_append_params &p, int pos, long long row, int d, f32x4 &cs, f32x4 &sn) {
+  const int half = p.b.hd / 2;
+  if constexpr (!AT) {
+    const long long at = (long long)pos * half + d;
+    cs = ld4(p.cosines + at);
+    sn = ld4(p.sines + at);
+  } else {
+    const uint32_t axes = p.axes ? p.axes[d >> 2] : 0u; /* two bits a pair */
+    auto place = [&](uint32_t axis) {
+      int at = p.at[(long long)axis * p.at_ld + row];
+      if ((unsigned)at >= (unsigned)p.rope_positions) {
+        note(p.b.faults, AOS_KV_FAULT_POSITION);
+        at = 0;
+      }
+      return (long long)at * half + d;
+    };
+    if (axes == (axes & 3u) * 0x55u) {
+      const long long at = place(axes & 3u);
+      cs = ld4(p.cosines + at);
+      sn = ld4(p.sines + at);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const long long at = place(axes >> (2 * i) & 3u) + i;
+        cs[i] = p.cosines[at];
+        sn[i] = p.sines[at];
+      }
+    }
+  }
+}
+
 /* Grid (blocks of 16 positions, groups of query heads then key/value heads). Bound by memory, by latency where there are
  * few rows: 8191 tokens of 40 query and 8 key/value heads of 128 at 16 bits 47 us (235 MB, 5.0 TB/s), 5 prompts of up to
  * 1531 tokens, 28/4 heads, at 4 bits 21 us, one token 3.9 us. */
-template <int FMT, int HDP>
+template <int FMT, int HDP, bool AT>
 __global__ void __launch_bounds__(256) aos_kv_append_kernel(aos_kv_append_params p, int qgroups) {
   constexpr int LD = HDP + 8; /* LDS row: 16 bytes of padding keep the column reads of a value unit apart */
   __shared__ __attribute__((aligned(16))) uint16_t ks[16 * LD], vs[16 * LD];
@@ -117,11 +150,7 @@ __global__ void __launch_bounds__(256) aos_kv_append_kernel(aos_kv_append_params
       if (c >= per || sub >= par) continue;
       const int t = c / chunks, d = 4 * (c % chunks);
       f32x4 cs = {}, sn = {};
-      if (rot) {
-        const long long at = (long long)(o.pos + o.lo + t) * half + d;
-        cs = ld4(p.cosines + at);
-        sn = ld4(p.sines + at);
-      }
+      if (rot) turn_of<AT>(p, o.pos + o.lo + t, o.row + t, d, cs, sn);
       const uint16_t *x = p.q + (long long)(o.row + t) * p.q_ld + d;
       uint16_t *y = p.q_out + (long long)(o.row + t) * p.out_ld + d;
       for (int h = h0 + sub; h < h1; h += par) {
@@ -169,11 +198,7 @@ __global__ void __launch_bounds__(256) aos_kv_append_kernel(aos_kv_append_params
     const int t = c / chunks, d = 4 * (c % chunks);
     const uint16_t *x = p.k + (long long)(o.row + t) * p.k_ld + h * hd + d;
     f32x4 cs = {}, sn = {}, ba = {}, bb = {};
-    if (rot) {
-      const long long at = (long long)(o.pos + o.lo + t) * half + d;
-      cs = ld4(p.cosines + at);
-      sn = ld4(p.sines + at);
-    }
+    if (rot) turn_of<AT>(p, o.pos + o.lo + t, o.row + t, d, cs, sn);
     if (p.kb) {
       ba = ld4(p.kb + h * hd + d);
       bb = ld4(p.kb + h * hd + d + half);
@@ -383,7 +408,11 @@ template <int FMT, int HDP>
 int append(const aos_kv_append_params *p, const aos_launch_ctx *ctx) {
   const int qg = p->q ? (p->nh + Q_HEADS - 1) / Q_HEADS : 0;
   aos_kv_append_params a = *p;
-  AOS_LAUNCH(ctx, (aos_kv_append_kernel<FMT, HDP>), dim3(blocks_of(p->b.max_new, p->b.n_seqs, p->b.n_tokens), qg + p->b.nkv), dim3(256), 0, a, qg);
+  const dim3 grid(blocks_of(p->b.max_new, p->b.n_seqs, p->b.n_tokens), qg + p->b.nkv);
+  if (p->at)
+    AOS_LAUNCH(ctx, (aos_kv_append_kernel<FMT, HDP, true>), grid, dim3(256), 0, a, qg);
+  else
+    AOS_LAUNCH(ctx, (aos_kv_append_kernel<FMT, HDP, false>), grid, dim3(256), 0, a, qg);
   return (int)hipGetLastError();
 }
 template <int FMT, int HDP>

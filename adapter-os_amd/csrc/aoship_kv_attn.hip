@@ -24,15 +24,9 @@ using namespace kv;
 
 namespace {
 
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int SC1 = 16; /* buffer cache policy: device-coherent (sc1) */
-constexpr float LOG2E = 1.44269504f;
-constexpr float NINF = -__builtin_inff();
-/* Running maximum of a row that has seen positions, whose scores were all minus infinity: its sum of zero makes it NaN,
- * that of a row that has seen nothing (NINF) zeros. */
-constexpr float LEAST = -3.40282347e38f;
 /* The running maximum of a row follows its scores only once they pass it by 2^SLACK (probabilities up to 256, an exact
  * power of two from what the true maximum would give): the accumulators are hardly ever rescaled. */
 constexpr float SLACK = 8.0f;
@@ -46,8 +40,6 @@ __device__ __forceinline__ uint32_t pack_bf16(float a, float b) { /* round to ne
   r[1] = (__bf16)b;
   return __builtin_bit_cast(uint32_t, r);
 }
-__device__ __forceinline__ float ex2(float x) { return __builtin_amdgcn_exp2f(x); }
-
 /* the four lanes l % 16 + 16 j combined; every lane gets the result */
 __device__ __forceinline__ float quad_max(float x) {
   const uint32_t u = __builtin_bit_cast(uint32_t, x);
@@ -65,36 +57,6 @@ __device__ __forceinline__ float quad_sum(float x) {
   const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
   return __builtin_bit_cast(float, (uint32_t)b[0]) + __builtin_bit_cast(float, (uint32_t)b[1]);
 }
-__device__ __forceinline__ float inverse(float sum, float m) {
-  return sum != 0.0f ? 1.0f / sum : m == NINF ? 0.0f : __builtin_nanf("");
-}
-/* exponent base of a running maximum: a row that has seen nothing yet keeps its zero sum free of inf - inf */
-__device__ __forceinline__ float safe_max(float m) { return m == NINF ? 0.0f : m; }
-
-/* eight consecutive codes (of W words each 8) as the bfloat16 operand of a matrix instruction */
-template <int FMT>
-__device__ __forceinline__ u32x4 decode8(const uint32_t *w, float scale) {
-  if constexpr (FMT == AOS_KV_BF16) {
-    return u32x4{w[0], w[1], w[2], w[3]};
-  } else if constexpr (FMT == AOS_KV_MXFP8) {
-    return u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[0], scale, false)),
-                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[0], scale, true)),
-                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[1], scale, false)),
-                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[1], scale, true))};
-  } else {
-    return u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[0], scale, 0)),
-                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[0], scale, 1)),
-                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[0], scale, 2)),
-                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[0], scale, 3))};
-  }
-}
-/* Scale byte j of a word (constant once unrolled) as its power of two; 255 gives infinity, which times its zero codes is
- * NaN. Plain operations, two where one that selects a byte would do (24 streams of 32768 at 4 bits: 126 us and 124):
- * beside matrix instructions the compiler places wait states for what it knows, not for an asm statement. */
-__device__ __forceinline__ float byte_scale(uint32_t w, int j) {
-  return __builtin_bit_cast(float, (w >> 8 * j & 255u) << 23);
-}
-
 /* Infinities and NaNs among the values. In a tile that a row sees only in part, the product of such a value with a
  * probability of zero would reach rows that do not see it. Once one has entered the cache (a word that append sets), the
  * kernels look for them in such tiles: the matrix product gets zeros in their place, another one counts for each row and
@@ -764,20 +726,6 @@ constexpr int tile_part_floats() { /* of a piece: maxima and sums [4 waves][2][3
   return 4 * 64 + TR * HDP;
 }
 
-__device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
-  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-}
-__device__ __forceinline__ float half_max(float x) { /* with the lane 32 away */
-  const uint32_t u = __builtin_bit_cast(uint32_t, x);
-  const auto a = __builtin_amdgcn_permlane32_swap(u, u, false, false);
-  return fmaxf(__builtin_bit_cast(float, (uint32_t)a[0]), __builtin_bit_cast(float, (uint32_t)a[1]));
-}
-__device__ __forceinline__ float half_sum(float x) {
-  const uint32_t u = __builtin_bit_cast(uint32_t, x);
-  const auto a = __builtin_amdgcn_permlane32_swap(u, u, false, false);
-  return __builtin_bit_cast(float, (uint32_t)a[0]) + __builtin_bit_cast(float, (uint32_t)a[1]);
-}
-
 /* Four positions of two dimensions (a word of 8-bit codes each, or the low halves of words of 4-bit ones) as bfloat16
  * pairs of positions {dimension 0: 01, 23, dimension 1: 01, 23}: the codes of a position side by side, so that one
  * conversion applies its scale to both, then the positions side by side. */
@@ -905,13 +853,6 @@ __host__ __device__ __forceinline__ int slot_base(const aos_kv_batch &b, int sta
   start = start < 0 ? 0 : start > b.n_tokens ? b.n_tokens : start;
   return (int)((long long)start * g / TR) + s;
 }
-/* whether the starts of every n-th sequence from the first-th on fall */
-__host__ __device__ __forceinline__ bool starts_fall(const aos_kv_batch &b, int first, int n) {
-  bool fall = false;
-  for (int s = first; s < b.n_seqs; s += n) fall |= b.starts[s + 1] < b.starts[s];
-  return fall;
-}
-
 /* Where a walk over the slots is: sequence s, which has the slots base .. next - 1. */
 struct Cursor {
   Seq q;

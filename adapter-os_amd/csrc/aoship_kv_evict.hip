@@ -1,0 +1,318 @@
+/*
+ * aoship_kv_evict.hip — shortening sequences of the paged cache to the positions that matter.
+ *
+ * Of each sequence of L positions and each key/value head, n = min(keep, L) stay: the first ones, the last ones, and of those
+ * between the ones of greatest weight (a NaN below everything; equal weights: the lower positions), in their order. They
+ * are moved to other pages, codes and scales as they are, so that nothing is rounded again.
+ *
+ *   select  the n-th greatest weight by bisection of its bits: a workgroup has a head's weights in registers (up to 32768,
+ *           else it reads them again for each bit) and counts those that reach a bound, 32 times at most; then the kept
+ *           positions' places by counting the kept ones before them.
+ *   move    a workgroup gathers a tile of 64 kept positions. Keys are 16-byte units of one position; values, whose units
+ *           hold 8 or 16 positions of a dimension, are taken apart and put together element by element.
+ */
+#include "aoship_internal.h"
+#include "aoship_kv.h"
+#include <hip/hip_ext.h>
+
+using namespace kv;
+
+namespace {
+
+constexpr int NT = 1024, NW = NT / 64;
+constexpr int PER = 32; /* weights of a thread at once */
+constexpr int SPAN = NT * PER;
+
+/* what stays of a sequence: n positions; n < 0: left out (a fault, noted) */
+struct Kept {
+  int len, n;
+};
+__device__ __forceinline__ Kept kept_of(const aos_kv_evict_params &p, int s) {
+  Kept k;
+  k.len = p.b.lens[s];
+  const int keep = p.keep[s];
+  k.n = keep < k.len ? keep : k.len;
+  const bool ok = k.len >= 0 && k.len <= p.b.max_len && keep >= 0 && k.n <= p.max_keep &&
+                  (keep >= k.len || (long long)p.first + p.recent <= keep);
+  if (!ok) {
+    k.n = -1;
+    note(p.b.faults, AOS_KV_FAULT_BATCH);
+  }
+  return k;
+}
+
+/* order of weights as unsigned numbers: a NaN first (0), both zeros alike */
+__device__ __forceinline__ uint32_t order_of(float w) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, w + 0.0f);
+  return w != w ? 0u : u ^ ((uint32_t)((int)u >> 31) | 0x80000000u);
+}
+
+/* inclusive sums over the wave's lanes */
+__device__ __forceinline__ int lane_scan(int x, int lane) {
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const int y = (int)aos_shfl((uint32_t)x, lane - d);
+    if (lane >= d) x += y;
+  }
+  return x;
+}
+
+/* Grid: sequences times key/value heads. Thread t has the positions t, t + 1024, ... of a span of 32768. */
+__global__ void __launch_bounds__(NT) aos_kv_select_kernel(aos_kv_evict_params p) {
+  __shared__ int count[2][NW];
+  __shared__ int above[PER * NW], ties[PER * NW]; /* of a wave's 64 positions: kept for sure, and of the bound's weight */
+  __shared__ int totals[2];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int s = (int)blockIdx.x / p.b.nkv, h = (int)blockIdx.x - s * p.b.nkv;
+  const Kept k = kept_of(p, s);
+  if (k.n < 0) return;
+  const float *w = p.weights + (long long)s * p.w_seq + (long long)h * p.w_head;
+  int32_t *kept = p.kept + (long long)s * p.kept_seq + (long long)h * p.kept_head;
+  float *wo = p.w_out ? p.w_out + (long long)s * p.wo_seq + (long long)h * p.wo_head : nullptr;
+  if (k.n == k.len) {
+    for (int i = tid; i < k.len; i += NT) {
+      kept[i] = i;
+      if (wo) wo[i] = w[i];
+    }
+    return;
+  }
+  const int lo = p.first, hi = k.len - p.recent; /* to choose from: lo .. hi - 1 (there are more than enough) */
+  const int m = k.n - p.first - p.recent;
+
+  /* x: a weight's order plus one, 0 for positions that are not to be chosen from (n < len <= 2^30, and the order of
+   * the greatest float stays below 2^32 - 1) */
+  auto load = [&](uint32_t (&x)[PER], int base) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int pos = base + i * NT + tid;
+      x[i] = pos >= lo && pos < hi ? order_of(w[pos]) + 1u : 0u;
+    }
+  };
+  const bool once = k.len <= SPAN;
+  uint32_t x[PER];
+  if (once) load(x, 0);
+  /* the greatest bound that at least m reach; with exactly m there are no ties to part */
+  uint32_t bound = 0;
+  int reach = 0; /* how many reach it (where bound > 0) */
+  if (m > 0) {
+    int turn = 0;
+    for (int bit = 31; bit >= 0; --bit, turn ^= 1) {
+      const uint32_t at = bound | (1u << bit);
+      int c = 0;
+      for (int base = 0; base < k.len; base += SPAN) {
+        if (!once) load(x, base);
+#pragma unroll
+        for (int i = 0; i < PER; ++i) c += (int)__popcll(__ballot(x[i] >= at));
+      }
+      if (lane == 0) count[turn][wave] = c;
+      __syncthreads();
+      int all = 0;
+#pragma unroll
+      for (int i = 0; i < NW; ++i) all += count[turn][i];
+      if (all >= m) {
+        bound = at;
+        reach = all;
+        if (all == m) break; /* uniform */
+      }
+    }
+  } else {
+    bound = 0xffffffffu; /* (no weight's) */
+  }
+  const bool exact = m == 0 || reach == m;
+  int taken = 0, left = 0; /* places before this span; ties that are still kept */
+  if (!exact) {
+    /* m less those above the bound */
+    int c = 0;
+    for (int base = 0; base < k.len; base += SPAN) {
+      if (!once) load(x, base);
+#pragma unroll
+      for (int i = 0; i < PER; ++i) c += (int)__popcll(__ballot(x[i] > bound));
+    }
+    __syncthreads();
+    if (lane == 0) count[0][wave] = c;
+    __syncthreads();
+    left = m;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) left -= count[0][i];
+  }
+
+  for (int base = 0; base < k.len; base += SPAN) {
+    if (!once) load(x, base);
+    auto sure = [&](int i) { /* kept whatever its ties */
+      const int pos = base + i * NT + tid;
+      return pos < k.len && (pos < lo || pos >= hi || (exact ? x[i] >= bound : x[i] > bound));
+    };
+    auto tie = [&](int i) { return !exact && x[i] == bound; }; /* (bound > 0) */
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int a = (int)__popcll(__ballot(sure(i))), t = (int)__popcll(__ballot(tie(i)));
+      if (lane == 0) {
+        above[i * NW + wave] = a;
+        ties[i * NW + wave] = t;
+      }
+    }
+    __syncthreads();
+    if (wave == 0) {
+      /* PER * NW groups of 64 positions in order, 8 a lane: ties before each, then places before each */
+      int t[PER * NW / 64], sum = 0;
+#pragma unroll
+      for (int i = 0; i < PER * NW / 64; ++i) {
+        t[i] = ties[lane * (PER * NW / 64) + i];
+        sum += t[i];
+      }
+      int before = lane_scan(sum, lane) - sum, places = 0;
+      const int all_ties = __builtin_amdgcn_readlane(before + sum, 63);
+      int a[PER * NW / 64];
+#pragma unroll
+      for (int i = 0; i < PER * NW / 64; ++i) {
+        const int at = lane * (PER * NW / 64) + i, room = left - before;
+        a[i] = above[at] + (room < 0 ? 0 : room < t[i] ? room : t[i]);
+        ties[at] = before;
+        before += t[i];
+        places += a[i];
+      }
+      int place = lane_scan(places, lane) - places;
+      if (lane == 63) {
+        totals[0] = place + places;
+        totals[1] = all_ties;
+      }
+#pragma unroll
+      for (int i = 0; i < PER * NW / 64; ++i) {
+        above[lane * (PER * NW / 64) + i] = place;
+        place += a[i];
+      }
+    }
+    __syncthreads();
+    const uint64_t below = (1ull << lane) - 1ull;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const bool y = sure(i), t = tie(i);
+      const uint64_t ys = __ballot(y), ts = __ballot(t);
+      const int room = left - ties[i * NW + wave], mine = (int)__popcll(ts & below);
+      const int at = taken + above[i * NW + wave] + (int)__popcll(ys & below) + (mine < room ? mine : room > 0 ? room : 0);
+      if (y || (t && mine < room)) {
+        const int pos = base + i * NT + tid;
+        kept[at] = pos;
+        if (wo) wo[at] = w[pos];
+      }
+    }
+    __syncthreads();
+    taken += totals[0];
+    left -= totals[1] < left ? totals[1] : left;
+    __syncthreads(); /* (totals are free again) */
+  }
+  if (wo)
+    for (int i = k.n + tid; i < k.len; i += NT) wo[i] = 0.0f;
+}
+
+/* Grid: tiles of 64 kept positions, key/value heads, sequences. */
+template <int FMT, int HDP>
+__global__ void __launch_bounds__(256) aos_kv_move_kernel(aos_kv_evict_params p, int tiles) {
+  __shared__ const unsigned char *src[TILE]; /* the tiles that the positions are in; NULL: none */
+  __shared__ int in[TILE];                   /* their places in them */
+  const int tid = threadIdx.x;
+  const int tile = (int)(blockIdx.x % (uint32_t)tiles), sh = (int)(blockIdx.x / (uint32_t)tiles);
+  const int s = sh / p.b.nkv, h = sh - s * p.b.nkv, i0 = tile * TILE;
+  const Kept k = kept_of(p, s);
+  if (i0 >= k.n) return;
+  const int n = k.n - i0 < TILE ? k.n - i0 : TILE;
+  const int to = page_checked(p.b, p.to[(long long)s * p.to_stride + (i0 >> p.b.page_shift)]);
+  if (to < 0) return; /* uniform */
+  unsigned char *dst = tile_ptr<FMT, HDP>(p.b, to, h, i0);
+  if (tid < TILE) {
+    const unsigned char *t = nullptr;
+    int pos = 0;
+    if (tid < n) {
+      pos = p.kept[(long long)s * p.kept_seq + (long long)h * p.kept_head + i0 + tid];
+      const int page = (unsigned)pos < (unsigned)k.len ? page_of(p.b, s, pos) : -1;
+      if (page >= 0) t = tile_ptr<FMT, HDP>(p.b, page, h, pos);
+    }
+    src[tid] = t;
+    in[tid] = pos & (TILE - 1);
+  }
+  __syncthreads();
+
+  constexpr int KU = HDP * bits<FMT>() / 128; /* key units of a position */
+#pragma unroll 4
+  for (int c = tid; c < KU * TILE; c += 256) {
+    const int i = c % TILE, u = c / TILE;
+    if (i >= n) continue;
+    const unsigned char *t = src[i];
+    *(u32x4 *)(dst + (u * TILE + i) * 16) = t ? aos_gld16(t + (u * TILE + in[i]) * 16) : u32x4{};
+  }
+  if constexpr (FMT == AOS_KV_BF16) {
+    for (int c = tid; c < (TILE / 8) * HDP; c += 256) {
+      const int d = c % HDP, u = c / HDP;
+      if (8 * u >= n) break;
+      uint32_t x[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const unsigned char *t = src[8 * u + e];
+        const int at = in[8 * u + e];
+        x[e] = t ? *(const __attribute__((address_space(1))) uint16_t *)(t + v_off<FMT, HDP>() + (at / 8 * HDP + d) * 16 + at % 8 * 2) : 0u;
+      }
+      *(u32x4 *)(dst + v_off<FMT, HDP>() + (u * HDP + d) * 16) =
+          u32x4{x[0] | x[1] << 16, x[2] | x[3] << 16, x[4] | x[5] << 16, x[6] | x[7] << 16};
+    }
+  } else {
+    constexpr int W = FMT == AOS_KV_MXFP8 ? 4 : 2; /* words of a value unit: 16 positions of a dimension */
+    for (int c = tid; c < (TILE / 16) * HDP; c += 256) {
+      const int d = c % HDP, u = c / HDP;
+      if (16 * u >= n) break;
+      uint32_t y[W] = {};
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const unsigned char *t = src[16 * u + e];
+        const int at = in[16 * u + e], byte = FMT == AOS_KV_MXFP8 ? at % 16 : at % 16 / 2;
+        uint32_t x = t ? *(const __attribute__((address_space(1))) unsigned char *)(t + v_off<FMT, HDP>() + (at / 16 * HDP + d) * (4 * W) + byte) : 0u;
+        if constexpr (FMT == AOS_KV_MXFP8) {
+          y[e / 4] |= x << (8 * (e % 4));
+        } else {
+          x = at & 1 ? x >> 4 : x & 15u;
+          y[e / 8] |= x << (4 * (e % 8));
+        }
+      }
+      if constexpr (FMT == AOS_KV_MXFP8)
+        *(u32x4 *)(dst + v_off<FMT, HDP>() + (u * HDP + d) * 16) = u32x4{y[0], y[1], y[W - 2], y[W - 1]};
+      else
+        *(u32x2 *)(dst + v_off<FMT, HDP>() + (u * HDP + d) * 8) = u32x2{y[0], y[1]};
+    }
+    for (int c = tid; c < 2 * (HDP / 32) * TILE; c += 256) {
+      const int i = c % TILE, b = c / TILE % (HDP / 32);
+      if (i >= n) continue;
+      const bool is_v = c >= (HDP / 32) * TILE;
+      const unsigned char *t = src[i];
+      const int from = is_v ? vs_off<FMT, HDP>() + b * TILE + in[i] : ks_off<FMT, HDP>() + b * TILE + ks_index(in[i]);
+      const int at = is_v ? vs_off<FMT, HDP>() + b * TILE + i : ks_off<FMT, HDP>() + b * TILE + ks_index(i);
+      dst[at] = t ? t[from] : 0;
+    }
+  }
+}
+
+template <int FMT, int HDP>
+int evict(const aos_kv_evict_params *p, const aos_launch_ctx *ctx) {
+  const uint32_t sh = (uint32_t)p->b.n_seqs * (uint32_t)p->b.nkv;
+  AOS_LAUNCH(ctx, aos_kv_select_kernel, dim3(sh), dim3(NT), 0, *p);
+  const hipError_t e = hipGetLastError();
+  const int tiles = (p->max_keep + TILE - 1) / TILE;
+  if (e != hipSuccess || tiles == 0) return (int)e;
+  AOS_LAUNCH(ctx, (aos_kv_move_kernel<FMT, HDP>), dim3(sh * (uint32_t)tiles), dim3(256), 0, *p, tiles);
+  return (int)hipGetLastError();
+}
+
+}  // namespace
+
+#define KV_DISPATCH(fn, fmt, hdp, ...)                                       \
+  ((hdp) == 64 ? ((fmt) == AOS_KV_BF16    ? fn<AOS_KV_BF16, 64>(__VA_ARGS__)    \
+                  : (fmt) == AOS_KV_MXFP8 ? fn<AOS_KV_MXFP8, 64>(__VA_ARGS__)   \
+                                          : fn<AOS_KV_MXFP4, 64>(__VA_ARGS__))  \
+   : (hdp) == 128 ? ((fmt) == AOS_KV_BF16    ? fn<AOS_KV_BF16, 128>(__VA_ARGS__)   \
+                     : (fmt) == AOS_KV_MXFP8 ? fn<AOS_KV_MXFP8, 128>(__VA_ARGS__)  \
+                                             : fn<AOS_KV_MXFP4, 128>(__VA_ARGS__)) \
+                  : ((fmt) == AOS_KV_BF16    ? fn<AOS_KV_BF16, 256>(__VA_ARGS__)   \
+                     : (fmt) == AOS_KV_MXFP8 ? fn<AOS_KV_MXFP8, 256>(__VA_ARGS__)  \
+                                             : fn<AOS_KV_MXFP4, 256>(__VA_ARGS__)))
+
+extern "C" int aos_launch_kv_evict(const aos_kv_evict_params *p, const aos_launch_ctx *ctx) {
+  return KV_DISPATCH(evict, p->b.format, p->b.hdp, p, ctx);
+}

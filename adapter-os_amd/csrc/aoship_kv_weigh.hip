@@ -1,0 +1,596 @@
+/*
+ * aoship_kv_weigh.hip — the attention weight that each position of the paged cache gets from a batch's rows.
+ *
+ * For key/value head h of a sequence, over its rows r (new token and query head of the group) that see position j:
+ *
+ *   w_j = prior_j + sum_r e^(s_rj - m_r) / l_r,   s_rj = scale q_r . k_j,  m_r = max_j s_rj,  l_r = sum_j e^(s_rj - m_r)
+ *
+ * A weight needs its rows' sums over all positions first. Sequences of up to 32 rows (a token, a few) read their keys
+ * once: the scores go to memory as they are formed (4 bytes for a row's position), with the rows' maxima and sums over
+ * pieces of the sequence, and a second launch makes weights of them. With more rows the scores would be more than the
+ * keys: they are formed twice, for the sums and for the weights. Scores, sums and weights are float32, added in one order.
+ *
+ * Matrix instructions' registers (aoship_device.h): every accumulator register is read.
+ */
+#include "aoship_internal.h"
+#include "aoship_kv.h"
+#include <hip/hip_ext.h>
+
+using namespace kv;
+
+namespace {
+
+constexpr int FEW = AOS_KV_WEIGH_FEW;      /* rows of a sequence whose scores are kept */
+constexpr int KB = AOS_KV_WEIGH_BLOCK;     /* positions of a workgroup: a tile of 64 a wave */
+constexpr int RC = AOS_KV_WEIGH_ROWS;      /* rows of a workgroup where there are many */
+constexpr int RT = 64;                     /* rows of a stage */
+
+/* A tile's keys of 32 positions a block, as the matrix instructions take them: lane l has the quarter of position
+ * l % 32 (through `at`) that half l / 32 of the dimensions makes, undecoded. */
+template <int FMT, int HDP>
+struct Keys {
+  static constexpr int UNITS = HDP * bits<FMT>() / 256; /* 16-byte units of a lane and block */
+  static constexpr int SB = FMT == AOS_KV_BF16 ? 0 : HDP / 64;
+  static constexpr int W8 = bits<FMT>() / 4; /* words of 8 codes */
+  uint32_t w[2][UNITS * 4];
+  uint32_t sb[2][SB ? SB : 1];
+  /* at: the position of this lane's row within a block */
+  __device__ __forceinline__ void load(const unsigned char *t, int at, int half) {
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const int pos = 32 * b + at;
+#pragma unroll
+      for (int i = 0; i < UNITS; ++i) {
+        const u32x4 x = aos_gld16(t + ((half * UNITS + i) * TILE + pos) * 16);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[b][4 * i + j] = x[j];
+      }
+      if constexpr (SB > 0)
+#pragma unroll
+        for (int i = 0; i < SB; ++i)
+          sb[b][i] = *(const __attribute__((address_space(1))) unsigned char *)(t + ks_off<FMT, HDP>() + (half * SB + i) * TILE + ks_index(pos));
+    }
+  }
+  /* step e of a block: 8 dimensions from half * HDP / 2 + 8 e on */
+  __device__ __forceinline__ u32x4 operand(int b, int e) const {
+    return decode8<FMT>(&w[b][e * W8], FMT == AOS_KV_BF16 ? 1.0f : byte_scale(sb[b][SB ? e / 4 : 0], 0));
+  }
+};
+
+/* a sequence's visible span, as row (token) t sees it: [lo, hi] */
+struct Span {
+  int p0, window;
+  __device__ __forceinline__ int hi(int t) const { return p0 + t; }
+  __device__ __forceinline__ int lo(int t) const { return window > 0 && p0 + t - window + 1 > 0 ? p0 + t - window + 1 : 0; }
+};
+
+__device__ __forceinline__ float score_factor(float scale) { /* (a scale of zero stays above it: masks keep -infinity) */
+  return fmaxf(fabsf(scale) * LOG2E, 1.17549435e-38f);
+}
+
+/* ---- few rows -------------------------------------------------------------------------------- */
+
+/* Grid: pieces of `tiles` position tiles, key/value heads, sequences. S^T = K . Q^T by v_mfma_f32_32x32x16_bf16: row
+ * 16 s + 8 a + 4 c + i of a block of 32 keys is position 16 c + 8 s + 4 a + i, so that a lane's 16 scores are 16
+ * consecutive positions of its row. The waves take a piece's tiles in turn. */
+template <int FMT, int HDP>
+__global__ void __launch_bounds__(256, 2) aos_kv_scores_kernel(aos_kv_weigh_params p) {
+  constexpr int KS = HDP / 16;
+  __shared__ float ml[4][2][32];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 31, half = lane >> 5;
+  const int piece = (int)(blockIdx.x % (uint32_t)p.pieces), sh = (int)(blockIdx.x / (uint32_t)p.pieces);
+  const int s = sh / p.b.nkv, h = sh - s * p.b.nkv;
+  const Seq q = seq_at(p.b, s);
+  const int g = p.nh / p.b.nkv, rows = q.count * g;
+  const Span v = {q.len - q.count, p.window};
+  if (rows == 0 || q.len == 0) return;
+  const int first = v.lo(0) / TILE, end = (q.len + TILE - 1) / TILE; /* tiles that some row sees */
+  int t0 = piece * p.tiles, t1 = t0 + p.tiles < end ? t0 + p.tiles : end;
+  if (t0 < first) t0 = first;
+  if (t0 >= t1) return;
+
+  const int rr = col < rows ? col : rows - 1, t = rr / g, hh = h * g + rr - t * g;
+  const int hi = v.hi(t), lo = v.lo(t), lo_max = v.lo(q.count - 1), hi_min = v.hi(0);
+  const float cs = score_factor(p.scale);
+  const uint32_t flip = p.scale < 0.0f ? 0x80008000u : 0u;
+  u32x4 qf[KS];
+  const uint16_t *qr = p.q + (long long)(q.row0 + t) * p.q_ld + hh * p.b.hd;
+#pragma unroll
+  for (int e = 0; e < KS; ++e) {
+    const int d = half * (HDP / 2) + 8 * e;
+    qf[e] = d < p.b.hd && col < rows ? aos_gld16(qr + d) : u32x4{};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) qf[e][i] ^= flip;
+  }
+  const int at = ((col & 4) << 2) | ((col & 16) >> 1) | ((col & 8) >> 1) | (col & 3);
+  float *out = p.scores + ((long long)sh * p.rows + col) * p.lpad + 16 * half;
+  float m = NINF, l = 0.0f;
+  for (int i = t0 + wave; i < t1; i += 4) {
+    const int tb = i * TILE, page = page_of(p.b, s, tb);
+    Keys<FMT, HDP> k;
+    k.load(tile_ptr<FMT, HDP>(p.b, page < 0 ? 0 : page, h, tb), at, half);
+    f32x16 sc[2] = {f32x16{}, f32x16{}};
+#pragma unroll
+    for (int e = 0; e < KS; ++e)
+#pragma unroll
+      for (int b = 0; b < 2; ++b) sc[b] = mfma32(k.operand(b, e), qf[e], sc[b]);
+    if (page < 0 || tb < lo_max || tb + TILE - 1 > hi_min) {
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const int pos = tb + 32 * b + 16 * half + j;
+          if (page < 0 || pos < lo || pos > hi) sc[b][j] = NINF;
+        }
+    }
+    float mx = NINF;
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) mx = fmaxf(mx, sc[b][j]);
+    mx = half_max(mx) * cs;
+    if (page >= 0 && lo < tb + TILE && hi >= tb) mx = fmaxf(mx, LEAST);
+    const float top = fmaxf(m, mx), ms = safe_max(top);
+    l = l * ex2(m - ms);
+    m = top;
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) l = l + ex2(fmaf(sc[b][j], cs, -ms));
+    if (col < rows)
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int j = 0; j < 16; j += 4)
+          *(f32x4 *)(out + tb + 32 * b + j) = f32x4{sc[b][j], sc[b][j + 1], sc[b][j + 2], sc[b][j + 3]};
+  }
+  l = half_sum(l);
+  if (half == 0) {
+    ml[wave][0][col] = m;
+    ml[wave][1][col] = l;
+  }
+  __syncthreads();
+  if (tid < rows) {
+    float top = NINF, sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) top = fmaxf(top, ml[w][0][tid]);
+    const float ms = safe_max(top);
+#pragma unroll
+    for (int w = 0; w < 4; ++w) sum = sum + ml[w][1][tid] * ex2(ml[w][0][tid] - ms);
+    float *part = p.part + ((long long)blockIdx.x * p.rows + tid) * 2;
+    part[0] = top;
+    part[1] = sum;
+  }
+}
+
+/* four weights at a position (a multiple of 4): prior + x, of positions below len */
+__device__ __forceinline__ void store4(const aos_kv_weigh_params &p, int s, int h, int pos, int len, const float *x) {
+  float *w = p.w + (long long)s * p.w_seq + (long long)h * p.w_head + pos;
+  const float *o = p.prior ? p.prior + (long long)s * p.prior_seq + (long long)h * p.prior_head + pos : nullptr;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (pos + i < len) w[i] = o ? o[i] + x[i] : x[i];
+}
+
+/* Grid: pieces of 1024 positions, key/value heads, sequences: the kept scores made weights. A thread has four positions. */
+constexpr int WB = 1024;
+__global__ void __launch_bounds__(256) aos_kv_weights_kernel(aos_kv_weigh_params p, int blocks) {
+  __shared__ float red[8][2][FEW], base[FEW], inv[FEW];
+  const int tid = threadIdx.x;
+  const int blk = (int)(blockIdx.x % (uint32_t)blocks), sh = (int)(blockIdx.x / (uint32_t)blocks);
+  const int s = sh / p.b.nkv, h = sh - s * p.b.nkv;
+  const Seq q = seq_at(p.b, s);
+  const int rows = q.count * (p.nh / p.b.nkv), pos = blk * WB + 4 * tid;
+  if (blk * WB >= q.len) return;
+  const Span v = {q.len - q.count, p.window};
+  const int first = rows ? v.lo(0) / TILE : 0; /* the scores of earlier tiles were not formed */
+  if (rows) {
+    /* the rows' maxima and sums over the pieces, eight threads a row */
+    const int c0 = first / p.tiles, c1 = ((q.len - 1) / TILE) / p.tiles, r = tid % FEW, k = tid / FEW;
+    const float *part = p.part + ((long long)sh * p.pieces * p.rows + r) * 2;
+    float m = NINF, l = 0.0f;
+    if (r < rows)
+      for (int c = c0 + k; c <= c1; c += 8) {
+        const float pm = part[(long long)c * p.rows * 2], pl = part[(long long)c * p.rows * 2 + 1];
+        const float top = fmaxf(m, pm), ms = safe_max(top);
+        l = l * ex2(m - ms) + pl * ex2(pm - ms);
+        m = top;
+      }
+    red[k][0][r] = m;
+    red[k][1][r] = l;
+    __syncthreads();
+    if (tid < FEW) {
+      float top = NINF, sum = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) top = fmaxf(top, red[i][0][tid]);
+      const float ms = safe_max(top);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum = sum + red[i][1][tid] * ex2(red[i][0][tid] - ms);
+      base[tid] = ms;
+      inv[tid] = inverse(sum, top);
+    }
+    __syncthreads();
+  }
+  if (pos >= q.len) return;
+  float x[4] = {};
+  if (rows && pos + 3 >= first * TILE) {
+    const float cs = score_factor(p.scale);
+    const float *sc = p.scores + (long long)sh * p.rows * p.lpad + pos;
+    for (int r = 0; r < rows; ++r) {
+      const f32x4 y = *(const f32x4 *)(sc + (long long)r * p.lpad);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = fmaf(ex2(fmaf(y[i], cs, -base[r])), inv[r], x[i]);
+    }
+    bool odd = false;
+    for (int r = 0; r < rows; ++r) odd |= inv[r] != inv[r];
+    if (odd) { /* rows without a distribution: what they do not see has no part of them */
+      const bool there = page_of(p.b, s, pos) >= 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        x[i] = 0.0f;
+        for (int r = 0; r < rows; ++r) {
+          const int t = r / (p.nh / p.b.nkv);
+          if (!there || pos + i < v.lo(t) || pos + i > v.hi(t)) continue;
+          x[i] = fmaf(ex2(fmaf(sc[(long long)r * p.lpad + i], cs, -base[r])), inv[r], x[i]);
+        }
+      }
+    }
+  }
+  store4(p, s, h, pos, q.len, x);
+}
+
+template <int FMT, int HDP>
+int launch_few(const aos_kv_weigh_params *p, const aos_launch_ctx *ctx) {
+  const uint32_t sh = (uint32_t)p->b.n_seqs * (uint32_t)p->b.nkv;
+  AOS_LAUNCH(ctx, (aos_kv_scores_kernel<FMT, HDP>), dim3(sh * (uint32_t)p->pieces), dim3(256), 0, *p);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return (int)e;
+  const int blocks = (p->b.max_len + WB - 1) / WB;
+  AOS_LAUNCH(ctx, aos_kv_weights_kernel, dim3(sh * (uint32_t)blocks), dim3(256), 0, *p, blocks);
+  return (int)hipGetLastError();
+}
+
+/* ---- many rows ------------------------------------------------------------------------------- */
+
+/* The rows of a sequence that see some of the positions k0 .. k1 - 1: [ra, rb) */
+struct Rows {
+  int ra, rb;
+};
+__device__ __forceinline__ Rows rows_of(const Seq &q, const Span &v, int g, int k0, int k1) {
+  Rows r;
+  const int ta = k0 - v.p0, tb = v.window > 0 && k1 - 1 + v.window - 1 - v.p0 < q.count - 1 ? k1 - 1 + v.window - 1 - v.p0 : q.count - 1;
+  r.ra = (ta > 0 ? ta : 0) * g;
+  r.rb = (tb + 1) * g;
+  return r;
+}
+
+/* Whether the batch's starts fall somewhere (noted): its sequences' rows may then be the same, and none of them is served. */
+__device__ __forceinline__ bool refused(const aos_kv_batch &b, int tid, int n) {
+  if (!__syncthreads_or(starts_fall(b, tid, n) ? 1 : 0)) return false;
+  if (tid == 0) note(b.faults, AOS_KV_FAULT_BATCH);
+  return true;
+}
+
+/* A stage: 64 rows' queries, [unit of 8 dimensions][row], a unit's rows 16 bytes more apart than they take (a row's
+ * units, which 16 lanes write, then lie in different banks), with the rows' maxima and factors or positions. */
+template <int HDP>
+struct Stage {
+  static constexpr int UNITS = HDP / 8, LD = RT * 16 + 16, N = UNITS * RT / 256;
+  unsigned char q[UNITS * LD];
+  int hi[RT];
+  float m[RT], f[RT];
+};
+
+/* A workgroup has the keys of KB positions in registers, a tile a wave, and the rows of one chunk (RC of them) that see
+ * some of them go by in stages of 64 through LDS.
+ *   SUM false: each row's maximum and sum over the block's positions, to part[head][block][row].
+ *   SUM true: the weights of the block's positions from the chunk's rows, to scores[sequence][head][chunk][position].
+ * Grid: blocks, chunks, key/value heads, sequences. */
+template <int FMT, int HDP, bool SUM>
+__global__ void __launch_bounds__(256, HDP == 256 ? 1 : 2) aos_kv_weigh_kernel(aos_kv_weigh_params p) {
+  constexpr int KS = HDP / 16, N = Stage<HDP>::N, LD = Stage<HDP>::LD, UNITS = Stage<HDP>::UNITS;
+  __shared__ __attribute__((aligned(16))) Stage<HDP> st[2];
+  __shared__ float red[SUM ? 1 : 2][4][2][SUM ? 1 : RT];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 31, half = lane >> 5;
+  if (refused(p.b, tid, 256)) return;
+  int x = (int)blockIdx.x;
+  const int blk = x % p.blocks;
+  x /= p.blocks;
+  const int chunk = x % p.chunks;
+  x /= p.chunks;
+  const int s = x / p.b.nkv, h = x - s * p.b.nkv;
+  const Seq q = seq_at(p.b, s);
+  const int g = p.nh / p.b.nkv, k0 = blk * KB, k1 = k0 + KB < q.len ? k0 + KB : q.len;
+  if (q.count == 0 || k0 >= q.len) return;
+  const Span v = {q.len - q.count, p.window};
+  const Rows vis = rows_of(q, v, g, k0, k1);
+  const int ra = vis.ra > chunk * RC ? vis.ra / RT * RT : chunk * RC;
+  const int rb = vis.rb < (chunk + 1) * RC ? vis.rb : (chunk + 1) * RC;
+  if (ra >= rb) return;
+
+  /* this wave's keys */
+  const int tb = k0 + TILE * wave;
+  const int page = tb < q.len ? page_of(p.b, s, tb) : -1;
+  u32x4 kf[2][KS];
+  {
+    Keys<FMT, HDP> k;
+    k.load(tile_ptr<FMT, HDP>(p.b, page < 0 ? 0 : page, h, tb), col, half);
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int e = 0; e < KS; ++e) kf[b][e] = k.operand(b, e);
+  }
+  const float cs = score_factor(p.scale);
+  const uint32_t flip = p.scale < 0.0f ? 0x80008000u : 0u;
+  const long long total = (long long)p.b.n_tokens * g; /* rows of a head */
+  const float2 *stat = (const float2 *)p.stat + h * total + (long long)q.row0 * g;
+
+  /* a thread's pieces of a stage: rows tid / UNITS + i * 256 / UNITS, unit tid % UNITS */
+  constexpr int STEP = 256 / UNITS;
+  const int unit = tid % UNITS, row1 = tid / UNITS;
+  u32x4 fq[N];
+  float2 fs = {0.0f, 0.0f};
+  int fh = 0;
+  auto fetch = [&](int r0) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int r = r0 + row1 + i * STEP, t = r / g, hh = h * g + r - t * g;
+      fq[i] = u32x4{};
+      if (r < rb && 8 * unit < p.b.hd) fq[i] = aos_gld16(p.q + (long long)(q.row0 + t) * p.q_ld + hh * p.b.hd + 8 * unit);
+    }
+    if (tid < RT) {
+      const int r = r0 + tid;
+      fh = r < rb ? v.hi(r / g) : -1;
+      if (SUM && r < rb) fs = stat[r];
+    }
+  };
+  auto put = [&](Stage<HDP> &d) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      u32x4 y = fq[i];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) y[j] ^= flip;
+      *(u32x4 *)(d.q + unit * LD + (row1 + i * STEP) * 16) = y;
+    }
+    if (tid < RT) {
+      d.hi[tid] = fh;
+      if (SUM) {
+        d.m[tid] = fs.x;
+        d.f[tid] = fs.y;
+      }
+    }
+  };
+  float acc[2] = {0.0f, 0.0f};
+  fetch(ra);
+  put(st[0]);
+  __syncthreads();
+  int i = 0;
+  for (int r0 = ra; r0 < rb; r0 += RT, ++i) {
+    const Stage<HDP> &d = st[i & 1];
+    if (r0 + RT < rb) fetch(r0 + RT);
+    /* the stage's rows see up to hi_min .. hi_max, from lo_min .. lo_max on */
+    const int last = r0 + RT < rb ? r0 + RT - 1 : rb - 1;
+    const int ta = r0 / g, tz = last / g;
+    const bool any = page >= 0 && tb <= v.hi(tz) && tb + TILE > v.lo(ta);
+    const bool edge = tb < v.lo(tz) || tb + TILE - 1 > v.hi(ta) || r0 + RT > rb;
+#pragma unroll
+    for (int sub = 0; sub < 2; ++sub) {
+      float m = NINF, l = 0.0f;
+      if (any) { /* uniform */
+        f32x16 sc[2] = {f32x16{}, f32x16{}};
+#pragma unroll
+        for (int e = 0; e < KS; ++e) {
+          const u32x4 qf = *(const u32x4 *)(d.q + (half * KS + e) * LD + (32 * sub + col) * 16);
+#pragma unroll
+          for (int b = 0; b < 2; ++b) sc[b] = SUM ? mfma32(qf, kf[b][e], sc[b]) : mfma32(kf[b][e], qf, sc[b]);
+        }
+        if constexpr (!SUM) {
+          const int hi = d.hi[32 * sub + col], lo = v.lo(hi - v.p0);
+          if (edge) {
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+              for (int j = 0; j < 16; ++j) {
+                const int pos = tb + 32 * b + 8 * (j >> 2) + 4 * half + (j & 3);
+                if (pos < lo || pos > hi) sc[b][j] = NINF;
+              }
+          }
+          float mx = NINF;
+#pragma unroll
+          for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) mx = fmaxf(mx, sc[b][j]);
+          mx = half_max(mx) * cs;
+          if (lo < tb + TILE && hi >= tb) mx = fmaxf(mx, LEAST);
+          m = mx;
+          const float ms = safe_max(m);
+#pragma unroll
+          for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) l = l + ex2(fmaf(sc[b][j], cs, -ms));
+          l = half_sum(l);
+        } else {
+#pragma unroll
+          for (int j4 = 0; j4 < 4; ++j4) {
+            const int at = 32 * sub + 8 * j4 + 4 * half; /* rows at .. at + 3 of the stage */
+            const f32x4 rm = *(const f32x4 *)(d.m + at), rf = *(const f32x4 *)(d.f + at);
+            const int4 hi = *(const int4 *)(d.hi + at);
+            const int his[4] = {hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                float e = ex2(fmaf(sc[b][4 * j4 + j], cs, -rm[j])) * rf[j];
+                if (edge) {
+                  const int pos = tb + 32 * b + col;
+                  e = pos >= v.lo(his[j] - v.p0) && pos <= his[j] ? e : 0.0f;
+                }
+                acc[b] = acc[b] + e;
+              }
+          }
+        }
+      }
+      if constexpr (!SUM) {
+        if (half == 0) {
+          red[i & 1][wave][0][32 * sub + col] = m;
+          red[i & 1][wave][1][32 * sub + col] = l;
+        }
+      }
+    }
+    if (r0 + RT < rb) put(st[(i + 1) & 1]);
+    __syncthreads();
+    if constexpr (!SUM) {
+      if (tid < RT && r0 + tid < rb) {
+        float top = NINF, sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) top = fmaxf(top, red[i & 1][w][0][tid]);
+        const float ms = safe_max(top);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) sum = sum + red[i & 1][w][1][tid] * ex2(red[i & 1][w][0][tid] - ms);
+        float2 *part = (float2 *)p.part + ((long long)h * p.blocks + blk) * total + (long long)q.row0 * g + r0 + tid;
+        *part = make_float2(top, sum);
+      }
+    }
+  }
+  if constexpr (SUM) {
+    float *out = p.scores + (((long long)s * p.b.nkv + h) * p.chunks + chunk) * p.lpad + tb;
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const float sum = half_sum(acc[b]);
+      if (half == 0 && tb < q.len) out[32 * b + col] = sum;
+    }
+  }
+}
+
+/* Grid: pieces of 256 rows, key/value heads, sequences: a row's maximum and the inverse of its sum over all blocks. */
+__global__ void __launch_bounds__(256) aos_kv_weigh_rows_kernel(aos_kv_weigh_params p, int pieces) {
+  if (refused(p.b, (int)threadIdx.x, 256)) return;
+  const int piece = (int)(blockIdx.x % (uint32_t)pieces), sh = (int)(blockIdx.x / (uint32_t)pieces);
+  const int s = sh / p.b.nkv, h = sh - s * p.b.nkv;
+  const Seq q = seq_at(p.b, s);
+  const int g = p.nh / p.b.nkv, r = piece * 256 + (int)threadIdx.x;
+  if (r >= q.count * g) return;
+  const Span v = {q.len - q.count, p.window};
+  const int t = r / g, hi = v.hi(t), lo = v.lo(t);
+  const long long total = (long long)p.b.n_tokens * g, at = (long long)q.row0 * g + r;
+  const float2 *part = (const float2 *)p.part + (long long)h * p.blocks * total + at;
+  float m = NINF, l = 0.0f;
+  if (hi >= 0)
+    for (int k = lo / KB; k <= hi / KB; ++k) {
+      const float2 y = part[(long long)k * total];
+      const float top = fmaxf(m, y.x), ms = safe_max(top);
+      l = l * ex2(m - ms) + y.y * ex2(y.x - ms);
+      m = top;
+    }
+  ((float2 *)p.stat)[h * total + at] = make_float2(safe_max(m), inverse(l, m));
+}
+
+/* Grid: blocks of KB positions, key/value heads, sequences: the chunks' weights added in order. */
+__global__ void __launch_bounds__(64) aos_kv_weigh_sum_kernel(aos_kv_weigh_params p) {
+  if (refused(p.b, (int)threadIdx.x, 64)) return;
+  const int blk = (int)(blockIdx.x % (uint32_t)p.blocks), sh = (int)(blockIdx.x / (uint32_t)p.blocks);
+  const int s = sh / p.b.nkv, h = sh - s * p.b.nkv;
+  const Seq q = seq_at(p.b, s);
+  const int g = p.nh / p.b.nkv, k0 = blk * KB, k1 = k0 + KB < q.len ? k0 + KB : q.len, pos = k0 + 4 * (int)threadIdx.x;
+  if (pos >= q.len) return;
+  float x[4] = {};
+  if (q.count) {
+    const Span v = {q.len - q.count, p.window};
+    const Rows vis = rows_of(q, v, g, k0, k1);
+    const float *in = p.scores + (long long)sh * p.chunks * p.lpad + pos;
+    for (int c = vis.ra / RC; c * RC < vis.rb; ++c) {
+      const f32x4 y = *(const f32x4 *)(in + (long long)c * p.lpad);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = x[i] + y[i];
+    }
+  }
+  store4(p, s, h, pos, q.len, x);
+}
+
+template <int FMT, int HDP>
+int launch_many(const aos_kv_weigh_params *p, const aos_launch_ctx *ctx) {
+  const uint32_t sh = (uint32_t)p->b.n_seqs * (uint32_t)p->b.nkv;
+  const uint32_t wgs = sh * (uint32_t)p->blocks * (uint32_t)p->chunks;
+  const int pieces = (p->rows + 255) / 256;
+  hipError_t e;
+  AOS_LAUNCH(ctx, (aos_kv_weigh_kernel<FMT, HDP, false>), dim3(wgs), dim3(256), 0, *p);
+  if ((e = hipGetLastError()) != hipSuccess) return (int)e;
+  AOS_LAUNCH(ctx, aos_kv_weigh_rows_kernel, dim3(sh * (uint32_t)pieces), dim3(256), 0, *p, pieces);
+  if ((e = hipGetLastError()) != hipSuccess) return (int)e;
+  AOS_LAUNCH(ctx, (aos_kv_weigh_kernel<FMT, HDP, true>), dim3(wgs), dim3(256), 0, *p);
+  if ((e = hipGetLastError()) != hipSuccess) return (int)e;
+  AOS_LAUNCH(ctx, aos_kv_weigh_sum_kernel, dim3(sh * (uint32_t)p->blocks), dim3(64), 0, *p);
+  return (int)hipGetLastError();
+}
+
+template <int FMT, int HDP>
+int weigh(const aos_kv_weigh_params *p, const aos_launch_ctx *ctx) {
+  return p->few ? launch_few<FMT, HDP>(p, ctx) : launch_many<FMT, HDP>(p, ctx);
+}
+
+}  // namespace
+
+/* The shape of a batch's launches and the workspace they need (which grows with each of the batch's sizes). */
+extern "C" int aos_kv_weigh_shape(aos_kv_weigh_params *p, size_t *bytes) {
+  const aos_kv_batch &b = p->b;
+  const long long g = p->nh / b.nkv, rows = b.max_new * g, sh = (long long)b.n_seqs * b.nkv;
+  const long long blocks = b.max_len > 0 ? ((long long)b.max_len + KB - 1) / KB : 1;
+  if (rows > (1ll << 30) || sh > 0x7fffffff) return 0;
+  p->rows = (int)rows;
+  p->blocks = (int)blocks;
+  p->lpad = p->blocks * KB;
+  /* few rows: pieces of one block where there are few, of up to eight, so that the sums of pieces stay few */
+  long long span = sh * blocks / 2048;
+  span = span < 1 ? 1 : span > 8 ? 8 : span;
+  p->tiles = (int)span * (KB / TILE);
+  p->pieces = (int)((blocks + span - 1) / span);
+  p->chunks = (int)((rows + RC - 1) / RC);
+  const double kept = (double)sh * rows * (4.0 * p->lpad + 8.0 * blocks);
+  p->few = rows <= FEW && kept <= AOS_KV_WEIGH_KEEP && !p->no_few;
+  double need = kept, wgs = (double)sh * blocks;
+  if (!p->few) {
+    need = 8.0 * b.n_tokens * p->nh * (blocks + 1) + 4.0 * sh * p->chunks * p->lpad;
+    const double pieces = (double)((rows + 255) / 256), work = (double)blocks * p->chunks;
+    wgs = sh * (pieces > work ? pieces : work);
+  }
+  if (need > AOS_KV_WEIGH_MOST || wgs > 2e9) return 0;
+  *bytes = (size_t)need;
+  return 1;
+}
+
+/* What every batch within these sizes needs, whichever way it goes; 0 where this batch cannot be counted. */
+extern "C" size_t aos_kv_weigh_most(const aos_kv_weigh_params *p) {
+  aos_kv_weigh_params a = *p;
+  a.no_few = 1;
+  size_t many = 0, few = 0;
+  if (!aos_kv_weigh_shape(&a, &many)) return 0;
+  a.no_few = 0;
+  if (a.b.max_new * (a.nh / a.b.nkv) > FEW) a.b.max_new = FEW / (a.nh / a.b.nkv);
+  if (a.b.max_new > 0 && aos_kv_weigh_shape(&a, &few) && !a.few) few = (size_t)AOS_KV_WEIGH_KEEP;
+  return many > few ? many : few;
+}
+
+/* the parts of a workspace of that many bytes */
+extern "C" void aos_kv_weigh_parts(aos_kv_weigh_params *p, void *ws) {
+  const size_t sh = (size_t)p->b.n_seqs * p->b.nkv, total = (size_t)p->b.n_tokens * p->nh;
+  p->scores = (float *)ws;
+  p->part = p->scores + sh * (size_t)(p->few ? p->rows : p->chunks) * (size_t)p->lpad;
+  p->stat = p->few ? nullptr : p->part + 2 * total * (size_t)p->blocks;
+}
+
+#define KV_DISPATCH(fn, fmt, hdp, ...)                                       \
+  ((hdp) == 64 ? ((fmt) == AOS_KV_BF16    ? fn<AOS_KV_BF16, 64>(__VA_ARGS__)    \
+                  : (fmt) == AOS_KV_MXFP8 ? fn<AOS_KV_MXFP8, 64>(__VA_ARGS__)   \
+                                          : fn<AOS_KV_MXFP4, 64>(__VA_ARGS__))  \
+   : (hdp) == 128 ? ((fmt) == AOS_KV_BF16    ? fn<AOS_KV_BF16, 128>(__VA_ARGS__)   \
+                     : (fmt) == AOS_KV_MXFP8 ? fn<AOS_KV_MXFP8, 128>(__VA_ARGS__)  \
+                                             : fn<AOS_KV_MXFP4, 128>(__VA_ARGS__)) \
+                  : ((fmt) == AOS_KV_BF16    ? fn<AOS_KV_BF16, 256>(__VA_ARGS__)   \
+                     : (fmt) == AOS_KV_MXFP8 ? fn<AOS_KV_MXFP8, 256>(__VA_ARGS__)  \
+                                             : fn<AOS_KV_MXFP4, 256>(__VA_ARGS__)))
+
+extern "C" int aos_launch_kv_weigh(const aos_kv_weigh_params *p, const aos_launch_ctx *ctx) {
+  return KV_DISPATCH(weigh, p->b.format, p->b.hdp, p, ctx);
+}

@@ -444,6 +444,13 @@ void aoship_kv_cache_free(aoship_kv_cache_t *cache);
  * Returns 0 / -1. */
 int aoship_kv_cache_set_rope(aoship_kv_cache_t *cache, const float *cosines, const float *sines, int positions);
 
+/* Rotary positions on several axes (time, height and width of images and video): axes[i] (host, copied, [head_dim / 2]) is the
+ * axis, 0 .. n_axes - 1, whose position turns pair i of a row in aoship_kv_append_at; NULL: all of them axis 0, as at first
+ * (n_axes is then 1). Synchronises the device; graphs captured before hold the old axes, which are gone. A call that fails
+ * leaves the axes that were set. Returns 0 / -1. */
+#define AOSHIP_KV_MAX_AXES 4
+int aoship_kv_cache_set_rope_axes(aoship_kv_cache_t *cache, const uint8_t *axes, int n_axes);
+
 /* Stream (hipStream_t) for this cache's launches; NULL = null stream. Returns 0 / -1. */
 int aoship_kv_cache_set_stream(aoship_kv_cache_t *cache, void *stream);
 
@@ -451,9 +458,11 @@ int aoship_kv_cache_set_stream(aoship_kv_cache_t *cache, void *stream);
  * a combination of the bits below, 0 for nothing, -1 on error. Synchronises the device. Such a sequence is left
  * out whole, its rows of the outputs left as they are (BATCH: starts that fall or pass n_tokens, more new rows than
  * max_new, a length outside 0..max_len; where starts does not ascend, others may be left out with it), or the positions
- * of such a page are (PAGE): not written, read as zeros, not attended to. */
+ * of such a page are (PAGE): not written, read as zeros, not attended to. A rotary position outside the tables counts as 0
+ * (POSITION). */
 #define AOSHIP_KV_FAULT_BATCH 1
 #define AOSHIP_KV_FAULT_PAGE 2
+#define AOSHIP_KV_FAULT_POSITION 4
 int aoship_kv_cache_faults(aoship_kv_cache_t *cache);
 
 /* The sequences of a call. Sequence s has the rows starts[s] .. starts[s + 1] - 1 of the call's row arrays as its new
@@ -494,6 +503,14 @@ typedef struct {
  * keys and values in the cache's format to the pages of `layer`. Asynchronous. Returns 0 / -1. */
 int aoship_kv_append(aoship_kv_cache_t *cache, int layer, const aoship_kv_batch_t *batch, const aoship_kv_rows_t *rows);
 
+/* aoship_kv_append with rotary positions of the rows' own: pair i of row t is turned by entry i of the tables' row
+ * positions[axis of i][t] (device int32 [n_axes][axis_stride]; axis_stride at least n_tokens, or 0 where all axes have the same
+ * positions), whatever the row's place in its sequence: images and video on several axes, and sequences that aoship_kv_evict has shortened, whose next token is at its
+ * place in the text and not in the cache. Needs rotary tables; rows->rotated must be 0. Keys in the cache are turned as they
+ * are written: attention, whose mask goes by places in the cache, needs no positions. Asynchronous. Returns 0 / -1. */
+int aoship_kv_append_at(aoship_kv_cache_t *cache, int layer, const aoship_kv_batch_t *batch, const aoship_kv_rows_t *rows,
+                        const int32_t *positions, int64_t axis_stride);
+
 /* The rows that an append of the same batch wrote, as the bfloat16 values that the cache holds for them (a batch
  * whose sequences' rows are all their positions reads them whole): k, v: device rows like those of append.
  * Asynchronous. Returns 0 / -1. */
@@ -516,6 +533,63 @@ int aoship_kv_read(aoship_kv_cache_t *cache, int layer, const aoship_kv_batch_t 
 int aoship_kv_attention(aoship_kv_cache_t *cache, int layer, const aoship_kv_batch_t *batch, const aoship_bf16_t *q,
                         int64_t q_stride, int num_heads, float scale, int window, aoship_bf16_t *out,
                         int64_t out_stride);
+
+/* ---- eviction from the paged cache: what attention looks at stays ------------------------------ */
+
+/* Weights [sequence][key/value head][position] of a batch (device float32; strides in elements: a head's positions side by
+ * side, max_len of them, heads and sequences apart). prior may be NULL (zeros) or `out` (with its strides), and must not
+ * overlap it otherwise. */
+typedef struct {
+  const float *prior;
+  int64_t prior_seq_stride, prior_head_stride;
+  float *out;
+  int64_t out_seq_stride, out_head_stride;
+} aoship_kv_weights_t;
+
+/* The attention weight of each position of the batch's sequences: out = prior + sum of the probabilities that the new rows
+ * (appended before), and the query heads of the position's key/value head, give it; the probabilities are those of
+ * aoship_kv_attention with the same q, scale and window. Every position below a sequence's length gets its weight (prior
+ * where no row sees it, or its page is not the cache's), others are left as they are. For the weights of a prompt's last
+ * rows only, give a batch of these rows. Everything is float32, in an order that follows from the batch: the same call
+ * gives the same bits. A batch without rows (n_tokens or max_new 0) is nothing to do. A row without probabilities (a
+ * NaN in it, or no score that float32 holds above minus infinity) makes the weights of all
+ * positions that it sees NaN. In a batch whose starts fall nothing may be written.
+ * Uses a workspace of the cache's, which calls of one cache share and a call grows if it must: that synchronises the
+ * device, and is refused while the cache's stream is captured. Asynchronous otherwise. Returns 0 / -1. */
+int aoship_kv_weigh(aoship_kv_cache_t *cache, int layer, const aoship_kv_batch_t *batch, const aoship_bf16_t *q,
+                    int64_t q_stride, int num_heads, float scale, int window, const aoship_kv_weights_t *weights);
+
+/* Sizes the workspace for batches of up to these sizes, so that calls allocate nothing (a captured call's graph holds the
+ * workspace of its time: reserve the largest before). Bytes, with H heads and 256-position blocks of max_len: 4 for a row
+ * of a sequence with up to 32 rows (new tokens times heads of a group), a head and a position, 1 GB at most; beyond that 8
+ * for a row, a head and a block. Returns 0 / -1. */
+int aoship_kv_weigh_reserve(aoship_kv_cache_t *cache, int num_heads, int n_seqs, int n_tokens, int max_new, int max_len);
+
+/* Arguments of aoship_kv_evict (device arrays). A sequence of L positions keeps n = min(keep, L) of them. */
+typedef struct {
+  const float *weights; /* [sequence][key/value head][position], as of aoship_kv_weigh */
+  int64_t weights_seq_stride, weights_head_stride;
+  const int32_t *keep;     /* [n_seqs] positions that each sequence keeps (L or more: all of them) */
+  int max_keep;            /* no sequence keeps more (a bound, like max_len) */
+  int first, recent;       /* its first and last positions stay whatever their weights: first + recent <= keep */
+  const int32_t *to_pages; /* [n_seqs][to_page_stride] pages that the kept positions are moved to */
+  int to_page_stride;      /* at least max_keep / page_size, rounded up */
+  int32_t *kept;           /* [sequence][key/value head][n] out: the kept positions, ascending (max_keep side by side) */
+  int64_t kept_seq_stride, kept_head_stride;
+  float *weights_out; /* NULL, or out: the kept positions' weights, then zeros up to L (max_len side by side); not weights */
+  int64_t weights_out_seq_stride, weights_out_head_stride;
+} aoship_kv_evict_t;
+
+/* Of each sequence (lens and pages of the batch; its starts, n_tokens and max_new are not used) and each key/value head of
+ * `layer`, moves the first and the last positions and those of greatest weight between to the first n positions of to_pages,
+ * in their order: of equal weights the lower positions stay, a NaN counts as the least. Keys and values move as they are
+ * held (nothing is rounded again). Each head may keep other positions; all keep n, so that the sequence is one of
+ * n positions in its new pages, its next row appended at place n with aoship_kv_append_at. Pages of to_pages must not be among
+ * the batch's pages (which keep what they hold, so that others may go on reading them) nor twice in to_pages; what they
+ * hold past n is unspecified. A sequence whose length, keep or first + recent does not fit is left out (BATCH), positions of
+ * a page outside the cache move as zeros, and to such a page not at all (PAGE). Run it for each layer, then give the old
+ * pages back. Asynchronous. Returns 0 / -1. */
+int aoship_kv_evict(aoship_kv_cache_t *cache, int layer, const aoship_kv_batch_t *batch, const aoship_kv_evict_t *args);
 
 /* ---- Liquid blend (crates/adapteros-lora-kernel-api/src/liquid.rs) ------------------------ */
 
