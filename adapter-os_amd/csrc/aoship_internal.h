@@ -705,7 +705,6 @@ typedef struct {
 /* Attention weights of cached positions (aoship_kv_weigh.hip). */
 #define AOS_KV_WEIGH_FEW 32
 #define AOS_KV_WEIGH_BLOCK 256
-#define AOS_KV_WEIGH_ROWS 1024
 #define AOS_KV_WEIGH_KEEP 1.0e9  /* bytes of kept scores at most: beyond, the keys are read twice instead */
 #define AOS_KV_WEIGH_MOST 6.4e10 /* bytes of workspace at most */
 typedef struct {
@@ -719,7 +718,8 @@ typedef struct {
   float *w;           /* [sequence][head][position]; may be prior */
   long long prior_seq, prior_head, w_seq, w_head;
   /* aos_kv_weigh_shape: */
-  int few, rows, blocks, lpad, tiles, pieces, chunks;
+  int few, rows, blocks, lpad, tiles, pieces, chunks, rc /* rows of a chunk */;
+  uint32_t g_mul, g_shift; /* of the division by the heads of a group */
   /* aos_kv_weigh_parts: */
   float *scores; /* few: [sequence][head][rows][lpad]; else the chunks' weights [sequence][head][chunks][lpad] */
   float *part;   /* maxima and sums: few: [sequence][head][pieces][rows][2]; else [head][blocks][all rows][2] */

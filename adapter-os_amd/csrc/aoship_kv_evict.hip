@@ -20,8 +20,8 @@ using namespace kv;
 namespace {
 
 constexpr int NT = 1024, NW = NT / 64;
-constexpr int PER = 32; /* weights of a thread at once */
-constexpr int SPAN = NT * PER;
+constexpr int MOST = 32;     /* weights of a thread at once, at most */
+constexpr int LIST = 4 * NT; /* weights that are listed */
 
 /* what stays of a sequence: n positions; n < 0: left out (a fault, noted) */
 struct Kept {
@@ -57,11 +57,14 @@ __device__ __forceinline__ int lane_scan(int x, int lane) {
   return x;
 }
 
-/* Grid: sequences times key/value heads. Thread t has the positions t, t + 1024, ... of a span of 32768. */
+/* Grid: sequences times key/value heads. Thread t has the positions t, t + 1024, ... of a span of PER * 1024. */
+template <int PER>
 __global__ void __launch_bounds__(NT) aos_kv_select_kernel(aos_kv_evict_params p) {
-  __shared__ int count[2][NW];
+  constexpr int SPAN = NT * PER;
+  __shared__ int total[3][3]; /* counts of three bounds, of this turn, the next and the last */
   __shared__ int above[PER * NW], ties[PER * NW]; /* of a wave's 64 positions: kept for sure, and of the bound's weight */
-  __shared__ int totals[2];
+  __shared__ int totals[2], listed;
+  __shared__ uint32_t list[LIST];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int s = (int)blockIdx.x / p.b.nkv, h = (int)blockIdx.x - s * p.b.nkv;
   const Kept k = kept_of(p, s);
@@ -81,39 +84,92 @@ __global__ void __launch_bounds__(NT) aos_kv_select_kernel(aos_kv_evict_params p
 
   /* x: a weight's order plus one, 0 for positions that are not to be chosen from (n < len <= 2^30, and the order of
    * the greatest float stays below 2^32 - 1) */
+  /* (loads without a condition, all on their way together) */
+  auto weight = [&](int pos) { /* (32-bit offsets: 2^30 positions at most) */
+    return *(const float *)((const char *)w + (uint32_t)(pos < k.len ? pos : k.len - 1) * 4u);
+  };
   auto load = [&](uint32_t (&x)[PER], int base) {
+    float v[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) v[i] = weight(base + i * NT + tid);
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int pos = base + i * NT + tid;
-      x[i] = pos >= lo && pos < hi ? order_of(w[pos]) + 1u : 0u;
+      x[i] = pos >= lo && pos < hi ? order_of(v[i]) + 1u : 0u;
     }
   };
   const bool once = k.len <= SPAN;
   uint32_t x[PER];
   if (once) load(x, 0);
-  /* the greatest bound that at least m reach; with exactly m there are no ties to part */
+  auto count_of = [&](auto &&counts) { /* adds up counts(i) of all rows and spans, a row's by its wave */
+    for (int base = 0; base < k.len; base += SPAN) {
+      if (!once) load(x, base);
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        counts(x[i]);
+      }
+    }
+  };
+  /* The greatest bound that at least m reach, two bits a turn; with exactly m there are no ties to part. After eight bits the
+   * weights between the bound and the next one are mostly few: listed, a thread has at most four of them to count. */
   uint32_t bound = 0;
-  int reach = 0; /* how many reach it (where bound > 0) */
+  int reach = hi - lo, over = 0; /* how many reach it, and the next bound that the bits so far can make */
   if (m > 0) {
     int turn = 0;
-    for (int bit = 31; bit >= 0; --bit, turn ^= 1) {
+    if (tid < 3) total[0][tid] = 0;
+    __syncthreads();
+    auto step = [&](int bit, const int (&c)[3], int more) { /* c: this wave's counts; more: what they leave out */
       const uint32_t at = bound | (1u << bit);
-      int c = 0;
-      for (int base = 0; base < k.len; base += SPAN) {
-        if (!once) load(x, base);
-#pragma unroll
-        for (int i = 0; i < PER; ++i) c += (int)__popcll(__ballot(x[i] >= at));
-      }
-      if (lane == 0) count[turn][wave] = c;
+      if (lane < 3) atomicAdd(&total[turn][lane], lane == 0 ? c[0] : lane == 1 ? c[1] : c[2]);
+      const int next = turn == 2 ? 0 : turn + 1;
+      if (tid < 3) total[next][tid] = 0; /* (read last two turns ago) */
       __syncthreads();
-      int all = 0;
+      const int all[3] = {total[turn][0], total[turn][1], total[turn][2]};
+      turn = next;
 #pragma unroll
-      for (int i = 0; i < NW; ++i) all += count[turn][i];
-      if (all >= m) {
-        bound = at;
-        reach = all;
-        if (all == m) break; /* uniform */
+      for (int j = 2; j >= 0; --j) {
+        const int n = __builtin_amdgcn_readfirstlane(all[j]) + more;
+        if (n >= m) {
+          bound = at + ((uint32_t)j << bit);
+          reach = n;
+          break;
+        }
+        over = n;
       }
+    };
+    auto count_of_one = [&](int bit, uint32_t y, int (&c)[3]) {
+#pragma unroll
+      for (int j = 0; j < 3; ++j) c[j] += (int)__popcll(__ballot(y >= (bound | (1u << bit)) + ((uint32_t)j << bit)));
+    };
+    int bit = 30;
+    for (; bit >= 24 && reach != m; bit -= 2) { /* (uniform) */
+      int c[3] = {};
+      count_of([&](uint32_t y) { count_of_one(bit, y, c); });
+      step(bit, c, 0);
+    }
+    if (reach != m && reach - over <= LIST) {
+      if (tid == 0) listed = 0;
+      __syncthreads();
+      count_of([&](uint32_t y) {
+        if (y > 0u && y >> 24 == bound >> 24) list[atomicAdd(&listed, 1)] = y; /* reach - over of them */
+      });
+      __syncthreads();
+      const int n = listed, rest = over;
+      uint32_t y[LIST / NT];
+#pragma unroll
+      for (int j = 0; j < LIST / NT; ++j) y[j] = j * NT + tid < n ? list[j * NT + tid] : 0u;
+      for (; bit >= 0 && reach != m; bit -= 2) {
+        int c[3] = {};
+#pragma unroll
+        for (int j = 0; j < LIST / NT; ++j)
+          if (j * NT < n) count_of_one(bit, y[j], c);
+        step(bit, c, rest);
+      }
+    }
+    for (; bit >= 0 && reach != m; bit -= 2) {
+      int c[3] = {};
+      count_of([&](uint32_t y) { count_of_one(bit, y, c); });
+      step(bit, c, 0);
     }
   } else {
     bound = 0xffffffffu; /* (no weight's) */
@@ -123,17 +179,13 @@ __global__ void __launch_bounds__(NT) aos_kv_select_kernel(aos_kv_evict_params p
   if (!exact) {
     /* m less those above the bound */
     int c = 0;
-    for (int base = 0; base < k.len; base += SPAN) {
-      if (!once) load(x, base);
-#pragma unroll
-      for (int i = 0; i < PER; ++i) c += (int)__popcll(__ballot(x[i] > bound));
-    }
+    count_of([&](uint32_t y) { c += (int)__popcll(__ballot(y > bound)); });
     __syncthreads();
-    if (lane == 0) count[0][wave] = c;
+    if (tid == 0) total[0][0] = 0;
     __syncthreads();
-    left = m;
-#pragma unroll
-    for (int i = 0; i < NW; ++i) left -= count[0][i];
+    if (lane == 0) atomicAdd(&total[0][0], c);
+    __syncthreads();
+    left = m - total[0][0];
   }
 
   for (int base = 0; base < k.len; base += SPAN) {
@@ -153,19 +205,20 @@ __global__ void __launch_bounds__(NT) aos_kv_select_kernel(aos_kv_evict_params p
     }
     __syncthreads();
     if (wave == 0) {
-      /* PER * NW groups of 64 positions in order, 8 a lane: ties before each, then places before each */
-      int t[PER * NW / 64], sum = 0;
+      /* PER * NW groups of 64 positions in order, EACH a lane: ties before each, then places before each */
+      constexpr int EACH = PER * NW / 64;
+      int t[EACH], sum = 0;
 #pragma unroll
-      for (int i = 0; i < PER * NW / 64; ++i) {
-        t[i] = ties[lane * (PER * NW / 64) + i];
+      for (int i = 0; i < EACH; ++i) {
+        t[i] = ties[lane * EACH + i];
         sum += t[i];
       }
       int before = lane_scan(sum, lane) - sum, places = 0;
       const int all_ties = __builtin_amdgcn_readlane(before + sum, 63);
-      int a[PER * NW / 64];
+      int a[EACH];
 #pragma unroll
-      for (int i = 0; i < PER * NW / 64; ++i) {
-        const int at = lane * (PER * NW / 64) + i, room = left - before;
+      for (int i = 0; i < EACH; ++i) {
+        const int at = lane * EACH + i, room = left - before;
         a[i] = above[at] + (room < 0 ? 0 : room < t[i] ? room : t[i]);
         ties[at] = before;
         before += t[i];
@@ -177,24 +230,31 @@ __global__ void __launch_bounds__(NT) aos_kv_select_kernel(aos_kv_evict_params p
         totals[1] = all_ties;
       }
 #pragma unroll
-      for (int i = 0; i < PER * NW / 64; ++i) {
-        above[lane * (PER * NW / 64) + i] = place;
+      for (int i = 0; i < EACH; ++i) {
+        above[lane * EACH + i] = place;
         place += a[i];
       }
     }
     __syncthreads();
     const uint64_t below = (1ull << lane) - 1ull;
+    constexpr int FLY = PER < 8 ? PER : 8;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const bool y = sure(i), t = tie(i);
-      const uint64_t ys = __ballot(y), ts = __ballot(t);
-      const int room = left - ties[i * NW + wave], mine = (int)__popcll(ts & below);
-      const int at = taken + above[i * NW + wave] + (int)__popcll(ys & below) + (mine < room ? mine : room > 0 ? room : 0);
-      if (y || (t && mine < room)) {
-        const int pos = base + i * NT + tid;
-        kept[at] = pos;
-        if (wo) wo[at] = w[pos];
+    for (int i0 = 0; i0 < PER; i0 += FLY) {
+      float v[FLY];
+#pragma unroll
+      for (int i = 0; i < FLY; ++i) v[i] = weight(base + (i0 + i) * NT + tid);
+#pragma unroll
+      for (int i = 0; i < FLY; ++i) {
+        const bool y = sure(i0 + i), t = tie(i0 + i);
+        const uint64_t ys = __ballot(y), ts = __ballot(t);
+        const int group = (i0 + i) * NW + wave, room = left - ties[group], mine = (int)__popcll(ts & below);
+        const uint32_t at = (uint32_t)(taken + above[group] + (int)__popcll(ys & below) + (mine < room ? mine : room > 0 ? room : 0));
+        if (y || (t && mine < room)) {
+          *(int32_t *)((char *)kept + at * 4u) = base + (i0 + i) * NT + tid;
+          if (wo) *(float *)((char *)wo + at * 4u) = v[i];
+        }
       }
+      aos_compiler_barrier(); /* (no more of them in registers at once) */
     }
     __syncthreads();
     taken += totals[0];
@@ -292,7 +352,14 @@ __global__ void __launch_bounds__(256) aos_kv_move_kernel(aos_kv_evict_params p,
 template <int FMT, int HDP>
 int evict(const aos_kv_evict_params *p, const aos_launch_ctx *ctx) {
   const uint32_t sh = (uint32_t)p->b.n_seqs * (uint32_t)p->b.nkv;
-  AOS_LAUNCH(ctx, aos_kv_select_kernel, dim3(sh), dim3(NT), 0, *p);
+  /* registers for the longest sequence */
+  const int len = p->b.max_len;
+  if (len <= 4 * NT)
+    AOS_LAUNCH(ctx, aos_kv_select_kernel<4>, dim3(sh), dim3(NT), 0, *p);
+  else if (len <= 16 * NT)
+    AOS_LAUNCH(ctx, aos_kv_select_kernel<16>, dim3(sh), dim3(NT), 0, *p);
+  else
+    AOS_LAUNCH(ctx, aos_kv_select_kernel<MOST>, dim3(sh), dim3(NT), 0, *p);
   const hipError_t e = hipGetLastError();
   const int tiles = (p->max_keep + TILE - 1) / TILE;
   if (e != hipSuccess || tiles == 0) return (int)e;

@@ -22,7 +22,6 @@ namespace {
 
 constexpr int FEW = AOS_KV_WEIGH_FEW;      /* rows of a sequence whose scores are kept */
 constexpr int KB = AOS_KV_WEIGH_BLOCK;     /* positions of a workgroup: a tile of 64 a wave */
-constexpr int RC = AOS_KV_WEIGH_ROWS;      /* rows of a workgroup where there are many */
 constexpr int RT = 64;                     /* rows of a stage */
 
 /* A tile's keys of 32 positions a block, as the matrix instructions take them: lane l has the quarter of position
@@ -68,6 +67,12 @@ __device__ __forceinline__ float score_factor(float scale) { /* (a scale of zero
   return fmaxf(fabsf(scale) * LOG2E, 1.17549435e-38f);
 }
 
+/* Workgroups go to the XCDs in turn: which part of a sequence each has turns with the sequence (or chunk), so that no XCD
+ * has the parts that short sequences, or rows before them, do not reach. */
+__device__ __forceinline__ int turned(int i, int by, int n) {
+  return (int)(((uint32_t)i + (uint32_t)by) % (uint32_t)n);
+}
+
 /* ---- few rows -------------------------------------------------------------------------------- */
 
 /* Grid: pieces of `tiles` position tiles, key/value heads, sequences. S^T = K . Q^T by v_mfma_f32_32x32x16_bf16: row
@@ -79,7 +84,8 @@ __global__ void __launch_bounds__(256, 2) aos_kv_scores_kernel(aos_kv_weigh_para
   __shared__ float ml[4][2][32];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 31, half = lane >> 5;
-  const int piece = (int)(blockIdx.x % (uint32_t)p.pieces), sh = (int)(blockIdx.x / (uint32_t)p.pieces);
+  const int sh = (int)(blockIdx.x / (uint32_t)p.pieces);
+  const int piece = turned((int)(blockIdx.x - (uint32_t)sh * (uint32_t)p.pieces), sh, p.pieces);
   const int s = sh / p.b.nkv, h = sh - s * p.b.nkv;
   const Seq q = seq_at(p.b, s);
   const int g = p.nh / p.b.nkv, rows = q.count * g;
@@ -158,7 +164,7 @@ __global__ void __launch_bounds__(256, 2) aos_kv_scores_kernel(aos_kv_weigh_para
     const float ms = safe_max(top);
 #pragma unroll
     for (int w = 0; w < 4; ++w) sum = sum + ml[w][1][tid] * ex2(ml[w][0][tid] - ms);
-    float *part = p.part + ((long long)blockIdx.x * p.rows + tid) * 2;
+    float *part = p.part + (((long long)sh * p.pieces + piece) * p.rows + tid) * 2;
     part[0] = top;
     part[1] = sum;
   }
@@ -184,18 +190,24 @@ __global__ void __launch_bounds__(256) aos_kv_weights_kernel(aos_kv_weigh_params
   const int rows = q.count * (p.nh / p.b.nkv), pos = blk * WB + 4 * tid;
   if (blk * WB >= q.len) return;
   const Span v = {q.len - q.count, p.window};
+  bool odd = false;                            /* some row has no distribution */
   const int first = rows ? v.lo(0) / TILE : 0; /* the scores of earlier tiles were not formed */
   if (rows) {
     /* the rows' maxima and sums over the pieces, eight threads a row */
     const int c0 = first / p.tiles, c1 = ((q.len - 1) / TILE) / p.tiles, r = tid % FEW, k = tid / FEW;
-    const float *part = p.part + ((long long)sh * p.pieces * p.rows + r) * 2;
+    const float2 *part = (const float2 *)p.part + (long long)sh * p.pieces * p.rows + r;
     float m = NINF, l = 0.0f;
     if (r < rows)
-      for (int c = c0 + k; c <= c1; c += 8) {
-        const float pm = part[(long long)c * p.rows * 2], pl = part[(long long)c * p.rows * 2 + 1];
-        const float top = fmaxf(m, pm), ms = safe_max(top);
-        l = l * ex2(m - ms) + pl * ex2(pm - ms);
-        m = top;
+      for (int c = c0 + k; c <= c1; c += 32) { /* (four on their way together) */
+        float2 y[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i] = c + 8 * i <= c1 ? part[(long long)(c + 8 * i) * p.rows] : make_float2(NINF, 0.0f);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float top = fmaxf(m, y[i].x), ms = safe_max(top);
+          l = l * ex2(m - ms) + y[i].y * ex2(y[i].x - ms);
+          m = top;
+        }
       }
     red[k][0][r] = m;
     red[k][1][r] = l;
@@ -210,20 +222,23 @@ __global__ void __launch_bounds__(256) aos_kv_weights_kernel(aos_kv_weigh_params
       base[tid] = ms;
       inv[tid] = inverse(sum, top);
     }
-    __syncthreads();
+    odd = __syncthreads_or(tid < FEW && inv[tid] != inv[tid]) != 0;
   }
   if (pos >= q.len) return;
   float x[4] = {};
   if (rows && pos + 3 >= first * TILE) {
     const float cs = score_factor(p.scale);
     const float *sc = p.scores + (long long)sh * p.rows * p.lpad + pos;
-    for (int r = 0; r < rows; ++r) {
-      const f32x4 y = *(const f32x4 *)(sc + (long long)r * p.lpad);
+    for (int r0 = 0; r0 < rows; r0 += 8) { /* (eight on their way together) */
+      f32x4 y[8];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = fmaf(ex2(fmaf(y[i], cs, -base[r])), inv[r], x[i]);
+      for (int k = 0; k < 8; ++k)
+        y[k] = r0 + k < rows ? *(const f32x4 *)(sc + (long long)(r0 + k) * p.lpad) : f32x4{NINF, NINF, NINF, NINF};
+#pragma unroll
+      for (int k = 0; k < 8; ++k) /* (rows past the last have factors of zero) */
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = fmaf(ex2(fmaf(y[k][i], cs, -base[r0 + k])), inv[r0 + k], x[i]);
     }
-    bool odd = false;
-    for (int r = 0; r < rows; ++r) odd |= inv[r] != inv[r];
     if (odd) { /* rows without a distribution: what they do not see has no part of them */
       const bool there = page_of(p.b, s, pos) >= 0;
 #pragma unroll
@@ -266,8 +281,8 @@ __device__ __forceinline__ Rows rows_of(const Seq &q, const Span &v, int g, int 
 }
 
 /* Whether the batch's starts fall somewhere (noted): its sequences' rows may then be the same, and none of them is served. */
-__device__ __forceinline__ bool refused(const aos_kv_batch &b, int tid, int n) {
-  if (!__syncthreads_or(starts_fall(b, tid, n) ? 1 : 0)) return false;
+__device__ __forceinline__ bool refused(const aos_kv_batch &b, bool fall, int tid) {
+  if (!__syncthreads_or(fall ? 1 : 0)) return false;
   if (tid == 0) note(b.faults, AOS_KV_FAULT_BATCH);
   return true;
 }
@@ -282,23 +297,21 @@ struct Stage {
   float m[RT], f[RT];
 };
 
-/* A workgroup has the keys of KB positions in registers, a tile a wave, and the rows of one chunk (RC of them) that see
+/* A workgroup has the keys of KB positions in registers, a tile a wave, and the rows of one chunk (p.rc of them) that see
  * some of them go by in stages of 64 through LDS.
  *   SUM false: each row's maximum and sum over the block's positions, to part[head][block][row].
  *   SUM true: the weights of the block's positions from the chunk's rows, to scores[sequence][head][chunk][position].
  * Grid: blocks, chunks, key/value heads, sequences. */
 template <int FMT, int HDP, bool SUM>
-__global__ void __launch_bounds__(256, HDP == 256 ? 1 : 2) aos_kv_weigh_kernel(aos_kv_weigh_params p) {
+__global__ void __launch_bounds__(256, HDP == 256 ? 1 : 3) aos_kv_weigh_kernel(aos_kv_weigh_params p) {
   constexpr int KS = HDP / 16, N = Stage<HDP>::N, LD = Stage<HDP>::LD, UNITS = Stage<HDP>::UNITS;
   __shared__ __attribute__((aligned(16))) Stage<HDP> st[2];
   __shared__ float red[SUM ? 1 : 2][4][2][SUM ? 1 : RT];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 31, half = lane >> 5;
-  if (refused(p.b, tid, 256)) return;
-  int x = (int)blockIdx.x;
-  const int blk = x % p.blocks;
-  x /= p.blocks;
-  const int chunk = x % p.chunks;
+  int x = (int)(blockIdx.x / (uint32_t)p.blocks);
+  const int b0 = (int)(blockIdx.x - (uint32_t)x * (uint32_t)p.blocks), chunk = x % p.chunks;
+  const int blk = turned(b0, x, p.blocks);
   x /= p.chunks;
   const int s = x / p.b.nkv, h = x - s * p.b.nkv;
   const Seq q = seq_at(p.b, s);
@@ -306,26 +319,17 @@ __global__ void __launch_bounds__(256, HDP == 256 ? 1 : 2) aos_kv_weigh_kernel(a
   if (q.count == 0 || k0 >= q.len) return;
   const Span v = {q.len - q.count, p.window};
   const Rows vis = rows_of(q, v, g, k0, k1);
-  const int ra = vis.ra > chunk * RC ? vis.ra / RT * RT : chunk * RC;
-  const int rb = vis.rb < (chunk + 1) * RC ? vis.rb : (chunk + 1) * RC;
+  const int ra = vis.ra > chunk * p.rc ? vis.ra / RT * RT : chunk * p.rc;
+  const int rb = vis.rb < (chunk + 1) * p.rc ? vis.rb : (chunk + 1) * p.rc;
   if (ra >= rb) return;
 
-  /* this wave's keys */
-  const int tb = k0 + TILE * wave;
+  const int tb = k0 + TILE * wave; /* this wave's keys */
   const int page = tb < q.len ? page_of(p.b, s, tb) : -1;
-  u32x4 kf[2][KS];
-  {
-    Keys<FMT, HDP> k;
-    k.load(tile_ptr<FMT, HDP>(p.b, page < 0 ? 0 : page, h, tb), col, half);
-#pragma unroll
-    for (int b = 0; b < 2; ++b)
-#pragma unroll
-      for (int e = 0; e < KS; ++e) kf[b][e] = k.operand(b, e);
-  }
   const float cs = score_factor(p.scale);
   const uint32_t flip = p.scale < 0.0f ? 0x80008000u : 0u;
   const long long total = (long long)p.b.n_tokens * g; /* rows of a head */
   const float2 *stat = (const float2 *)p.stat + h * total + (long long)q.row0 * g;
+  auto token = [&](int r) { return (int)(((uint64_t)(uint32_t)r * p.g_mul) >> p.g_shift); }; /* r / g */
 
   /* a thread's pieces of a stage: rows tid / UNITS + i * 256 / UNITS, unit tid % UNITS */
   constexpr int STEP = 256 / UNITS;
@@ -336,13 +340,13 @@ __global__ void __launch_bounds__(256, HDP == 256 ? 1 : 2) aos_kv_weigh_kernel(a
   auto fetch = [&](int r0) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int r = r0 + row1 + i * STEP, t = r / g, hh = h * g + r - t * g;
+      const int r = r0 + row1 + i * STEP, t = token(r), hh = h * g + r - t * g;
       fq[i] = u32x4{};
       if (r < rb && 8 * unit < p.b.hd) fq[i] = aos_gld16(p.q + (long long)(q.row0 + t) * p.q_ld + hh * p.b.hd + 8 * unit);
     }
     if (tid < RT) {
       const int r = r0 + tid;
-      fh = r < rb ? v.hi(r / g) : -1;
+      fh = r < rb ? v.hi(token(r)) : -1;
       if (SUM && r < rb) fs = stat[r];
     }
   };
@@ -362,22 +366,32 @@ __global__ void __launch_bounds__(256, HDP == 256 ? 1 : 2) aos_kv_weigh_kernel(a
       }
     }
   };
+  fetch(ra); /* (on their way with the keys) */
+  const bool fall = starts_fall(p.b, tid, 256);
+  u32x4 kf[2][KS];
+  {
+    Keys<FMT, HDP> k;
+    k.load(tile_ptr<FMT, HDP>(p.b, page < 0 ? 0 : page, h, tb), col, half);
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int e = 0; e < KS; ++e) kf[b][e] = k.operand(b, e);
+  }
   float acc[2] = {0.0f, 0.0f};
-  fetch(ra);
   put(st[0]);
-  __syncthreads();
+  if (refused(p.b, fall, tid)) return;
   int i = 0;
   for (int r0 = ra; r0 < rb; r0 += RT, ++i) {
     const Stage<HDP> &d = st[i & 1];
     if (r0 + RT < rb) fetch(r0 + RT);
-    /* the stage's rows see up to hi_min .. hi_max, from lo_min .. lo_max on */
-    const int last = r0 + RT < rb ? r0 + RT - 1 : rb - 1;
-    const int ta = r0 / g, tz = last / g;
-    const bool any = page >= 0 && tb <= v.hi(tz) && tb + TILE > v.lo(ta);
-    const bool edge = tb < v.lo(tz) || tb + TILE - 1 > v.hi(ta) || r0 + RT > rb;
 #pragma unroll
     for (int sub = 0; sub < 2; ++sub) {
       float m = NINF, l = 0.0f;
+      /* what the 32 rows see of the tile: something, and whether all of them all of it */
+      const int rs = r0 + 32 * sub, re = rs + 32 < rb ? rs + 32 : rb;
+      const int ta = token(rs), tz = token(re - 1); /* (no rows: not used) */
+      const bool any = page >= 0 && rs < rb && tb <= v.hi(tz) && tb + TILE > v.lo(ta);
+      const bool edge = tb < v.lo(tz) || tb + TILE - 1 > v.hi(ta) || re < rs + 32;
       if (any) { /* uniform */
         f32x16 sc[2] = {f32x16{}, f32x16{}};
 #pragma unroll
@@ -416,19 +430,23 @@ __global__ void __launch_bounds__(256, HDP == 256 ? 1 : 2) aos_kv_weigh_kernel(a
           for (int j4 = 0; j4 < 4; ++j4) {
             const int at = 32 * sub + 8 * j4 + 4 * half; /* rows at .. at + 3 of the stage */
             const f32x4 rm = *(const f32x4 *)(d.m + at), rf = *(const f32x4 *)(d.f + at);
-            const int4 hi = *(const int4 *)(d.hi + at);
-            const int his[4] = {hi.x, hi.y, hi.z, hi.w};
+            if (edge) {
+              const int4 hi = *(const int4 *)(d.hi + at);
+              const int his[4] = {hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
-            for (int b = 0; b < 2; ++b)
+              for (int b = 0; b < 2; ++b)
 #pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                float e = ex2(fmaf(sc[b][4 * j4 + j], cs, -rm[j])) * rf[j];
-                if (edge) {
+                for (int j = 0; j < 4; ++j) {
                   const int pos = tb + 32 * b + col;
-                  e = pos >= v.lo(his[j] - v.p0) && pos <= his[j] ? e : 0.0f;
+                  const float e = fmaf(ex2(fmaf(sc[b][4 * j4 + j], cs, -rm[j])), rf[j], acc[b]);
+                  acc[b] = pos >= v.lo(his[j] - v.p0) && pos <= his[j] ? e : acc[b];
                 }
-                acc[b] = acc[b] + e;
-              }
+            } else {
+#pragma unroll
+              for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[b] = fmaf(ex2(fmaf(sc[b][4 * j4 + j], cs, -rm[j])), rf[j], acc[b]);
+            }
           }
         }
       }
@@ -466,7 +484,7 @@ __global__ void __launch_bounds__(256, HDP == 256 ? 1 : 2) aos_kv_weigh_kernel(a
 
 /* Grid: pieces of 256 rows, key/value heads, sequences: a row's maximum and the inverse of its sum over all blocks. */
 __global__ void __launch_bounds__(256) aos_kv_weigh_rows_kernel(aos_kv_weigh_params p, int pieces) {
-  if (refused(p.b, (int)threadIdx.x, 256)) return;
+  if (refused(p.b, starts_fall(p.b, (int)threadIdx.x, 256), (int)threadIdx.x)) return;
   const int piece = (int)(blockIdx.x % (uint32_t)pieces), sh = (int)(blockIdx.x / (uint32_t)pieces);
   const int s = sh / p.b.nkv, h = sh - s * p.b.nkv;
   const Seq q = seq_at(p.b, s);
@@ -477,19 +495,24 @@ __global__ void __launch_bounds__(256) aos_kv_weigh_rows_kernel(aos_kv_weigh_par
   const long long total = (long long)p.b.n_tokens * g, at = (long long)q.row0 * g + r;
   const float2 *part = (const float2 *)p.part + (long long)h * p.blocks * total + at;
   float m = NINF, l = 0.0f;
-  if (hi >= 0)
-    for (int k = lo / KB; k <= hi / KB; ++k) {
-      const float2 y = part[(long long)k * total];
-      const float top = fmaxf(m, y.x), ms = safe_max(top);
-      l = l * ex2(m - ms) + y.y * ex2(y.x - ms);
+  const int k1 = hi < 0 ? -1 : hi / KB;
+  for (int k0 = lo / KB; k0 <= k1; k0 += 8) { /* (eight on their way together) */
+    float2 y[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = k0 + i <= k1 ? part[(long long)(k0 + i) * total] : make_float2(NINF, 0.0f);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float top = fmaxf(m, y[i].x), ms = safe_max(top);
+      l = l * ex2(m - ms) + y[i].y * ex2(y[i].x - ms);
       m = top;
     }
+  }
   ((float2 *)p.stat)[h * total + at] = make_float2(safe_max(m), inverse(l, m));
 }
 
 /* Grid: blocks of KB positions, key/value heads, sequences: the chunks' weights added in order. */
 __global__ void __launch_bounds__(64) aos_kv_weigh_sum_kernel(aos_kv_weigh_params p) {
-  if (refused(p.b, (int)threadIdx.x, 64)) return;
+  if (refused(p.b, starts_fall(p.b, (int)threadIdx.x, 64), (int)threadIdx.x)) return;
   const int blk = (int)(blockIdx.x % (uint32_t)p.blocks), sh = (int)(blockIdx.x / (uint32_t)p.blocks);
   const int s = sh / p.b.nkv, h = sh - s * p.b.nkv;
   const Seq q = seq_at(p.b, s);
@@ -500,10 +523,15 @@ __global__ void __launch_bounds__(64) aos_kv_weigh_sum_kernel(aos_kv_weigh_param
     const Span v = {q.len - q.count, p.window};
     const Rows vis = rows_of(q, v, g, k0, k1);
     const float *in = p.scores + (long long)sh * p.chunks * p.lpad + pos;
-    for (int c = vis.ra / RC; c * RC < vis.rb; ++c) {
-      const f32x4 y = *(const f32x4 *)(in + (long long)c * p.lpad);
+    const int c1 = (vis.rb + p.rc - 1) / p.rc;
+    for (int c0 = vis.ra / p.rc; c0 < c1; c0 += 8) {
+      f32x4 y[8];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = x[i] + y[i];
+      for (int j = 0; j < 8; ++j) y[j] = c0 + j < c1 ? *(const f32x4 *)(in + (long long)(c0 + j) * p.lpad) : f32x4{};
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = x[i] + y[j][i];
     }
   }
   store4(p, s, h, pos, q.len, x);
@@ -540,18 +568,31 @@ extern "C" int aos_kv_weigh_shape(aos_kv_weigh_params *p, size_t *bytes) {
   if (rows > (1ll << 30) || sh > 0x7fffffff) return 0;
   p->rows = (int)rows;
   p->blocks = (int)blocks;
+  /* r / g for r < 2^30: r M >> 31 + s with 2^s >= g, M = 2^(31 + s) / g rounded up: off by less than 2^30 g / 2^(31 + s) < 1 / 2
+   * of the least distance to the next whole number */
+  int sh2 = 0;
+  while ((1ll << sh2) < g) ++sh2;
+  p->g_mul = (uint32_t)(((1ull << (31 + sh2)) + (uint64_t)g - 1) / (uint64_t)g);
+  p->g_shift = 31 + sh2;
   p->lpad = p->blocks * KB;
-  /* few rows: pieces of one block where there are few, of up to eight, so that the sums of pieces stay few */
-  long long span = sh * blocks / 2048;
+  /* few rows: pieces of a block where there are few, of up to eight, so that the sums of pieces stay few (64 streams of up
+   * to 16001 positions, 16128 blocks: 181 us in pieces of one, 186 of three, 200 of seven, whose last round is half empty) */
+  long long span = sh * blocks / 8192;
   span = span < 1 ? 1 : span > 8 ? 8 : span;
   p->tiles = (int)span * (KB / TILE);
   p->pieces = (int)((blocks + span - 1) / span);
-  p->chunks = (int)((rows + RC - 1) / RC);
+  /* many rows: chunks of 64 where there are few, of up to 512 (prompt of 4001, 28 heads: 222 us, 234 in chunks of 256, 238 of
+   * 1024, whose second round is half empty) */
+  const double stages = (double)((rows + RT - 1) / RT), units = stages * sh * blocks;
+  const int k = units < 4096 ? 1 : units > 16384 ? 8 : (int)(units / 2048);
+  p->rc = RT * k;
+  p->chunks = (int)((rows + p->rc - 1) / p->rc);
   const double kept = (double)sh * rows * (4.0 * p->lpad + 8.0 * blocks);
   p->few = rows <= FEW && kept <= AOS_KV_WEIGH_KEEP && !p->no_few;
   double need = kept, wgs = (double)sh * blocks;
   if (!p->few) {
-    need = 8.0 * b.n_tokens * p->nh * (blocks + 1) + 4.0 * sh * p->chunks * p->lpad;
+    /* (chunks are at most units / 8 or 4096 of them, and one more for each block) */
+    need = 8.0 * b.n_tokens * p->nh * (blocks + 1) + 4.0 * KB * ((units > 32768 ? units / 8 : 4096) + (double)sh * blocks);
     const double pieces = (double)((rows + 255) / 256), work = (double)blocks * p->chunks;
     wgs = sh * (pieces > work ? pieces : work);
   }
