@@ -753,13 +753,18 @@ def _logprobs_out(what: str, T: int, targets, logprob, entropy, rank, top_ids, t
     """(the outputs' struct, the targets' pointer), checked: device tensors of T rows, contiguous."""
     import torch
 
-    n = next((t.shape[-1] for t in (top_ids, top_logprobs) if t is not None and t.dim() == 2), 0)
-    for t, kind, shape in ((targets, torch.int32, (T,)), (logprob, torch.float32, (T,)), (entropy, torch.float32, (T,)),
-                           (rank, torch.int32, (T,)), (top_ids, torch.int32, (T, n)), (top_logprobs, torch.float32, (T, n))):
-        if t is not None and (t.dtype != kind or tuple(t.shape) != shape or not t.is_contiguous()
-                              or t.get_device() != _initialised):
-            raise AosError(f"{what}: targets and rank [T], logprob and entropy [T], top_ids and top_logprobs [T, n] must be "
-                           "contiguous int32 and float32 tensors on the device")
+    n, one = 0, (T,)
+    if top_ids is not None or top_logprobs is not None:
+        n = (top_logprobs if top_ids is None else top_ids).shape[-1]
+
+    def ok(t, kind, shape):
+        return t is None or t.dtype is kind and t.shape == shape and t.is_contiguous() and t.get_device() == _initialised
+
+    i, f = torch.int32, torch.float32
+    if not (ok(targets, i, one) and ok(logprob, f, one) and ok(entropy, f, one) and ok(rank, i, one)
+            and ok(top_ids, i, (T, n)) and ok(top_logprobs, f, (T, n))):
+        raise AosError(f"{what}: targets and rank [T], logprob and entropy [T], top_ids and top_logprobs [T, n] must be "
+                       "contiguous int32 and float32 tensors on the device")
     return _LogProbsOut(_ptr(logprob), _ptr(rank), _ptr(entropy), _ptr(top_ids), _ptr(top_logprobs), n), _ptr(targets)
 
 
@@ -770,6 +775,9 @@ class LogProbs:
         self.h = lib().aoship_logprobs_new()
         if not self.h:
             raise AosError(f"aoship_logprobs_new: {last_error()}")
+        import torch
+
+        self._dtypes = (torch.float32, torch.bfloat16)
 
     def set_stream(self, stream_ptr) -> None:
         _check(lib().aoship_logprobs_set_stream(self.h, stream_ptr), "aoship_logprobs_set_stream")
@@ -778,16 +786,15 @@ class LogProbs:
                  top_logprobs=None) -> None:
         """logits: device float32 or bfloat16 [T, vocab] (rows may be set apart); targets: device int32 [T]. Outputs, each
         may be None: logprob, entropy float32 [T], rank int32 [T], top_ids int32 and top_logprobs float32 [T, n]."""
-        import torch
-
-        if logits.dim() != 2 or logits.dtype not in (torch.float32, torch.bfloat16) \
-                or logits.get_device() != _initialised or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        shape, stride, kind = logits.shape, logits.stride(), logits.dtype
+        if len(shape) != 2 or kind not in self._dtypes or logits.get_device() != _initialised \
+                or shape[1] > 1 and stride[1] != 1:
             raise AosError("LogProbs: logits must be a float32 or bfloat16 tensor [T, vocab] on the device, the logits of a "
                            "row side by side")
-        T, vocab = logits.shape
+        T, vocab = shape
         out, tp = _logprobs_out("LogProbs", T, targets, logprob, entropy, rank, top_ids, top_logprobs)
-        if _lib.aoship_logprobs(self.h, logits.data_ptr(), logits.dtype is torch.bfloat16, T, vocab,
-                                logits.stride(0) if T > 1 else vocab, tp, C.byref(out)):
+        if _lib.aoship_logprobs(self.h, logits.data_ptr(), kind is self._dtypes[1], T, vocab,
+                                stride[0] if T > 1 else vocab, tp, C.byref(out)):
             raise AosError(f"aoship_logprobs: {last_error()}")
 
     def __del__(self):
@@ -870,6 +877,7 @@ class KVCache:
         import torch
 
         self._rows, self._scale = _KVRows(), head_dim ** -0.5
+        self._weights, self._evict = _KVWeights(), _KVEvict()
         self._dtypes, self._f32, self._i32 = (torch.bfloat16, torch.int16), torch.float32, torch.int32
         self._device = _initialised
 
@@ -992,20 +1000,22 @@ class KVCache:
 
     def _table(self, what: str, t, n: int, width: int, kind) -> tuple[int, int, int]:
         """(pointer, sequence stride, head stride) of a device tensor [n, num_kv_heads, at least width], checked."""
-        if t.dim() != 3 or t.dtype is not kind or t.get_device() != self._device or t.shape[0] != n \
-                or t.shape[1] != self.num_kv_heads or t.shape[2] < width or (t.shape[2] > 1 and t.stride(2) != 1):
-            raise AosError(f"KVCache.{what}: a device {str(kind)[6:]} tensor [{n}, {self.num_kv_heads}, {width} or more], the "
-                           "positions of a head side by side")
-        head = t.stride(1) if self.num_kv_heads > 1 else max(t.stride(1), t.shape[2])
-        return t.data_ptr(), t.stride(0) if n > 1 else self.num_kv_heads * head, head
+        shape, stride, nkv = t.shape, t.stride(), self.num_kv_heads
+        if len(shape) != 3 or shape[0] != n or shape[1] != nkv or shape[2] < width or t.dtype is not kind \
+                or t.get_device() != self._device or stride[2] != 1 and shape[2] > 1:
+            raise AosError(f"KVCache.{what}: a device {str(kind)[6:]} tensor [{n}, {nkv}, {width} or more], the positions of a "
+                           "head side by side")
+        head = stride[1] if nkv > 1 else max(stride[1], shape[2])
+        return t.data_ptr(), stride[0] if n > 1 else nkv * head, head
 
     def weigh(self, layer: int, batch: KVBatch, q, weights, scale: float | None = None, window: int = 0, prior=None) -> None:
         """The attention weight of each cached position of the batch's sequences from the batch's rows (appended before),
         into weights, device float32 [sequences, num_kv_heads, max_len or more]; added to those of prior (may be
         weights itself) where given."""
-        n, c, w = q.shape[0], batch.c, _KVWeights()
+        n, c, w = q.shape[0], batch.c, self._weights
         qp, qs = self._row(q, n)
         seqs = c.n_seqs
+        w.prior = None
         w.out, w.out_seq, w.out_head = self._table("weigh: weights", weights, seqs, c.max_len, self._f32)
         if prior is not None:
             w.prior, w.prior_seq, w.prior_head = self._table("weigh: prior", prior, seqs, c.max_len, self._f32)
@@ -1025,20 +1035,20 @@ class KVCache:
         between, keep [sequences] (device int32) in all, to the pages of to_pages (device int32 [sequences, pages]); writes the
         kept positions of each key/value head to kept, device int32 [sequences, num_kv_heads, most], and their weights
         to weights_out."""
-        c, e = batch.c, _KVEvict()
+        c, e, i32, dev = batch.c, self._evict, self._i32, self._device
         n = c.n_seqs
-        for t, dims in ((keep, 1), (to_pages, 2)):
-            if t.dtype is not self._i32 or t.dim() != dims or t.shape[0] != n or t.get_device() != self._device \
-                    or (t.numel() and t.shape[-1] > 1 and t.stride(-1) != 1):
-                raise AosError("KVCache.evict: keep [n] and to_pages [n, pages] must be device int32 tensors")
+        width, to_stride = to_pages.shape[-1], to_pages.stride()
+        if keep.dtype is not i32 or keep.shape != (n,) or n > 1 and keep.stride() != (1,) or keep.get_device() != dev \
+                or to_pages.dtype is not i32 or to_pages.shape != (n, width) or width > 1 and to_stride[1] != 1 \
+                or to_pages.get_device() != dev:
+            raise AosError("KVCache.evict: keep [n] and to_pages [n, pages] must be device int32 tensors")
         e.weights, e.weights_seq, e.weights_head = self._table("evict: weights", weights, n, c.max_len, self._f32)
         e.kept, e.kept_seq, e.kept_head = self._table("evict: kept", kept, n, 0, self._i32)
+        e.weights_out = None
         if weights_out is not None:
             e.weights_out, e.out_seq, e.out_head = self._table("evict: weights_out", weights_out, n, c.max_len, self._f32)
-        e.keep, e.to_pages, e.to_stride = keep.data_ptr(), to_pages.data_ptr(), to_pages.shape[1]
-        if n > 1 and to_pages.stride(0) != to_pages.shape[1]:
-            e.to_stride = to_pages.stride(0)
-        e.max_keep = min(kept.shape[2], to_pages.shape[1] * self.page_size)
+        e.keep, e.to_pages, e.to_stride = keep.data_ptr(), to_pages.data_ptr(), to_stride[0] if n > 1 else width
+        e.max_keep = min(kept.shape[2], width * self.page_size)
         e.first, e.recent = first, recent
         if _lib.aoship_kv_evict(self.h, layer, self._batch(batch, c.n_tokens), C.byref(e)):
             raise AosError(f"aoship_kv_evict: {last_error()}")

@@ -293,7 +293,8 @@ template <int HDP>
 struct Stage {
   static constexpr int UNITS = HDP / 8, LD = RT * 16 + 16, N = UNITS * RT / 256;
   unsigned char q[UNITS * LD];
-  int hi[RT];
+  long long next[RT]; /* where the queries of the stage after this one begin (elements; past the last row: that row's) */
+  int hi[RT];         /* the last position that a row sees; -1 past the last row */
   float m[RT], f[RT];
 };
 
@@ -334,39 +335,38 @@ __global__ void __launch_bounds__(256, HDP == 256 ? 1 : 3) aos_kv_weigh_kernel(a
   /* a thread's pieces of a stage: rows tid / UNITS + i * 256 / UNITS, unit tid % UNITS */
   constexpr int STEP = 256 / UNITS;
   const int unit = tid % UNITS, row1 = tid / UNITS;
+  const bool real = 8 * unit < p.b.hd; /* (zeros past head_dim) */
+  auto place = [&](int r) {
+    const int x = r < rb ? r : rb - 1, t = token(x);
+    return (long long)(q.row0 + t) * p.q_ld + (long long)(h * g + x - t * g) * p.b.hd;
+  };
+  const uint16_t *qu = p.q + (real ? 8 * unit : 0);
   u32x4 fq[N];
   float2 fs = {0.0f, 0.0f};
   int fh = 0;
-  auto fetch = [&](int r0) {
+  auto fetch = [&](int r0, auto &&at) { /* the queries of a stage's rows, at(i) from qu, and what goes with them */
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int r = r0 + row1 + i * STEP, t = token(r), hh = h * g + r - t * g;
-      fq[i] = u32x4{};
-      if (r < rb && 8 * unit < p.b.hd) fq[i] = aos_gld16(p.q + (long long)(q.row0 + t) * p.q_ld + hh * p.b.hd + 8 * unit);
-    }
+    for (int i = 0; i < N; ++i) fq[i] = aos_gld16(qu + at(row1 + i * STEP));
     if (tid < RT) {
       const int r = r0 + tid;
       fh = r < rb ? v.hi(token(r)) : -1;
       if (SUM && r < rb) fs = stat[r];
     }
   };
-  auto put = [&](Stage<HDP> &d) {
+  auto put = [&](Stage<HDP> &d, int r0) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      u32x4 y = fq[i];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) y[j] ^= flip;
-      *(u32x4 *)(d.q + unit * LD + (row1 + i * STEP) * 16) = y;
-    }
+    for (int i = 0; i < N; ++i) *(u32x4 *)(d.q + unit * LD + (row1 + i * STEP) * 16) = real ? fq[i] : u32x4{};
     if (tid < RT) {
       d.hi[tid] = fh;
       if (SUM) {
         d.m[tid] = fs.x;
         d.f[tid] = fs.y;
       }
+    } else if (tid < 2 * RT) {
+      d.next[tid - RT] = place(r0 + RT + tid - RT);
     }
   };
-  fetch(ra); /* (on their way with the keys) */
+  fetch(ra, [&](int i) { return place(ra + i); }); /* (on their way with the keys) */
   const bool fall = starts_fall(p.b, tid, 256);
   u32x4 kf[2][KS];
   {
@@ -375,15 +375,19 @@ __global__ void __launch_bounds__(256, HDP == 256 ? 1 : 3) aos_kv_weigh_kernel(a
 #pragma unroll
     for (int b = 0; b < 2; ++b)
 #pragma unroll
-      for (int e = 0; e < KS; ++e) kf[b][e] = k.operand(b, e);
+      for (int e = 0; e < KS; ++e) {
+        kf[b][e] = k.operand(b, e);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) kf[b][e][j] ^= flip; /* a negative scale: negated keys */
+      }
   }
   float acc[2] = {0.0f, 0.0f};
-  put(st[0]);
+  put(st[0], ra);
   if (refused(p.b, fall, tid)) return;
   int i = 0;
   for (int r0 = ra; r0 < rb; r0 += RT, ++i) {
     const Stage<HDP> &d = st[i & 1];
-    if (r0 + RT < rb) fetch(r0 + RT);
+    if (r0 + RT < rb) fetch(r0 + RT, [&](int i) { return d.next[i]; });
 #pragma unroll
     for (int sub = 0; sub < 2; ++sub) {
       float m = NINF, l = 0.0f;
@@ -457,7 +461,7 @@ __global__ void __launch_bounds__(256, HDP == 256 ? 1 : 3) aos_kv_weigh_kernel(a
         }
       }
     }
-    if (r0 + RT < rb) put(st[(i + 1) & 1]);
+    if (r0 + RT < rb) put(st[(i + 1) & 1], r0 + RT);
     __syncthreads();
     if constexpr (!SUM) {
       if (tid < RT && r0 + tid < rb) {

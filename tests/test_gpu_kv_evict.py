@@ -270,6 +270,47 @@ def test_weights_with_infinities_and_nans(hip, fmt, new):
     _check_weigh(hip, fmt, 4, nkv, hd, 64, [new] * 4, lens, k_rows=k, q_rows=q, small=new < 50)
 
 
+@pytest.mark.parametrize("fmt", P.FORMATS)
+@pytest.mark.parametrize("hd,nkv,nh,new,window", [(128, 8, 24, 1, 0), (128, 8, 24, 20, 700), (256, 2, 16, 1, 0), (64, 4, 28, 45, 0)])
+def test_weights_with_the_chip_full(hip, fmt, hd, nkv, nh, new, window):
+    """More workgroups than the chip holds, converting and multiplying at once, against float64 sums over the values that the
+    cache holds, and the same bits three times."""
+    import torch
+
+    rng = np.random.default_rng(hd + new)
+    lens = rng.integers(new, 3000, 64).tolist()
+    pool = P.Pool(hip, lens, nkv, hd, 128, fmt)
+    total, T, g = sum(lens), 64 * new, nh // nkv
+    gen = torch.Generator(device="cuda").manual_seed(hd)
+    k = torch.randn((total, nkv, hd), generator=gen, device="cuda").bfloat16()
+    pool.cache.append(0, pool.batch(lens, lens), k, k)
+    held = [torch.empty_like(k) for _ in range(2)]
+    pool.cache.read(0, pool.batch(lens, lens), *held)
+    q = torch.randn((T, nh, hd), generator=gen, device="cuda").bfloat16()
+    out = torch.zeros((64, nkv, max(lens)), device="cuda")
+    b = pool.batch([new] * 64, lens)
+    pool.cache.weigh(0, b, q, out, window=window)
+    first = out.clone()
+    S = hd ** -0.5 * float(q.float().abs().sum(-1).max()) * float(held[0].float().abs().max())
+    rel = 2.2 * (hd + 4) * 2.0 ** -24 * S + 2.0 ** -13  # (_tolerance)
+    at = 0
+    for s, L in enumerate(lens):
+        x = held[0][at:at + L].double().permute(1, 2, 0).contiguous()
+        at += L
+        y = q[s * new:(s + 1) * new].double().unflatten(1, (nkv, g)).permute(1, 0, 2, 3).reshape(nkv, new * g, hd)
+        far = (L - new + torch.arange(new, device="cuda"))[:, None] - torch.arange(L, device="cuda")
+        hidden = (far < 0) | (far >= window) if window else far < 0
+        z = torch.matmul(y, x) * hd ** -0.5
+        z = z.masked_fill(hidden.repeat_interleave(g, 0), float("-inf"))
+        want = torch.softmax(z, -1).sum(1)
+        got = first[s, :, :L].double()
+        assert ((got - want).abs() <= rel * want + 1e-30).all(), (s, float(((got - want).abs() / (want + 1e-30)).max()))
+    for _ in range(2):
+        out.zero_()
+        pool.cache.weigh(0, b, q, out, window=window)
+        assert torch.equal(out, first)
+
+
 def _state(pool, n, nkv, L):
     import torch
 
