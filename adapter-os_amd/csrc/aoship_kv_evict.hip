@@ -57,7 +57,9 @@ __device__ __forceinline__ int lane_scan(int x, int lane) {
   return x;
 }
 
-/* Grid: sequences times key/value heads. Thread t has the positions t, t + 1024, ... of a span of PER * 1024. */
+/* Bound by the latency of its turns and by how few workgroups there are: 2 heads of 2047 weights 11 us, 128 of up to 12000 26,
+ * 32 of up to 32767 52.
+ * Grid: sequences times key/value heads. Thread t has the positions t, t + 1024, ... of a span of PER * 1024. */
 template <int PER>
 __global__ void __launch_bounds__(NT) aos_kv_select_kernel(aos_kv_evict_params p) {
   constexpr int SPAN = NT * PER;
@@ -265,7 +267,9 @@ __global__ void __launch_bounds__(NT) aos_kv_select_kernel(aos_kv_evict_params p
     for (int i = k.n + tid; i < k.len; i += NT) wo[i] = 0.0f;
 }
 
-/* Grid: tiles of 64 kept positions, key/value heads, sequences. */
+/* Grid: tiles of 64 kept positions, key/value heads, sequences. Bound by memory at 16 bits: 4 sequences of up to 32767 down to
+ * 15000, 8 heads of 128, 127 us (233 MB written, most of 330 MB read: every line holds some kept position); by the taking
+ * apart of values at 4: 16 of up to 12000 down to 4096, 77 us (71 and 130 MB). */
 template <int FMT, int HDP>
 __global__ void __launch_bounds__(256) aos_kv_move_kernel(aos_kv_evict_params p, int tiles) {
   __shared__ const unsigned char *src[TILE]; /* the tiles that the positions are in; NULL: none */
@@ -301,18 +305,32 @@ __global__ void __launch_bounds__(256) aos_kv_move_kernel(aos_kv_evict_params p,
     *(u32x4 *)(dst + (u * TILE + i) * 16) = t ? aos_gld16(t + (u * TILE + in[i]) * 16) : u32x4{};
   }
   if constexpr (FMT == AOS_KV_BF16) {
-    for (int c = tid; c < (TILE / 8) * HDP; c += 256) {
-      const int d = c % HDP, u = c / HDP;
+    /* a thread per unit of 8 positions of a dimension. Where its positions come from is the same for all lanes of a
+     * wave, so a source unit is loaded once for the run of positions that are in it (127 us where a load for each position
+     * took 143; for the quantised formats, whose units are cheaper to load, 81 and 77 the other way) */
+    for (int c = tid; c < TILE / 8 * HDP; c += 256) {
+      const int u = __builtin_amdgcn_readfirstlane(c / HDP), d = c % HDP;
       if (8 * u >= n) break;
-      uint32_t x[8];
+      u32x4 x = {};
+      uint32_t y[4] = {};
+      const unsigned char *from = nullptr;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const unsigned char *t = src[8 * u + e];
-        const int at = in[8 * u + e];
-        x[e] = t ? *(const __attribute__((address_space(1))) uint16_t *)(t + v_off<FMT, HDP>() + (at / 8 * HDP + d) * 16 + at % 8 * 2) : 0u;
+        const uint64_t t = (uint64_t)src[8 * u + e];
+        const unsigned char *unit = (const unsigned char *)(((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(t >> 32)) << 32) |
+                                                            (uint32_t)__builtin_amdgcn_readfirstlane((int)t));
+        const int at = __builtin_amdgcn_readfirstlane(in[8 * u + e]);
+        if (unit) unit += v_off<FMT, HDP>() + at / 8 * HDP * 16;
+        if (e == 0 || unit != from) { /* uniform */
+          from = unit;
+          x = unit ? aos_gld16(unit + d * 16) : u32x4{};
+        }
+        uint32_t w = x[0];
+#pragma unroll
+        for (int i = 1; i < 4; ++i) w = at % 8 / 2 == i ? x[i] : w;
+        y[e / 2] |= (w >> (at & 1) * 16 & 0xffffu) << (e % 2 * 16);
       }
-      *(u32x4 *)(dst + v_off<FMT, HDP>() + (u * HDP + d) * 16) =
-          u32x4{x[0] | x[1] << 16, x[2] | x[3] << 16, x[4] | x[5] << 16, x[6] | x[7] << 16};
+      *(u32x4 *)(dst + v_off<FMT, HDP>() + (u * HDP + d) * 16) = u32x4{y[0], y[1], y[2], y[3]};
     }
   } else {
     constexpr int W = FMT == AOS_KV_MXFP8 ? 4 : 2; /* words of a value unit: 16 positions of a dimension */

@@ -503,14 +503,15 @@ def test_evict_of_long_sequences(hip, L):
     _evicted(hip, "mxfp4", 1, 64, 256, [L, L - 1000], [L // 3, L // 2], 4, 100, w)
 
 
-def test_evict_and_bad_batches(hip):
+@pytest.mark.parametrize("fmt", P.FORMATS)
+def test_evict_and_bad_batches(hip, fmt):
     """Sequences that do not fit are left out, positions of bad pages move as zeros and not to bad pages, others are served."""
     import torch
 
     rng = np.random.default_rng(2)
     nkv, hd, L = 2, 64, 200
     lens = [200, 200, 200, 201, 200]
-    pool = P.Pool(hip, [200] * 5, nkv, hd, 64, "bf16", spare=20)
+    pool = P.Pool(hip, [200] * 5, nkv, hd, 64, fmt, spare=20)
     rows = P.bf16(rng.standard_normal((1000, nkv, hd)) + 5)
     pool.cache.append(0, pool.batch([200] * 5, [200] * 5), P.to_gpu(rows), P.to_gpu(rows))
     pool.pages[0, 1] = 999
@@ -532,7 +533,7 @@ def test_evict_and_bad_batches(hip):
     for s in (0, 4):
         b = hip.KVBatch(_i32([0, 64]), _i32([64]), _i32(to[s:s + 1, :1]), 64, 64)
         pool.cache.read(0, b, *back)
-        x = rows[200 * s + want[:64]].copy()
+        x = P.quantised(rows, fmt)[200 * s + want[:64]]
         if s == 0:
             x[(want[:64] >= 64) & (want[:64] < 128)] = 0
         _same(P.to_cpu(back[0]), x)
