@@ -12,12 +12,12 @@
  * each of which it keeps the largest value and the unit it is in. The n largest elements lie in the n groups whose
  * largest come first; these few groups are read again (from the L2), what is not before the last of their largest
  * goes to a list (about n entries), and an entry's place in the answer is the number of entries before it. The n groups
- * are found in the same way: a bound that n of a wave's lanes reach, by bisection of the bits, then a list and places in it.
+ * are found in the same way: a bound that n of a wave's lanes reach, then a list and places in it.
  *
- * Few rows are cut into slices, whose pieces the row's last workgroup joins (a second launch cost 5 us more).
+ * Few rows are cut into slices, whose pieces the row's last workgroup joins.
  *
  * Bound by reading the logits once, and nearly as much by the vector instructions (an exponential and nine others a logit):
- * 4000 rows of 50257 bfloat16 99 us, 4.1 TB/s. Few rows by the latencies of the choice: 1 row of 152064 with 5 tokens 14
+ * 4000 rows of 50257 bfloat16 97 us, 4.1 TB/s. Few rows by the latencies of the choice: 1 row of 152064 with 5 tokens 14
  * us, 64 of 128256 with 20 24 us (taking the n one after the other from 64 lanes 72).
  */
 #include "aoship_device.h"
@@ -129,34 +129,18 @@ __device__ __forceinline__ void push(Shared &sh, uint64_t k) {
   if (at < LIST) sh.list[at] = k;
 }
 
-/* A bound that exactly n of the wave's keys reach (0 where there are no n): the value's bits from the highest on, as far as
- * it takes to part n from the others, the index's where values are alike. Uniform. */
-__device__ __forceinline__ uint64_t wave_nth(uint64_t k, int n) {
-  const uint32_t hi = (uint32_t)(k >> 32), lo = (uint32_t)k;
-  uint32_t v = 0;
-  for (uint32_t bit = 1u << 31; bit; bit >>= 1) {
-    const int c = (int)__popcll(__ballot(hi >= (v | bit)));
-    if (c < n) continue;
-    v |= bit;
-    if (c == n) return (uint64_t)v << 32;
-  }
-  n -= (int)__popcll(__ballot(hi > v));
-  uint32_t i = 0;
-  for (uint32_t bit = 1u << 31; bit; bit >>= 1) {
-    const int c = (int)__popcll(__ballot(hi == v && lo >= (i | bit)));
-    if (c < n) continue;
-    i |= bit;
-    if (c == n) break;
-  }
-  return ((uint64_t)v << 32) | i;
-}
-
 /* The n largest of all threads' four keys (distinct, zeros for none), in order, into sh.top. Of a wave's lanes' largest the
  * n-th is no more than the n-th of all keys: those from the largest such bound on are listed, about twice n. */
 __device__ __forceinline__ void largest(Shared &sh, const uint64_t (&k)[4], int n) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const uint64_t a = k[0] > k[1] ? k[0] : k[1], b = k[2] > k[3] ? k[2] : k[3], mine = a > b ? a : b;
-  const uint64_t bound = wave_nth(mine, n);
+  /* a lane counts the lanes before its own (bisecting the bound's bits by ballots, a chain of scalar turns, made 1 row of
+   * 152064 19.3 us for 14.5, 64 of 128256 28.3 for 24.4) */
+  int before = 0;
+#pragma unroll 16
+  for (int j = 0; j < 64; ++j) before += lane_key(mine, j) > mine ? 1 : 0;
+  const uint64_t nth = __ballot(mine != 0 && before == n - 1); /* (none: fewer than n keys) */
+  const uint64_t bound = nth ? lane_key(mine, __builtin_ctzll(nth)) : 0;
   if (lane == 0) sh.wave[wave] = bound;
   if (tid == 0) sh.listed = 0;
   __syncthreads();
@@ -479,8 +463,8 @@ static_assert(AOS_LOGPROBS_MAX_TOP <= 32 && AOS_LOGPROBS_MAX_TOP * AOS_LOGPROBS_
 static_assert(AOS_LOGPROBS_MAX_SLICES <= SEGS * NT, "a thread takes SEGS slices");
 
 /* Slices of a row: as many as give the rows 512 workgroups, of at least 2048 elements. A workgroup's choice of candidates
- * costs as much as reading some 10000 elements: 64 rows of 128256 with 20 of them 34 us in 2048 workgroups, 35 in 1024,
- * 24 in 512, 25 in 256. */
+ * costs as much as reading some 10000 elements: 64 rows of 128256 with 20 of them 36 us in 1024 workgroups, 24.5 in 512,
+ * 25.4 in 256. */
 extern "C" void aos_logprobs_shape(int T, int vocab, int *slices, int *span) {
   long long s = T > 0 ? (512 + T - 1) / T : 1;
   if (s > vocab / 2048) s = vocab / 2048;
