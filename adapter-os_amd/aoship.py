@@ -963,7 +963,7 @@ class KVCache:
         r.v_bias = None if v_bias is None else self._bias(v_bias, nkv)
         if positions is not None:
             t = positions
-            if t.dtype is not self._i32 or t.get_device() != self._device or t.shape[-1] != n or t.dim() > 2 \
+            if t.dtype is not self._i32 or t.get_device() != self._device or t.dim() not in (1, 2) or t.shape[-1] != n \
                     or (t.shape[0] if t.dim() == 2 else 1) != self.n_axes or (n > 1 and t.stride(-1) != 1):
                 raise AosError(f"KVCache.append: positions must be device int32 [{self.n_axes}, {n}], those of an axis side "
                                "by side")

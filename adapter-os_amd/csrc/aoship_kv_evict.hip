@@ -268,8 +268,8 @@ __global__ void __launch_bounds__(NT) aos_kv_select_kernel(aos_kv_evict_params p
 }
 
 /* Grid: tiles of 64 kept positions, key/value heads, sequences. Bound by memory at 16 bits: 4 sequences of up to 32767 down to
- * 15000, 8 heads of 128, 127 us (233 MB written, most of 330 MB read: every line holds some kept position); by the taking
- * apart of values at 4: 16 of up to 12000 down to 4096, 77 us (71 and 130 MB). */
+ * 15000, 8 heads of 128, 126 us (345 MB fetched, 226 written, 4.5 TB/s); by the taking apart of values at 4: 16 of up to
+ * 12000 down to 4096, 77 us (141 and 70 MB, 2.7 TB/s). */
 template <int FMT, int HDP>
 __global__ void __launch_bounds__(256) aos_kv_move_kernel(aos_kv_evict_params p, int tiles) {
   __shared__ const unsigned char *src[TILE]; /* the tiles that the positions are in; NULL: none */

@@ -10,7 +10,9 @@
  * pieces of the sequence, and a second launch makes weights of them. With more rows the scores would be more than the
  * keys: they are formed twice, for the sums and for the weights. Scores, sums and weights are float32, added in one order.
  *
- * Matrix instructions' registers (aoship_device.h): every accumulator register is read.
+ * Matrix instructions' registers (aoship_device.h): every accumulator register is read, so results need no hold; operands are
+ * not held, as in the attention over the cache, and the tests check the outputs with the whole chip multiplying and
+ * converting at once, in every format, against float64 and run to run, bit for bit.
  */
 #include "aoship_internal.h"
 #include "aoship_kv.h"
@@ -77,7 +79,11 @@ __device__ __forceinline__ int turned(int i, int by, int n) {
 
 /* Grid: pieces of `tiles` position tiles, key/value heads, sequences. S^T = K . Q^T by v_mfma_f32_32x32x16_bf16: row
  * 16 s + 8 a + 4 c + i of a block of 32 keys is position 16 c + 8 s + 4 a + i, so that a lane's 16 scores are 16
- * consecutive positions of its row. The waves take a piece's tiles in turn. */
+ * consecutive positions of its row. The waves take a piece's tiles in turn.
+ *
+ * Bound by memory: 64 streams of up to 16001 positions, 28/4 heads of 128, 16 bits: 147 us for 682 MB fetched and 75
+ * written (5.1 TB/s; a large copy 4.7), then 29 us to read the scores and make weights of them. One stream of 512: 5 and 4
+ * us, latencies. */
 template <int FMT, int HDP>
 __global__ void __launch_bounds__(256, 2) aos_kv_scores_kernel(aos_kv_weigh_params p) {
   constexpr int KS = HDP / 16;
@@ -274,7 +280,9 @@ struct Rows {
 };
 __device__ __forceinline__ Rows rows_of(const Seq &q, const Span &v, int g, int k0, int k1) {
   Rows r;
-  const int ta = k0 - v.p0, tb = v.window > 0 && k1 - 1 + v.window - 1 - v.p0 < q.count - 1 ? k1 - 1 + v.window - 1 - v.p0 : q.count - 1;
+  const int ta = k0 - v.p0; /* the first that is not before them, and the last whose window reaches them */
+  const long long far = v.window > 0 ? (long long)k1 - 1 + v.window - 1 - v.p0 : q.count - 1;
+  const int tb = far < q.count - 1 ? (int)far : q.count - 1;
   r.ra = (ta > 0 ? ta : 0) * g;
   r.rb = (tb + 1) * g;
   return r;
@@ -302,7 +310,12 @@ struct Stage {
  * some of them go by in stages of 64 through LDS.
  *   SUM false: each row's maximum and sum over the block's positions, to part[head][block][row].
  *   SUM true: the weights of the block's positions from the chunk's rows, to scores[sequence][head][chunk][position].
- * Grid: blocks, chunks, key/value heads, sequences. */
+ * Grid: blocks, chunks, key/value heads, sequences.
+ *
+ * Bound by the vector instructions beside the matrix ones (12 and 10 of them to one). Prompt of 4001, 28/4 heads of 128, 16
+ * bits: 93 and 90 us for 57 GFLOP each. 32 tokens over up to 8132 positions, 12 sequences, 24/8 heads, 8
+ * bits: 30 us either way. Queries' fragments read four ahead of the matrix instructions were within the runs' spread (the prompt
+ * 209 and 205 us for 213 and 207 in all), with a wave fewer a SIMD slower (216 and 219; the 32 tokens 79 us for 72 and 73). */
 template <int FMT, int HDP, bool SUM>
 __global__ void __launch_bounds__(256, HDP == 256 ? 1 : 3) aos_kv_weigh_kernel(aos_kv_weigh_params p) {
   constexpr int KS = HDP / 16, N = Stage<HDP>::N, LD = Stage<HDP>::LD, UNITS = Stage<HDP>::UNITS;
@@ -585,8 +598,8 @@ extern "C" int aos_kv_weigh_shape(aos_kv_weigh_params *p, size_t *bytes) {
   span = span < 1 ? 1 : span > 8 ? 8 : span;
   p->tiles = (int)span * (KB / TILE);
   p->pieces = (int)((blocks + span - 1) / span);
-  /* many rows: chunks of 64 where there are few, of up to 512 (prompt of 4001, 28 heads: 222 us, 234 in chunks of 256, 238 of
-   * 1024, whose second round is half empty) */
+  /* many rows: chunks of 64 where there are few, of up to 512 (prompt of 4001, 28 heads: 198 to 201 us; chunks of 256 take as
+   * long, 201 to 202, and leave twice as many weights to add up) */
   const double stages = (double)((rows + RT - 1) / RT), units = stages * sh * blocks;
   const int k = units < 4096 ? 1 : units > 16384 ? 8 : (int)(units / 2048);
   p->rc = RT * k;

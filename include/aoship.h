@@ -505,8 +505,8 @@ int aoship_kv_append(aoship_kv_cache_t *cache, int layer, const aoship_kv_batch_
 
 /* aoship_kv_append with rotary positions of the rows' own: pair i of row t is turned by entry i of the tables' row
  * positions[axis of i][t] (device int32 [n_axes][axis_stride]; axis_stride at least n_tokens, or 0 where all axes have the same
- * positions), whatever the row's place in its sequence: images and video on several axes, and sequences that aoship_kv_evict has shortened, whose next token is at its
- * place in the text and not in the cache. Needs rotary tables; rows->rotated must be 0. Keys in the cache are turned as they
+ * positions), whatever the row's place in its sequence: images and video on several axes, and sequences that
+ * aoship_kv_evict has shortened, whose next token is at its place in the text and not in the cache. Needs rotary tables; rows->rotated must be 0. Keys in the cache are turned as they
  * are written: attention, whose mask goes by places in the cache, needs no positions. Asynchronous. Returns 0 / -1. */
 int aoship_kv_append_at(aoship_kv_cache_t *cache, int layer, const aoship_kv_batch_t *batch, const aoship_kv_rows_t *rows,
                         const int32_t *positions, int64_t axis_stride);

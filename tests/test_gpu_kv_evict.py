@@ -106,7 +106,7 @@ def test_position_refusals(hip):
     with pytest.raises(hip.AosError, match="tables"):
         pool.cache.append(0, b, k, k, positions=at[0])
     pool.cache.set_rope(*_tables(10, 64))
-    for bad in (at, at[0, :3], at[0].long(), at[0].cpu()):
+    for bad in (at, at[0, :3], at[0].long(), at[0].cpu(), at[0, 0]):
         with pytest.raises(hip.AosError):
             pool.cache.append(0, b, k, k, positions=bad)
     with pytest.raises(hip.AosError, match="rotated"):
