@@ -61,8 +61,8 @@ struct Keys {
 /* a sequence's visible span, as row (token) t sees it: [lo, hi] */
 struct Span {
   int p0, window;
-  __device__ __forceinline__ int hi(int t) const { return p0 + t; }
-  __device__ __forceinline__ int lo(int t) const { return window > 0 && p0 + t - window + 1 > 0 ? p0 + t - window + 1 : 0; }
+  __host__ __device__ __forceinline__ int hi(int t) const { return p0 + t; }
+  __host__ __device__ __forceinline__ int lo(int t) const { return window > 0 && p0 + t - window + 1 > 0 ? p0 + t - window + 1 : 0; }
 };
 
 __device__ __forceinline__ float score_factor(float scale) { /* (a scale of zero stays above it: masks keep -infinity) */
@@ -278,11 +278,12 @@ int launch_few(const aos_kv_weigh_params *p, const aos_launch_ctx *ctx) {
 struct Rows {
   int ra, rb;
 };
-__device__ __forceinline__ Rows rows_of(const Seq &q, const Span &v, int g, int k0, int k1) {
+__host__ __device__ __forceinline__ Rows rows_of(const Seq &q, const Span &v, int g, int k0, int k1) {
   Rows r;
   const int ta = k0 - v.p0; /* the first that is not before them, and the last whose window reaches them */
   const long long far = v.window > 0 ? (long long)k1 - 1 + v.window - 1 - v.p0 : q.count - 1;
-  const int tb = far < q.count - 1 ? (int)far : q.count - 1;
+  /* (-1: none; a block's distance before the rows, 2^30 at most, passes 2^31 times g) */
+  const int tb = far < -1 ? -1 : far < q.count - 1 ? (int)far : q.count - 1;
   r.ra = (ta > 0 ? ta : 0) * g;
   r.rb = (tb + 1) * g;
   return r;
@@ -636,6 +637,14 @@ extern "C" void aos_kv_weigh_parts(aos_kv_weigh_params *p, void *ws) {
   p->scores = (float *)ws;
   p->part = p->scores + sh * (size_t)(p->few ? p->rows : p->chunks) * (size_t)p->lpad;
   p->stat = p->few ? nullptr : p->part + 2 * total * (size_t)p->blocks;
+}
+
+/* Diagnostic, for tests without a device: the rows (heads of a group times `count` new tokens) of a sequence of `len` positions
+ * that see some of the positions k0 .. k1 - 1, as the kernels of many rows find them: [out[0], out[1]). */
+extern "C" void aoship_internal_kv_weigh_rows(int g, int window, int count, int len, int k0, int k1, int *out) {
+  const Rows r = rows_of(Seq{0, count, len}, Span{len - count, window}, g, k0, k1);
+  out[0] = r.ra;
+  out[1] = r.rb;
 }
 
 #define KV_DISPATCH(fn, fmt, hdp, ...)                                       \
