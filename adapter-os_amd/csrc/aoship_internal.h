@@ -718,10 +718,12 @@ typedef struct {
   float *w;           /* [sequence][head][position]; may be prior */
   long long prior_seq, prior_head, w_seq, w_head;
   /* aos_kv_weigh_shape: */
-  int few, rows, blocks, lpad, tiles, pieces, chunks, rc /* rows of a chunk */;
+  int few, rows, blocks, lpad, tiles, pieces;
+  int rc, chunks, slots;     /* rows of a chunk; chunks of each sequence (0: as many as its rows need); all of them */
+  int row_pieces, row_slots; /* the same of 256 rows */
   uint32_t g_mul, g_shift; /* of the division by the heads of a group */
   /* aos_kv_weigh_parts: */
-  float *scores; /* few: [sequence][head][rows][lpad]; else the chunks' weights [sequence][head][chunks][lpad] */
+  float *scores; /* few: [sequence][head][rows][lpad]; else the chunks' weights [slots][head][lpad] */
   float *part;   /* maxima and sums: few: [sequence][head][pieces][rows][2]; else [head][blocks][all rows][2] */
   float *stat;   /* [head][all rows][2] maxima and inverse sums */
 } aos_kv_weigh_params;

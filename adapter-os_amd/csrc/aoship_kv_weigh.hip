@@ -289,6 +289,63 @@ __host__ __device__ __forceinline__ Rows rows_of(const Seq &q, const Span &v, in
   return r;
 }
 
+/* The rows of a head are dealt out in shares of `unit`, one or more a sequence: `each` of every sequence, or (each 0) as
+ * many as its own rows need and one at most to spare, sequence s's from number (first row) / unit + s on. The second,
+ * whose shares follow the batch's rows, is for batches of which the first would make more than twice as many, like single
+ * tokens beside a prompt (63 and one of 4001, up to 16000 positions, 28/4 heads of 128: 454 us and 107 MB, 1933 us and
+ * 979 MB by the first; prompts of 900, 400, 1200 and 700, whose sequences it has to search for, 70 us, 66 by the first). */
+struct Shares {
+  int unit, each;
+  __host__ __device__ __forceinline__ long long base(int g, int s, int row0) const {
+    return each ? (long long)s * each : (long long)row0 * g / unit + s;
+  }
+};
+/* how many there are of each kind */
+inline double shares_of_each(const aos_kv_batch &b, long long g, int unit) {
+  return (double)((b.max_new * g + unit - 1) / unit) * b.n_seqs;
+}
+inline double shares_of_own(const aos_kv_batch &b, long long g, int unit) {
+  return (double)(b.n_tokens * g / unit + b.n_seqs);
+}
+
+/* Share number x of head h of sequence s is its part-th; s -1: none. From the number i of a head's share (of all of a
+ * sequence's, head by head, where each sequence has as many). Uniform: each wave searches for the sequence, 64 at a time. */
+struct Share {
+  int s, h;
+  long long part, x;
+};
+__device__ __forceinline__ Share share_at(const aos_kv_batch &b, const Shares &d, int g, uint32_t i, int lane) {
+  Share o;
+  if (d.each) {
+    const int sh = (int)(i / (uint32_t)d.each);
+    o.part = (int)(i - (uint32_t)sh * (uint32_t)d.each);
+    o.s = sh / b.nkv;
+    o.h = sh - o.s * b.nkv;
+    o.x = (long long)o.s * d.each + o.part;
+    return o;
+  }
+  const uint32_t x = i / (uint32_t)b.nkv;
+  o.h = (int)(i - x * (uint32_t)b.nkv);
+  o.x = x;
+  int at = 0, n = b.n_seqs; /* the last of at .. at + n - 1 whose shares begin at or before x (where starts fall, any) */
+  for (;;) {
+    const int step = (n + 63) / 64, k = lane * step;
+    const bool yes = k < n && d.base(g, at + k, b.starts[at + k]) <= x;
+    const int c = (int)__popcll(__ballot(yes));
+    if (c == 0) {
+      o.s = -1;
+      return o;
+    }
+    at += (c - 1) * step;
+    n = n - (c - 1) * step < step ? n - (c - 1) * step : step;
+    if (step == 1) break;
+  }
+  o.s = __builtin_amdgcn_readfirstlane(at);
+  o.part = o.x - d.base(g, o.s, b.starts[o.s]);
+  if (o.part < 0) o.s = -1; /* (only where starts fall) */
+  return o;
+}
+
 /* Whether the batch's starts fall somewhere (noted): its sequences' rows may then be the same, and none of them is served. */
 __device__ __forceinline__ bool refused(const aos_kv_batch &b, bool fall, int tid) {
   if (!__syncthreads_or(fall ? 1 : 0)) return false;
@@ -310,8 +367,8 @@ struct Stage {
 /* A workgroup has the keys of KB positions in registers, a tile a wave, and the rows of one chunk (p.rc of them) that see
  * some of them go by in stages of 64 through LDS.
  *   SUM false: each row's maximum and sum over the block's positions, to part[head][block][row].
- *   SUM true: the weights of the block's positions from the chunk's rows, to scores[sequence][head][chunk][position].
- * Grid: blocks, chunks, key/value heads, sequences.
+ *   SUM true: the weights of the block's positions from the chunk's rows, to scores[chunk][head][position].
+ * Grid: blocks, shares (chunks) of the rows.
  *
  * Bound by the vector instructions beside the matrix ones (12 and 10 of them to one). Prompt of 4001, 28/4 heads of 128, 16
  * bits: 93 and 90 us for 57 GFLOP each. 32 tokens over up to 8132 positions, 12 sequences, 24/8 heads, 8
@@ -324,18 +381,19 @@ __global__ void __launch_bounds__(256, HDP == 256 ? 1 : 3) aos_kv_weigh_kernel(a
   __shared__ float red[SUM ? 1 : 2][4][2][SUM ? 1 : RT];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 31, half = lane >> 5;
-  int x = (int)(blockIdx.x / (uint32_t)p.blocks);
-  const int b0 = (int)(blockIdx.x - (uint32_t)x * (uint32_t)p.blocks), chunk = x % p.chunks;
-  const int blk = turned(b0, x, p.blocks);
-  x /= p.chunks;
-  const int s = x / p.b.nkv, h = x - s * p.b.nkv;
+  const int x = (int)(blockIdx.x / (uint32_t)p.blocks), b0 = (int)(blockIdx.x - (uint32_t)x * (uint32_t)p.blocks);
+  const int blk = turned(b0, x, p.blocks), g = p.nh / p.b.nkv;
+  const Share chunk = share_at(p.b, Shares{p.rc, p.chunks}, g, (uint32_t)x, lane);
+  const int s = chunk.s, h = chunk.h;
+  if (s < 0) return;
   const Seq q = seq_at(p.b, s);
-  const int g = p.nh / p.b.nkv, k0 = blk * KB, k1 = k0 + KB < q.len ? k0 + KB : q.len;
+  const int k0 = blk * KB, k1 = k0 + KB < q.len ? k0 + KB : q.len;
   if (q.count == 0 || k0 >= q.len) return;
   const Span v = {q.len - q.count, p.window};
   const Rows vis = rows_of(q, v, g, k0, k1);
-  const int ra = vis.ra > chunk * p.rc ? vis.ra / RT * RT : chunk * p.rc;
-  const int rb = vis.rb < (chunk + 1) * p.rc ? vis.rb : (chunk + 1) * p.rc;
+  if (chunk.part * p.rc >= vis.rb) return; /* (a share to spare) */
+  const int r1 = (int)chunk.part * p.rc;
+  const int ra = vis.ra > r1 ? vis.ra / RT * RT : r1, rb = vis.rb < r1 + p.rc ? vis.rb : r1 + p.rc;
   if (ra >= rb) return;
 
   const int tb = k0 + TILE * wave; /* this wave's keys */
@@ -491,7 +549,7 @@ __global__ void __launch_bounds__(256, HDP == 256 ? 1 : 3) aos_kv_weigh_kernel(a
     }
   }
   if constexpr (SUM) {
-    float *out = p.scores + (((long long)s * p.b.nkv + h) * p.chunks + chunk) * p.lpad + tb;
+    float *out = p.scores + (chunk.x * p.b.nkv + h) * p.lpad + tb;
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
       const float sum = half_sum(acc[b]);
@@ -500,14 +558,16 @@ __global__ void __launch_bounds__(256, HDP == 256 ? 1 : 3) aos_kv_weigh_kernel(a
   }
 }
 
-/* Grid: pieces of 256 rows, key/value heads, sequences: a row's maximum and the inverse of its sum over all blocks. */
-__global__ void __launch_bounds__(256) aos_kv_weigh_rows_kernel(aos_kv_weigh_params p, int pieces) {
+/* Grid: shares of 256 rows: a row's maximum and the inverse of its sum over all blocks. */
+__global__ void __launch_bounds__(256) aos_kv_weigh_rows_kernel(aos_kv_weigh_params p) {
   if (refused(p.b, starts_fall(p.b, (int)threadIdx.x, 256), (int)threadIdx.x)) return;
-  const int piece = (int)(blockIdx.x % (uint32_t)pieces), sh = (int)(blockIdx.x / (uint32_t)pieces);
-  const int s = sh / p.b.nkv, h = sh - s * p.b.nkv;
+  const int g = p.nh / p.b.nkv;
+  const Share piece = share_at(p.b, Shares{256, p.row_pieces}, g, blockIdx.x, (int)threadIdx.x & 63);
+  const int s = piece.s, h = piece.h;
+  if (s < 0) return;
   const Seq q = seq_at(p.b, s);
-  const int g = p.nh / p.b.nkv, r = piece * 256 + (int)threadIdx.x;
-  if (r >= q.count * g) return;
+  if (piece.part * 256 + (int)threadIdx.x >= (long long)q.count * g) return;
+  const int r = (int)piece.part * 256 + (int)threadIdx.x;
   const Span v = {q.len - q.count, p.window};
   const int t = r / g, hi = v.hi(t), lo = v.lo(t);
   const long long total = (long long)p.b.n_tokens * g, at = (long long)q.row0 * g + r;
@@ -540,12 +600,13 @@ __global__ void __launch_bounds__(64) aos_kv_weigh_sum_kernel(aos_kv_weigh_param
   if (q.count) {
     const Span v = {q.len - q.count, p.window};
     const Rows vis = rows_of(q, v, g, k0, k1);
-    const float *in = p.scores + (long long)sh * p.chunks * p.lpad + pos;
+    const long long step = (long long)p.b.nkv * p.lpad; /* from a chunk to the next */
+    const float *in = p.scores + Shares{p.rc, p.chunks}.base(g, s, q.row0) * step + (long long)h * p.lpad + pos;
     const int c1 = (vis.rb + p.rc - 1) / p.rc;
     for (int c0 = vis.ra / p.rc; c0 < c1; c0 += 8) {
       f32x4 y[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) y[j] = c0 + j < c1 ? *(const f32x4 *)(in + (long long)(c0 + j) * p.lpad) : f32x4{};
+      for (int j = 0; j < 8; ++j) y[j] = c0 + j < c1 ? *(const f32x4 *)(in + (c0 + j) * step) : f32x4{};
 #pragma unroll
       for (int j = 0; j < 8; ++j)
 #pragma unroll
@@ -558,12 +619,11 @@ __global__ void __launch_bounds__(64) aos_kv_weigh_sum_kernel(aos_kv_weigh_param
 template <int FMT, int HDP>
 int launch_many(const aos_kv_weigh_params *p, const aos_launch_ctx *ctx) {
   const uint32_t sh = (uint32_t)p->b.n_seqs * (uint32_t)p->b.nkv;
-  const uint32_t wgs = sh * (uint32_t)p->blocks * (uint32_t)p->chunks;
-  const int pieces = (p->rows + 255) / 256;
+  const uint32_t wgs = (uint32_t)p->slots * (uint32_t)p->b.nkv * (uint32_t)p->blocks;
   hipError_t e;
   AOS_LAUNCH(ctx, (aos_kv_weigh_kernel<FMT, HDP, false>), dim3(wgs), dim3(256), 0, *p);
   if ((e = hipGetLastError()) != hipSuccess) return (int)e;
-  AOS_LAUNCH(ctx, aos_kv_weigh_rows_kernel, dim3(sh * (uint32_t)pieces), dim3(256), 0, *p, pieces);
+  AOS_LAUNCH(ctx, aos_kv_weigh_rows_kernel, dim3((uint32_t)p->row_slots * (uint32_t)p->b.nkv), dim3(256), 0, *p);
   if ((e = hipGetLastError()) != hipSuccess) return (int)e;
   AOS_LAUNCH(ctx, (aos_kv_weigh_kernel<FMT, HDP, true>), dim3(wgs), dim3(256), 0, *p);
   if ((e = hipGetLastError()) != hipSuccess) return (int)e;
@@ -601,20 +661,29 @@ extern "C" int aos_kv_weigh_shape(aos_kv_weigh_params *p, size_t *bytes) {
   p->pieces = (int)((blocks + span - 1) / span);
   /* many rows: chunks of 64 where there are few, of up to 512 (prompt of 4001, 28 heads: 198 to 201 us; chunks of 256 take as
    * long, 201 to 202, and leave twice as many weights to add up) */
-  const double stages = (double)((rows + RT - 1) / RT), units = stages * sh * blocks;
+  const double one = shares_of_each(b, g, RT), own = shares_of_own(b, g, RT);
+  const bool each = one <= 2 * own;
+  const double heads = b.nkv * (double)blocks, units = (each ? one : own) * heads;
   const int k = units < 4096 ? 1 : units > 16384 ? 8 : (int)(units / 2048);
   p->rc = RT * k;
-  p->chunks = (int)((rows + p->rc - 1) / p->rc);
+  p->chunks = each ? (int)((rows + p->rc - 1) / p->rc) : 0;
+  p->row_pieces = each ? (int)((rows + 255) / 256) : 0;
+  const double slots = each ? shares_of_each(b, g, p->rc) : shares_of_own(b, g, p->rc);
+  const double row_slots = each ? shares_of_each(b, g, 256) : shares_of_own(b, g, 256);
   const double kept = (double)sh * rows * (4.0 * p->lpad + 8.0 * blocks);
   p->few = rows <= FEW && kept <= AOS_KV_WEIGH_KEEP && !p->no_few;
   double need = kept, wgs = (double)sh * blocks;
   if (!p->few) {
-    /* (chunks are at most units / 8 or 4096 of them, and one more for each block) */
-    need = 8.0 * b.n_tokens * p->nh * (blocks + 1) + 4.0 * KB * ((units > 32768 ? units / 8 : 4096) + (double)sh * blocks);
-    const double pieces = (double)((rows + 255) / 256), work = (double)blocks * p->chunks;
-    wgs = sh * (pieces > work ? pieces : work);
+    /* (chunks times blocks are at most units / 8 or 4096, and one more for each sequence's head and block; units are at
+     * most those of `most`, which grow with each of the batch's sizes, whichever way is taken) */
+    const double most = fmin(one, 2 * own) * heads;
+    need = 8.0 * b.n_tokens * p->nh * (blocks + 1) + 4.0 * KB * ((most > 32768 ? most / 8 : 4096) + (double)sh * blocks);
+    const double work = slots * (double)blocks;
+    wgs = fmax(wgs, b.nkv * fmax(work, row_slots));
   }
   if (need > AOS_KV_WEIGH_MOST || wgs > 2e9) return 0;
+  p->slots = p->few ? 0 : (int)slots;
+  p->row_slots = p->few ? 0 : (int)row_slots;
   *bytes = (size_t)need;
   return 1;
 }
@@ -635,7 +704,7 @@ extern "C" size_t aos_kv_weigh_most(const aos_kv_weigh_params *p) {
 extern "C" void aos_kv_weigh_parts(aos_kv_weigh_params *p, void *ws) {
   const size_t sh = (size_t)p->b.n_seqs * p->b.nkv, total = (size_t)p->b.n_tokens * p->nh;
   p->scores = (float *)ws;
-  p->part = p->scores + sh * (size_t)(p->few ? p->rows : p->chunks) * (size_t)p->lpad;
+  p->part = p->scores + (p->few ? sh * (size_t)p->rows : (size_t)p->slots * p->b.nkv) * (size_t)p->lpad;
   p->stat = p->few ? nullptr : p->part + 2 * total * (size_t)p->blocks;
 }
 
@@ -645,6 +714,27 @@ extern "C" void aoship_internal_kv_weigh_rows(int g, int window, int count, int 
   const Rows r = rows_of(Seq{0, count, len}, Span{len - count, window}, g, k0, k1);
   out[0] = r.ra;
   out[1] = r.rb;
+}
+
+/* The launches of a batch, for tests without a device: out = {few, rows of a chunk, chunks of each sequence (0: their own),
+ * chunks, 256-row pieces of each, pieces, padded length}; returns the workspace's bytes, 0 for a batch too large. */
+extern "C" size_t aoship_internal_kv_weigh_shape(int nkv, int nh, int n_seqs, int n_tokens, int max_new, int max_len, int *out) {
+  aos_kv_weigh_params p = {};
+  p.b.nkv = nkv;
+  p.b.n_seqs = n_seqs;
+  p.b.n_tokens = n_tokens;
+  p.b.max_new = max_new < n_tokens ? max_new : n_tokens;
+  p.b.max_len = max_len;
+  p.nh = nh;
+  size_t bytes = 0;
+  if (!aos_kv_weigh_shape(&p, &bytes)) return 0;
+  const int got[7] = {p.few, p.rc, p.chunks, p.slots, p.row_pieces, p.row_slots, p.lpad};
+  for (int i = 0; i < 7; ++i) out[i] = got[i];
+  return bytes;
+}
+/* number of sequence s's first share */
+extern "C" long long aoship_internal_kv_weigh_share(int unit, int each, int g, int s, int row0) {
+  return Shares{unit, each}.base(g, s, row0);
 }
 
 #define KV_DISPATCH(fn, fmt, hdp, ...)                                       \

@@ -672,3 +672,50 @@ def test_a_sequences_life(hip, fmt):
                 got = acc[layer][s, :, :lens_now[s]].double().cpu().numpy()
                 assert (np.abs(got - pr - want) <= _tolerance(qr[s:s + 1], h[0], hd ** -0.5, want, pr)).all()
     assert cache.faults() == 0
+
+
+# ---- attention weights of batches whose sequences differ much ----------------------------------
+
+
+@pytest.mark.parametrize("fmt,nh,nkv,hd,window", [("bf16", 28, 4, 128, 0), ("mxfp8", 24, 8, 128, 300), ("mxfp4", 14, 2, 64, 0),
+                                                  ("bf16", 4, 1, 256, 100)])
+@pytest.mark.parametrize("place", ["first", "last", "middle"])
+def test_weights_of_one_prompt_beside_single_tokens(hip, fmt, nh, nkv, hd, window, place):
+    """What a serving step has: a prompt's chunk and many streams of a token each, some of none"""
+    new, lens = [1, 0, 1] * 24, [5 + 17 * i for i in range(72)]
+    at = {"first": 0, "last": 72, "middle": 31}[place]
+    new.insert(at, 260)
+    lens.insert(at, 700)
+    _check_weigh(hip, fmt, nh, nkv, hd, 64, new, lens, window, seed=at)
+
+
+def test_weights_of_ragged_prompts(hip):
+    """More sequences than one round of the search for a row's sequence takes, rows in front of the first one's and behind
+    the last one's, and a workspace for batches of any spread"""
+    import torch
+
+    rng = np.random.default_rng(2)
+    n, nkv, nh, hd = 150, 1, 3, 64
+    new = np.where(rng.random(n) < 0.8, rng.integers(0, 3, n), rng.integers(3, 200, n))
+    lens = (new + rng.integers(0, 100, n)).tolist()
+    _check_weigh(hip, "bf16", nh, nkv, hd, 64, new.tolist(), lens, seed=3)
+    pool = P.Pool(hip, lens, nkv, hd, 64, "bf16")
+    k = P.to_gpu(P.bf16(rng.standard_normal((sum(lens), nkv, hd))))
+    pool.cache.append(0, pool.batch(lens, lens), k, k)
+    starts = np.concatenate([[0], np.cumsum(new)])
+    T = int(starts[-1])
+    q = torch.zeros((T + 60, nh, hd), dtype=torch.bfloat16, device="cuda")
+    q[40:40 + T] = P.to_gpu(P.bf16(rng.standard_normal((T, nh, hd))))
+    got = [torch.full((n, nkv, max(lens)), 7.0, device="cuda") for _ in range(2)]
+    pool.cache.weigh(0, pool.batch(new, lens), q[40:40 + T], got[0])
+    pool.cache.weigh(0, pool.batch(new, lens, starts=starts + 40), q, got[1])
+    assert torch.allclose(got[0], got[1], rtol=1e-5, atol=1e-7) and pool.cache.faults() == 0
+    # starts that fall, sequences with rows before 0 and behind n_tokens: noted, and the rest within bounds
+    for bad in (starts[::-1], np.where(np.arange(n + 1) == 70, 0, starts + 40)):
+        pool.cache.weigh(0, pool.batch(new, lens, starts=bad), q, got[1])
+        assert pool.cache.faults() & hip.KV_FAULT_BATCH
+    out = torch.full((n, nkv, max(lens)), 7.0, device="cuda")
+    pool.cache.weigh(0, pool.batch(new, lens, starts=starts - 5), q, out)
+    assert pool.cache.faults() == hip.KV_FAULT_BATCH and (out[0] == 7).all() and (out[-1, 0, :lens[-1]] != 7).all()
+    pool.cache.weigh(0, pool.batch(new, lens, starts=starts + 61), q, out)
+    assert pool.cache.faults() == hip.KV_FAULT_BATCH
