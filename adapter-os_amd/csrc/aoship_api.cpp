@@ -4156,6 +4156,15 @@ extern "C" int aoship_internal_kv_evict_check(const aoship_kv_config_t *c, int l
   return kv_evict_check(*c, layer, batch, e);
 }
 
+/* Diagnostic (no counterpart in the reference): most workgroups of a launch where a call's may be cut into several (0: as at
+ * first). Returns the number before. */
+uint32_t aos_launch_most = AOS_LAUNCH_MOST;
+extern "C" uint32_t aoship_internal_set_launch_most(uint32_t n) {
+  const uint32_t before = aos_launch_most;
+  aos_launch_most = n ? n : AOS_LAUNCH_MOST;
+  return before;
+}
+
 /* Diagnostic (no counterpart in the reference): with `on` 0 the cache's attention and weigh calls take the kernels of
  * large batches whatever a batch's size, so that tests reach these at small sizes. Same results within the tolerance. */
 extern "C" int aoship_internal_kv_cache_set_small_batches(aoship_kv_cache_t *m, int on) {

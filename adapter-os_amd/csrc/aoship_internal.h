@@ -637,6 +637,13 @@ typedef struct {
       hipLaunchKernelGGL(kernel, grid, block, lds, (hipStream_t)(ctx)->stream, __VA_ARGS__);      \
   } while (0)
 
+/* Workgroups that a launch gets of `left` ones: a grid has fewer than 2^32 threads, of up to 1024 a workgroup. Where a
+ * call can need more (attention weights, eviction, log probabilities), its kernels count workgroups from wg0 on and it
+ * launches them one piece after the other. aos_launch_most is a variable for tests of such pieces at small sizes. */
+#define AOS_LAUNCH_MOST (1u << 21)
+extern uint32_t aos_launch_most;
+#define AOS_LAUNCH_PIECE(left) ((left) < aos_launch_most ? (left) : aos_launch_most)
+
 /* A launcher with nothing to do still closes its profiling interval (zero length), so that
  * pooled events never report a stale time. */
 #define AOS_SKIP(ctx)                                                                             \
@@ -722,6 +729,7 @@ typedef struct {
   int rc, chunks, slots;     /* rows of a chunk; chunks of each sequence (0: as many as its rows need); all of them */
   int row_pieces, row_slots; /* the same of 256 rows */
   uint32_t g_mul, g_shift; /* of the division by the heads of a group */
+  uint32_t wg0;            /* number of the launch's first workgroup */
   /* aos_kv_weigh_parts: */
   float *scores; /* few: [sequence][head][rows][lpad]; else the chunks' weights [slots][head][lpad] */
   float *part;   /* maxima and sums: few: [sequence][head][pieces][rows][2]; else [head][blocks][all rows][2] */
@@ -739,6 +747,7 @@ typedef struct {
   const int32_t *to;    /* [n_seqs][to_stride] pages */
   int to_stride;
   int32_t *kept;        /* [sequence][head][kept position] */
+  uint32_t wg0;         /* number of the launch's first workgroup */
 } aos_kv_evict_params;
 
 /* Attention splits its work evenly over its workgroups, whatever sequence a share falls in; a row tile cut between
@@ -772,7 +781,8 @@ typedef struct {
   int32_t *top_ids;             /* [T][n_top] or NULL */
   float *top_logprobs;          /* [T][n_top] or NULL */
   uint64_t *part;               /* [AOS_LOGPROBS_WGS][AOS_LOGPROBS_PART] */
-  uint32_t *counters;           /* [AOS_LOGPROBS_WGS] arrivals of a row's slices, zero between launches */
+  uint32_t *counters;           /* [AOS_LOGPROBS_WGS] arrivals of a row's slices, zero between calls */
+  uint32_t wg0;                 /* number of the launch's first workgroup */
 } aos_logprobs_params;
 
 #ifdef __cplusplus

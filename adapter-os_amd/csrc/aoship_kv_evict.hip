@@ -68,7 +68,7 @@ __global__ void __launch_bounds__(NT) aos_kv_select_kernel(aos_kv_evict_params p
   __shared__ int totals[2], listed;
   __shared__ uint32_t list[LIST];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int s = (int)blockIdx.x / p.b.nkv, h = (int)blockIdx.x - s * p.b.nkv;
+  const int sh = (int)(p.wg0 + blockIdx.x), s = sh / p.b.nkv, h = sh - s * p.b.nkv;
   const Kept k = kept_of(p, s);
   if (k.n < 0) return;
   const float *w = p.weights + (long long)s * p.w_seq + (long long)h * p.w_head;
@@ -275,7 +275,8 @@ __global__ void __launch_bounds__(256) aos_kv_move_kernel(aos_kv_evict_params p,
   __shared__ const unsigned char *src[TILE]; /* the tiles that the positions are in; NULL: none */
   __shared__ int in[TILE];                   /* their places in them */
   const int tid = threadIdx.x;
-  const int tile = (int)(blockIdx.x % (uint32_t)tiles), sh = (int)(blockIdx.x / (uint32_t)tiles);
+  const uint32_t wg = p.wg0 + blockIdx.x;
+  const int tile = (int)(wg % (uint32_t)tiles), sh = (int)(wg / (uint32_t)tiles);
   const int s = sh / p.b.nkv, h = sh - s * p.b.nkv, i0 = tile * TILE;
   const Kept k = kept_of(p, s);
   if (i0 >= k.n) return;
@@ -372,17 +373,26 @@ int evict(const aos_kv_evict_params *p, const aos_launch_ctx *ctx) {
   const uint32_t sh = (uint32_t)p->b.n_seqs * (uint32_t)p->b.nkv;
   /* registers for the longest sequence */
   const int len = p->b.max_len;
-  if (len <= 4 * NT)
-    AOS_LAUNCH(ctx, aos_kv_select_kernel<4>, dim3(sh), dim3(NT), 0, *p);
-  else if (len <= 16 * NT)
-    AOS_LAUNCH(ctx, aos_kv_select_kernel<16>, dim3(sh), dim3(NT), 0, *p);
-  else
-    AOS_LAUNCH(ctx, aos_kv_select_kernel<MOST>, dim3(sh), dim3(NT), 0, *p);
-  const hipError_t e = hipGetLastError();
+  aos_kv_evict_params a = *p;
+  for (a.wg0 = 0; a.wg0 < sh; a.wg0 += AOS_LAUNCH_PIECE(sh - a.wg0)) {
+    const uint32_t n = AOS_LAUNCH_PIECE(sh - a.wg0);
+    if (len <= 4 * NT)
+      AOS_LAUNCH(ctx, aos_kv_select_kernel<4>, dim3(n), dim3(NT), 0, a);
+    else if (len <= 16 * NT)
+      AOS_LAUNCH(ctx, aos_kv_select_kernel<16>, dim3(n), dim3(NT), 0, a);
+    else
+      AOS_LAUNCH(ctx, aos_kv_select_kernel<MOST>, dim3(n), dim3(NT), 0, a);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return (int)e;
+  }
   const int tiles = (p->max_keep + TILE - 1) / TILE;
-  if (e != hipSuccess || tiles == 0) return (int)e;
-  AOS_LAUNCH(ctx, (aos_kv_move_kernel<FMT, HDP>), dim3(sh * (uint32_t)tiles), dim3(256), 0, *p, tiles);
-  return (int)hipGetLastError();
+  const uint32_t wgs = sh * (uint32_t)tiles;
+  for (a.wg0 = 0; a.wg0 < wgs; a.wg0 += AOS_LAUNCH_PIECE(wgs - a.wg0)) {
+    AOS_LAUNCH(ctx, (aos_kv_move_kernel<FMT, HDP>), dim3(AOS_LAUNCH_PIECE(wgs - a.wg0)), dim3(256), 0, a, tiles);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return (int)e;
+  }
+  return 0;
 }
 
 }  // namespace

@@ -90,8 +90,9 @@ __global__ void __launch_bounds__(256, 2) aos_kv_scores_kernel(aos_kv_weigh_para
   __shared__ float ml[4][2][32];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 31, half = lane >> 5;
-  const int sh = (int)(blockIdx.x / (uint32_t)p.pieces);
-  const int piece = turned((int)(blockIdx.x - (uint32_t)sh * (uint32_t)p.pieces), sh, p.pieces);
+  const uint32_t wg = p.wg0 + blockIdx.x;
+  const int sh = (int)(wg / (uint32_t)p.pieces);
+  const int piece = turned((int)(wg - (uint32_t)sh * (uint32_t)p.pieces), sh, p.pieces);
   const int s = sh / p.b.nkv, h = sh - s * p.b.nkv;
   const Seq q = seq_at(p.b, s);
   const int g = p.nh / p.b.nkv, rows = q.count * g;
@@ -190,7 +191,8 @@ constexpr int WB = 1024;
 __global__ void __launch_bounds__(256) aos_kv_weights_kernel(aos_kv_weigh_params p, int blocks) {
   __shared__ float red[8][2][FEW], base[FEW], inv[FEW];
   const int tid = threadIdx.x;
-  const int blk = (int)(blockIdx.x % (uint32_t)blocks), sh = (int)(blockIdx.x / (uint32_t)blocks);
+  const uint32_t wg = p.wg0 + blockIdx.x;
+  const int blk = (int)(wg % (uint32_t)blocks), sh = (int)(wg / (uint32_t)blocks);
   const int s = sh / p.b.nkv, h = sh - s * p.b.nkv;
   const Seq q = seq_at(p.b, s);
   const int rows = q.count * (p.nh / p.b.nkv), pos = blk * WB + 4 * tid;
@@ -261,15 +263,30 @@ __global__ void __launch_bounds__(256) aos_kv_weights_kernel(aos_kv_weigh_params
   store4(p, s, h, pos, q.len, x);
 }
 
+/* a kernel's wgs workgroups, in as many launches as they take */
+template <class Launch>
+int in_pieces(const aos_kv_weigh_params *p, uint32_t wgs, Launch &&launch) {
+  aos_kv_weigh_params a = *p;
+  for (a.wg0 = 0; a.wg0 < wgs; a.wg0 += AOS_LAUNCH_PIECE(wgs - a.wg0)) {
+    launch(a, AOS_LAUNCH_PIECE(wgs - a.wg0));
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return (int)e;
+  }
+  return 0;
+}
+
 template <int FMT, int HDP>
 int launch_few(const aos_kv_weigh_params *p, const aos_launch_ctx *ctx) {
   const uint32_t sh = (uint32_t)p->b.n_seqs * (uint32_t)p->b.nkv;
-  AOS_LAUNCH(ctx, (aos_kv_scores_kernel<FMT, HDP>), dim3(sh * (uint32_t)p->pieces), dim3(256), 0, *p);
-  const hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return (int)e;
   const int blocks = (p->b.max_len + WB - 1) / WB;
-  AOS_LAUNCH(ctx, aos_kv_weights_kernel, dim3(sh * (uint32_t)blocks), dim3(256), 0, *p, blocks);
-  return (int)hipGetLastError();
+  int e = in_pieces(p, sh * (uint32_t)p->pieces, [&](const aos_kv_weigh_params &a, uint32_t n) {
+    AOS_LAUNCH(ctx, (aos_kv_scores_kernel<FMT, HDP>), dim3(n), dim3(256), 0, a);
+  });
+  if (!e)
+    e = in_pieces(p, sh * (uint32_t)blocks, [&](const aos_kv_weigh_params &a, uint32_t n) {
+      AOS_LAUNCH(ctx, aos_kv_weights_kernel, dim3(n), dim3(256), 0, a, blocks);
+    });
+  return e;
 }
 
 /* ---- many rows ------------------------------------------------------------------------------- */
@@ -381,7 +398,8 @@ __global__ void __launch_bounds__(256, HDP == 256 ? 1 : 3) aos_kv_weigh_kernel(a
   __shared__ float red[SUM ? 1 : 2][4][2][SUM ? 1 : RT];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 31, half = lane >> 5;
-  const int x = (int)(blockIdx.x / (uint32_t)p.blocks), b0 = (int)(blockIdx.x - (uint32_t)x * (uint32_t)p.blocks);
+  const uint32_t wg = p.wg0 + blockIdx.x;
+  const int x = (int)(wg / (uint32_t)p.blocks), b0 = (int)(wg - (uint32_t)x * (uint32_t)p.blocks);
   const int blk = turned(b0, x, p.blocks), g = p.nh / p.b.nkv;
   const Share chunk = share_at(p.b, Shares{p.rc, p.chunks}, g, (uint32_t)x, lane);
   const int s = chunk.s, h = chunk.h;
@@ -562,7 +580,7 @@ __global__ void __launch_bounds__(256, HDP == 256 ? 1 : 3) aos_kv_weigh_kernel(a
 __global__ void __launch_bounds__(256) aos_kv_weigh_rows_kernel(aos_kv_weigh_params p) {
   if (refused(p.b, starts_fall(p.b, (int)threadIdx.x, 256), (int)threadIdx.x)) return;
   const int g = p.nh / p.b.nkv;
-  const Share piece = share_at(p.b, Shares{256, p.row_pieces}, g, blockIdx.x, (int)threadIdx.x & 63);
+  const Share piece = share_at(p.b, Shares{256, p.row_pieces}, g, p.wg0 + blockIdx.x, (int)threadIdx.x & 63);
   const int s = piece.s, h = piece.h;
   if (s < 0) return;
   const Seq q = seq_at(p.b, s);
@@ -591,7 +609,8 @@ __global__ void __launch_bounds__(256) aos_kv_weigh_rows_kernel(aos_kv_weigh_par
 /* Grid: blocks of KB positions, key/value heads, sequences: the chunks' weights added in order. */
 __global__ void __launch_bounds__(64) aos_kv_weigh_sum_kernel(aos_kv_weigh_params p) {
   if (refused(p.b, starts_fall(p.b, (int)threadIdx.x, 64), (int)threadIdx.x)) return;
-  const int blk = (int)(blockIdx.x % (uint32_t)p.blocks), sh = (int)(blockIdx.x / (uint32_t)p.blocks);
+  const uint32_t wg = p.wg0 + blockIdx.x;
+  const int blk = (int)(wg % (uint32_t)p.blocks), sh = (int)(wg / (uint32_t)p.blocks);
   const int s = sh / p.b.nkv, h = sh - s * p.b.nkv;
   const Seq q = seq_at(p.b, s);
   const int g = p.nh / p.b.nkv, k0 = blk * KB, k1 = k0 + KB < q.len ? k0 + KB : q.len, pos = k0 + 4 * (int)threadIdx.x;
@@ -620,15 +639,22 @@ template <int FMT, int HDP>
 int launch_many(const aos_kv_weigh_params *p, const aos_launch_ctx *ctx) {
   const uint32_t sh = (uint32_t)p->b.n_seqs * (uint32_t)p->b.nkv;
   const uint32_t wgs = (uint32_t)p->slots * (uint32_t)p->b.nkv * (uint32_t)p->blocks;
-  hipError_t e;
-  AOS_LAUNCH(ctx, (aos_kv_weigh_kernel<FMT, HDP, false>), dim3(wgs), dim3(256), 0, *p);
-  if ((e = hipGetLastError()) != hipSuccess) return (int)e;
-  AOS_LAUNCH(ctx, aos_kv_weigh_rows_kernel, dim3((uint32_t)p->row_slots * (uint32_t)p->b.nkv), dim3(256), 0, *p);
-  if ((e = hipGetLastError()) != hipSuccess) return (int)e;
-  AOS_LAUNCH(ctx, (aos_kv_weigh_kernel<FMT, HDP, true>), dim3(wgs), dim3(256), 0, *p);
-  if ((e = hipGetLastError()) != hipSuccess) return (int)e;
-  AOS_LAUNCH(ctx, aos_kv_weigh_sum_kernel, dim3(sh * (uint32_t)p->blocks), dim3(64), 0, *p);
-  return (int)hipGetLastError();
+  int e = in_pieces(p, wgs, [&](const aos_kv_weigh_params &a, uint32_t n) {
+    AOS_LAUNCH(ctx, (aos_kv_weigh_kernel<FMT, HDP, false>), dim3(n), dim3(256), 0, a);
+  });
+  if (!e)
+    e = in_pieces(p, (uint32_t)p->row_slots * (uint32_t)p->b.nkv, [&](const aos_kv_weigh_params &a, uint32_t n) {
+      AOS_LAUNCH(ctx, aos_kv_weigh_rows_kernel, dim3(n), dim3(256), 0, a);
+    });
+  if (!e)
+    e = in_pieces(p, wgs, [&](const aos_kv_weigh_params &a, uint32_t n) {
+      AOS_LAUNCH(ctx, (aos_kv_weigh_kernel<FMT, HDP, true>), dim3(n), dim3(256), 0, a);
+    });
+  if (!e)
+    e = in_pieces(p, sh * (uint32_t)p->blocks, [&](const aos_kv_weigh_params &a, uint32_t n) {
+      AOS_LAUNCH(ctx, aos_kv_weigh_sum_kernel, dim3(n), dim3(64), 0, a);
+    });
+  return e;
 }
 
 template <int FMT, int HDP>

@@ -249,7 +249,8 @@ __global__ void __launch_bounds__(NT, 4) aos_logprobs_kernel(aos_logprobs_params
   constexpr int FLY = 2; /* units of a thread on their way while as many are worked on */
   __shared__ Shared sh;
   const int tid = threadIdx.x;
-  const int row = (int)(blockIdx.x / (uint32_t)p.slices), slice = (int)(blockIdx.x - (uint32_t)row * (uint32_t)p.slices);
+  const uint32_t wg = p.wg0 + blockIdx.x;
+  const int row = (int)(wg / (uint32_t)p.slices), slice = (int)(wg - (uint32_t)row * (uint32_t)p.slices);
   const char *x = (const char *)p.logits + (long long)row * p.ld * SIZE;
   const int a0 = slice * p.span, a1 = a0 + p.span < p.vocab ? a0 + p.span : p.vocab;
   const int lead = (int)((16u - (uint32_t)((uintptr_t)(x + (long long)a0 * SIZE) & 15u)) & 15u) / SIZE;
@@ -402,7 +403,7 @@ __global__ void __launch_bounds__(NT, 4) aos_logprobs_kernel(aos_logprobs_params
     answer(p, sh, row, st, xt, target, before);
     return;
   }
-  uint64_t *part = p.part + (size_t)blockIdx.x * AOS_LOGPROBS_PART;
+  uint64_t *part = p.part + (size_t)wg * AOS_LOGPROBS_PART;
   if (tid == 0) {
     publish(part, pair(st.m, st.l));
     publish(part + 1, pair(st.s, __builtin_bit_cast(float, before)));
@@ -453,8 +454,14 @@ __global__ void __launch_bounds__(NT, 4) aos_logprobs_kernel(aos_logprobs_params
 
 template <bool BF16>
 int launch(const aos_logprobs_params *p, const aos_launch_ctx *ctx) {
-  AOS_LAUNCH(ctx, (aos_logprobs_kernel<BF16>), dim3((uint32_t)p->T * (uint32_t)p->slices), dim3(NT), 0, *p);
-  return (int)hipGetLastError();
+  const uint32_t wgs = (uint32_t)p->T * (uint32_t)p->slices;
+  aos_logprobs_params a = *p;
+  for (a.wg0 = 0; a.wg0 < wgs; a.wg0 += AOS_LAUNCH_PIECE(wgs - a.wg0)) {
+    AOS_LAUNCH(ctx, (aos_logprobs_kernel<BF16>), dim3(AOS_LAUNCH_PIECE(wgs - a.wg0)), dim3(NT), 0, a);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return (int)e;
+  }
+  return 0;
 }
 
 }  // namespace
