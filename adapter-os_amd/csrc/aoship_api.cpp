@@ -3639,6 +3639,8 @@ struct aoship_kv_cache {
   DevBuf faults; /* two words: faults, and whether an infinity or a NaN has entered the values */
   int rope_positions = 0;
   DevBuf weigh; /* aoship_kv_weigh's workspace */
+  bool weigh_held = false;          /* a captured call's graph has it */
+  std::vector<DevBuf> weigh_before; /* smaller ones that graphs have */
   DevBuf axes; /* of the rotated pairs, four to a byte */
   int n_axes = 1;
   bool small_batches = true; /* diagnostic: aoship_internal_kv_cache_set_small_batches */
@@ -4028,6 +4030,8 @@ static int kv_weigh_grow(aoship_kv_cache *m, const char *what, size_t bytes) {
                                        "(aoship_kv_weigh_reserve)");
   }
   HIP_OR_FAIL(hipDeviceSynchronize(), "hipDeviceSynchronize"); /* (a launch may still use the old one) */
+  if (m->weigh_held) m->weigh_before.push_back(std::move(m->weigh)); /* (a replay writes to it) */
+  m->weigh_held = false;
   return m->weigh.alloc(bytes, false);
 }
 
@@ -4065,6 +4069,9 @@ extern "C" int aoship_kv_weigh(aoship_kv_cache_t *m, int layer, const aoship_kv_
   p.no_few = !m->small_batches;
   if (p.no_few && !aos_kv_weigh_shape(&p, &bytes)) return set_err("aoship_kv_weigh: rows times positions of the batch too large");
   if (kv_weigh_grow(m, "aoship_kv_weigh", bytes)) return -1;
+  hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+  if (hipStreamIsCapturing(m->stream, &st) != hipSuccess) (void)hipGetLastError(); /* (the launch says why) */
+  if (st == hipStreamCaptureStatusActive) m->weigh_held = true;
   aos_kv_weigh_parts(&p, m->weigh.p);
   p.q = q;
   p.q_ld = q_stride;

@@ -560,7 +560,7 @@ int aoship_kv_weigh(aoship_kv_cache_t *cache, int layer, const aoship_kv_batch_t
                     int64_t q_stride, int num_heads, float scale, int window, const aoship_kv_weights_t *weights);
 
 /* Sizes the workspace for batches of up to these sizes, so that calls allocate nothing (a captured call's graph holds the
- * workspace of its time: reserve the largest before). Bytes, with max_len in blocks of 256 positions: where no sequence has
+ * workspace of its time, which stays until the cache is freed: reserve the largest before). Bytes, with max_len in blocks of 256 positions: where no sequence has
  * more than 32 rows (new tokens times heads of a group), 4 for a row, a key/value head and a position, 1 GB at most;
  * else, for a batch of n_tokens and n_seqs however its rows are spread, 8 for a new token, a query head and a block
  * (and one block more), 4 for a position of a key/value head and each 256 rows, 5 for one and each sequence, and 4 MB. A

@@ -719,3 +719,44 @@ def test_weights_of_ragged_prompts(hip):
     assert pool.cache.faults() == hip.KV_FAULT_BATCH and (out[0] == 7).all() and (out[-1, 0, :lens[-1]] != 7).all()
     pool.cache.weigh(0, pool.batch(new, lens, starts=starts + 61), q, out)
     assert pool.cache.faults() == hip.KV_FAULT_BATCH
+
+
+@pytest.mark.parametrize("new", [1, 40])
+def test_a_graph_keeps_its_workspace(hip, new):
+    """Eager calls and a second graph that need a larger one, between the replays of a graph captured before"""
+    import torch
+
+    rng = np.random.default_rng(new)
+    lens, nkv, hd, nh = [200, 400], 2, 64, 6
+    pool = P.Pool(hip, [2048, 2048], nkv, hd, 64, "bf16")
+    k = P.to_gpu(P.bf16(rng.standard_normal((4096, nkv, hd))))
+    pool.cache.append(0, pool.batch([2048] * 2, [2048] * 2), k, k)
+    small, large = pool.batch([new] * 2, lens), pool.batch([300, 200], [2048, 1900])
+    q = [P.to_gpu(P.bf16(rng.standard_normal((n, nh, hd)))) for n in (2 * new, 500)]
+    out = [torch.zeros((2, nkv, n), device="cuda") for n in (400, 2048)]
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    pool.cache.set_stream(s.cuda_stream)
+    pool.cache.reserve_weigh(nh, small, 2 * new)
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+    with torch.cuda.graph(graphs[0], stream=s):
+        pool.cache.weigh(0, small, q[0], out[0])
+    free = torch.cuda.mem_get_info()[0]
+    pool.cache.weigh(0, large, q[1], out[1])
+    torch.cuda.synchronize()
+    want = [torch.zeros_like(out[0]), out[1].clone()]
+    assert torch.cuda.mem_get_info()[0] < free
+    with torch.cuda.graph(graphs[1], stream=s):
+        pool.cache.weigh(0, large, q[1], out[1])
+    pool.cache.weigh(0, small, q[0], want[0])
+    torch.cuda.synchronize()
+    for i in range(3):
+        filler = torch.full((1 << 22,), 5.0, device="cuda")  # (as what would be freed might be used again)
+        for g, o, w in zip(graphs, out, want):
+            o.zero_()
+            torch.cuda.synchronize()
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(o, w) and float(o.sum()) > 0
+        assert (filler == 5).all()
+        del filler
