@@ -522,7 +522,8 @@ int aoship_kv_read(aoship_kv_cache_t *cache, int layer, const aoship_kv_batch_t 
  * consecutive groups. A row that sees nothing gives zeros. q, out: device rows of num_heads * head_dim (out must
  * not overlap q). Scores, probabilities and sums are float32; each probability is rounded to bfloat16 (by at most 2^-8 of
  * it, beside its exact sum) where it multiplies a value, and the result at the end. Probabilities times values are summed
- * before the division by their sum: magnitudes above some 2^90 can come out as infinities or NaN. The order of these sums
+ * before the division by their sum: magnitudes above some 2^90 can come out as infinities or NaN. Scores are to stay within
+ * 2^30: a row with one beyond, whose exponent's rounding passes what float32 holds, can be NaN. The order of these sums
  * follows from the whole batch (its sequences' rows and lengths, and the device): the same call gives the same bits each
  * time, but a sequence among other neighbours may differ in its last bits.
  * An infinity or a NaN reaches the rows that see its position and no others (an infinity whose probability rounds to zero,
@@ -553,7 +554,7 @@ typedef struct {
  * rows only, give a batch of these rows. Everything is float32, in an order that follows from the batch: the same call
  * gives the same bits. A batch without rows (n_tokens or max_new 0) is nothing to do. A row without probabilities (a
  * NaN in it, or no score that float32 holds above minus infinity) makes the weights of all
- * positions that it sees NaN. In a batch whose starts fall nothing may be written.
+ * positions that it sees NaN, and one with a score beyond 2^30 in magnitude can, as in aoship_kv_attention. In a batch whose starts fall nothing may be written.
  * Uses a workspace of the cache's, which calls of one cache share and a call grows if it must: that synchronises the
  * device, and is refused while the cache's stream is captured. Asynchronous otherwise. Returns 0 / -1. */
 int aoship_kv_weigh(aoship_kv_cache_t *cache, int layer, const aoship_kv_batch_t *batch, const aoship_bf16_t *q,

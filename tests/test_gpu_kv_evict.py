@@ -760,3 +760,28 @@ def test_a_graph_keeps_its_workspace(hip, new):
             assert torch.equal(o, w) and float(o.sum()) > 0
         assert (filler == 5).all()
         del filler
+
+
+@pytest.mark.parametrize("new", [1, 60])
+@pytest.mark.parametrize("e", [10, 20, 29])
+def test_weights_of_large_scores(hip, new, e):
+    """Scores of up to 2^30, as documented, exact in float32 (one product each) and hundreds apart or equal: a row's weight
+    goes to its largest ones alike. 100 equal terms are added (half a step each, 2^-24), an exponential and an inverse
+    taken, and 120 rows added up: 2^-16 of a weight in all."""
+    import torch
+
+    lens, nkv, nh, hd = [300, 65], 2, 4, 64
+    k = np.zeros((sum(lens), nkv, hd))
+    for o, n in ((0, 300), (300, 65)):
+        k[o:o + n:3, :, 0], k[o + 1:o + n:3, :, 0] = 2.0 ** e * 1.171875, 2.0 ** (e - 1)
+    q = np.zeros((2 * new, nh, hd))
+    q[..., 0] = 1.6875  # (products of up to 1.98 2^e)
+    q[::2, 1, 0] = -1.6875
+    pool = P.Pool(hip, lens, nkv, hd, 64, "bf16")
+    pool.cache.append(0, pool.batch(lens, lens), P.to_gpu(k), P.to_gpu(k))
+    out = torch.full((2, nkv, 300), 7.0, device="cuda")
+    pool.cache.weigh(0, pool.batch([new] * 2, lens), P.to_gpu(q), out, scale=1.0)
+    got = out.double().cpu().numpy()
+    for s, (o, n) in enumerate(((0, 300), (300, 65))):
+        want = _weights(q[s * new:(s + 1) * new], k[o:o + n], 1.0, 0, nkv)
+        assert want.max() > 0.003 and (np.abs(got[s, :, :n] - want) <= 2.0 ** -16 * want + 1e-30).all()
