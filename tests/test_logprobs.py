@@ -59,3 +59,16 @@ def test_slices_cover_a_row_within_the_workspace(T, vocab):
     assert 1 <= n <= 1024 and n * span.value >= vocab and (n - 1) * span.value < vocab
     if n > 1:
         assert T * n <= 2048 and span.value % 32 == 0 and span.value >= 2048
+
+
+@pytest.mark.parametrize("T", [1, 2, 3, 7, 100, 255, 256, 257, 341, 342, 511, 512, 513, 1023, 1024, 1025, 1 << 26])
+@pytest.mark.parametrize("vocab", [4096, 50257, 152064, 524287, 1 << 20, (1 << 21) + 1, 1 << 24, 1 << 30])
+def test_slices_stay_within_the_handles_workspace(T, vocab):
+    """The workspace holds the pieces of 1024 workgroups and as many rows' counters, and a thread joins four slices of a row."""
+    f = aoship.lib().aoship_internal_logprobs_shape
+    f.restype, f.argtypes = C.c_int, [C.c_int, C.c_int, C.POINTER(C.c_int)]
+    span = C.c_int()
+    n = f(T, vocab, C.byref(span))
+    assert 1 <= n <= 1024
+    if n > 1:
+        assert T * n <= 1024 and T <= 1024
