@@ -130,7 +130,8 @@ __device__ __forceinline__ void turn_of(const aos_kv_append_params &p, int pos, 
 /* Grid (blocks of 16 positions, groups of query heads then key/value heads). Bound by memory, by latency where there are
  * few rows: 8191 tokens of 40 query and 8 key/value heads of 128 at 16 bits 47 us (235 MB, 5.0 TB/s), 5 prompts of up to
  * 1531 tokens, 28/4 heads, at 4 bits 21 us, one token 3.9 us. With positions given (AT; on three axes in turn, so that each pair
- * is looked up by itself) two prompts of up to 6111 tokens, 24/8 heads, at 8 bits 39 us, 48 tokens of 28/4 heads 4.7. */
+ * is looked up by itself) two prompts of up to 6111 tokens, 24/8 heads, at 8 bits 52 us (171 MB, 3.3 TB/s; 40 where the caches
+ * still hold the rows), 48 tokens of 28/4 heads 4.7. */
 template <int FMT, int HDP, bool AT>
 __global__ void __launch_bounds__(256) aos_kv_append_kernel(aos_kv_append_params p, int qgroups) {
   constexpr int LD = HDP + 8; /* LDS row: 16 bytes of padding keep the column reads of a value unit apart */

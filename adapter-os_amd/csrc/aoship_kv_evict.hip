@@ -5,9 +5,10 @@
  * between the ones of greatest weight (a NaN below everything; equal weights: the lower positions), in their order. They
  * are moved to other pages, codes and scales as they are, so that nothing is rounded again.
  *
- *   select  the n-th greatest weight by bisection of its bits: a workgroup has a head's weights in registers (up to 32768,
- *           else it reads them again for each bit) and counts those that reach a bound, 32 times at most; then the kept
- *           positions' places by counting the kept ones before them.
+ *   select  the n-th greatest weight by its bits, two a turn: a workgroup counts the weights that reach each of three bounds, 16
+ *           times at most and once more where equal weights part; after eight bits those still in question, if few, are
+ *           listed and only they counted. It holds a head's weights itself up to 32768, and reads longer ones again each
+ *           turn; then the kept positions' places by counting the kept ones before them.
  *   move    a workgroup gathers a tile of 64 kept positions. Keys are 16-byte units of one position; values, whose units
  *           hold 8 or 16 positions of a dimension, are taken apart and put together element by element.
  */
@@ -58,7 +59,8 @@ __device__ __forceinline__ int lane_scan(int x, int lane) {
 }
 
 /* Bound by the latency of its turns and by how few workgroups there are: 2 heads of 2047 weights 11 us, 128 of up to 12000 26,
- * 32 of up to 32767 52.
+ * 32 of up to 32767 52. The instance of 32 weights a thread (max_len past 16384) is at its 128 registers and keeps 31 of a
+ * thread's words in private memory.
  * Grid: sequences times key/value heads. Thread t has the positions t, t + 1024, ... of a span of PER * 1024. */
 template <int PER>
 __global__ void __launch_bounds__(NT) aos_kv_select_kernel(aos_kv_evict_params p) {
@@ -103,7 +105,7 @@ __global__ void __launch_bounds__(NT) aos_kv_select_kernel(aos_kv_evict_params p
   const bool once = k.len <= SPAN;
   uint32_t x[PER];
   if (once) load(x, 0);
-  auto count_of = [&](auto &&counts) { /* adds up counts(i) of all rows and spans, a row's by its wave */
+  auto count_of = [&](auto &&counts) { /* counts(x) of each of a thread's weights, span by span */
     for (int base = 0; base < k.len; base += SPAN) {
       if (!once) load(x, base);
 #pragma unroll

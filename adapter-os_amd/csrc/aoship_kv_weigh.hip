@@ -387,8 +387,11 @@ struct Stage {
  *   SUM true: the weights of the block's positions from the chunk's rows, to scores[chunk][head][position].
  * Grid: blocks, shares (chunks) of the rows.
  *
- * Bound by the vector instructions beside the matrix ones (12 and 10 of them to one). Prompt of 4001, 28/4 heads of 128, 16
- * bits: 93 and 90 us for 57 GFLOP each. 32 tokens over up to 8132 positions, 12 sequences, 24/8 heads, 8
+ * Prompt of 4001, 28/4 heads of 128, 16 bits: 93 and 90 us for 57 GFLOP each, more than any one unit's part of it: a SIMD has 34 us
+ * of vector instructions (12 and 10 of them to a matrix one), 17 of the exponentials' lower rate and 23 of matrix
+ * instructions. They overlap little: both position blocks' products end in the same step, so that a wave has no exponentials
+ * to form while its products run, and registers leave three waves a SIMD (heads wider than 128: one, two where the weights of
+ * quantised keys are formed); waves wait for 35% of their cycles. 32 tokens over up to 8132 positions, 12 sequences, 24/8 heads, 8
  * bits: 30 us either way. Queries' fragments read four ahead of the matrix instructions were within the runs' spread (the prompt
  * 209 and 205 us for 213 and 207 in all), with a wave fewer a SIMD slower (216 and 219; the 32 tokens 79 us for 72 and 73). */
 template <int FMT, int HDP, bool SUM>

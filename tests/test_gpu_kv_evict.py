@@ -690,7 +690,7 @@ def test_weights_of_one_prompt_beside_single_tokens(hip, fmt, nh, nkv, hd, windo
 
 
 def test_weights_of_ragged_prompts(hip):
-    """More sequences than one round of the search for a row's sequence takes, rows in front of the first one's and behind
+    """More sequences than one step of the search for a row's sequence takes, rows in front of the first one's and behind
     the last one's, and a workspace for batches of any spread"""
     import torch
 
@@ -785,3 +785,14 @@ def test_weights_of_large_scores(hip, new, e):
     for s, (o, n) in enumerate(((0, 300), (300, 65))):
         want = _weights(q[s * new:(s + 1) * new], k[o:o + n], 1.0, 0, nkv)
         assert want.max() > 0.003 and (np.abs(got[s, :, :n] - want) <= 2.0 ** -16 * want + 1e-30).all()
+
+
+def test_weights_of_thousands_of_sequences(hip):
+    """A row's sequence searched for in three steps"""
+    rng = np.random.default_rng(4)
+    n = 5000
+    new = (rng.random(n) < 0.5).astype(int)
+    lens = new + rng.integers(0, 4, n)
+    new[4321], lens[4321] = 300, 333
+    new[77], lens[77] = 40, 40
+    _check_weigh(hip, "bf16", 2, 1, 64, 64, new.tolist(), lens.tolist(), seed=9)
